@@ -10,6 +10,7 @@ from .attention import decode_attention
 from .paged import PageTable, PagedCompressedKV, PagedBF16KV
 from .codec import encode_reference, decode_reference, bits_per_value
 from .kernels import attention_compressed, attention_reference, decode_to_bf16, encode_pages
+from .layer import prompt_attention, rotate_prompt, rope_append, rope_append_paged, add_norm
 
 
 def __getattr__(name):
@@ -23,4 +24,5 @@ __version__ = "0.1.0"
 __all__ = ["CompressedKV", "BF16KV", "check_overflow", "decode_attention", "Engine",
            "encode_reference", "decode_reference", "bits_per_value",
            "attention_compressed", "attention_reference", "decode_to_bf16", "encode_pages",
-           "PageTable", "PagedCompressedKV", "PagedBF16KV", "PagedEngine"]
+           "PageTable", "PagedCompressedKV", "PagedBF16KV", "PagedEngine",
+           "prompt_attention", "rotate_prompt", "rope_append", "rope_append_paged", "add_norm"]

@@ -13,7 +13,7 @@ _PATH = os.environ.get("EXACTKV_LIB") or os.path.join(os.path.dirname(os.path.ab
 # EXACTKV_CHECK_ERRORS=1: after every kernel-launching call, wait for its stream and raise if
 # a kernel set a sticky error bit (exkv_error_bits); slow, for debugging
 _CHECK = os.environ.get("EXACTKV_CHECK_ERRORS", "") not in ("", "0")
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _p, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -74,11 +74,27 @@ SIGNATURES = {
     "exkv_noalloc_scratch_bytes": [],
     "exkv_plan_splits": [_i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32)],
     "exkv_plan_splits_hd": [_i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32)],
+    "exkv_prompt_attention": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
+                              _i32, _i32, _i32, _f32, _p],
     "exkv_abi_version": [],
     "exkv_last_error": [],
     "exkv_error_bits": [_p, _i32, _p],
     "exkv_set_wait_limit": [_i32],
 }
+
+# token rows with their tables, norms and output: the first arguments of every rotated append
+_ROPE_ROWS = [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _p, _p, _f32, _p, _i32, _i32, _i32]
+_CACHE = [_p, _p, _p, _p, _p, _p, _p, _p]          # six arrays, cnt, before
+SIGNATURES.update({
+    "exkv_rotate_prompt": [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _p, _p, _f32, _p, _p, _p, _p, _i32, _i32, _i32,
+                           _i32, _i32, _p],
+    "exkv_rope_append": _ROPE_ROWS + [*_CACHE, _p, _i64, _i64, *_CACHE, _p, _i64, _i64, _i32, _i32, _p],
+    "exkv_rope_append_bf16": _ROPE_ROWS + [_p, _p, _p, _p, _i32, _i32, _p],
+    "exkv_rope_append_paged": _ROPE_ROWS + [*_CACHE, _p, _i64, _i64, *_CACHE, _i64, _i64, _p, _p, _p, _i64, _i32, _i32,
+                                            _i32, _i32, _p],
+    "exkv_rope_append_paged_bf16": _ROPE_ROWS + [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
+    "exkv_add_norm": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _f32, _f32, _p, _p, _i32, _i32, _p],
+})
 
 _lib = None
 
@@ -125,6 +141,8 @@ ERROR_BITS = {
     0x4: "encoder: the slot scan's look-back gave up on a predecessor",
     0x8: "encoder: inconsistent scan workspace",
     0x10: "wire pack: a raw row's pool slot lay outside the pool (clamped)",
+    0x20: "packed prompts: sequence offsets that do not ascend from 0 within the rows (clamped)",
+    0x40: "rotation: a position outside the cosine and sine tables (clamped)",
 }
 
 

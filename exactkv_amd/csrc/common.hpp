@@ -123,6 +123,8 @@ int wait_for_tag(const char* what, const int32_t* host, int32_t tag, hipStream_t
 hipError_t fetch_errors_attention(uint32_t* out, int first, int clear, hipStream_t stream);
 hipError_t fetch_errors_encode(uint32_t* out, int first, int clear, hipStream_t stream);
 hipError_t fetch_errors_wire(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_prompt(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_rope(uint32_t* out, int first, int clear, hipStream_t stream);
 }  // namespace exkv
 
 #define EXKV_OK 0

@@ -23,6 +23,7 @@
 // head dim (64, 128 or 256); the entry points pick the instance.
 #include <type_traits>
 
+#include "rope.hpp"
 #include "tile.hpp"
 #include "../../include/exactkv.h"
 
@@ -919,9 +920,21 @@ __device__ inline void copy_row_thread(uint16_t* dst, const uint16_t* src) {
     }
 }
 
+// The same of a row that other workgroups of this launch may have stored (device-coherently).
+template <int D>
+__device__ inline void copy_fresh_row_thread(uint16_t* dst, const uint16_t* src) {
+    for (int c0 = 0; c0 < D / 2; c0 += 16) {
+        uint32_t v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = (uint32_t)ld_dev_i32(reinterpret_cast<const int32_t*>(src) + c0 + c);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) reinterpret_cast<uint32_t*>(dst)[c0 + c] = v[c];
+    }
+}
+
 // Raw-row slots and rows of n units whose pages have just been encoded (all kAppendThreads
 // threads of one block call it), in unit order from slot cnt0 on: `units` gives the index of a
-// unit's page and the source of its row r. Thread t takes
+// unit's page and copies its row r. Thread t takes
 // units [t * per, (t + 1) * per): their rowmasks (device-coherent loads, eight in flight),
 // the block's exclusive scan of their raw-row counts (the codec's slot order),
 // rowoff. Then the raw rows (rows 0-14 from the unit's tail area, written by earlier
@@ -972,7 +985,7 @@ __device__ inline int place_raw_rows(const Units& units, int n, int cnt0, const 
                 for (int r = 0; r < kPage; ++r)
                     if ((m[k] >> r) & 1u) {
                         const int64_t slot = (int64_t)cnt0 + run + j++;
-                        if (slot < pool.cap) copy_row_thread<D>(pool.raw + slot * D, units.src_row(u, r));
+                        if (slot < pool.cap) units.copy(pool.raw + slot * D, u, r);
                     }
             }
             run += popc32(m[k]);
@@ -991,7 +1004,7 @@ __device__ inline int place_raw_rows(const Units& units, int n, int cnt0, const 
             int k = g - s_rank[lo], r = 0;             // g is the k-th raw row of unit lo's page
             for (; r < kPage - 1; ++r)
                 if (((mk >> r) & 1u) && k-- == 0) break;
-            copy_row_thread<D>(pool.raw + ((int64_t)cnt0 + g) * D, units.src_row(lo, r));
+            units.copy(pool.raw + ((int64_t)cnt0 + g) * D, lo, r);
         }
     }
     return total;
@@ -1033,7 +1046,9 @@ struct AppendUnits {
     }
     __device__ const uint16_t* x(int u) const { return a.x + (u / a.H) * a.sx_b + (u % a.H) * a.sx_h; }
     __device__ uint16_t* tail(int u) const { return a.raw + (a.cap + (int64_t)u * kPage) * D; }
-    __device__ const uint16_t* src_row(int u, int r) const { return r == kPage - 1 ? x(u) : tail(u) + r * D; }
+    __device__ void copy(uint16_t* dst, int u, int r) const {
+        copy_row_thread<D>(dst, r == kPage - 1 ? x(u) : tail(u) + r * D);
+    }
 };
 
 template <int D, bool ONE>
@@ -1197,8 +1212,8 @@ struct FilledUnits {
     const int* pidx;
     __device__ int64_t page(int u) const { return (int64_t)pidx[u / all.a.H] * all.a.H + u % all.a.H; }
     __device__ int unit(int u) const { return row[u / all.a.H] * all.a.H + u % all.a.H; }
-    __device__ const uint16_t* src_row(int u, int r) const {
-        return r == kPage - 1 ? all.x(unit(u)) : all.tail(unit(u)) + r * D;
+    __device__ void copy(uint16_t* dst, int u, int r) const {
+        copy_row_thread<D>(dst, r == kPage - 1 ? all.x(unit(u)) : all.tail(unit(u)) + r * D);
     }
 };
 
@@ -1316,6 +1331,254 @@ __global__ void __launch_bounds__(256) paged_bf16_append_kernel(PagedAppendArgs 
     if (T < 0) return;
     const int64_t row = paged_pidx(a, s, T / kPage) * kPage + T % kPage;
     copy_row<D>(buf + (row * a.H + h) * D, a.x + i * a.sx_b + h * a.sx_h, lane);
+}
+
+// ---------------------------------------------------------------- rotated append
+
+// One token of every sequence with the rotation on the way (rope.hpp), keys and values in one
+// launch: the token's query rows are rotated to q_out, its key rows into the key cache and its
+// value rows copied into the value cache, for the four kinds of cache. Bytes and counters are
+// those of the two appends above given the rotated keys.
+//
+// D / 16 lanes hold a row and a thread takes at most a few rows, so an ordinary step is one round
+// trip (length, table row and token rows) and its stores: bound by those and the launch.
+//
+// Compressed caches at a page end: a block stores its rows, key and value rows of tokens that
+// fill a page device-coherently, waits for them, and its wavefronts encode those units' pages (all
+// 16 rows now lie in the open page; the block's own stores are seen through its CU's cache). The
+// last block of the grid to arrive places both caches' raw rows, row 15 by device-coherent loads.
+// Contiguous caches count every step in, since the last block advances their token counts.
+enum CacheKind { kContiguous, kContiguousBf16, kPaged, kPagedBf16 };
+
+struct RopeCaches {
+    AppendArgs k, v;          // kContiguous (x unused; arrivals: k.state + 1)
+    PagedAppendArgs pk, pv;   // kPaged, and kPagedBf16 for the table (x unused)
+    uint16_t *kbuf, *vbuf;    // the bf16 kinds
+    int32_t *kstate, *vstate; // kContiguousBf16 (arrivals: kstate + 1)
+    int32_t* arrivals;        // kPaged
+    int TS;                   // kContiguousBf16
+};
+
+// Units whose pages fill, of contiguous caches (all of them) and of paged ones (listed rows).
+template <int D>
+struct RopeUnits {
+    const AppendArgs& a;
+    int T;
+    __device__ int64_t page(int u) const { return AppendUnits<D>{a, T}.page(u); }
+    __device__ void copy(uint16_t* dst, int u, int r) const {
+        const uint16_t* src = AppendUnits<D>{a, T}.tail(u) + r * D;
+        if (r == kPage - 1) copy_fresh_row_thread<D>(dst, src); else copy_row_thread<D>(dst, src);
+    }
+};
+template <int D>
+struct RopeFilledUnits {
+    const PagedUnits<D>& all;
+    const int* row;
+    const int* pidx;
+    __device__ int64_t page(int u) const { return (int64_t)pidx[u / all.a.H] * all.a.H + u % all.a.H; }
+    __device__ void copy(uint16_t* dst, int u, int r) const {
+        const uint16_t* src = all.tail(row[u / all.a.H] * all.a.H + u % all.a.H) + r * D;
+        if (r == kPage - 1) copy_fresh_row_thread<D>(dst, src); else copy_row_thread<D>(dst, src);
+    }
+};
+
+// A row's 16 values of a lane, device-coherently.
+template <int D>
+__device__ inline void store_row16_dev(uint16_t* row, int g, const uint32_t (&u)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        st_dev_i32(reinterpret_cast<int32_t*>(row + 8 * g) + i, (int32_t)u[i]);
+        st_dev_i32(reinterpret_cast<int32_t*>(row + D / 2 + 8 * g) + i, (int32_t)u[4 + i]);
+    }
+}
+
+constexpr int kRopeBf16Threads = 256;
+constexpr int rope_threads(int kind) { return kind == kPagedBf16 ? kRopeBf16Threads : kAppendThreads; }
+
+// Encodes the page that unit u (token i, head h) of one cache fills, at row0 of its arrays.
+template <int D, class Args>
+__device__ inline void encode_unit(const Args& a, const uint16_t* tail, int64_t page, int64_t row0, int lane, int64_t next,
+                                   int64_t next_off) {
+    const uint32_t rm = encode_page<D>(tail, D, nullptr, lane, a.sm + row0 * D, a.code + row0 * (D / 2), a.H,
+                                       a.base + page * D, nullptr);
+    if (lane == 0) {
+        st_dev_i32(a.rowmask + page, (int32_t)rm);
+        if (next >= 0) {
+            a.rowmask[next] = 0xFFFF;
+            a.rowoff[next] = (int32_t)next_off;
+        }
+    }
+}
+
+template <int D, int KIND, bool V16>
+__global__ void __launch_bounds__(rope_threads(KIND)) rope_append_kernel(RopeRows r, RopeCaches c) {
+    constexpr int THREADS = rope_threads(KIND), GL = D / 16, RB = THREADS / GL;   // rows of a block's pass
+    constexpr bool PAGED = KIND == kPaged || KIND == kPagedBf16, COMP = KIND == kContiguous || KIND == kPaged;
+    const int g = threadIdx.x % GL, heads = r.Hq + 2 * r.Hkv, rows = r.n * heads;
+    int T = 0;
+    bool full = false;
+    if constexpr (KIND == kContiguous) T = c.k.state[0];
+    if constexpr (KIND == kContiguousBf16) T = c.kstate[0];
+    if constexpr (KIND == kContiguous) full = T < 0 || T >= c.k.TS;
+    if constexpr (KIND == kContiguousBf16) full = T < 0 || T >= c.TS;
+    bool fills = COMP && !PAGED && !full && T % kPage == kPage - 1;
+    for (int row = (int)blockIdx.x * RB + (int)threadIdx.x / GL; row < rows; row += (int)gridDim.x * RB) {
+        const int i = row / heads, j = row % heads;
+        int slot = i, tok = T;
+        if constexpr (PAGED) {
+            slot = paged_slot(c.pk, i);
+            tok = paged_new_token(c.pk, slot);
+        }
+        const bool isq = j < r.Hq, isv = j >= r.Hq + r.Hkv;
+        const int h = isq ? j : isv ? j - r.Hq - r.Hkv : j - r.Hq;
+        uint32_t u[8];
+        load_row16<D, V16>(isq ? r.q + i * r.sq_n + h * r.sq_h
+                               : isv ? r.v + i * r.sv_n + h * r.sv_h : r.k + i * r.sk_n + h * r.sk_h, g, u);
+        if (!isv) {
+            float cs[8], sn[8];
+            const int64_t at = (int64_t)table_row(r.t, tok) * (D / 2) + 8 * g;
+            load_angles(r.t.cos + at, cs);
+            load_angles(r.t.sin + at, sn);
+            turn_row<D>(u, isq ? r.q_norm : r.k_norm, r.eps, cs, sn, g);
+        }
+        if (isq) {
+            store_row16<D>(r.q_out + ((int64_t)i * r.Hq + h) * D, g, u);
+            continue;
+        }
+        if (PAGED ? tok < 0 : full) continue;          // no room: nothing is written
+        if constexpr (COMP) {
+            const int64_t cap = PAGED ? (isv ? c.pv.cap : c.pk.cap) : (isv ? c.v.cap : c.k.cap);
+            uint16_t* raw = PAGED ? (isv ? c.pv.raw : c.pk.raw) : (isv ? c.v.raw : c.k.raw);
+            uint16_t* dst = raw + (cap + ((int64_t)slot * r.Hkv + h) * kPage + tok % kPage) * D;
+            if (tok % kPage == kPage - 1)
+                store_row16_dev<D>(dst, g, u);
+            else
+                store_row16<D>(dst, g, u);
+        } else {
+            int64_t at;
+            if constexpr (PAGED)
+                at = paged_pidx(c.pk, slot, tok / kPage) * kPage + tok % kPage;
+            else
+                at = (int64_t)i * c.TS + T;
+            store_row16<D>((isv ? c.vbuf : c.kbuf) + (at * r.Hkv + h) * D, g, u);
+        }
+    }
+    if constexpr (KIND == kPagedBf16) return;
+    if constexpr (KIND == kContiguousBf16) {
+        if (full) return;                              // uniform over the grid
+        if (gridDim.x == 1)
+            __syncthreads();                           // every wave has read the count
+        else if (!last_block(c.kstate + 1, false))
+            return;
+        if (threadIdx.x == 0) {
+            if (gridDim.x > 1) st_dev_i32(c.kstate + 1, 0);
+            c.kstate[0] = T + 1;
+            c.vstate[0] = T + 1;
+        }
+    }
+    if constexpr (COMP) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        __shared__ int s_row[kFillRows], s_pidx[kFillRows];
+        int nf = 0;
+        if constexpr (PAGED) {
+            int any = 0;
+            for (int c0 = 0; c0 < r.n; c0 += kFillRows) {
+                if (c0 > 0) __syncthreads();           // the lists are read
+                nf = list_fills(c0, fill_page(c.pk, c0 + (int)threadIdx.x), s_row, s_pidx);
+                any += nf;
+            }
+            if (any == 0) return;                      // uniform over the grid
+            fills = true;
+        } else if (full) {
+            return;
+        }
+        if (fills) {                                   // uniform
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            for (int first = (int)blockIdx.x * RB; first < rows; first += (int)gridDim.x * RB)
+                for (int row = first + wave; row < min(first + RB, rows); row += kAppendWaves) {
+                    const int i = row / heads, j = row % heads;
+                    if (j < r.Hq) continue;
+                    const bool isv = j >= r.Hq + r.Hkv;
+                    const int h = isv ? j - r.Hq - r.Hkv : j - r.Hq;
+                    if constexpr (PAGED) {
+                        const PagedAppendArgs& a = isv ? c.pv : c.pk;
+                        const int slot = paged_slot(a, i), tok = paged_new_token(a, slot);
+                        if (tok < 0 || tok % kPage != kPage - 1) continue;
+                        const int64_t pidx = paged_pidx(a, slot, tok / kPage);
+                        const int64_t tail_row = a.cap + ((int64_t)slot * a.H + h) * kPage;
+                        const int64_t next = tok / kPage + 1 < a.max_pages ? paged_pidx(a, slot, tok / kPage + 1) * a.H + h : -1;
+                        encode_unit<D>(a, a.raw + tail_row * D, pidx * a.H + h, pidx * kPage * a.H + h, lane, next, tail_row);
+                    } else {
+                        const AppendArgs& a = isv ? c.v : c.k;
+                        const int u = i * a.H + h, pg = T / kPage, NP = a.TS / kPage;
+                        const int64_t page = ((int64_t)i * NP + pg) * a.H + h, tail_row = a.cap + (int64_t)u * kPage;
+                        encode_unit<D>(a, a.raw + tail_row * D, page, ((int64_t)i * a.TS + (int64_t)pg * kPage) * a.H + h, lane,
+                                       pg + 1 < NP ? page + a.H : -1, tail_row);
+                    }
+                }
+        }
+        int32_t* arrivals;
+        if constexpr (PAGED) arrivals = c.arrivals; else arrivals = c.k.state + 1;
+        if (gridDim.x == 1) {
+            if (fills) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        } else if (!last_block(arrivals, fills)) {
+            return;
+        }
+        if (fills)
+            for (int which = 0; which < 2; ++which) {
+                __syncthreads();                       // the lists and the tables of the other cache are read
+                if constexpr (PAGED) {
+                    const PagedAppendArgs& a = which ? c.pv : c.pk;
+                    const PagedUnits<D> units{a};
+                    const int cnt0 = *a.cnt;
+                    int cnt = cnt0;
+                    for (int c0 = 0; c0 < r.n; c0 += kFillRows) {
+                        if (r.n > kFillRows) {
+                            __syncthreads();
+                            nf = list_fills(c0, fill_page(a, c0 + (int)threadIdx.x), s_row, s_pidx);
+                        }
+                        if (nf == 0) continue;         // uniform
+                        cnt += place_raw_rows<D, kAppendLdsUnits>(RopeFilledUnits<D>{units, s_row, s_pidx}, nf * a.H, cnt,
+                                                                  RawPool{a.rowmask, a.rowoff, a.raw, a.cap});
+                    }
+                    __syncthreads();                   // every thread has read the counter
+                    if (threadIdx.x == 0) {
+                        *a.before = cnt0;
+                        *a.cnt = cnt;
+                    }
+                } else {
+                    const AppendArgs& a = which ? c.v : c.k;
+                    const int cnt0 = *a.cnt;
+                    const int placed = place_raw_rows<D, kAppendLdsUnits>(RopeUnits<D>{a, T}, a.B * a.H, cnt0,
+                                                                          RawPool{a.rowmask, a.rowoff, a.raw, a.cap});
+                    __syncthreads();
+                    if (threadIdx.x == 0) {
+                        *a.before = cnt0;
+                        *a.cnt = cnt0 + placed;
+                    }
+                }
+            }
+        if (threadIdx.x == 0) {
+            if (gridDim.x > 1) st_dev_i32(arrivals, 0);
+            if constexpr (!PAGED) {
+                c.k.state[0] = T + 1;
+                c.v.state[0] = T + 1;
+            }
+        }
+    }
+}
+
+template <int D, int KIND>
+static void launch_rope_append(const RopeRows& r, const RopeCaches& c, bool v16, hipStream_t stream) {
+    constexpr int per = rope_threads(KIND) / (D / 16);
+    int64_t blocks = ((int64_t)r.n * (r.Hq + 2 * r.Hkv) + per - 1) / per;
+    if (KIND != kPagedBf16 && blocks > kAppendBlocks) blocks = kAppendBlocks;
+    if (v16)
+        hipLaunchKernelGGL((rope_append_kernel<D, KIND, true>), dim3((unsigned)blocks), dim3(rope_threads(KIND)), 0, stream, r, c);
+    else
+        hipLaunchKernelGGL((rope_append_kernel<D, KIND, false>), dim3((unsigned)blocks), dim3(rope_threads(KIND)), 0, stream, r, c);
 }
 
 // ---------------------------------------------------------------- decode to bf16
@@ -1709,6 +1972,135 @@ extern "C" int exkv_bf16_append_paged(const void* x, int64_t sx_b, int64_t sx_h,
     hipLaunchKernelGGL(EXKV_FOR_D(paged_bf16_append_kernel, D), dim3((unsigned)((n * H + 3) / 4)), dim3(256), 0,
                        stream, a, (uint16_t*)buf);
     return launch_status("bf16_append_paged");
+}
+
+// ---------------------------------------------------------------- rotated append
+
+static bool rows_even(const void* p, int64_t s_n, int64_t s_h, int bytes) {
+    return ((uintptr_t)p | (uintptr_t)(2 * s_n) | (uintptr_t)(2 * s_h)) % bytes == 0;
+}
+
+static int check_rope(const char* what, const RopeRows& r, int32_t D) {
+    EXKV_REQUIRE(head_dim_ok(D), "%s: head dim must be 64, 128 or 256 (got %d)", what, D);
+    EXKV_REQUIRE(r.n >= 0 && r.Hq > 0 && r.Hkv > 0 && r.t.rows > 0, "%s: bad shape n=%d Hq=%d Hkv=%d table rows=%d", what,
+                 r.n, r.Hq, r.Hkv, r.t.rows);
+    EXKV_REQUIRE((int64_t)r.n * (r.Hq + 2 * r.Hkv) * (D / 16) <= INT32_MAX / 2, "%s: too many rows (n=%d)", what, r.n);
+    EXKV_REQUIRE(r.n == 0 || (r.q && r.k && r.v && r.t.cos && r.t.sin && r.q_out), "%s: null pointer", what);
+    EXKV_REQUIRE(rows_even(r.q, r.sq_n, r.sq_h, 4) && rows_even(r.k, r.sk_n, r.sk_h, 4) && rows_even(r.v, r.sv_n, r.sv_h, 4),
+                 "%s: token rows must start at even elements (4-byte aligned)", what);
+    EXKV_REQUIRE(((uintptr_t)r.q_out | (uintptr_t)r.t.cos | (uintptr_t)r.t.sin | (uintptr_t)r.q_norm | (uintptr_t)r.k_norm) %
+                         16 == 0,
+                 "%s: tables, norms and the output must be 16-byte aligned", what);
+    return EXKV_OK;
+}
+
+template <int KIND>
+static int run_rope_append(const char* what, const RopeRows& r, const RopeCaches& c, int32_t D, hipStream_t stream) {
+    if (r.n == 0) return EXKV_OK;
+    const bool v16 = rows_even(r.q, r.sq_n, r.sq_h, 16) && rows_even(r.k, r.sk_n, r.sk_h, 16) && rows_even(r.v, r.sv_n, r.sv_h, 16);
+    if (D == 64)
+        launch_rope_append<64, KIND>(r, c, v16, stream);
+    else if (D == 128)
+        launch_rope_append<128, KIND>(r, c, v16, stream);
+    else
+        launch_rope_append<256, KIND>(r, c, v16, stream);
+    return launch_status(what);
+}
+
+#define EXKV_ROPE_PARAMS                                                                                                   \
+    const void *q, int64_t sq_n, int64_t sq_h, const void *k, int64_t sk_n, int64_t sk_h, const void *v, int64_t sv_n,     \
+        int64_t sv_h, const float *cos, const float *sin, int32_t table_rows, const void *q_norm, const void *k_norm,      \
+        float eps, void *q_out, int32_t n, int32_t Hq, int32_t Hkv
+#define EXKV_ROPE_ROWS                                                                                                     \
+    RopeRows {                                                                                                             \
+        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, sq_n, sq_h, sk_n, sk_h, sv_n, sv_h,                    \
+            {cos, sin, table_rows}, (const uint16_t*)q_norm, (const uint16_t*)k_norm, eps, (uint16_t*)q_out, n, Hq, Hkv    \
+    }
+
+extern "C" int exkv_rope_append(EXKV_ROPE_PARAMS, void* k_sm, void* k_code, void* k_base, int32_t* k_rowmask,
+                                int32_t* k_rowoff, void* k_raw, int32_t* k_cnt, int32_t* k_before, int32_t* k_state,
+                                int64_t k_cap, int64_t k_raw_rows, void* v_sm, void* v_code, void* v_base,
+                                int32_t* v_rowmask, int32_t* v_rowoff, void* v_raw, int32_t* v_cnt, int32_t* v_before,
+                                int32_t* v_state, int64_t v_cap, int64_t v_raw_rows, int32_t TS, int32_t D,
+                                hipStream_t stream) {
+    const RopeRows r = EXKV_ROPE_ROWS;
+    const int rc = check_rope("rope_append", r, D);
+    if (rc != EXKV_OK) return rc;
+    EXKV_REQUIRE(TS > 0 && TS % kPage == 0, "rope_append: bad shape TS=%d", TS);
+    const int64_t tails = (int64_t)n * Hkv * kPage;
+    EXKV_REQUIRE(k_cap >= 0 && k_cap + tails <= k_raw_rows && v_cap >= 0 && v_cap + tails <= v_raw_rows,
+                 "rope_append: raw pool (%lld and %lld rows) smaller than cap + tail area", (long long)k_raw_rows,
+                 (long long)v_raw_rows);
+    EXKV_REQUIRE(k_sm && k_code && k_base && k_rowmask && k_rowoff && k_raw && k_cnt && k_before && k_state && v_sm && v_code &&
+                     v_base && v_rowmask && v_rowoff && v_raw && v_cnt && v_before && v_state && k_raw != v_raw,
+                 "rope_append: null pointer, or one cache for both");
+    RopeCaches c{};
+    c.k = AppendArgs{nullptr, 0, 0, (uint8_t*)k_sm, (uint8_t*)k_code, (uint8_t*)k_base, k_rowmask, k_rowoff, (uint16_t*)k_raw,
+                     k_cnt, k_before, k_state, k_cap, n, Hkv, TS};
+    c.v = AppendArgs{nullptr, 0, 0, (uint8_t*)v_sm, (uint8_t*)v_code, (uint8_t*)v_base, v_rowmask, v_rowoff, (uint16_t*)v_raw,
+                     v_cnt, v_before, v_state, v_cap, n, Hkv, TS};
+    return run_rope_append<kContiguous>("rope_append", r, c, D, stream);
+}
+
+extern "C" int exkv_rope_append_bf16(EXKV_ROPE_PARAMS, void* kbuf, int32_t* k_state, void* vbuf, int32_t* v_state, int32_t TS,
+                                     int32_t D, hipStream_t stream) {
+    const RopeRows r = EXKV_ROPE_ROWS;
+    const int rc = check_rope("rope_append_bf16", r, D);
+    if (rc != EXKV_OK) return rc;
+    EXKV_REQUIRE(TS > 0, "rope_append_bf16: bad shape TS=%d", TS);
+    EXKV_REQUIRE(kbuf && vbuf && k_state && v_state && kbuf != vbuf, "rope_append_bf16: null pointer, or one cache for both");
+    RopeCaches c{};
+    c.kbuf = (uint16_t*)kbuf;
+    c.vbuf = (uint16_t*)vbuf;
+    c.kstate = k_state;
+    c.vstate = v_state;
+    c.TS = TS;
+    return run_rope_append<kContiguousBf16>("rope_append_bf16", r, c, D, stream);
+}
+
+extern "C" int exkv_rope_append_paged(EXKV_ROPE_PARAMS, void* k_sm, void* k_code, void* k_base, int32_t* k_rowmask,
+                                      int32_t* k_rowoff, void* k_raw, int32_t* k_cnt, int32_t* k_before, int32_t* arrivals,
+                                      int64_t k_cap, int64_t k_raw_rows, void* v_sm, void* v_code, void* v_base,
+                                      int32_t* v_rowmask, int32_t* v_rowoff, void* v_raw, int32_t* v_cnt, int32_t* v_before,
+                                      int64_t v_cap, int64_t v_raw_rows, const int32_t* slots, const int32_t* lens,
+                                      const int32_t* block_table, int64_t bt_stride, int32_t max_seqs, int32_t max_pages,
+                                      int32_t pool_pages, int32_t D, hipStream_t stream) {
+    const RopeRows r = EXKV_ROPE_ROWS;
+    int rc = check_rope("rope_append_paged", r, D);
+    if (rc == EXKV_OK) rc = check_paged_append("rope_append_paged", n, Hkv, D, max_seqs, max_pages, bt_stride, pool_pages);
+    if (rc != EXKV_OK) return rc;
+    const int64_t tails = (int64_t)max_seqs * Hkv * kPage;
+    EXKV_REQUIRE(k_cap >= 0 && k_cap + tails <= k_raw_rows && v_cap >= 0 && v_cap + tails <= v_raw_rows,
+                 "rope_append_paged: raw pool (%lld and %lld rows) smaller than cap + tail area", (long long)k_raw_rows,
+                 (long long)v_raw_rows);
+    EXKV_REQUIRE(k_sm && k_code && k_base && k_rowmask && k_rowoff && k_raw && k_cnt && k_before && arrivals && v_sm && v_code &&
+                     v_base && v_rowmask && v_rowoff && v_raw && v_cnt && v_before && lens && block_table && k_raw != v_raw,
+                 "rope_append_paged: null pointer, or one cache for both");
+    RopeCaches c{};
+    c.pk = PagedAppendArgs{nullptr, 0, 0, (uint8_t*)k_sm, (uint8_t*)k_code, (uint8_t*)k_base, k_rowmask, k_rowoff,
+                           (uint16_t*)k_raw, k_cnt, k_before, slots, lens, block_table, bt_stride, k_cap, n, Hkv, max_seqs,
+                           max_pages, pool_pages};
+    c.pv = PagedAppendArgs{nullptr, 0, 0, (uint8_t*)v_sm, (uint8_t*)v_code, (uint8_t*)v_base, v_rowmask, v_rowoff,
+                           (uint16_t*)v_raw, v_cnt, v_before, slots, lens, block_table, bt_stride, v_cap, n, Hkv, max_seqs,
+                           max_pages, pool_pages};
+    c.arrivals = arrivals;
+    return run_rope_append<kPaged>("rope_append_paged", r, c, D, stream);
+}
+
+extern "C" int exkv_rope_append_paged_bf16(EXKV_ROPE_PARAMS, void* kbuf, void* vbuf, const int32_t* slots, const int32_t* lens,
+                                           const int32_t* block_table, int64_t bt_stride, int32_t max_seqs,
+                                           int32_t max_pages, int32_t pool_pages, int32_t D, hipStream_t stream) {
+    const RopeRows r = EXKV_ROPE_ROWS;
+    int rc = check_rope("rope_append_paged_bf16", r, D);
+    if (rc == EXKV_OK) rc = check_paged_append("rope_append_paged_bf16", n, Hkv, D, max_seqs, max_pages, bt_stride, pool_pages);
+    if (rc != EXKV_OK) return rc;
+    EXKV_REQUIRE(kbuf && vbuf && lens && block_table && kbuf != vbuf, "rope_append_paged_bf16: null pointer, or one pool for both");
+    RopeCaches c{};
+    c.kbuf = (uint16_t*)kbuf;
+    c.vbuf = (uint16_t*)vbuf;
+    c.pk = PagedAppendArgs{nullptr, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, slots, lens,
+                           block_table, bt_stride, 0, n, Hkv, max_seqs, max_pages, pool_pages};
+    return run_rope_append<kPagedBf16>("rope_append_paged_bf16", r, c, D, stream);
 }
 
 extern "C" int exkv_decode_to_bf16_paged(const void* sm, const void* code, const void* base,

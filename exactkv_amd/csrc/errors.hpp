@@ -23,6 +23,8 @@ enum : uint32_t {
     kErrLookback = 1u << 2,  // encoder: the slot scan's look-back gave up on a predecessor
     kErrScanWs = 1u << 3,    // encoder: the scan workspace was inconsistent (more tickets than blocks)
     kErrWire = 1u << 4,      // wire unpack / pack: a raw row's pool slot fell outside the pool
+    kErrOffsets = 1u << 5,   // packed prompts: sequence offsets that do not ascend from 0 within the rows
+    kErrPosition = 1u << 6,  // rotation: a position outside the cosine / sine tables
 };
 
 static __device__ uint32_t file_error_word;

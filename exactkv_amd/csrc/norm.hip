@@ -1,0 +1,181 @@
+// The residual stream between two blocks of a decoder layer, for gfx950: a block's output x
+// (normed, gated, scaled, each where asked for) added to the stream r, and the norm that feeds the
+// next block:
+//     u = x                         or  x rsqrt(mean(x^2) + eps) post_w
+//     u = u gate                    (where a gate is given)
+//     h = r + scale u               (without r: scale u)
+//     y = h rsqrt(mean(h^2) + eps) w.
+// bf16 rows in and out, fp32 between; h and y are rounded once each (y from the unrounded h).
+// No kernel of the reference (its model's own modules do this, engine.py:75-91).
+//
+// Bound by HBM: x, r and a row-wise gate are read once, h and y written once. One workgroup of
+// 64 WAVES threads holds a row in registers, eight channels a thread and piece, CH pieces; the
+// two sums go through the wavefront's lanes and, with several wavefronts, through LDS.
+#include "rope.hpp"
+#include "../../include/exactkv.h"
+
+namespace exkv {
+
+struct NormArgs {
+    const uint16_t *x, *r, *w, *post_w, *gate;     // r, post_w, gate may be nullptr
+    int64_t sx, sr, sg;                            // row strides in elements (sg 0: one gate row for all)
+    uint16_t *h, *y;                               // [N, C]; h may be nullptr
+    float eps, scale;
+    int N, C;
+};
+
+__device__ inline float wave_total(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+template <int WAVES>
+__device__ inline float block_total(float x, float* s) {
+    x = wave_total(x);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) x += s[i];
+    }
+    return x;
+}
+
+// Eight channels of a row from channel c0 on (V16: one 16-byte piece, all of it in the row; else
+// one by one, those past C as zeros).
+template <bool V16>
+__device__ inline void load8(const uint16_t* row, int c0, int C, float (&v)[8]) {
+    if constexpr (V16) {
+        uint32_t u[4];
+        ld_words<4>(row + c0, u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = lo_float(u[i]);
+            v[2 * i + 1] = hi_float(u[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < C ? lo_float(row[c0 + i]) : 0.f;
+    }
+}
+template <bool V16>
+__device__ inline void store8(uint16_t* row, int c0, int C, const float (&v)[8]) {
+    if constexpr (V16) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+        st_words<4>(row + c0, u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < C) row[c0 + i] = (uint16_t)bf16_pair(v[i], 0.f);
+    }
+}
+
+template <int WAVES, int CH, bool V16>
+__global__ void __launch_bounds__(64 * WAVES) norm_kernel(NormArgs a) {
+    __shared__ float s_sum[2][WAVES];
+    const int64_t row = blockIdx.x;
+    const uint16_t *x = a.x + row * a.sx, *r = a.r + row * a.sr, *gate = a.gate + row * a.sg;
+    const float inv_c = 1.f / (float)a.C;
+    float v[CH][8];
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int c0 = (i * 64 * WAVES + (int)threadIdx.x) * 8;
+        if (c0 < a.C)
+            load8<V16>(x, c0, a.C, v[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+    float k = a.scale;
+    if (a.post_w != nullptr) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+        k *= rsqrtf(fmaf(block_total<WAVES>(sq, s_sum[0]), inv_c, a.eps));
+        sq = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int c0 = (i * 64 * WAVES + (int)threadIdx.x) * 8;
+        if (c0 < a.C) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= k;
+            if (a.post_w != nullptr) {
+                load8<V16>(a.post_w, c0, a.C, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+            }
+            if (a.gate != nullptr) {
+                load8<V16>(gate, c0, a.C, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+            }
+            if (a.r != nullptr) {
+                load8<V16>(r, c0, a.C, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+            }
+            if (a.h != nullptr) store8<V16>(a.h + row * a.C, c0, a.C, v[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+        }
+    }
+    const float rs = rsqrtf(fmaf(block_total<WAVES>(sq, s_sum[1]), inv_c, a.eps));
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int c0 = (i * 64 * WAVES + (int)threadIdx.x) * 8;
+        if (c0 < a.C) {
+            float f[8];
+            load8<V16>(a.w, c0, a.C, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= rs * f[j];
+            store8<V16>(a.y + row * a.C, c0, a.C, v[i]);
+        }
+    }
+}
+
+template <int WAVES, int CH>
+static void launch_norm(const NormArgs& a, bool v16, hipStream_t stream) {
+    if (v16)
+        hipLaunchKernelGGL((norm_kernel<WAVES, CH, true>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
+    else
+        hipLaunchKernelGGL((norm_kernel<WAVES, CH, false>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
+}
+
+}  // namespace exkv
+
+using namespace exkv;
+
+extern "C" int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t sr, const void* w, const void* post_w,
+                             const void* gate, int64_t sg, float scale, float eps, void* h, void* y, int32_t N, int32_t C,
+                             hipStream_t stream) {
+    EXKV_REQUIRE(N >= 0 && C > 0 && C <= 16384, "add_norm: 1 to 16384 channels (got %d, N=%d)", C, N);
+    if (N == 0) return EXKV_OK;
+    EXKV_REQUIRE(x && w && y, "add_norm: null pointer");
+    EXKV_REQUIRE(sx >= 0 && sr >= 0 && sg >= 0, "add_norm: negative row stride");
+    EXKV_REQUIRE(((uintptr_t)x | (uintptr_t)r | (uintptr_t)w | (uintptr_t)post_w | (uintptr_t)gate | (uintptr_t)h |
+                  (uintptr_t)y) % 2 == 0, "add_norm: unaligned bf16 pointer");
+    const NormArgs a{(const uint16_t*)x, (const uint16_t*)r, (const uint16_t*)w, (const uint16_t*)post_w,
+                     (const uint16_t*)gate, sx, r ? sr : 0, gate ? sg : 0, (uint16_t*)h, (uint16_t*)y, eps, scale, N, C};
+    const bool v16 = (((uintptr_t)x | (uintptr_t)r | (uintptr_t)w | (uintptr_t)post_w | (uintptr_t)gate | (uintptr_t)h |
+                       (uintptr_t)y) % 16 == 0) && C % 8 == 0 && sx % 8 == 0 && a.sr % 8 == 0 && a.sg % 8 == 0;
+    if (C <= 512)
+        launch_norm<1, 1>(a, v16, stream);
+    else if (C <= 1024)
+        launch_norm<1, 2>(a, v16, stream);
+    else if (C <= 2048)
+        launch_norm<4, 1>(a, v16, stream);
+    else if (C <= 4096)
+        launch_norm<4, 2>(a, v16, stream);
+    else if (C <= 8192)
+        launch_norm<4, 4>(a, v16, stream);
+    else
+        launch_norm<8, 4>(a, v16, stream);
+    return hip_status(hipGetLastError(), "add_norm");
+}

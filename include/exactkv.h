@@ -39,7 +39,8 @@ extern "C" {
 typedef struct ihipStream_t* hipStream_t;
 
 /* ABI version of the library (2: the encoders take a scan workspace; 3: head dims 64 and
- * 256 and exkv_plan_splits_hd; 4: exkv_error_bits and exkv_set_wait_limit). */
+ * 256 and exkv_plan_splits_hd; 4: exkv_error_bits and exkv_set_wait_limit; 5: the operators of a
+ * decoder layer around the caches, exkv_prompt_attention and below). */
 int exkv_abi_version(void);
 
 /* Sticky error bits of the kernels. A kernel that gives up a bounded wait (a correct call
@@ -54,9 +55,11 @@ int exkv_abi_version(void);
 #define EXKV_ERR_LOOKBACK 0x4u  /* encoder: the slot scan's look-back gave up on a predecessor */
 #define EXKV_ERR_SCAN_WS 0x8u   /* encoder: an inconsistent scan workspace (more blocks than tickets) */
 #define EXKV_ERR_WIRE 0x10u     /* wire pack: a raw row's pool slot lay outside the pool */
+#define EXKV_ERR_OFFSETS 0x20u  /* packed prompts: sequence offsets that do not ascend from 0 within the rows */
+#define EXKV_ERR_POSITION 0x40u /* rotation: a position outside the cosine and sine tables (clamped) */
 
 /* out (a device uint32 on the GPU of `stream`) = the OR of the error words of that GPU, in
- * stream order (three small kernels; nothing synchronizes, nothing is allocated); clear != 0
+ * stream order (a small kernel for each; nothing synchronizes, nothing is allocated); clear != 0
  * resets the words. Bits set by kernels on other streams of the GPU are included once they
  * have completed.
  * No counterpart in the reference, whose one such condition, raw-pool overflow, is a
@@ -435,6 +438,93 @@ int exkv_plan_splits(int32_t B, int32_t Hkv, int32_t Hq, int32_t T, int32_t targ
  * No counterpart in the reference (head dim 128 only, cache.py:21). */
 int exkv_plan_splits_hd(int32_t B, int32_t Hkv, int32_t Hq, int32_t T, int32_t D, int32_t* nsplit,
                         int32_t* split_len);
+
+/* Causal attention of packed prompts. Sequence s (of S) holds the query rows cu_q[s] ..
+ * cu_q[s+1] - 1 of q and the key rows cu_k[s] .. cu_k[s+1] - 1 of k and v (int32 [S+1] on the
+ * GPU, ascending from 0; equal ones: an empty sequence); its queries are its last tokens, query
+ * i at key position p = i + keys - queries, and attend to the keys j <= p of their sequence,
+ * with window > 0 only those with j > p - window; a row that sees no key is 0. q [N, Hq, D]
+ * with element strides sq_t (token) and sq_h (head), k and v [NK, Hkv, D] alike, channels
+ * contiguous; rows and strides of whole 16 bytes, key and value rows D to 2^23 elements apart.
+ * out [N, Hq, D] contiguous; rows that no sequence holds are left as they are, or set to 0 if
+ * zero_tail. qk_scale = log2(e) / sqrt(D). Offsets that leave the rows are clamped to them and
+ * reported (EXKV_ERR_OFFSETS). One launch.
+ * No counterpart in the reference (its prefill is the model's own forward pass,
+ * engine.py:42-49). */
+int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                          const void* v, int64_t sv_t, int64_t sv_h, void* out, const int32_t* cu_q,
+                          const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv,
+                          int32_t D, int32_t window, int32_t zero_tail, float qk_scale, hipStream_t stream);
+
+/* The rotation of a packed prompt's queries and keys, for exkv_prompt_attention and the
+ * caches' prefill: row t of sequence s (offsets cu as there) stands at position start[s] + t -
+ * cu[s] (start: int32 [S], or NULL: 0); its heads are rotated half-split with that row of cos and
+ * sin (fp32 [table_rows, D/2]), after the RMS norm over the head with weights q_norm / k_norm
+ * (bf16 [D], or NULL: none) and eps. fp32 inside, rounded once to q_out [N, Hq, D] and k_out
+ * [N, Hkv, D]; rows that no sequence holds become 0. q, k: token and head strides in elements,
+ * rows 4-byte aligned; tables, norms and outputs 16-byte aligned. A position outside the tables is
+ * clamped and reported (EXKV_ERR_POSITION). One launch.
+ * No counterpart in the reference (the model's own modules rotate, engine.py:42-49,75-91). */
+int exkv_rotate_prompt(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                       const float* cos, const float* sin, int32_t table_rows, const void* q_norm,
+                       const void* k_norm, float eps, void* q_out, void* k_out, const int32_t* cu,
+                       const int32_t* start, int32_t S, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                       hipStream_t stream);
+
+/* One token of n sequences with the rotation on the way, in one launch: q rows (strides sq_n,
+ * sq_h) rotated to q_out [n, Hq, D], k rows rotated and appended to the key cache, v rows appended
+ * to the value cache -- what exkv_cache_append (n = B) leaves in both caches given the rotated keys,
+ * counters and raw rows included. A token's position is the number of tokens before it (k_state[0],
+ * or lens - 1). Norms, tables and alignment as in exkv_rotate_prompt. k_state[1] is zero between
+ * calls; both states advance.
+ * Replaces: engine.py:75-91 (rotation) with cache.py:100-112 (append). */
+int exkv_rope_append(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v,
+                     int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int32_t table_rows,
+                     const void* q_norm, const void* k_norm, float eps, void* q_out, int32_t n, int32_t Hq, int32_t Hkv,
+                     void* k_sm, void* k_code, void* k_base, int32_t* k_rowmask, int32_t* k_rowoff,
+                     void* k_raw, int32_t* k_cnt, int32_t* k_before, int32_t* k_state, int64_t k_cap,
+                     int64_t k_raw_rows, void* v_sm, void* v_code, void* v_base, int32_t* v_rowmask,
+                     int32_t* v_rowoff, void* v_raw, int32_t* v_cnt, int32_t* v_before, int32_t* v_state,
+                     int64_t v_cap, int64_t v_raw_rows, int32_t TS, int32_t D, hipStream_t stream);
+
+/* The same into plain bf16 caches [n, TS, Hkv, D] (exkv_bf16_append); states of two words, the
+ * second zero between calls. */
+int exkv_rope_append_bf16(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v,
+                          int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int32_t table_rows,
+                          const void* q_norm, const void* k_norm, float eps, void* q_out, int32_t n, int32_t Hq, int32_t Hkv,
+                          void* kbuf, int32_t* k_state, void* vbuf, int32_t* v_state, int32_t TS, int32_t D,
+                          hipStream_t stream);
+
+/* The same into paged compressed caches (exkv_cache_append_paged_counted: slots, lens counting the
+ * new token, block table, and one arrival word, zero between calls, for both caches). */
+int exkv_rope_append_paged(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v,
+                           int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int32_t table_rows,
+                           const void* q_norm, const void* k_norm, float eps, void* q_out, int32_t n, int32_t Hq, int32_t Hkv,
+                           void* k_sm, void* k_code, void* k_base, int32_t* k_rowmask, int32_t* k_rowoff,
+                           void* k_raw, int32_t* k_cnt, int32_t* k_before, int32_t* arrivals, int64_t k_cap,
+                           int64_t k_raw_rows, void* v_sm, void* v_code, void* v_base, int32_t* v_rowmask,
+                           int32_t* v_rowoff, void* v_raw, int32_t* v_cnt, int32_t* v_before, int64_t v_cap,
+                           int64_t v_raw_rows, const int32_t* slots, const int32_t* lens,
+                           const int32_t* block_table, int64_t bt_stride, int32_t max_seqs, int32_t max_pages,
+                           int32_t pool_pages, int32_t D, hipStream_t stream);
+
+/* The same into paged bf16 pools [16 * pool_pages, Hkv, D] (exkv_bf16_append_paged). */
+int exkv_rope_append_paged_bf16(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v,
+                                int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int32_t table_rows,
+                                const void* q_norm, const void* k_norm, float eps, void* q_out, int32_t n, int32_t Hq, int32_t Hkv,
+                                void* kbuf, void* vbuf, const int32_t* slots, const int32_t* lens,
+                                const int32_t* block_table, int64_t bt_stride, int32_t max_seqs, int32_t max_pages,
+                                int32_t pool_pages, int32_t D, hipStream_t stream);
+
+/* The residual stream between two blocks: u = x, normed over its C channels with post_w if given;
+ * times gate if given; h = r + scale u (r NULL: scale u); y = h rsqrt(mean(h^2) + eps) w. bf16
+ * rows of C (1 to 16384) channels, x, r and gate with row strides sx, sr, sg in elements (sg 0: one
+ * gate row for all), w and post_w [C], h (may be NULL) and y [N, C] contiguous; fp32 inside, h and y
+ * rounded once each. One launch.
+ * Replaces: engine.py:75-91 (the residual adds and norms of the model's own modules). */
+int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t sr, const void* w, const void* post_w,
+                  const void* gate, int64_t sg, float scale, float eps, void* h, void* y, int32_t N, int32_t C,
+                  hipStream_t stream);
 
 #ifdef __cplusplus
 }
