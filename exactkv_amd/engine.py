@@ -13,7 +13,12 @@ MI355X specifics:
     later step replays it. A pool growth at a page boundary changes the raw-pool
     buffers, so the graph is captured again on the next step;
   * prefill runs one sequence at a time through the model's own forward pass, with SDPA
-    restricted to its fused (flash / memory-efficient) kernels.
+    restricted to its fused (flash / memory-efficient) kernels;
+  * layer_kernels=True (PagedEngine.add_many: always) walks the layers here instead, with this
+    package's kernels between the model's projections: rotation and appends in one launch, each
+    residual add with the norm behind it in one, and prompts packed, several sequences in one
+    pass of prompt attention. It rounds less often than the model's modules (once per kernel),
+    so its logits are near theirs, not their bits; the two caches agree bit for bit either way.
 """
 import importlib
 
@@ -22,6 +27,7 @@ import torch
 from .cache import BF16KV, CompressedKV, check_overflow
 from .attention import decode_attention
 from .kernels import HEAD_DIMS, attention_compressed, attention_reference, P
+from .layer import add_norm, launch_rope_append, prompt_attention, rope_append, rotate_prompt
 
 BACKENDS = {"exactkv": CompressedKV, "bf16": BF16KV}
 
@@ -74,6 +80,87 @@ def _project(eng, att, x, B, cos, sin):
     return q, k, v
 
 
+class _LayerKernels:
+    """A decoder's layers with this package's kernels between its projections."""
+
+    PACK = 16384                                # prompt tokens of one pass
+
+    def __init__(self, eng, positions):
+        m = eng.m.model
+        kind = getattr(m.rotary_emb, "rope_type", "default")
+        if kind in ("dynamic", "longrope"):
+            raise AssertionError(f"layer kernels take fixed rotary tables (the model's are {kind!r})")
+        if next(m.parameters()).dtype != torch.bfloat16:
+            raise AssertionError("layer kernels take a bf16 model")
+        self.eng = eng
+        # the model's own tables, in fp32
+        like = torch.zeros(1, dtype=torch.float32, device=eng.dev)
+        cos, sin = m.rotary_emb(like, torch.arange(positions, device=eng.dev)[None])
+        half = eng.D // 2
+        if cos.shape[-1] != eng.D or not torch.equal(cos[..., :half], cos[..., half:]):
+            raise AssertionError("layer kernels rotate half-split over the whole head")
+        self.cos, self.sin = (t[0, :, :half].float().contiguous() for t in (cos, sin))
+
+    def _norm(self, x, residual, norm):
+        return add_norm(x, residual, norm.weight, eps=norm.variance_epsilon)
+
+    def _head_norms(self, att):
+        if not self.eng.qk_norm:
+            return {}
+        return dict(q_norm=att.q_norm.weight, k_norm=att.k_norm.weight, eps=att.q_norm.variance_epsilon)
+
+    def _walk(self, tok, attend):
+        """tok: token ids [n]; attend(i, q, k, v, norms) gives layer i's attention [n, Hq, D] from
+        its projections. Returns the normed hidden state [n, C]."""
+        eng, m = self.eng, self.eng.m.model
+        n = tok.shape[0]
+        h, x = self._norm(m.embed_tokens(tok), None, m.layers[0].input_layernorm)
+        for i, layer in enumerate(m.layers):
+            att = layer.self_attn
+            q = att.q_proj(x).view(n, eng.Hq, eng.D)
+            k = att.k_proj(x).view(n, eng.Hkv, eng.D)
+            v = att.v_proj(x).view(n, eng.Hkv, eng.D)
+            o = attend(i, q, k, v, self._head_norms(att))
+            h, x = self._norm(att.o_proj(o.view(n, eng.Hq * eng.D)), h, layer.post_attention_layernorm)
+            after = m.layers[i + 1].input_layernorm if i + 1 < eng.L else m.norm
+            h, x = self._norm(layer.mlp(x), h, after)
+        return x
+
+    def step(self, tok, attend, device_only):
+        """Logits of one decode step: attend(i, q) over layer i's caches, its token appended."""
+        append = launch_rope_append if device_only else rope_append
+
+        def layer(i, q, k, v, norms):
+            return attend(i, append(q, k, v, self.cos, self.sin, *self.eng.kv[i], **norms))
+        return self.eng.m.lm_head(self._walk(tok, layer))
+
+    def prompts(self, prompts, slots):
+        """Prompts (1-D token ids) into the caches' slots, packed: the normed hidden state of each
+        prompt's last token [len(prompts), C]."""
+        eng, last, i = self.eng, [], 0
+        while i < len(prompts):
+            j, total = i, 0                        # as many as one pass takes, one at least
+            while j < len(prompts) and (j == i or total + prompts[j].numel() <= self.PACK):
+                total += prompts[j].numel()
+                j += 1
+            ends = [0]
+            for p in prompts[i:j]:
+                ends.append(ends[-1] + p.numel())
+            cu = torch.tensor(ends, dtype=torch.int32).to(eng.dev)
+
+            def layer(li, q, k, v, norms):
+                q, k = rotate_prompt(q, k, self.cos, self.sin, cu, **norms)
+                kc, vc = eng.kv[li]
+                for slot, a, e in zip(slots[i:j], ends, ends[1:]):
+                    kc.prefill_slot(slot, k[None, a:e])
+                    vc.prefill_slot(slot, v[None, a:e])
+                return prompt_attention(q, k, v, cu, window=eng.windows[li])
+            x = self._walk(torch.cat([p.reshape(-1) for p in prompts[i:j]]), layer)
+            last.append(x[torch.tensor(ends[1:]).to(eng.dev) - 1])
+            i = j
+        return torch.cat(last)
+
+
 def _write_through(engine, b):
     """A prefill-only transformers cache whose update() encodes the layer's keys and values
     into sequence slot b of the engine's caches and keeps nothing, so the model's forward
@@ -108,11 +195,14 @@ def _layer_kv(pkv, i):
 
 
 class Engine:
-    def __init__(self, model, B, T_max, backend="exactkv", attn=None, before_step=None, graph=True):
+    def __init__(self, model, B, T_max, backend="exactkv", attn=None, before_step=None, graph=True,
+                 layer_kernels=False):
         """backend: 'exactkv' / 'bf16', or a cache class with the same interface.
         attn(q, k_cache, v_cache) and before_step(engine, T) let benchmarks plug in other
         kernels (reference engine.py:30-33); with either plug-in the step runs eagerly.
-        graph: capture the decode step in a HIP graph (default)."""
+        graph: capture the decode step in a HIP graph (default).
+        layer_kernels: rotation, norms and prompt attention by this package's kernels (its own
+        caches only)."""
         # sliding-window layers: decode attention reads each sequence's last `window` tokens,
         # the keys the model's own mask admits (positions > p - window)
         _describe(self, model)
@@ -126,6 +216,9 @@ class Engine:
         self.before_step = before_step
         self.grows = 0
         ours = isinstance(cls, type) and issubclass(cls, (CompressedKV, BF16KV))
+        if layer_kernels and not ours:
+            raise AssertionError("layer kernels append to this package's caches only")
+        self._layers = _LayerKernels(self, self.TS) if layer_kernels else None
         self.use_graph = bool(graph) and attn is None and before_step is None and ours
         self._stream = torch.cuda.Stream(device=self.dev) if self.use_graph else None
         self._graph = None
@@ -147,7 +240,15 @@ class Engine:
         as a [1, T, H, D] view), so the model's DynamicCache never holds the prompt's K/V
         (reference engine.py:42-49 builds it, then cache.py:87-98 copies each layer out of
         it). fused=False keeps that order (the K/V of all layers live until the forward
-        pass ends); both give the same cache bytes."""
+        pass ends); both give the same cache bytes.
+        With layer_kernels the prompts go through packed, several at a time (fused is not used)."""
+        if self._layers is not None:
+            if ids.shape[1] == 0 or b0 + ids.shape[0] > self.B or ids.shape[1] > self.TS:
+                raise AssertionError(f"{ids.shape[0]} prompts of {ids.shape[1]} tokens do not fit slots {b0} to {self.B - 1} "
+                                     f"of {self.TS}")
+            hidden = self._layers.prompts(list(ids), list(range(b0, b0 + ids.shape[0])))
+            self._graph = None                  # buffers may have grown
+            return self._prefill_next(hidden[:, None])
         nxt = []
         with _fused_sdpa():
             for i0 in range(ids.shape[0]):
@@ -193,6 +294,8 @@ class Engine:
         advances its cache's host count, as the reference does, so an attention plug-in
         sees the current length."""
         m, B, Hq, Hkv, D = self.m, self.B, self.Hq, self.Hkv, self.D
+        if self._layers is not None:
+            return self._layers.step(tok, lambda i, q: self._attend(q, *self.kv[i], self.windows[i]), device_only)
         h = m.model.embed_tokens(tok.view(B, 1))
         self._pos.copy_(self.kv[0][0].state[:1].view(1, 1))                 # position = tokens so far
         cos, sin = m.model.rotary_emb(h, self._pos)
@@ -290,9 +393,11 @@ class PagedEngine:
     Engine's. Steps run eagerly: the block table and lengths change on the host between
     steps (begin_step claims a page whenever a token fills one)."""
 
-    def __init__(self, model, max_seqs, T_max, backend="exactkv", num_pages=None, graph=True):
+    def __init__(self, model, max_seqs, T_max, backend="exactkv", num_pages=None, graph=True, layer_kernels=False):
         """graph: replay the step from a HIP graph when the step's slots are 0..n-1 (default);
-        the graph is captured again when n or a raw pool's buffer changes."""
+        the graph is captured again when n or a raw pool's buffer changes.
+        layer_kernels: steps and add() by this package's kernels around the projections, as in
+        Engine (add_many always)."""
         from .paged import PageTable, PagedBF16KV, PagedCompressedKV
         _describe(self, model)
         max_pages = -(-T_max // P)
@@ -306,11 +411,41 @@ class PagedEngine:
         self._tok = torch.zeros(max_seqs, dtype=torch.long, device=self.dev)
         self._logits = None
         self.captures = 0
+        self._positions = P * max_pages
+        self._own_layers = bool(layer_kernels)
+        self._layers = _LayerKernels(self, self._positions) if layer_kernels else None
+
+    @torch.no_grad()
+    def add_many(self, prompts):
+        """Prefill several prompts (1-D token ids of any lengths) into new sequence slots, packed:
+        one pass over the model's layers for about 16K tokens of them. Returns (slots, the greedy
+        next tokens [len(prompts)]). Where a prompt does not fit, none is added."""
+        if self._layers is None:
+            self._layers = _LayerKernels(self, self._positions)
+        prompts = list(prompts)
+        if not prompts or any(p.numel() == 0 for p in prompts):
+            raise ValueError("add_many takes one or more prompts of at least one token")
+        slots = []
+        try:
+            for p in prompts:
+                slots.append(self.table.add(int(p.numel())))
+        except (RuntimeError, ValueError):
+            for s in slots:
+                self.table.release(s)
+            raise
+        hidden = self._layers.prompts(prompts, slots)
+        return slots, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)
 
     @torch.no_grad()
     def add(self, ids, slot=None):
         """Prefill one prompt (1-D token ids) into a new sequence slot. Returns (slot, the
         greedy next token)."""
+        if self._own_layers:
+            if ids.numel() == 0:
+                raise ValueError("a prompt of no tokens")
+            s = self.table.add(int(ids.numel()), slot)
+            hidden = self._layers.prompts([ids.view(-1)], [s])
+            return s, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)[0]
         s = self.table.add(int(ids.numel()), slot)
         with _fused_sdpa():
             out = self.m.model(ids.view(1, -1), use_cache=True, past_key_values=_write_through(self, s))
@@ -322,6 +457,8 @@ class PagedEngine:
     def _forward(self, tok, n):
         """The step's kernels for n rows (appends, attention, the model): no host state."""
         m = self.m
+        if self._own_layers:
+            return self._layers.step(tok, lambda i, q: decode_attention(q, *self.kv[i], window=self.windows[i]), True)
         _, _, lens = self.table.step_rows()
         pos = (lens - 1).view(n, 1).long()                                   # each sequence's position
         h = m.model.embed_tokens(tok.view(n, 1))
