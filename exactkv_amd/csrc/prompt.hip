@@ -41,11 +41,12 @@ namespace exkv {
 #define EXKV_LDS __attribute__((address_space(3)))
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kKeys = 64;              // keys per tile
 constexpr float kLowest = -1e30f;      // the running maximum before any key, in log2 units
 constexpr float kRaise = 8.f;          // a score this far above the running maximum raises it
 
@@ -58,9 +59,11 @@ struct PromptArgs {
     float qk_scale;                    // log2(e) / sqrt(D)
 };
 
+// Two values to bf16 (nearest even): one v_cvt_pk_bf16_f32. Converted one by one they take three
+// more instructions a pair.
 __device__ inline uint32_t pack_bf16(float a, float b) {
-    const __bf16 lo = (__bf16)a, hi = (__bf16)b;
-    return (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+    const f32x2 x = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
 }
 __device__ inline float bf16_float(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -193,12 +196,13 @@ __device__ inline void zero_rows(const PromptArgs& a, int64_t end, int part, int
         out[i] = make_uint4(0, 0, 0, 0);
 }
 
-template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, 2)))
+template <int D, int NW, int KEYS, int WPE>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 prompt_kernel(PromptArgs a, int tiles) {
+    constexpr int KB = KEYS / 32;                                // 32-key blocks of a tile
     constexpr int ROWS = 32 * NW, KS = D / 16, NB = D / 32;      // rows, score k-steps, 32-channel blocks
     constexpr int PIECES = D / 8, RPI = 64 / PIECES;             // 16-byte pieces of a row, rows per load
-    constexpr int TILE = kKeys * 2 * D, LOADS = TILE / 1024 / NW;
+    constexpr int TILE = KEYS * 2 * D, LOADS = TILE / 1024 / NW;
     static_assert(TILE % (1024 * NW) == 0, "whole loads");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];     // K, V of stage 0, K, V of stage 1
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -221,7 +225,7 @@ prompt_kernel(PromptArgs a, int tiles) {
     const int w_lo = __builtin_amdgcn_readfirstlane(pos), w_hi = __builtin_amdgcn_readlane(pos, 31);
     const bool wave_on = wrow0 < nrows;
     const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
-    const int first = k_lo / kKeys, last = k_hi < 0 ? first - 1 : k_hi / kKeys;
+    const int first = k_lo / KEYS, last = k_hi < 0 ? first - 1 : k_hi / KEYS;
 
     bf16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)(tile.q0 + tok) * a.sq_t + hq * a.sq_h + 8 * half;
@@ -238,7 +242,7 @@ prompt_kernel(PromptArgs a, int tiles) {
         v_off[i] = (uint32_t)(r * (int)a.sv_t * 2 + (c ^ value_swizzle<D>(r)) * 16);
     }
     auto load_tile = [&](int it, int stage) {
-        const int j0 = it * kKeys, n = min(kKeys, tile.Lk - j0);
+        const int j0 = it * KEYS, n = min(KEYS, tile.Lk - j0);
         const u32x4 kb = buffer_of(a.k + (int64_t)(tile.k0 + j0) * a.sk_t + hk * a.sk_h, (uint32_t)(((n - 1) * (int)a.sk_t + D) * 2));
         const u32x4 vb = buffer_of(a.v + (int64_t)(tile.k0 + j0) * a.sv_t + hk * a.sv_h, (uint32_t)(((n - 1) * (int)a.sv_t + D) * 2));
         const uint32_t at = lds0 + stage * 2 * TILE + w * 1024;
@@ -265,32 +269,34 @@ prompt_kernel(PromptArgs a, int tiles) {
     float m = kLowest, l = 0.f;
 
     auto tile_step = [&](int it, int stage) {
-        const int j0 = it * kKeys;
-        if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + kKeys - 1 <= w_lo - a.window)) return;   // uniform: none visible
+        const int j0 = it * KEYS;
+        if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + KEYS - 1 <= w_lo - a.window)) return;   // uniform: none visible
         const EXKV_LDS uint8_t* ks = (const EXKV_LDS uint8_t*)lds + stage * 2 * TILE;
         const EXKV_LDS uint8_t* vs = ks + TILE;
-        f32x16 sc[2];
+        f32x16 sc[KB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
                 const bf16x8 kf = *(const EXKV_LDS bf16x8*)(ks + (k_rd ^ (s << 5)) + kb * 32 * 2 * D);
                 sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], sc[kb], 0, 0, 0);
             }
-        }
-        if (!(j0 + kKeys - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window))) {     // uniform: some hidden
+        if (!(j0 + KEYS - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window))) {     // uniform: some hidden
+            asm volatile("");                          // a branch, not selects in every tile
             const int rel = pos - j0 - 4 * half;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if ((uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) sc[kb][i] = -INFINITY;
         }
         float mx = sc[0][0];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
         mx = halves_max(mx) * a.qk_scale;
@@ -303,9 +309,9 @@ prompt_kernel(PromptArgs a, int tiles) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
         }
-        bf16x8 pf[4];
+        bf16x8 pf[2 * KB];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < 2 * KB; ++s) {
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -316,7 +322,7 @@ prompt_kernel(PromptArgs a, int tiles) {
             pf[s] = __builtin_bit_cast(bf16x8, u);
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 2 * KB; ++s)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 union {
@@ -364,11 +370,11 @@ prompt_kernel(PromptArgs a, int tiles) {
     }
 }
 
-template <int D, int NW>
+template <int D, int NW, int KEYS, int WPE>
 static void launch_prompt(const PromptArgs& a, hipStream_t stream) {
     // every sequence's last tile may be partial, and one more for rows behind the last sequence
     const int64_t tiles = (int64_t)a.N * a.G / (32 * NW) + a.S + 1;
-    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)(tiles * a.Hkv)), dim3(64 * NW), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_kernel<D, NW, KEYS, WPE>), dim3((unsigned)(tiles * a.Hkv)), dim3(64 * NW), 0, stream, a, (int)tiles);
 }
 
 hipError_t fetch_errors_prompt(uint32_t* out, int first, int clear, hipStream_t stream) {
@@ -406,10 +412,10 @@ extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, 
     const PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_t, sq_h, sk_t, sk_h,
                        sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale};
     if (D == 64)
-        launch_prompt<64, 8>(a, stream);
+        launch_prompt<64, 4, 64, 4>(a, stream);
     else if (D == 128)
-        launch_prompt<128, 8>(a, stream);
+        launch_prompt<128, 4, 64, 2>(a, stream);
     else
-        launch_prompt<256, 4>(a, stream);
+        launch_prompt<256, 4, 32, 2>(a, stream);
     return hip_status(hipGetLastError(), "prompt_attention");
 }
