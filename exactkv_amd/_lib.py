@@ -75,7 +75,8 @@ SIGNATURES = {
     "exkv_plan_splits": [_i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32)],
     "exkv_plan_splits_hd": [_i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32)],
     "exkv_prompt_attention": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
-                              _i32, _i32, _i32, _f32, _p],
+                              _i32, _i32, _i32, _f32, _p, _i64, _p],
+    "exkv_prompt_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32],
     "exkv_abi_version": [],
     "exkv_last_error": [],
     "exkv_error_bits": [_p, _i32, _p],
@@ -117,7 +118,7 @@ def load():
         f = getattr(lib, name)
         f.argtypes = args
         f.restype = {"exkv_last_error": ctypes.c_char_p, "exkv_wire_bytes": ctypes.c_int64,
-                     "exkv_noalloc_scratch_bytes": ctypes.c_int64,
+                     "exkv_noalloc_scratch_bytes": ctypes.c_int64, "exkv_prompt_workspace": ctypes.c_int64,
                      "exkv_merge_counters": ctypes.c_int64}.get(name, ctypes.c_int)
     v = lib.exkv_abi_version()
     if v != ABI_VERSION:
@@ -130,7 +131,7 @@ def load():
 
 
 # entry points that take no stream (host-only, or hooks)
-_NO_STREAM = {"exkv_wire_bytes", "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
+_NO_STREAM = {"exkv_wire_bytes", "exkv_prompt_workspace", "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
               "exkv_plan_splits", "exkv_plan_splits_hd", "exkv_abi_version", "exkv_last_error", "exkv_error_bits",
               "exkv_set_wait_limit"}
 

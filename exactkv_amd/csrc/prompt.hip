@@ -57,6 +57,10 @@ struct PromptArgs {
     const int32_t *cu_q, *cu_k;        // [S + 1]
     int S, N, NK, Hq, Hkv, G, window, zero_tail;
     float qk_scale;                    // log2(e) / sqrt(D)
+    // keys split into up to `split` parts a tile, of about the tiles that fill `slots` workgroups: partial results
+    int split, slots;
+    float* part_o;                     // [split, N * Hq, D]
+    float2* part_ml;                   // [split, N * Hq]: running maximum (log2 units), sum
 };
 
 // Two values to bf16 (nearest even): one v_cvt_pk_bf16_f32. Converted one by one they take three
@@ -78,6 +82,12 @@ __device__ inline float halves_sum(float x) {
     return __uint_as_float(c[0]) + __uint_as_float(c[1]);
 }
 
+// f(0), .. f(N - 1) with constants.
+template <int N, class F, int... I>
+__device__ inline void each_of(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ inline void each(F f) { each_of<N>(f, std::make_integer_sequence<int, N>{}); }
+
 // A buffer descriptor over `bytes` bytes from p: loads past them return zeros.
 __device__ inline u32x4 buffer_of(const void* p, uint32_t bytes) {
     const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -88,10 +98,16 @@ __device__ inline u32x4 buffer_of(const void* p, uint32_t bytes) {
     b.w = 0x00020000u;
     return b;
 }
-// Direct-to-LDS load of 16 bytes a lane (lane l's land at lds + 16 l), ordered by the kernel's own
-// s_waitcnt: inline, since the compiler would wait for every such load before each LDS read.
-__device__ inline void load_lds16(u32x4 buf, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buf), "{m0}"(lds) : "memory");
+// Piece I of a wavefront's share of a tile straight to LDS: 16 bytes a lane, lane l's to lds + 1024 I
+// + 16 l. Inline, since the compiler would wait for every such load before each LDS read; no memory
+// clobber either, so that LDS reads of other stages may move past it: the wait and the barrier
+// before a stage is read, and the barrier before it is loaded again, order them.
+template <int I>
+__device__ inline void load_piece(u32x4 buf, uint32_t off, uint32_t lds) {
+    if constexpr (I == 0)                              // M0 may have been written just before
+        asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buf), "{m0}"(lds));
+    else
+        asm volatile("buffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds" ::"v"(off), "s"(buf), "{m0}"(lds), "n"(1024 * I));
 }
 
 // Which piece of a row's 16-byte pieces lies where: piece c of key row r at c ^ swizzle(r). Keys are
@@ -105,6 +121,29 @@ __host__ __device__ constexpr int value_swizzle(int r) { return D == 64 ? ((r >>
 // One sequence's share of a workgroup: rows row0 .. of its Lq * G, key rows k0 .. k0 + Lk - 1.
 struct PromptTile {
     int q0, Lq, k0, Lk, row0;
+};
+
+// The descriptor of a tile of KEYS key or value rows of one sequence and head (wave-uniform), and of
+// the next ones. Rows behind the sequence's end lie past its size.
+template <int D, int KEYS>
+struct Stream {
+    u32x4 buf;
+    int left;                          // rows from the tile on
+    uint32_t pitch, step;              // bytes between rows; of a tile
+    __device__ Stream(const uint16_t* p, int64_t s_t, int64_t at_head, const PromptTile& t, int key)
+        : left(t.Lk - key), pitch((uint32_t)s_t * 2) {
+        buf = buffer_of(p + (int64_t)(t.k0 + key) * s_t + at_head, 0);
+        step = KEYS * pitch;
+        size();
+    }
+    __device__ void size() { buf.z = left > 0 ? (min(left, KEYS) - 1) * pitch + 2 * D : 0; }
+    __device__ void next() {
+        const uint64_t a = (((uint64_t)buf.y << 32) | buf.x) + step;
+        buf.x = (uint32_t)a;
+        buf.y = (uint32_t)(a >> 32);
+        left -= KEYS;
+        size();
+    }
 };
 
 // The offsets of sequence s, made fit for use where they are not: 0 <= begin <= end <= rows.
@@ -125,10 +164,13 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, i
     before = 0;
     end = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-        int begin = 0, len = 0;
-        bool bad = false;
-        if (s0 + lane < a.S) sequence_of(a.cu_q, s0 + lane, a.N, begin, len, bad);
-        if (bad) report_error(kErrOffsets);
+        int begin = 0, len = 0, begin_k = 0, len_k = 0;
+        bool bad = false, bad_k = false;
+        if (s0 + lane < a.S) {
+            sequence_of(a.cu_q, s0 + lane, a.N, begin, len, bad);
+            sequence_of(a.cu_k, s0 + lane, a.NK, begin_k, len_k, bad_k);
+        }
+        if (bad || bad_k) report_error(kErrOffsets);
         const int n = (int)(((int64_t)len * a.G + ROWS - 1) / ROWS);
         const int incl = wave_incl_scan(n);
         const int total = __builtin_amdgcn_readlane(incl, 63);
@@ -138,11 +180,8 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, i
             tile.q0 = __builtin_amdgcn_readlane(begin, l);
             tile.Lq = __builtin_amdgcn_readlane(len, l);
             tile.row0 = last * ROWS;
-            bool bad_k = false;
-            sequence_of(a.cu_k, s0 + l, a.NK, tile.k0, tile.Lk, bad_k);
-            if (bad_k) report_error(kErrOffsets);
-            tile.k0 = __builtin_amdgcn_readfirstlane(tile.k0);
-            tile.Lk = __builtin_amdgcn_readfirstlane(tile.Lk);
+            tile.k0 = __builtin_amdgcn_readlane(begin_k, l);
+            tile.Lk = __builtin_amdgcn_readlane(len_k, l);
             return true;
         }
         before += total;
@@ -196,7 +235,96 @@ __device__ inline void zero_rows(const PromptArgs& a, int64_t end, int part, int
         out[i] = make_uint4(0, 0, 0, 0);
 }
 
-template <int D, int NW, int KEYS, int WPE>
+// Key tiles that row tile `row0` of a sequence walks: first .. last.
+template <int ROWS, int KEYS>
+__device__ inline void key_tiles(const PromptArgs& a, const PromptTile& tile, int& first, int& last) {
+    const int shift = tile.Lk - tile.Lq, nrows = tile.Lq * a.G;
+    const int t_lo = tile.row0 / a.G, t_hi = min(tile.row0 + ROWS - 1, nrows - 1) / a.G;
+    const int k_lo = a.window > 0 ? max(0, t_lo + shift - a.window + 1) : 0, k_hi = t_hi + shift;
+    first = k_lo / KEYS;
+    last = k_hi < 0 ? first - 1 : k_hi / KEYS;
+}
+
+// Key tiles of a part, where the keys are split: of the ways to cut the longest tile into 1 to
+// `split` parts, the one that a model of the time finds best. Lane k - 1 takes k parts; every
+// wavefront of both kernels computes it from the offsets. In steps of one tile (1.07 us with one
+// workgroup on a CU): with r workgroups on every CU a step takes 0.8 r; the parts' results, written
+// and read, cost 0.04 a part at head dim 128 (64 KB each) and the second launch 3. The tiles' lengths ascend
+// evenly within a sequence, from n0 to n1, so its tiles have on average
+// (F(n1 / most) - F(n0 / most)) / (n1 / most - n0 / most) parts, F the integral of ceil.
+// Measured against no split (us): 68 rows on 32K keys 489 -> 52, 512 rows on 16K 255 -> 140.
+__device__ inline float ceil_integral(float x) {
+    const float f = floorf(x);
+    return 0.5f * f * (f + 1.f) + (x - f) * (f + 1.f);
+}
+constexpr int kLeast = 8;                              // tiles of keys a split call has, per part
+template <int N>
+__device__ inline float ror(float x) {                 // lane i of a 16-lane row: lane (i - N) % 16 of it
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ inline float wave_least(float x) {
+    x = fminf(x, ror<8>(x));
+    x = fminf(x, ror<4>(x));
+    x = fminf(x, ror<2>(x));
+    x = fminf(x, ror<1>(x));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fminf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fminf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+template <int D, int ROWS, int KEYS>
+__device__ inline int tiles_per_part(const PromptArgs& a) {
+    const int lane = threadIdx.x & 63, k = lane + 1, span = (ROWS - 1) / a.G;
+    // lane's sequence: its row tiles, key tiles of the first and of the last one
+    auto lengths = [&](int s, int& tiles, int& n0, int& n1) {
+        int q0, k0, Lq = 0, Lk = 0;
+        bool bad;
+        if (s < a.S) {
+            sequence_of(a.cu_q, s, a.N, q0, Lq, bad);
+            sequence_of(a.cu_k, s, a.NK, k0, Lk, bad);
+        }
+        tiles = (Lq * a.G + ROWS - 1) / ROWS;
+        auto walked = [&](int t_hi) {
+            const int keys = max(0, t_hi + Lk - Lq + 1), window = a.window > 0 ? min(a.window, a.NK) + span : keys;
+            return (min(keys, window) + KEYS - 1) / KEYS;
+        };
+        n0 = walked(min(span, Lq - 1));
+        n1 = walked(Lq - 1);
+    };
+    int tiles, n0, n1;
+    float far = 1.f;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        lengths(s0 + lane, tiles, n0, n1);
+        far = fmaxf(far, tiles > 0 ? (float)max(n0, n1) : 0.f);
+    }
+    const int longest = (int)-wave_least(-far), most = (longest + k - 1) / k;
+    const float per = 1.f / (float)most;
+    float parts = 0.f;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        if (a.S > 64) lengths(s0 + lane, tiles, n0, n1);
+        for (int i = 0; i < min(64, a.S - s0); ++i) {
+            const int t = __builtin_amdgcn_readlane(tiles, i), m0 = __builtin_amdgcn_readlane(n0, i), m1 = __builtin_amdgcn_readlane(n1, i);
+            const float x0 = (float)min(m0, m1) * per, x1 = (float)max(m0, m1) * per;
+            parts += (float)t * (x1 - x0 < 0.01f ? ceilf(x1 - 1e-4f) : (ceil_integral(x1) - ceil_integral(x0)) / (x1 - x0));
+        }
+    }
+    parts = ceilf(parts - 0.01f) * (float)a.Hkv;
+    const float slots = (float)a.slots, side = ceilf(fminf(parts, slots) * (1.f / 256.f));
+    float time = ceilf(parts / slots) * (float)most * (side <= 1.f ? 1.07f : 0.8f * side);
+    if (k > 1) time += 3.f + 0.04f / 128.f * D * parts;
+    if (k > a.split) time = INFINITY;
+    return __builtin_amdgcn_readlane(most, __builtin_ctzll(__ballot(time == wave_least(time))));
+}
+
+// Into how many parts the key tiles first .. last are split.
+template <int D, int ROWS, int KEYS>
+__device__ inline int parts_of(const PromptArgs& a, int first, int last) {
+    if (a.split == 1) return 1;                        // uniform
+    const int most = tiles_per_part<D, ROWS, KEYS>(a);
+    return max(1, (last - first + most) / most);
+}
+
+template <int D, int NW, int KEYS, int WPE, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 prompt_kernel(PromptArgs a, int tiles) {
     constexpr int KB = KEYS / 32;                                // 32-key blocks of a tile
@@ -204,14 +332,16 @@ prompt_kernel(PromptArgs a, int tiles) {
     constexpr int PIECES = D / 8, RPI = 64 / PIECES;             // 16-byte pieces of a row, rows per load
     constexpr int TILE = KEYS * 2 * D, LOADS = TILE / 1024 / NW;
     static_assert(TILE % (1024 * NW) == 0, "whole loads");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];     // K, V of stage 0, K, V of stage 1
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];     // two key stages, then two value stages
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int hk = (int)blockIdx.x % a.Hkv, t = (int)blockIdx.x / a.Hkv;
+    // first parts first: a tile that has fewer leaves workgroups that end at once, and between the
+    // others those would take every second CU's slot as the grid is handed out
+    const int hk = (int)blockIdx.x % a.Hkv, t = (int)blockIdx.x / a.Hkv % tiles, part = (int)blockIdx.x / a.Hkv / tiles;
     PromptTile tile;
     int before, end;
     if (!find_tile<ROWS>(a, t, tile, before, end)) {
         if (a.zero_tail && end < a.N)
-            zero_rows<D, 64 * NW>(a, end, (t - before) * a.Hkv + hk, (tiles - before) * a.Hkv);
+            zero_rows<D, 64 * NW>(a, end, (part * (tiles - before) + t - before) * a.Hkv + hk, (tiles - before) * a.split * a.Hkv);
         return;
     }
     // the lane's row
@@ -219,46 +349,61 @@ prompt_kernel(PromptArgs a, int tiles) {
     const int wrow0 = tile.row0 + 32 * w, row = min(wrow0 + col, nrows - 1);
     const int tok = row / G, hq = hk * G + row % G;
     const int shift = tile.Lk - tile.Lq, pos = tok + shift;      // the key it stands at; < 0: none visible
-    // keys that the workgroup's and the wavefront's rows see
-    const int t_lo = tile.row0 / G, t_hi = min(tile.row0 + ROWS - 1, nrows - 1) / G;
-    const int k_lo = a.window > 0 ? max(0, t_lo + shift - a.window + 1) : 0, k_hi = t_hi + shift;
+    // keys that the wavefront's first and last row, and the workgroup's, see
     const int w_lo = __builtin_amdgcn_readfirstlane(pos), w_hi = __builtin_amdgcn_readlane(pos, 31);
     const bool wave_on = wrow0 < nrows;
     const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
-    const int first = k_lo / KEYS, last = k_hi < 0 ? first - 1 : k_hi / KEYS;
+    int first, last;
+    key_tiles<ROWS, KEYS>(a, tile, first, last);
+    const int parts = parts_of<D, ROWS, KEYS>(a, first, last);
+    if (part >= parts) return;
+    if (parts > 1) {
+        const int per = (last - first + parts) / parts;
+        first += part * per;
+        last = min(last, first + per - 1);
+    }
 
     bf16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)(tile.q0 + tok) * a.sq_t + hq * a.sq_h + 8 * half;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * s));
+    // waited for here, once (`settled`, behind the first tile's loads): the compiler would otherwise
+    // wait for them at every use in the loop, and so for the next tiles' loads in flight
+    auto settled = [&] {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
+    };
 
-    // loads: the wavefront's pieces of a tile
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(EXKV_LDS uint8_t*)lds);
+    // Loads: a wavefront brings LOADS KiB of a tile, one after the other, so that the instruction's
+    // offset moves both addresses and M0 is written once a tile (the offset is taken off the lane's:
+    // rows lie at least a row apart, so that stays >= 0). A tile's descriptor is the last one's, a
+    // tile further; rows past the sequence's end lie past its size.
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(EXKV_LDS uint8_t*)lds) + w * LOADS * 1024;
     uint32_t k_off[LOADS], v_off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int r = (i * NW + w) * RPI + lane / PIECES, c = lane % PIECES;
-        k_off[i] = (uint32_t)(r * (int)a.sk_t * 2 + (c ^ key_swizzle<D>(r)) * 16);
-        v_off[i] = (uint32_t)(r * (int)a.sv_t * 2 + (c ^ value_swizzle<D>(r)) * 16);
+        const int r = (w * LOADS + i) * RPI + lane / PIECES, c = lane % PIECES;
+        k_off[i] = (uint32_t)(r * (int)a.sk_t * 2 + (c ^ key_swizzle<D>(r)) * 16 - i * 1024);
+        v_off[i] = (uint32_t)(r * (int)a.sv_t * 2 + (c ^ value_swizzle<D>(r)) * 16 - i * 1024);
     }
-    auto load_tile = [&](int it, int stage) {
-        const int j0 = it * KEYS, n = min(KEYS, tile.Lk - j0);
-        const u32x4 kb = buffer_of(a.k + (int64_t)(tile.k0 + j0) * a.sk_t + hk * a.sk_h, (uint32_t)(((n - 1) * (int)a.sk_t + D) * 2));
-        const u32x4 vb = buffer_of(a.v + (int64_t)(tile.k0 + j0) * a.sv_t + hk * a.sv_h, (uint32_t)(((n - 1) * (int)a.sv_t + D) * 2));
-        const uint32_t at = lds0 + stage * 2 * TILE + w * 1024;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_lds16(kb, k_off[i], at + i * NW * 1024);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_lds16(vb, v_off[i], at + TILE + i * NW * 1024);
+    Stream<D, KEYS> keys(a.k, a.sk_t, hk * a.sk_h, tile, first * KEYS), vals(a.v, a.sv_t, hk * a.sv_h, tile, first * KEYS);
+    auto load_keys = [&](int st) {
+        each<LOADS>([&](auto i) { load_piece<i.value>(keys.buf, k_off[i.value], lds0 + st * TILE); });
+        keys.next();
+    };
+    auto load_values = [&](int st) {
+        each<LOADS>([&](auto i) { load_piece<i.value>(vals.buf, v_off[i.value], lds0 + (2 + st) * TILE); });
+        vals.next();
     };
 
     // reads: K piece 2 s + half of row 32 kb + col; V four keys x 16 channels per 16 lanes
     const int k_rd = col * 2 * D + (half ^ key_swizzle<D>(col)) * 16;
     const int vi = lane & 15, v_row = 4 * half + (vi >> 2);
     const int v_piece = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
-    int v_rd[NB];
+    constexpr int VA = NB < 4 ? NB : 4;                // the swizzle turns two bits of a block's index
+    int v_rd[VA];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < VA; ++nb)
         v_rd[nb] = v_row * 2 * D + ((4 * nb + v_piece) ^ value_swizzle<D>(v_row)) * 16 + (vi & 1) * 8;
 
     f32x16 o[NB];
@@ -268,12 +413,50 @@ prompt_kernel(PromptArgs a, int tiles) {
         for (int i = 0; i < 16; ++i) o[nb][i] = 0.f;
     float m = kLowest, l = 0.f;
 
-    auto tile_step = [&](int it, int stage) {
+    // the 16-byte K pieces of block kb, k-step s in K stage st, as the scores' operand
+    auto key_piece = [&](int st, int kb, int s) {
+        return *(const EXKV_LDS bf16x8*)((const EXKV_LDS uint8_t*)lds + st * TILE + (k_rd ^ ((s & 7) << 5)) + (s >> 3) * 256 + kb * 32 * 2 * D);
+    };
+    auto value_piece = [&](int st, int s, int nb) {
+        const EXKV_LDS uint8_t* p = (const EXKV_LDS uint8_t*)lds + (2 + st) * TILE + v_rd[nb % VA] + nb / VA * 256 + 16 * s * 2 * D;
+        union {
+            s16x4 q[2];
+            bf16x8 v;
+        } u;
+        u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EXKV_LDS s16x4*)p);
+        u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EXKV_LDS s16x4*)(p + 8 * 2 * D));
+        return u.v;
+    };
+    auto hide = [&](f32x16 (&sc)[KB], int it) {
         const int j0 = it * KEYS;
-        if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + KEYS - 1 <= w_lo - a.window)) return;   // uniform: none visible
-        const EXKV_LDS uint8_t* ks = (const EXKV_LDS uint8_t*)lds + stage * 2 * TILE;
-        const EXKV_LDS uint8_t* vs = ks + TILE;
-        f32x16 sc[KB];
+        if (j0 + KEYS - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window)) return;   // uniform: all seen
+        asm volatile("");
+        const int rel = pos - j0 - 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) sc[kb][i] = -INFINITY;
+    };
+    auto top = [&](const f32x16 (&sc)[KB]) {
+        float mx = sc[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
+        return halves_max(mx) * a.qk_scale;
+    };
+    auto raise = [&](float mx) {
+        if (__ballot(mx > m + kRaise) == 0) return;    // uniform
+        const float mn = fmaxf(m, mx), alpha = exp2_fast(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
+    };
+    auto scores = [&](int st, f32x16 (&sc)[KB]) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -281,35 +464,18 @@ prompt_kernel(PromptArgs a, int tiles) {
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const bf16x8 kf = *(const EXKV_LDS bf16x8*)(ks + (k_rd ^ (s << 5)) + kb * 32 * 2 * D);
-                sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], sc[kb], 0, 0, 0);
-            }
-        if (!(j0 + KEYS - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window))) {     // uniform: some hidden
-            asm volatile("");                          // a branch, not selects in every tile
-            const int rel = pos - j0 - 4 * half;
-#pragma unroll
             for (int kb = 0; kb < KB; ++kb)
+                sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_piece(st, kb, s), qf[s], sc[kb], 0, 0, 0);
+        if constexpr (PIPE) {                          // two k-steps' reads ahead of the products
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB, 0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if ((uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) sc[kb][i] = -INFINITY;
+            for (int i = 0; i < KS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, KB, 0);
+            }
         }
-        float mx = sc[0][0];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
-        mx = halves_max(mx) * a.qk_scale;
-        if (__ballot(mx > m + kRaise) != 0) {
-            const float mn = fmaxf(m, mx), alpha = exp2_fast(m - mn);
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
-        }
-        bf16x8 pf[2 * KB];
+    };
+    auto weights = [&](const f32x16 (&sc)[KB], bf16x8 (&pf)[2 * KB]) {
 #pragma unroll
         for (int s = 0; s < 2 * KB; ++s) {
             float p[8];
@@ -321,33 +487,99 @@ prompt_kernel(PromptArgs a, int tiles) {
             const u32x4 u = {pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
             pf[s] = __builtin_bit_cast(bf16x8, u);
         }
+    };
+    auto values = [&](int st, const bf16x8 (&pf)[2 * KB]) {
 #pragma unroll
         for (int s = 0; s < 2 * KB; ++s)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                union {
-                    s16x4 q[2];
-                    bf16x8 v;
-                } u;
-                u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EXKV_LDS s16x4*)(vs + v_rd[nb] + (16 * s) * 2 * D));
-                u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EXKV_LDS s16x4*)(vs + v_rd[nb] + (16 * s + 8) * 2 * D));
-                o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, pf[s], o[nb], 0, 0, 0);
-            }
+            for (int nb = 0; nb < NB; ++nb) o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_piece(st, s, nb), pf[s], o[nb], 0, 0, 0);
+    };
+    // every load so far has landed, and every wavefront is done with the stages loaded into next
+    auto next_stage = [&] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
-    if (first <= last) load_tile(first, 0);
-    for (int it = first; it <= last; ++it) {
-        const int stage = (it - first) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                  // tile `it` is whole, and every wavefront is done with the one before
-        asm volatile("" ::: "memory");
-        if (it < last) load_tile(it + 1, stage ^ 1);
-        tile_step(it, stage);
+    if constexpr (PIPE) {
+        // One tile a step: its scores `cur` become weights and meet the values while the next tile's
+        // scores `nxt` are made, so that matrix products and exponentials of one wavefront overlap.
+        auto step = [&](int it, auto stage, f32x16 (&cur)[KB], f32x16 (&nxt)[KB]) {
+            constexpr int st = decltype(stage)::value;
+            const bool more = it < last;               // uniform
+            next_stage();
+            if (it + 2 <= last) load_keys(st);
+            if (more) load_values(st ^ 1);
+            if (!wave_on) return;
+            bf16x8 pf[2 * KB];
+            float mx = kLowest;
+            if (more) {
+                scores(st ^ 1, nxt);
+                hide(nxt, it + 1);
+                mx = top(nxt);
+            }
+            weights(cur, pf);
+            values(st, pf);
+            raise(mx);
+        };
+        if (first <= last) {
+            f32x16 s0[KB], s1[KB];
+            load_keys(0);
+            load_values(0);
+            settled();
+            next_stage();
+            if (first < last) load_keys(1);
+            if (wave_on) {
+                scores(0, s0);
+                hide(s0, first);
+                m = fmaxf(m, top(s0));
+            }
+            for (int it = first; it <= last; it += 2) {
+                step(it, std::integral_constant<int, 0>{}, s0, s1);
+                if (it == last) break;
+                step(it + 1, std::integral_constant<int, 1>{}, s1, s0);
+            }
+        }
+    } else {
+        if (first <= last) {
+            load_keys(0);
+            load_values(0);
+        }
+        settled();
+        for (int it = first; it <= last; ++it) {
+            const int st = (it - first) & 1;
+            next_stage();
+            if (it < last) {
+                load_keys(st ^ 1);
+                load_values(st ^ 1);
+            }
+            const int j0 = it * KEYS;
+            if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + KEYS - 1 <= w_lo - a.window)) continue;   // uniform: none seen
+            f32x16 sc[KB];
+            bf16x8 pf[2 * KB];
+            scores(st, sc);
+            hide(sc, it);
+            raise(top(sc));
+            weights(sc, pf);
+            values(st, pf);
+        }
     }
 
     if (!wave_on) return;
     l = halves_sum(l);
     const bool live = wrow0 + col < nrows, seen = pos >= 0;
+    if (parts > 1) {
+        const int64_t row_out = (int64_t)part * a.N * a.Hq + (int64_t)(tile.q0 + tok) * a.Hq + hq;
+        if (!live) return;
+        if (half == 0) a.part_ml[row_out] = make_float2(m, l);
+        float* op = a.part_o + row_out * D + 4 * half;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(op + 32 * nb + 2 * i) = make_float4(o[nb][i], o[nb][i + 1], o[nb][i + 2], o[nb][i + 3]);
+        return;
+    }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     float finite = 0.f;                                // NaN once a value is not finite
     uint16_t* op = a.out + ((int64_t)(tile.q0 + tok) * a.Hq + hq) * D + 4 * half;
@@ -370,11 +602,95 @@ prompt_kernel(PromptArgs a, int tiles) {
     }
 }
 
-template <int D, int NW, int KEYS, int WPE>
-static void launch_prompt(const PromptArgs& a, hipStream_t stream) {
+// The parts of a split joined: with M the largest of a row's maxima m_i,
+//     out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
+// kMergeShare workgroups take a tile of prompt_kernel's rows. D / 4 lanes hold a row, four channels each,
+// and at first a part's maximum and sum each (hence no more parts than that); then every part's
+// factor goes to all of them, and the parts' loads do not wait for one another.
+constexpr int kMergeShare = 16;
+template <int D, int NW, int KEYS>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
+    constexpr int ROWS = 32 * NW, LPR = D / 4, RPW = 64 / LPR, PER = ROWS / kMergeShare;
+    const int sub = (int)blockIdx.x % kMergeShare, hk = (int)blockIdx.x / kMergeShare % a.Hkv;
+    const int t = (int)blockIdx.x / kMergeShare / a.Hkv;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane % LPR;
+    PromptTile tile;
+    int before, end;
+    if (!find_tile<ROWS>(a, t, tile, before, end)) return;
+    int first, last;
+    key_tiles<ROWS, KEYS>(a, tile, first, last);
+    const int parts = parts_of<D, ROWS, KEYS>(a, first, last);
+    if (parts == 1) return;
+    const int nrows = tile.Lq * a.G, shift = tile.Lk - tile.Lq, row0 = tile.row0 + PER * sub, stop = min(row0 + PER, nrows);
+    const int64_t stride = (int64_t)a.N * a.Hq;
+    uint32_t again = 0;                                // bit c: row row0 + c
+    for (int r0 = row0 + w * RPW; r0 < stop; r0 += 4 * RPW) {
+        const int r = r0 + lane / LPR, rc = min(r, stop - 1), tok = rc / a.G;
+        const int64_t row = (int64_t)(tile.q0 + tok) * a.Hq + hk * a.G + rc % a.G;
+        const float2 ml = j < parts ? a.part_ml[j * stride + row] : make_float2(kLowest, 0.f);
+        float M = ml.x;
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+        const float f = exp2_fast(ml.x - M);
+        float l = ml.y * f;
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* po = a.part_o + row * D + 4 * j;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(po + i * stride * D);
+            const float fi = __shfl(f, i, LPR);
+            o.x = fmaf(x.x, fi, o.x);
+            o.y = fmaf(x.y, fi, o.y);
+            o.z = fmaf(x.z, fi, o.z);
+            o.w = fmaf(x.w, fi, o.w);
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+        const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
+        if (r < stop)
+            *reinterpret_cast<uint2*>(a.out + row * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+        const uint64_t bad = __ballot(r < stop && tok + shift >= 0 && (finite != finite || !(l > 0.f && l < INFINITY)));
+#pragma unroll
+        for (int i = 0; i < RPW; ++i)
+            if ((bad >> (i * LPR) & (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull)) != 0) again |= 1u << (r0 + i - row0);
+    }
+    if (again != 0) {                                  // uniform over the wavefront
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        careful_rows<D>(a, tile, row0, hk, again);
+    }
+}
+
+// How a call is laid out. Keys are split where the row tiles give no CU two workgroups, the number
+// that it runs at a time at least: into up to twice the parts that fill the slots (a call's tiles
+// differ in length; tiles_per_part says how many are used).
+constexpr int kRows = 128, kWaves = 4;
+constexpr int keys_per_tile(int D) { return D == 256 ? 32 : 64; }
+struct PromptPlan {
+    int64_t tiles;                     // row tiles, at most
+    int split, slots;
+};
+static PromptPlan plan_prompt(int64_t N, int64_t NK, int64_t S, int64_t Hq, int64_t Hkv, int D, int64_t window) {
     // every sequence's last tile may be partial, and one more for rows behind the last sequence
-    const int64_t tiles = (int64_t)a.N * a.G / (32 * NW) + a.S + 1;
-    hipLaunchKernelGGL((prompt_kernel<D, NW, KEYS, WPE>), dim3((unsigned)(tiles * a.Hkv)), dim3(64 * NW), 0, stream, a, (int)tiles);
+    PromptPlan p{N * (Hq / Hkv) / kRows + S + 1, 1, D == 64 ? 1024 : 512};
+    const int64_t reach = window > 0 && window + kRows < NK ? window + kRows : NK;
+    const int64_t keys = (reach + keys_per_tile(D) - 1) / keys_per_tile(D), units = p.tiles * Hkv;
+    if (2 * units > p.slots) return p;
+    int64_t split = 2 * p.slots / units;
+    if (split > D / 4) split = D / 4;
+    if (split > keys / kLeast) split = keys / kLeast;
+    if (split > 1) p.split = (int)split;
+    return p;
+}
+
+template <int D, int WPE, bool PIPE>
+static void launch_prompt(const PromptArgs& a, int64_t tiles, hipStream_t stream) {
+    constexpr int KEYS = keys_per_tile(D);
+    hipLaunchKernelGGL((prompt_kernel<D, kWaves, KEYS, WPE, PIPE>), dim3((unsigned)(tiles * a.split * a.Hkv)), dim3(64 * kWaves), 0,
+                       stream, a, (int)tiles);
+    if (a.split > 1)
+        hipLaunchKernelGGL((prompt_merge_kernel<D, kWaves, KEYS>), dim3((unsigned)(kMergeShare * tiles * a.Hkv)), dim3(256), 0, stream, a);
 }
 
 hipError_t fetch_errors_prompt(uint32_t* out, int first, int clear, hipStream_t stream) {
@@ -389,10 +705,17 @@ static bool rows_ok(const void* p, int64_t s_t, int64_t s_h) {
     return (uintptr_t)p % 16 == 0 && s_t % 8 == 0 && s_h % 8 == 0 && s_t >= 0 && s_h >= 0;
 }
 
+extern "C" int64_t exkv_prompt_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window) {
+    if (!head_dim_ok(D) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || S < 0 || N <= 0 || NK <= 0 || window < 0) return 0;
+    const PromptPlan p = plan_prompt(N, NK, S, Hq, Hkv, D, window);
+    return p.split > 1 ? (int64_t)p.split * N * Hq * (D + 2) * 4 : 0;
+}
+
 extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
                                      const void* v, int64_t sv_t, int64_t sv_h, void* out, const int32_t* cu_q,
                                      const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv,
-                                     int32_t D, int32_t window, int32_t zero_tail, float qk_scale, hipStream_t stream) {
+                                     int32_t D, int32_t window, int32_t zero_tail, float qk_scale, void* ws, int64_t ws_bytes,
+                                     hipStream_t stream) {
     EXKV_REQUIRE(head_dim_ok(D), "prompt_attention: head dim must be 64, 128 or 256 (got %d)", D);
     EXKV_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "prompt_attention: %d query heads over %d KV heads", Hq, Hkv);
     EXKV_REQUIRE(S >= 0 && N >= 0 && NK >= 0 && window >= 0, "prompt_attention: bad shape S=%d N=%d NK=%d window=%d", S, N,
@@ -407,15 +730,25 @@ extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, 
                  "prompt_attention: key and value rows must lie %d to %d elements apart", D, 1 << 23);
     const int64_t G = Hq / Hkv;
     EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 &&
-                     ((int64_t)N * G / 128 + S + 1) * Hkv * 512 <= (int64_t)UINT32_MAX,
+                     ((int64_t)N * G / kRows + S + 1) * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX,
                  "prompt_attention: too many rows (N=%d, %d heads per KV head, %d KV heads, S=%d)", N, (int)G, Hkv, S);
-    const PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_t, sq_h, sk_t, sk_h,
-                       sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale};
+    PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_t, sq_h, sk_t, sk_h,
+                 sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale, 1, 0, nullptr, nullptr};
+    PromptPlan p = plan_prompt(N, NK, S, Hq, Hkv, D, window);
+    if (ws != nullptr && p.split > 1) {
+        const int64_t rows = (int64_t)p.split * N * Hq;
+        EXKV_REQUIRE((uintptr_t)ws % 16 == 0 && ws_bytes >= rows * (D + 2) * 4, "prompt_attention: workspace of %lld bytes, %lld needed",
+                     (long long)ws_bytes, (long long)(rows * (D + 2) * 4));
+        a.split = p.split;
+        a.slots = p.slots;
+        a.part_o = (float*)ws;
+        a.part_ml = (float2*)((float*)ws + rows * D);
+    }
     if (D == 64)
-        launch_prompt<64, 4, 64, 4>(a, stream);
+        launch_prompt<64, 4, false>(a, p.tiles, stream);
     else if (D == 128)
-        launch_prompt<128, 4, 64, 2>(a, stream);
+        launch_prompt<128, 2, true>(a, p.tiles, stream);
     else
-        launch_prompt<256, 4, 32, 2>(a, stream);
+        launch_prompt<256, 2, false>(a, p.tiles, stream);
     return hip_status(hipGetLastError(), "prompt_attention");
 }

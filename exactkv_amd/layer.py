@@ -134,9 +134,12 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, window=0, out=No
         with torch.cuda.device(dev):
             prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, window=window, out=out.zero_() if fresh else out)
         return out
+    # a call with few rows splits its keys: partial results, this call's own (in a graph: the graph's)
+    need = _lib.load().exkv_prompt_workspace(S, N, NK, Hq, Hkv, D, window)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call("exkv_prompt_attention", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, v.data_ptr(), sv_t, sv_h,
               out.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), S, N, NK, Hq, Hkv, D, window, int(fresh),
-              _QK_SCALE[D], _lib.stream(dev.index))
+              _QK_SCALE[D], None if ws is None else ws.data_ptr(), need, _lib.stream(dev.index))
     return out
 
 

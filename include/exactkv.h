@@ -448,13 +448,20 @@ int exkv_plan_splits_hd(int32_t B, int32_t Hkv, int32_t Hq, int32_t T, int32_t D
  * contiguous; rows and strides of whole 16 bytes, key and value rows D to 2^23 elements apart.
  * out [N, Hq, D] contiguous; rows that no sequence holds are left as they are, or set to 0 if
  * zero_tail. qk_scale = log2(e) / sqrt(D). Offsets that leave the rows are clamped to them and
- * reported (EXKV_ERR_OFFSETS). One launch.
+ * reported (EXKV_ERR_OFFSETS). ws (16-byte aligned, may be NULL): with the
+ * exkv_prompt_workspace bytes of the call, the keys of calls with few rows are split over more
+ * workgroups and joined by a second launch; without, or where that is 0, one launch. Calls that
+ * overlap need workspaces of their own.
  * No counterpart in the reference (its prefill is the model's own forward pass,
  * engine.py:42-49). */
 int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
                           const void* v, int64_t sv_t, int64_t sv_h, void* out, const int32_t* cu_q,
                           const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv,
-                          int32_t D, int32_t window, int32_t zero_tail, float qk_scale, hipStream_t stream);
+                          int32_t D, int32_t window, int32_t zero_tail, float qk_scale, void* ws,
+                          int64_t ws_bytes, hipStream_t stream);
+/* Bytes of workspace with which exkv_prompt_attention splits the keys of such a call; 0: none. Host
+ * only. */
+int64_t exkv_prompt_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window);
 
 /* The rotation of a packed prompt's queries and keys, for exkv_prompt_attention and the
  * caches' prefill: row t of sequence s (offsets cu as there) stands at position start[s] + t -

@@ -111,6 +111,45 @@ def test_rows_that_see_no_key_are_zero(D):
     assert (got[:30] == 0).all() and (got[40:49] == 0).all() and (got[49:110] == 0).all()
 
 
+SPLIT = [([1], [3000], 8, 8, 0), ([40, 1, 200], [2500, 40, 900], 8, 2, 0), ([17, 0, 130], [1500, 0, 130], 14, 2, 700),
+         ([700], [700], 4, 1, 0), ([3, 5, 2, 8], [5, 1000, 2, 700], 32, 8, 0), ([1] * 70, list(range(600, 670)), 4, 1, 0),
+         ([64, 30], [20, 1200], 8, 2, 0), ([17, 0, 130], [3500, 0, 130], 14, 2, 2000)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,keys,Hq,Hkv,window", SPLIT, ids=lambda x: str(x)[:24])
+def test_few_rows_split_their_keys(lens, keys, Hq, Hkv, window, D):
+    """Calls with few rows and many keys take a workspace and split the keys; rows without a key
+    among them are 0, rows that no sequence holds as without a split."""
+    from exactkv_amd import _lib
+    # at head dim 64 and 128, 700 keys (all, or a window's) are too few tiles to split
+    if max(keys) > 700 and window != 700:
+        assert _lib.load().exkv_prompt_workspace(len(lens), sum(lens), sum(keys), Hq, Hkv, D, window) > 0
+    got = _run(lens, Hq, Hkv, D, window=window, keys=keys, seed=41)
+    q, k, v = _inputs(lens, keys, Hq, Hkv, D, 41)
+    tail = torch.cat([q, q[:3]])
+    assert same_bits(exactkv.prompt_attention(tail, k, v, _cu(lens), cu_seqlens_k=_cu(keys), window=window)[:sum(lens)], got)
+    out = torch.full_like(tail, 7.0)
+    exactkv.prompt_attention(tail, k, v, _cu(lens), cu_seqlens_k=_cu(keys), window=window, out=out)
+    assert (out[sum(lens):] == 7).all() and same_bits(out[:sum(lens)], got)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_split_rows_with_bad_values(D):
+    """The joined result of split keys is checked for the rows that must not see a bad value, too."""
+    lens, keys = [30], [2000]
+    q, k, v = _inputs(lens, keys, 4, 2, D, 43)
+    v[1985, 1] = float("nan")                          # seen by the queries from key 1985 on, of KV head 1
+    got = exactkv.prompt_attention(q, k, v, _cu(lens), cu_seqlens_k=_cu(keys))
+    seen = torch.zeros(30, 4, dtype=torch.bool, device=DEV)
+    seen[15:, 2:] = True
+    v[1985, 1] = 0
+    want, mag = _formula(q, k, v, lens, keys, 0)
+    assert got[seen].isnan().all() and torch.isfinite(got[~seen]).all()
+    err = (got.double() - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * mag)
+    assert (err[~seen] <= 0).all()
+
+
 def test_more_sequences_than_a_wavefront_scans():
     g = torch.Generator().manual_seed(5)
     lens = torch.randint(0, 9, (200,), generator=g).tolist()
@@ -233,6 +272,27 @@ def test_captured_and_replayed():
         g.replay()
         torch.cuda.synchronize()
         assert same_bits(out, eager)
+
+
+def test_split_keys_captured():
+    """Two captured calls with split keys (a workspace each), replayed in either order."""
+    graphs, stream = [], torch.cuda.Stream()
+    for seed, lens, keys in ((3, [20], [3000]), (4, [7, 9], [2000, 1500])):
+        q, k, v = _inputs(lens, keys, 8, 2, 128, seed)
+        cu, ck = _cu(lens), _cu(keys)
+        want = exactkv.prompt_attention(q, k, v, cu, cu_seqlens_k=ck)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = exactkv.prompt_attention(q, k, v, cu, cu_seqlens_k=ck)
+        graphs.append((g, out, want, (q, k, v, cu, ck)))
+    for order in ((0, 1), (1, 0), (1, 1)):
+        for i in order:
+            graphs[i][1].zero_()
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for i in order:
+            assert same_bits(graphs[i][1], graphs[i][2])
 
 
 def test_on_another_stream():

@@ -16,7 +16,7 @@ def _fails(name, args, words):
 
 def _prompt(**kw):
     a = dict(q=16, sq_t=4096, sq_h=128, k=16, sk_t=1024, sk_h=128, v=16, sv_t=1024, sv_h=128, out=16, cu_q=4, cu_k=4, S=1,
-             N=10, NK=10, Hq=32, Hkv=8, D=128, window=0, zero=0, scale=0.1)
+             N=10, NK=10, Hq=32, Hkv=8, D=128, window=0, zero=0, scale=0.1, ws=None, wsb=0)
     a.update(kw)
     return (*a.values(), None)
 
