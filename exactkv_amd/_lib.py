@@ -278,6 +278,19 @@ def stream(index=None):
     return torch.cuda.current_stream(index).cuda_stream
 
 
+def current_device():
+    """The current device's index (through torch's raw query when it has one: a call of 0.1 us, not
+    0.3)."""
+    global _device_query
+    if _device_query is None:
+        import torch
+        _device_query = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    return _device_query()
+
+
+_device_query = None
+
+
 def ptr(t, align=16, what="tensor"):
     """Device pointer of a CUDA (HIP) tensor, checked for device and alignment."""
     if t is None:

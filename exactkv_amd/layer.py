@@ -14,6 +14,8 @@ No counterpart in the reference, whose engine leaves all of this to the model's 
 The tensors of a call are on one GPU; the work goes to that GPU's current stream, allocates
 nothing but the outputs, waits for nothing, and can be captured in a HIP graph.
 """
+import operator
+
 import torch
 
 from . import _lib
@@ -24,15 +26,24 @@ from .paged import PagedBF16KV, PagedCompressedKV
 BF16 = torch.bfloat16
 
 
-def _rows(t, what):
-    """(tokens, heads, D, token stride, head stride) of bf16 rows [n, H, D] on the GPU."""
-    if t.dim() != 3 or t.dtype != BF16 or not t.is_cuda:
-        raise ValueError(f"{what} must be a bf16 [tokens, heads, D] GPU tensor")
+# The checks below run in every call of a decode step, so each reads an attribute once and names
+# what is wrong only when something is.
+
+def _rows(t, dev, what):
+    """(tokens, heads, D, token stride, head stride) of bf16 rows [n, H, D] on GPU `dev` (an index)."""
+    if t.dtype is not BF16 or t.dim() != 3 or t.get_device() != dev or dev < 0:
+        _bad_tensor(t, dev, what, "a bf16 [tokens, heads, D] GPU tensor", t.dtype is BF16 and t.dim() == 3)
     n, H, D = t.shape
     s_t, s_h, s_d = t.stride()
     if s_d != 1 and D > 1:
         raise ValueError(f"{what}: rows (the last axis) must be contiguous")
     return n, H, D, (s_t if n > 1 else H * D), (s_h if H > 1 else D)
+
+
+def _bad_tensor(t, dev, what, kind, form):
+    if form and t.is_cuda and dev >= 0:
+        raise ValueError(f"all tensors of a call must be on one GPU: {what} is on {t.device}, the first on cuda:{dev}")
+    raise ValueError(f"{what} must be {kind}")
 
 
 def _check_heads(Hq, Hkv, D):
@@ -42,33 +53,52 @@ def _check_heads(Hq, Hkv, D):
         raise ValueError(f"{Hq} query heads do not divide over {Hkv} KV heads")
 
 
-def _offsets(cu, what):
-    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_cuda or not cu.is_contiguous():
+def _int32(t, dims, dev, what, kind):
+    """Pointer of a contiguous int32 tensor on GPU `dev`."""
+    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != dev or not t.is_contiguous():
+        _bad_tensor(t, dev, what, kind, t.dtype is torch.int32 and t.dim() == dims and t.is_contiguous())
+    return t.data_ptr()
+
+
+def _offsets(cu, dev, what):
+    """(pointer, sequences) of packed sequences' offsets."""
+    p = _int32(cu, 1, dev, what, "a contiguous int32 [sequences + 1] GPU tensor")
+    n = cu.shape[0]
+    if n < 1:
         raise ValueError(f"{what} must be a contiguous int32 [sequences + 1] GPU tensor")
-    return cu.numel() - 1
+    return p, n - 1
 
 
-def _one_device(dev, *tensors):
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"all tensors of a call must be on {dev} (got one on {t.device})")
-
-
-def _vector(w, n, what):
+def _vector(w, n, dev, what):
     """Pointer of a bf16 [n] weight, or None."""
     if w is None:
         return None
-    if w.dtype != BF16 or w.shape != (n,) or not w.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous bf16 [{n}] GPU tensor")
-    return _lib.ptr(w, 16, what)
+    if w.dtype is not BF16 or w.get_device() != dev or w.shape != (n,) or not w.is_contiguous():
+        _bad_tensor(w, dev, what, f"a contiguous bf16 [{n}] GPU tensor",
+                    w.dtype is BF16 and w.shape == (n,) and w.is_contiguous())
+    return w.data_ptr()
 
 
-def _tables(cos, sin, D):
+def _tables(cos, sin, D, dev):
     """(cos pointer, sin pointer, rows) of fp32 tables [positions, D / 2]."""
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != D // 2
-            or cos.shape != sin.shape or cos.shape[0] < 1 or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise ValueError(f"cos and sin must be contiguous fp32 [positions, {D // 2}] GPU tensors of one shape")
-    return _lib.ptr(cos, 16, "cos"), _lib.ptr(sin, 16, "sin"), cos.shape[0]
+    shape = cos.shape
+    f32 = torch.float32
+    if (cos.dtype is not f32 or sin.dtype is not f32 or cos.get_device() != dev or sin.get_device() != dev
+            or len(shape) != 2 or shape[1] != D // 2 or sin.shape != shape or shape[0] < 1
+            or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError(f"cos and sin must be contiguous fp32 [positions, {D // 2}] tensors of one shape on the call's GPU")
+    return cos.data_ptr(), sin.data_ptr(), shape[0]
+
+
+def _out_like(out, q, shape, *inputs):
+    """out, checked, or a new tensor of q's shape."""
+    if out is None:
+        return torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    if out.shape != shape or out.dtype is not BF16 or out.get_device() != q.get_device() or not out.is_contiguous():
+        raise ValueError("out must be a contiguous bf16 tensor shaped like q, on its GPU")
+    if _overlap(out, q) or any(_overlap(out, t) for t in inputs):
+        raise ValueError("out overlaps an input")
+    return out
 
 
 def _overlap(a, b):
@@ -82,10 +112,10 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
-def _elsewhere(dev):
-    """Whether dev is not the current device (calls then make it so: its current stream may be the
-    null stream, which is the current device's)."""
-    return dev.index != torch.cuda.current_device()
+def _on(dev):
+    """The context in which a call on GPU `dev` launches when that is not the current device: its
+    current stream may be the null stream, which is the current device's."""
+    return torch.cuda.device(dev)
 
 
 def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, window=0, out=None):
@@ -104,42 +134,36 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, window=0, out=No
     and v may be strided views (of a fused projection, of [1, H, N, D]): rows contiguous, 16-byte
     aligned. out: a contiguous tensor shaped like q that overlaps no input; its rows behind the
     last sequence are left as they were (without out they are 0)."""
-    N, Hq, D, sq_t, sq_h = _rows(q, "q")
-    NK, Hkv, Dk, sk_t, sk_h = _rows(k, "k")
-    NV, Hv, Dv, sv_t, sv_h = _rows(v, "v")
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, window=window, out=out)
+    N, Hq, D, sq_t, sq_h = _rows(q, dev, "q")
+    NK, Hkv, Dk, sk_t, sk_h = _rows(k, dev, "k")
+    NV, Hv, Dv, sv_t, sv_h = _rows(v, dev, "v")
     _check_heads(Hq, Hkv, D)
-    if Dk != D or (NV, Hv, Dv) != (NK, Hkv, D):
+    if Dk != D or NV != NK or Hv != Hkv or Dv != D:
         raise ValueError(f"k and v must be of one shape [keys, heads, {D}] (got {tuple(k.shape)}, {tuple(v.shape)})")
-    S = _offsets(cu_seqlens, "cu_seqlens")
+    cu, S = _offsets(cu_seqlens, dev, "cu_seqlens")
     if cu_seqlens_k is None:
-        cu_seqlens_k = cu_seqlens
+        cu_k = cu
         if NK != N:
             raise ValueError(f"{NK} keys for {N} queries: give cu_seqlens_k")
-    elif _offsets(cu_seqlens_k, "cu_seqlens_k") != S:
-        raise ValueError("cu_seqlens and cu_seqlens_k must hold as many sequences")
+    else:
+        cu_k, Sk = _offsets(cu_seqlens_k, dev, "cu_seqlens_k")
+        if Sk != S:
+            raise ValueError("cu_seqlens and cu_seqlens_k must hold as many sequences")
     window = int(window or 0)
     if window < 0 or window > 0x7FFFFFFF:
         raise ValueError(f"window must be >= 0 (got {window})")
-    dev = q.device
-    _one_device(dev, k, v, cu_seqlens, cu_seqlens_k, out)
     fresh = out is None
-    if fresh:
-        out = torch.empty((N, Hq, D), dtype=BF16, device=dev)
-    else:
-        if out.shape != q.shape or out.dtype != BF16 or not out.is_contiguous():
-            raise ValueError("out must be a contiguous bf16 tensor shaped like q")
-        if any(_overlap(out, t) for t in (q, k, v)):
-            raise ValueError("out overlaps an input")
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, window=window, out=out.zero_() if fresh else out)
-        return out
+    out = _out_like(out, q, (N, Hq, D), k, v)
     # a call with few rows splits its keys: partial results, this call's own (in a graph: the graph's)
     need = _lib.load().exkv_prompt_workspace(S, N, NK, Hq, Hkv, D, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.call("exkv_prompt_attention", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, v.data_ptr(), sv_t, sv_h,
-              out.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), S, N, NK, Hq, Hkv, D, window, int(fresh),
-              _QK_SCALE[D], None if ws is None else ws.data_ptr(), need, _lib.stream(dev.index))
+              out.data_ptr(), cu, cu_k, S, N, NK, Hq, Hkv, D, window, fresh, _QK_SCALE[D],
+              ws.data_ptr() if need else None, need, _lib.stream(dev))
     return out
 
 
@@ -152,61 +176,72 @@ def rotate_prompt(q, k, cos, sin, cu_seqlens, *, start=None, q_norm=None, k_norm
     prompt_attention and the caches' prefill; rows that no sequence holds are 0.
 
     A position outside the tables is clamped to them and sets an error bit (kernels.check_errors)."""
-    N, Hq, D, sq_t, sq_h = _rows(q, "q")
-    NK, Hkv, Dk, sk_t, sk_h = _rows(k, "k")
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return rotate_prompt(q, k, cos, sin, cu_seqlens, start=start, q_norm=q_norm, k_norm=k_norm, eps=eps)
+    N, Hq, D, sq_t, sq_h = _rows(q, dev, "q")
+    NK, Hkv, Dk, sk_t, sk_h = _rows(k, dev, "k")
     if D not in HEAD_DIMS or Dk != D or NK != N or Hq == 0 or Hkv == 0:
         raise ValueError(f"q and k must be [N, heads, D] with D in {HEAD_DIMS} (got {tuple(q.shape)}, {tuple(k.shape)})")
-    S = _offsets(cu_seqlens, "cu_seqlens")
-    dev = q.device
-    _one_device(dev, k, cos, sin, cu_seqlens, start, q_norm, k_norm)
-    if start is not None and (start.dtype != torch.int32 or start.shape != (S,) or not start.is_contiguous()):
-        raise ValueError(f"start must be a contiguous int32 [{S}] GPU tensor")
-    cp, sp, rows = _tables(cos, sin, D)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return rotate_prompt(q, k, cos, sin, cu_seqlens, start=start, q_norm=q_norm, k_norm=k_norm, eps=eps)
-    qo = torch.empty((N, Hq, D), dtype=BF16, device=dev)
-    ko = torch.empty((N, Hkv, D), dtype=BF16, device=dev)
-    _lib.call("exkv_rotate_prompt", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, cp, sp, rows,
-              _vector(q_norm, D, "q_norm"), _vector(k_norm, D, "k_norm"), eps, qo.data_ptr(), ko.data_ptr(),
-              cu_seqlens.data_ptr(), None if start is None else start.data_ptr(), S, N, Hq, Hkv, D, _lib.stream(dev.index))
+    cu, S = _offsets(cu_seqlens, dev, "cu_seqlens")
+    first = None
+    if start is not None:
+        first = _int32(start, 1, dev, "start", f"a contiguous int32 [{S}] GPU tensor")
+        if start.shape[0] != S:
+            raise ValueError(f"start must be a contiguous int32 [{S}] GPU tensor")
+    cp, sp, rows = _tables(cos, sin, D, dev)
+    qw, kw = _vector(q_norm, D, dev, "q_norm"), _vector(k_norm, D, dev, "k_norm")
+    qo, ko = _out_like(None, q, (N, Hq, D)), _out_like(None, k, (N, Hkv, D))
+    _lib.call("exkv_rotate_prompt", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, cp, sp, rows, qw, kw, eps,
+              qo.data_ptr(), ko.data_ptr(), cu, first, S, N, Hq, Hkv, D, _lib.stream(dev))
     return qo, ko
 
 
-def _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out):
+def _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out, dev):
     """The rows' arguments of a rotated append, and (out, n, Hkv, D)."""
-    n, Hq, D, sq_n, sq_h = _rows(q, "q")
-    nk, Hkv, Dk, sk_n, sk_h = _rows(k, "k")
-    nv, Hv, Dv, sv_n, sv_h = _rows(v, "v")
-    if D not in HEAD_DIMS or (nk, Dk) != (n, D) or (nv, Hv, Dv) != (n, Hkv, D) or Hq == 0 or Hkv == 0:
+    n, Hq, D, sq_n, sq_h = _rows(q, dev, "q")
+    nk, Hkv, Dk, sk_n, sk_h = _rows(k, dev, "k")
+    nv, Hv, Dv, sv_n, sv_h = _rows(v, dev, "v")
+    if D not in HEAD_DIMS or nk != n or Dk != D or nv != n or Hv != Hkv or Dv != D or Hq == 0 or Hkv == 0:
         raise ValueError(f"q [n, Hq, D], k and v [n, Hkv, D] with D in {HEAD_DIMS} expected (got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)})")
-    _one_device(q.device, k, v, cos, sin, q_norm, k_norm, out)
-    cp, sp, rows = _tables(cos, sin, D)
-    if out is None:
-        out = torch.empty((n, Hq, D), dtype=BF16, device=q.device)
-    elif out.shape != q.shape or out.dtype != BF16 or not out.is_contiguous():
-        raise ValueError("out must be a contiguous bf16 tensor shaped like q")
-    elif any(_overlap(out, t) for t in (q, k, v)):
-        raise ValueError("out overlaps an input")
-    return (q.data_ptr(), sq_n, sq_h, k.data_ptr(), sk_n, sk_h, v.data_ptr(), sv_n, sv_h, cp, sp, rows,
-            _vector(q_norm, D, "q_norm"), _vector(k_norm, D, "k_norm"), eps, _lib.ptr(out, 16, "out"), n, Hq, Hkv), out, n, Hkv, D
+    cp, sp, rows = _tables(cos, sin, D, dev)
+    qw, kw = _vector(q_norm, D, dev, "q_norm"), _vector(k_norm, D, dev, "k_norm")
+    out = _out_like(out, q, (n, Hq, D), k, v)
+    return (q.data_ptr(), sq_n, sq_h, k.data_ptr(), sk_n, sk_h, v.data_ptr(), sv_n, sv_h, cp, sp, rows, qw, kw, eps,
+            out.data_ptr(), n, Hq, Hkv), out, n, Hkv, D
 
 
-_ARRAYS = ("sm", "code", "base", "rowmask", "rowoff", "raw")
+_ARRAYS = operator.itemgetter("sm", "code", "base", "rowmask", "rowoff", "raw")
 
 
-def _compressed_args(buf, n, H, D, dev, what):
-    """A compressed cache's arrays and counters (its encoder view) as a call takes them, checked."""
-    raw = buf["raw"]
-    if (buf["H"], buf["D"]) != (H, D) or buf["sm"].shape[-1] != D or raw.shape[-1] != D:
+def _pool_args(buf, H, D, dev, what):
+    """A paged compressed cache's arrays and counters (its encoder view) as a call takes them, its
+    cap, raw rows and pages, checked."""
+    arrays = sm, code, base, rowmask, rowoff, raw = _ARRAYS(buf)
+    pages, units = buf["TS"] // P, buf["TS"] // P * H
+    if buf["H"] != H or buf["D"] != D or raw.shape[-1] != D:
         raise ValueError(f"{what} holds {buf['H']} heads of {buf['D']}, the rows {H} of {D}")
-    for name in _ARRAYS:
-        if not buf[name].is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous")
-    _one_device(dev, *(buf[name] for name in _ARRAYS))
-    return ([_lib.ptr(buf[name], 16, name) for name in _ARRAYS]
-            + [_lib.ptr(buf["cnt"], 4, "cnt"), _lib.ptr(buf["before"], 4, "before")], int(buf["cap"]), raw.shape[0])
+    if (sm.numel() != units * P * D or code.numel() * 2 != units * P * D or base.numel() != units * D
+            or rowmask.numel() != units or rowoff.numel() != units):
+        raise ValueError(f"{what}: the arrays are not those of {pages} pages")
+    low, ptrs = 0, []
+    for t in arrays:
+        if t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: the arrays must be contiguous, on the rows' GPU")
+        p = t.data_ptr()
+        low |= p
+        ptrs.append(p)
+    for t in (buf["cnt"], buf["before"]):
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: the counters must be on the rows' GPU")
+        p = t.data_ptr()
+        low |= p << 2
+        ptrs.append(p)
+    if low & 15:
+        raise ValueError(f"{what}: the arrays must be 16-byte aligned, the counters 4-byte")
+    return ptrs, int(buf["cap"]), raw.shape[0], pages
 
 
 def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=None, *, q_norm=None, k_norm=None,
@@ -221,48 +256,43 @@ def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=No
     in one launch. A slot whose lens is 0 or past the table is left alone.
 
     This is rope_append on tensors: it changes no host state."""
-    rows, out, n, H, D = _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out)
-    dev = q.device
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-        raise ValueError("block_table must be an int32 [sequences, pages] tensor with contiguous rows")
-    if lens.dtype != torch.int32 or lens.dim() != 1 or not lens.is_contiguous() or lens.shape[0] < block_table.shape[0]:
-        raise ValueError("lens must be a contiguous int32 [sequences] tensor")
-    if slots is not None and (slots.dtype != torch.int32 or slots.shape != (n,) or not slots.is_contiguous()):
-        raise ValueError("slots must be a contiguous int32 tensor with one entry per row")
-    _one_device(dev, lens, block_table, slots)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
             return rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots, q_norm=q_norm,
                                      k_norm=k_norm, eps=eps, out=out)
+    rows, out, n, H, D = _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out, dev)
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.get_device() != dev or block_table.stride(1) != 1:
+        raise ValueError("block_table must be an int32 [sequences, pages] tensor with contiguous rows, on the rows' GPU")
     seqs, max_pages = block_table.shape
-    table = (None if slots is None else slots.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
-             block_table.stride(0) if seqs > 1 else max_pages, seqs, max_pages)
-    st = _lib.stream(dev.index)
+    lp = _int32(lens, 1, dev, "lens", "a contiguous int32 [sequences] GPU tensor")
+    if lens.shape[0] < seqs:
+        raise ValueError(f"lens has {lens.shape[0]} entries for {seqs} sequences")
+    sp = None
+    if slots is not None:
+        sp = _int32(slots, 1, dev, "slots", "a contiguous int32 GPU tensor with one entry per row")
+        if slots.shape[0] != n:
+            raise ValueError("slots must be a contiguous int32 GPU tensor with one entry per row")
+    table = (sp, lp, block_table.data_ptr(), block_table.stride(0) if seqs > 1 else max_pages, seqs, max_pages)
+    st = _lib.stream(dev)
     if isinstance(kbuf, dict):
-        (*kp, kcap, krows), (*vp, vcap, vrows) = _flat(kbuf, n, H, D, dev, "kbuf"), _flat(vbuf, n, H, D, dev, "vbuf")
+        kp, kcap, krows, pages = _pool_args(kbuf, H, D, dev, "kbuf")
+        vp, vcap, vrows, vpages = _pool_args(vbuf, H, D, dev, "vbuf")
         arrivals = kbuf.get("arrivals")
         if arrivals is None:
             raise ValueError("kbuf has no arrival word ('arrivals', int32, zero between calls)")
-        pages = kbuf["TS"] // P
-        if vbuf["TS"] != kbuf["TS"] or kbuf["sm"].shape[0] * kbuf["sm"].shape[1] != kbuf["TS"]:
+        if vpages != pages:
             raise ValueError("kbuf and vbuf must be pools of as many pages")
         _lib.call("exkv_rope_append_paged", *rows, *kp, _lib.ptr(arrivals, 4, "arrivals"), kcap, krows, *vp, vcap, vrows,
                   *table, pages, D, st)
         return out
+    shape = kbuf.shape
     for t in (kbuf, vbuf):
-        if t.dtype != BF16 or t.dim() != 4 or t.shape[2:] != (H, D) or not t.is_contiguous() or t.shape[1] % P:
-            raise ValueError(f"kbuf and vbuf must be contiguous bf16 [1, {P} * pages, {H}, {D}] tensors")
-    _one_device(dev, kbuf, vbuf)
-    pages = kbuf.shape[0] * kbuf.shape[1] // P
-    if vbuf.shape != kbuf.shape or pages < 1:
-        raise ValueError("kbuf and vbuf must be pools of as many pages")
-    _lib.call("exkv_rope_append_paged_bf16", *rows, _lib.ptr(kbuf), _lib.ptr(vbuf), *table, pages, D, st)
+        if (t.dtype is not BF16 or t.shape != shape or len(shape) != 4 or shape[2] != H or shape[3] != D or shape[1] % P
+                or t.get_device() != dev or not t.is_contiguous()):
+            raise ValueError(f"kbuf and vbuf must be contiguous bf16 [1, {P} * pages, {H}, {D}] tensors on the rows' GPU")
+    _lib.call("exkv_rope_append_paged_bf16", *rows, _lib.ptr(kbuf), _lib.ptr(vbuf), *table, shape[0] * shape[1] // P, D, st)
     return out
-
-
-def _flat(buf, n, H, D, dev, what):
-    ptrs, cap, rows = _compressed_args(buf, n, H, D, dev, what)
-    return [*ptrs, cap, rows]
 
 
 def launch_rope_append(q, k, v, cos, sin, kc, vc, *, q_norm=None, k_norm=None, eps=1e-6, out=None):
@@ -274,17 +304,22 @@ def launch_rope_append(q, k, v, cos, sin, kc, vc, *, q_norm=None, k_norm=None, e
         kb, vb = (kc._buf(), vc._buf()) if isinstance(kc, PagedCompressedKV) else (kc.buf, vc.buf)
         return rope_append_paged(q, k, v, cos, sin, kb, vb, t.lens, t.block_table, slots, q_norm=q_norm, k_norm=k_norm,
                                  eps=eps, out=out)
-    if _elsewhere(q.device):
-        with torch.cuda.device(q.device):
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
             return launch_rope_append(q, k, v, cos, sin, kc, vc, q_norm=q_norm, k_norm=k_norm, eps=eps, out=out)
-    rows, out, n, H, D = _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out)
-    st = _lib.stream(q.device.index)
+    rows, out, n, H, D = _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out, dev)
+    if (kc.B, kc.H, kc.D, kc.TS) != (n, H, D, vc.TS) or (vc.B, vc.H, vc.D) != (n, H, D):
+        raise ValueError(f"the caches do not hold {n} sequences of {H} heads of {D}")
+    st = _lib.stream(dev)
     if isinstance(kc, CompressedKV):
-        _one_device(q.device, kc.sm, vc.sm)
+        if kc.raw.get_device() != dev or vc.raw.get_device() != dev:
+            raise ValueError("the caches must be on the rows' GPU")
         _lib.call("exkv_rope_append", *rows, *kc._ptrs(), kc.cap, kc.raw.shape[0], *vc._ptrs(), vc.cap, vc.raw.shape[0],
                   kc.TS, D, st)
     else:
-        _one_device(q.device, kc.buf, vc.buf)
+        if kc.buf.get_device() != dev or vc.buf.get_device() != dev:
+            raise ValueError("the caches must be on the rows' GPU")
         _lib.call("exkv_rope_append_bf16", *rows, _lib.ptr(kc.buf), _lib.ptr(kc.state, 4), _lib.ptr(vc.buf),
                   _lib.ptr(vc.state, 4), kc.TS, D, st)
     return out
@@ -348,61 +383,51 @@ def add_norm(x, residual, weight, *, eps=1e-6, post_weight=None, gate=None, scal
     fp32 inside; h and y are rounded once each, y from the unrounded h. Rows (the last axis)
     contiguous; x, residual and gate may have a stride between rows. With nothing to add, gate,
     norm or scale, h is x itself."""
-    if x.dim() < 1 or x.dtype != BF16 or not x.is_cuda:
+    shape, dev = x.shape, x.get_device()
+    if not shape or x.dtype is not BF16 or dev < 0:
         raise ValueError("x must be a bf16 GPU tensor [..., C]")
-    C = x.shape[-1]
+    if dev != _lib.current_device():
+        with _on(dev):
+            return add_norm(x, residual, weight, eps=eps, post_weight=post_weight, gate=gate, scale=scale)
+    C = shape[-1]
     if not 1 <= C <= 16384:
         raise ValueError(f"add_norm takes 1 to 16384 channels (got {C})")
-    dev = x.device
-    _one_device(dev, residual, weight, post_weight, gate)
-    _vec(weight, C, "weight")
-    _vec(post_weight, C, "post_weight")
-    scale = float(scale)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return add_norm(x, residual, weight, eps=eps, post_weight=post_weight, gate=gate, scale=scale)
-    xr, sx = _row_view(x, "x")
-    N = xr.shape[0]
-    rr = gr = None
+    wp, pp = _vector(weight, C, dev, "weight"), _vector(post_weight, C, dev, "post_weight")
+    if wp is None:
+        raise ValueError("add_norm needs the norm's weight")
+    xp, N, sx = _row_view(x, shape, dev, "x")
+    rp = gp = None
     sr = sg = 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != BF16:
-            raise ValueError("residual must be a bf16 tensor of x's shape")
-        rr, sr = _row_view(residual, "residual")
+        rp, _, sr = _row_view(residual, shape, dev, "residual")
     if gate is not None:
-        if gate.dtype != BF16 or (gate.shape != x.shape and gate.shape != (C,)):
-            raise ValueError(f"gate must be a bf16 tensor of x's shape or [{C}]")
-        if gate.shape == (C,) and x.dim() > 1:
-            gr = _vec(gate, C, "gate")
+        if gate.dim() == 1 and len(shape) > 1:
+            gp = _vector(gate, C, dev, "gate")
         else:
-            gr, sg = _row_view(gate, "gate")
-            gr = gr.data_ptr()
-    plain = residual is None and post_weight is None and gate is None and scale == 1.0
-    h = x if plain else torch.empty(x.shape, dtype=BF16, device=dev)
-    y = torch.empty(x.shape, dtype=BF16, device=dev)
-    _lib.call("exkv_add_norm", xr.data_ptr(), sx, None if rr is None else rr.data_ptr(), sr, weight.data_ptr(),
-              None if post_weight is None else post_weight.data_ptr(), gr, sg, scale, eps, None if plain else h.data_ptr(),
-              y.data_ptr(), N, C, _lib.stream(dev.index))
+            gp, _, sg = _row_view(gate, shape, dev, "gate")
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(shape)
+    if rp is None and pp is None and gp is None and scale == 1.0:
+        h, hp = x, None
+    else:
+        h = torch.empty_like(y)
+        hp = h.data_ptr()
+    _lib.call("exkv_add_norm", xp, sx, rp, sr, wp, pp, gp, sg, scale, eps, hp, y.data_ptr(), N, C, _lib.stream(dev))
     return h, y
 
 
-def _vec(w, C, what):
-    """Pointer of a bf16 [C] vector, or None."""
-    if w is None:
-        return None
-    if w.dtype != BF16 or w.shape != (C,) or (C > 1 and w.stride(0) != 1):
-        raise ValueError(f"{what} must be a contiguous bf16 [{C}] GPU tensor")
-    return w.data_ptr()
-
-
-def _row_view(t, what):
-    """t [..., C] as rows [N, C] and their stride."""
-    C = t.shape[-1]
+def _row_view(t, shape, dev, what):
+    """(pointer, rows, row stride) of a bf16 tensor of this shape [..., C], seen as rows."""
+    if t.dtype is not BF16 or t.shape != shape or t.get_device() != dev:
+        _bad_tensor(t, dev, what, f"a bf16 tensor of x's shape {tuple(shape)}", t.dtype is BF16 and t.shape == shape)
+    C = shape[-1]
+    n = t.numel() // C
+    if t.is_contiguous():
+        return t.data_ptr(), n, C
     if C > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: rows (the last axis) must be contiguous")
     if t.dim() != 2:
         try:
-            t = t.view(-1, C) if t.numel() else t.reshape(0, C)
+            t = t.view(-1, C)
         except RuntimeError:
             raise ValueError(f"{what}: the axes before the last must have one stride") from None
-    return t, (t.stride(0) if t.shape[0] > 1 else C)
+    return t.data_ptr(), n, (t.stride(0) if n > 1 else C)
