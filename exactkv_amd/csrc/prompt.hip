@@ -8,10 +8,11 @@
 //     out[t, h] = sum_j softmax_j(q[t, h] . k[j, h / G] / sqrt(D)) v[j, h / G],
 // and 0 where no key is visible.
 //
-// One workgroup takes 32 NW rows of one sequence and KV head, where row r is query head r % G of
-// token r / G: the G query heads of a KV head share its key and value tiles, and a tile of rows
-// spans few tokens, so little of it lies beyond the causal edge, at any G. Each wavefront owns
-// 32 rows and walks the visible keys 64 at a time:
+// One workgroup of four wavefronts takes 128 rows of one sequence and KV head, where row r is query
+// head r % G of token r / G: the G query heads of a KV head share its key and value tiles, and a tile
+// of rows spans few tokens, so little of it lies beyond the causal edge, at any G. Each wavefront owns
+// 32 rows and walks the visible keys 64 at a time (32 at head dim 256, whose registers then hold two
+// wavefronts a SIMD: 8K tokens at 16q/4kv 677 -> 546 us):
 //   S^T = K Q^T   v_mfma_f32_32x32x16_bf16, keys as rows, the wavefront's rows as columns, so a
 //                 lane holds one column (row of the tile) and half of its 64 scores: maximum and
 //                 sum are in-lane plus one exchange between the two halves of the wavefront;
@@ -21,17 +22,26 @@
 //                 of one channel per lane and read).
 // Key and value tiles arrive in LDS by direct loads (buffer_load ... lds, 16 bytes a lane; rows
 // past the sequence's end read as zeros), two stages, one barrier per tile. The 16-byte pieces of
-// a row are XOR-swizzled so that the reads of one piece over 16 or 32 rows hit every bank.
+// a row are XOR-swizzled so that the reads of one piece over 16 or 32 rows hit every bank (no bank
+// conflict counted).
+//
+// What bounds it: at 8K tokens, 32q/8kv, head dim 128, 490 us = 1,120 TFLOP/s, 0.85 of what a large
+// library product reaches here; both are held by power (1.76 GHz; the same call on zeros takes 359 us).
+// Two workgroups a CU (four at head dim 64) overlap one's matrix products with the other's
+// exponentials; one of eight wavefronts does so less (mixed prompts 79 / 68 us), three stages of keys
+// with a second barrier a tile cost more than they hide (continued prompts 78 / 93). A workgroup alone
+// on its CU needs 0.92 us a tile, of which the matrix products are 0.43.
 //
 // Numbers: scores, maxima, sums and the accumulator are fp32; the weights are rounded to bf16 for
-// the matrix product (half a step, 2^-9 of each weight, no more than the bf16 output loses).
+// the matrix product (half a step, at most 2^-8 of each weight, as the bf16 output's own rounding).
 // Weights are taken relative to a running maximum that is raised only when some score passes it
 // by 2^8 (the accumulator is then rescaled), so they stay below 256.
 //
 // Values that a row does not attend to must not reach it, also where they are infinite or NaN,
-// but the matrix product multiplies them by a weight of zero. A wavefront whose result is not
-// finite therefore computes the rows in question again, key by key over their visible keys
-// (careful_rows): what the formula gives then stands, and finite inputs never pay for it.
+// but the matrix product multiplies them by a weight of zero. A wavefront whose result is not finite
+// therefore looks through the values that some of its rows do not see, and where one of those is not
+// finite computes the rows in question again over their visible keys alone (careful_rows); so do rows
+// whose weights are all zero. What the formula gives then stands; finite results pay for none of it.
 #include "errors.hpp"
 #include "tile.hpp"
 #include "../../include/exactkv.h"
@@ -216,37 +226,78 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, i
     return false;
 }
 
-// Rows (bit c of `rows`: the wavefront's row c) computed again from their visible keys alone, one row
-// at a time with D / 64 channels a lane: the maximum first, then the sum.
+// Whether a value that some row standing at keys p_lo .. p_hi does not see, of the key tiles first ..
+// last that they walk, is infinite or NaN: only such values can have reached a row wrongly.
+template <int D, int KEYS>
+__device__ inline bool hidden_values_bad(const PromptArgs& a, const PromptTile& tile, int hk, int p_lo, int p_hi, int first, int last) {
+    constexpr int PIECES = D / 8;
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    auto scan = [&](int from, int to) {                // keys from .. to - 1
+        for (int i = lane; i < (to - from) * PIECES; i += 64) {
+            const uint4 x = ld16(a.v + (int64_t)(tile.k0 + from + i / PIECES) * a.sv_t + hk * a.sv_h + i % PIECES * 8);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= (~xs[j] & 0x7F80u) == 0 || (~xs[j] & 0x7F800000u) == 0;
+        }
+    };
+    scan(max(0, p_lo + 1), min((last + 1) * KEYS, tile.Lk));
+    if (a.window > 0) scan(first * KEYS, min(p_hi - a.window + 1, tile.Lk));
+    return __ballot(bad) != 0;
+}
+
+// Rows (bit c of `rows`: row wrow0 + c) computed again from their visible keys alone, one row at a
+// time: 64 scores at once, a lane each, for the maximum and again for the weights, then the values
+// with D / 64 channels a lane. About 1,500 cycles a row and 64 keys.
 template <int D>
 __device__ __attribute__((always_inline)) inline void careful_rows(const PromptArgs& a, const PromptTile& tile, int wrow0, int hk,
-                                                       uint32_t rows) {
+                                                                   uint32_t rows) {
     constexpr int C = D / 64;
     const int lane = threadIdx.x & 63;
-    while (rows != 0) {
+    while (rows != 0) {                                // uniform
         const int r = wrow0 + __builtin_ctz(rows);
         rows &= rows - 1;
         const int t = r / a.G, h = hk * a.G + r % a.G, p = t + tile.Lk - tile.Lq;
-        const uint16_t* q = a.q + (int64_t)(tile.q0 + t) * a.sq_t + h * a.sq_h + C * lane;
+        const uint16_t* q = a.q + (int64_t)(tile.q0 + t) * a.sq_t + h * a.sq_h;
         const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-        float m = -INFINITY, l = 0.f, o[C];
-        for (int c = 0; c < C; ++c) o[c] = 0.f;
-        for (int pass = 0; pass < 2; ++pass)
-            for (int j = first; j <= p; ++j) {
-                const uint16_t* k = a.k + (int64_t)(tile.k0 + j) * a.sk_t + hk * a.sk_h + C * lane;
-                float s = 0.f;
-                for (int c = 0; c < C; ++c) s = fmaf(bf16_float(q[c]), bf16_float(k[c]), s);
-                for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-                s *= a.qk_scale;
-                if (pass == 0) {
-                    m = s != s ? s : (m != m ? m : fmaxf(m, s));           // a NaN stays
-                } else {
-                    const uint16_t* v = a.v + (int64_t)(tile.k0 + j) * a.sv_t + hk * a.sv_h + C * lane;
-                    const float w = exp2_fast(s - m);
-                    l += w;
-                    for (int c = 0; c < C; ++c) o[c] = fmaf(w, bf16_float(v[c]), o[c]);
+        auto score = [&](int j) {                      // of key j, in log2 units
+            const uint16_t* k = a.k + (int64_t)(tile.k0 + j) * a.sk_t + hk * a.sk_h;
+            float s = 0.f;
+#pragma unroll 2
+            for (int c = 0; c < D; c += 8) {
+                const uint4 x = ld16(q + c), y = ld16(k + c);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), s);
+                    s = fmaf(__uint_as_float(xs[i] & 0xFFFF0000u), __uint_as_float(ys[i] & 0xFFFF0000u), s);
                 }
             }
+            return s * a.qk_scale;
+        };
+        float m = -INFINITY, l = 0.f, o[C];
+        bool nan = false;
+        for (int j0 = first; j0 <= p; j0 += 64) {
+            const float s = score(min(j0 + lane, p));  // the last key once more where there is none
+            nan |= s != s;
+            m = fmaxf(m, s);
+        }
+        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+        if (__ballot(nan) != 0) m = NAN;
+        for (int c = 0; c < C; ++c) o[c] = 0.f;
+        // (every weight is NaN where a score is: the first keys say so)
+        for (int j0 = first; j0 <= (m != m ? first : p); j0 += 64) {
+            const int n = min(64, p - j0 + 1);
+            const float w = lane < n ? exp2_fast(score(min(j0 + lane, p)) - m) : 0.f;
+            l += w;
+            const uint16_t* v = a.v + (int64_t)(tile.k0 + j0) * a.sv_t + hk * a.sv_h + C * lane;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const float wi = __shfl(w, i);
+                for (int c = 0; c < C; ++c) o[c] = fmaf(wi, bf16_float(v[i * a.sv_t + c]), o[c]);
+            }
+        }
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
         uint16_t* out = a.out + ((int64_t)(tile.q0 + t) * a.Hq + h) * D + C * lane;
         for (int c = 0; c < C; ++c) out[c] = __builtin_bit_cast(uint16_t, (__bf16)(p < first ? 0.f : o[c] / l));
     }
@@ -494,33 +545,18 @@ prompt_kernel(PromptArgs a, int tiles) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
                 sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_piece(st, kb, s), qf[s], sc[kb], 0, 0, 0);
-        if constexpr (PIPE) {                          // two k-steps' reads ahead of the products
-            __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB, 0);
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, KB, 0);
-            }
-        }
     };
-    auto weights = [&](const f32x16 (&sc)[KB], bf16x8 (&pf)[2 * KB]) {
-#pragma unroll
-        for (int s = 0; s < 2 * KB; ++s) {
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = exp2_fast(fmaf(sc[s >> 1][8 * (s & 1) + i], a.qk_scale, -m));
-                l += p[i];
-            }
-            const u32x4 u = {pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
-            pf[s] = __builtin_bit_cast(bf16x8, u);
-        }
+    // weights of scores 2 i, 2 i + 1 of the operand's order: dword i % 4 of operand piece i / 4
+    auto weigh = [&](const f32x16 (&sc)[KB], uint32_t (&pw)[8 * KB], int i) {
+        const int r = 8 * (i >> 2 & 1) + 2 * (i & 3);
+        const float p0 = exp2_fast(fmaf(sc[i >> 3][r], a.qk_scale, -m)), p1 = exp2_fast(fmaf(sc[i >> 3][r + 1], a.qk_scale, -m));
+        l += p0;
+        l += p1;
+        pw[i] = pack_bf16(p0, p1);
     };
-    auto values = [&](int st, const bf16x8 (&pf)[2 * KB]) {
-#pragma unroll
-        for (int s = 0; s < 2 * KB; ++s)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_piece(st, s, nb), pf[s], o[nb], 0, 0, 0);
+    auto weight_piece = [&](const uint32_t (&pw)[8 * KB], int s) {
+        const u32x4 u = {pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
+        return __builtin_bit_cast(bf16x8, u);
     };
     // every load so far has landed, and every wavefront is done with the stages loaded into next
     auto next_stage = [&] {
@@ -531,23 +567,81 @@ prompt_kernel(PromptArgs a, int tiles) {
 
     if constexpr (PIPE) {
         // One tile a step: its scores `cur` become weights and meet the values while the next tile's
-        // scores `nxt` are made, so that matrix products and exponentials of one wavefront overlap.
+        // scores `nxt` are made, and what one wavefront waits for is issued before other work: the
+        // scores' products (512 of a step's 1,024 matrix cycles) go two at a time with a piece of the
+        // loads of the tiles after (their issue costs 350 cycles on their own), half of the weights,
+        // and the first value pieces, which the products after the maximum need. A step of a
+        // workgroup alone on its CU takes 0.92 us so, 0.97 with the compiler's order.
+        constexpr int EARLY = 4 * KB, AHEAD = 2;       // weight pairs among the scores; key k-steps read ahead
         auto step = [&](int it, auto stage, f32x16 (&cur)[KB], f32x16 (&nxt)[KB]) {
             constexpr int st = decltype(stage)::value;
             const bool more = it < last;               // uniform
             next_stage();
-            if (it + 2 <= last) load_keys(st);
-            if (more) load_values(st ^ 1);
-            if (!wave_on) return;
-            bf16x8 pf[2 * KB];
+            if (!wave_on) {
+                if (more) {
+                    load_keys(st);
+                    load_values(st ^ 1);
+                }
+                return;
+            }
+            uint32_t pw[8 * KB];
             float mx = kLowest;
+            bf16x8 vf[2][NB];
             if (more) {
-                scores(st ^ 1, nxt);
+                bf16x8 kf[KS][KB];
+                each<AHEAD>([&](auto s) {
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) kf[s.value][kb] = key_piece(st ^ 1, kb, s.value);
+                });
+                each<KS>([&](auto step) {
+                    constexpr int s = decltype(step)::value;
+                    if constexpr (s + AHEAD < KS)
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb) kf[s + AHEAD][kb] = key_piece(st ^ 1, kb, s + AHEAD);
+                    if constexpr (s >= KS - 2)
+#pragma unroll
+                        for (int nb = NB / 2 * (s - KS + 2); nb < NB / 2 * (s - KS + 3); ++nb) vf[0][nb] = value_piece(st, 0, nb);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        if constexpr (s == 0)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) nxt[kb][i] = 0.f;
+                        nxt[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s][kb], qf[s], nxt[kb], 0, 0, 0);
+                    }
+                    // (past the last tile: loads of no bytes, zeros to a stage that nothing reads)
+                    if constexpr (s < LOADS) load_piece<s>(keys.buf, k_off[s], lds0 + st * TILE);
+                    if constexpr (s == LOADS - 1) keys.next();
+                    if constexpr (s >= KS - LOADS)
+                        load_piece<s - (KS - LOADS)>(vals.buf, v_off[s - (KS - LOADS)], lds0 + (2 + (st ^ 1)) * TILE);
+                    if constexpr (s == KS - 1) vals.next();
+#pragma unroll
+                    for (int i = EARLY * s / KS; i < EARLY * (s + 1) / KS; ++i) {
+                        weigh(cur, pw, i);
+                        asm volatile("" : "+v"(pw[i]), "+v"(l));     // here, not sunk to its use
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
                 hide(nxt, it + 1);
                 mx = top(nxt);
+            } else {
+#pragma unroll
+                for (int i = 0; i < EARLY; ++i) weigh(cur, pw, i);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) vf[0][nb] = value_piece(st, 0, nb);
             }
-            weights(cur, pf);
-            values(st, pf);
+#pragma unroll
+            for (int s = 0; s < 2 * KB; ++s) {
+                if (s + 1 < 2 * KB)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) vf[(s + 1) & 1][nb] = value_piece(st, s + 1, nb);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s & 1][nb], weight_piece(pw, s), o[nb], 0, 0, 0);
+                if (s + 1 < 2 * KB)
+#pragma unroll
+                    for (int i = 4 * (s + 1); i < 4 * (s + 2); ++i)
+                        if (i >= EARLY) weigh(cur, pw, i);
+            }
             raise(mx);
         };
         if (first <= last) {
@@ -584,12 +678,17 @@ prompt_kernel(PromptArgs a, int tiles) {
             const int j0 = it * KEYS;
             if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + KEYS - 1 <= w_lo - a.window)) continue;   // uniform: none seen
             f32x16 sc[KB];
-            bf16x8 pf[2 * KB];
+            uint32_t pw[8 * KB];
             scores(st, sc);
             hide(sc, it);
             raise(top(sc));
-            weights(sc, pf);
-            values(st, pf);
+#pragma unroll
+            for (int i = 0; i < 8 * KB; ++i) weigh(sc, pw, i);
+#pragma unroll
+            for (int s = 0; s < 2 * KB; ++s)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_piece(st, s, nb), weight_piece(pw, s), o[nb], 0, 0, 0);
         }
     }
 
@@ -623,7 +722,9 @@ prompt_kernel(PromptArgs a, int tiles) {
             }
             if (live) *reinterpret_cast<uint2*>(op + 32 * nb + 2 * i) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
-    const uint64_t again = __ballot(live && seen && (finite != finite || !(l > 0.f && l < INFINITY)));
+    const uint64_t empty = __ballot(live && seen && l == 0.f), odd = __ballot(live && seen && finite != finite);
+    uint64_t again = empty;
+    if (odd != 0 && hidden_values_bad<D, KEYS>(a, tile, hk, w_lo, w_hi, first, last)) again |= odd;
     if (again != 0) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // these rows' stores come first
         careful_rows<D>(a, tile, wrow0, hk, (uint32_t)again | (uint32_t)(again >> 32));
@@ -651,7 +752,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     if (parts == 1) return;
     const int nrows = tile.Lq * a.G, shift = tile.Lk - tile.Lq, row0 = tile.row0 + PER * sub, stop = min(row0 + PER, nrows);
     const int64_t stride = (int64_t)a.N * a.Hq;
-    uint32_t again = 0;                                // bit c: row row0 + c
+    uint32_t empty = 0, odd = 0;                       // bit c: row row0 + c
     for (int r0 = row0 + w * RPW; r0 < stop; r0 += 4 * RPW) {
         const int r = r0 + lane / LPR, rc = min(r, stop - 1), tok = rc / a.G;
         const int64_t row = (int64_t)(tile.q0 + tok) * a.Hq + hk * a.G + rc % a.G;
@@ -679,11 +780,17 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
         const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
         if (r < stop)
             *reinterpret_cast<uint2*>(a.out + row * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-        const uint64_t bad = __ballot(r < stop && tok + shift >= 0 && (finite != finite || !(l > 0.f && l < INFINITY)));
+        const uint64_t none = __ballot(r < stop && tok + shift >= 0 && l == 0.f);
+        const uint64_t bad = __ballot(r < stop && tok + shift >= 0 && finite != finite);
 #pragma unroll
-        for (int i = 0; i < RPW; ++i)
-            if ((bad >> (i * LPR) & (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull)) != 0) again |= 1u << (r0 + i - row0);
+        for (int i = 0; i < RPW; ++i) {
+            const uint64_t lanes = (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull) << (i * LPR);
+            if ((none & lanes) != 0) empty |= 1u << (r0 + i - row0);
+            if ((bad & lanes) != 0) odd |= 1u << (r0 + i - row0);
+        }
     }
+    uint32_t again = __builtin_amdgcn_readfirstlane(empty);
+    if (odd != 0 && hidden_values_bad<D, KEYS>(a, tile, hk, row0 / a.G + shift, (stop - 1) / a.G + shift, first, last)) again |= odd;
     if (again != 0) {                                  // uniform over the wavefront
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         careful_rows<D>(a, tile, row0, hk, again);
