@@ -869,9 +869,10 @@ extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, 
     EXKV_REQUIRE(NK == 0 || (sk_t >= D && sv_t >= D && sk_t <= (1 << 23) && sv_t <= (1 << 23)),
                  "prompt_attention: key and value rows must lie %d to %d elements apart", D, 1 << 23);
     const int64_t G = Hq / Hkv;
-    EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 &&
+    if (window > NK) window = NK;                      // no sequence is longer; sums of positions stay in 32 bits
+    EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 && (int64_t)N + 2 * (int64_t)NK < INT32_MAX - 1024 &&
                      ((int64_t)N * G / kRows + S + 1) * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX,
-                 "prompt_attention: too many rows (N=%d, %d heads per KV head, %d KV heads, S=%d)", N, (int)G, Hkv, S);
+                 "prompt_attention: too many rows (N=%d, NK=%d, %d heads per KV head, %d KV heads, S=%d)", N, NK, (int)G, Hkv, S);
     PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_t, sq_h, sk_t, sk_h,
                  sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale, 1, 0, INT32_MAX, nullptr, nullptr};
     PromptPlan p = plan_prompt(N, NK, S, Hq, Hkv, D, window);

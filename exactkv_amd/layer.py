@@ -169,7 +169,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, window=0, out=No
 
 def rotate_prompt(q, k, cos, sin, cu_seqlens, *, start=None, q_norm=None, k_norm=None, eps=1e-6):
     """A packed prompt's queries and keys rotated (half-split rotary embedding): q bf16 [N, Hq, D],
-    k bf16 [N, Hkv, D], strided views allowed, sequences as in prompt_attention; token i of
+    k bf16 [N, Hkv, D], strided views allowed (rows 4-byte aligned), sequences as in prompt_attention; token i of
     sequence s stands at position i, or start[s] + i (start: int32 [S] on the GPU), whose row of
     cos and sin (fp32 [positions, D / 2]) turns it. q_norm, k_norm (bf16 [D]): the heads are
     RMS-normed with these weights and eps first (Qwen3). Returns the two, contiguous, ready for
@@ -247,7 +247,7 @@ def _pool_args(buf, H, D, dev, what):
 def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=None, *, q_norm=None, k_norm=None,
                       eps=1e-6, out=None):
     """One token of each of n sequences into pages, the rotation on the way: q bf16 [n, Hq, D], k
-    and v bf16 [n, Hkv, D] (not rotated; strided views allowed). Row i belongs to sequence slot
+    and v bf16 [n, Hkv, D] (not rotated; strided views allowed, rows 4-byte aligned). Row i belongs to sequence slot
     slots[i] (int32 [n], distinct; default: i), which has lens[slot] tokens, this one included: its
     position, whose row of cos and sin (fp32 [positions, D / 2]) turns it, is lens[slot] - 1, and
     its page block_table[slot, position // 16] (int32). kbuf, vbuf: bf16 pools [1, 16 * pages,

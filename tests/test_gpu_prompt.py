@@ -150,6 +150,33 @@ def test_split_rows_with_bad_values(D):
     assert (err[~seen] <= 0).all()
 
 
+def test_no_keys_at_all_and_the_widest_windows():
+    q, k, v = _inputs([9], [9], 8, 2, 128, 45)
+    got = exactkv.prompt_attention(q, k[:0], v[:0], _cu([4, 5]), cu_seqlens_k=_cu([0, 0]))
+    assert (got == 0).all()
+    whole = exactkv.prompt_attention(q, k, v, _cu([9]))
+    for window in (9, 10, 1 << 30, 0x7FFFFFFF):
+        assert same_bits(exactkv.prompt_attention(q, k, v, _cu([9]), window=window), whole)
+    lens, keys = [12, 9], [5, 9]                        # queries before the first key, with a wide window
+    q, k, v = _inputs(lens, keys, 8, 2, 128, 46)
+    whole = exactkv.prompt_attention(q, k, v, _cu(lens), cu_seqlens_k=_cu(keys))
+    got = exactkv.prompt_attention(q, k, v, _cu(lens), cu_seqlens_k=_cu(keys), window=0x7FFFFFFF)
+    assert same_bits(got, whole)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_offsets_past_32_bits(D):
+    """Rows so far apart that element offsets pass 2^31, for queries, keys and values."""
+    n, pitch = 300, 1 << 23
+    q, k, v = _inputs([n], [n], 2, 1, D, 47)
+    want = exactkv.prompt_attention(q, k, v, _cu([n]))
+    wide = torch.empty(n * pitch, dtype=torch.bfloat16, device=DEV)
+    far = [wide.as_strided(t.shape, (pitch, D, 1), at) for t, at in ((q, 0), (k, 4096), (v, 8192))]
+    for dst, src in zip(far, (q, k, v)):
+        dst.copy_(src)
+    assert same_bits(exactkv.prompt_attention(*far, _cu([n])), want)
+
+
 def test_more_sequences_than_a_wavefront_scans():
     g = torch.Generator().manual_seed(5)
     lens = torch.randint(0, 9, (200,), generator=g).tolist()

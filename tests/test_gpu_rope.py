@@ -104,6 +104,24 @@ def test_rotate_prompt_strides_and_rows_behind():
     assert same_bits(got[0][:30], want[0][:30]) and (got[0][30:] == 0).all() and (got[1][30:] == 0).all()
 
 
+def test_offsets_past_32_bits():
+    """Rows so far apart that element offsets pass 2^31, whole prompts and appends."""
+    n, pitch, Hq, Hkv, D = 300, 1 << 23, 4, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(21)
+    q, k, v = _rows(g, n, Hq, D), _rows(g, n, Hkv, D), _rows(g, n, Hkv, D)
+    cos, sin = _tables(n, D)
+    wide = torch.empty(n * pitch, dtype=torch.bfloat16, device=DEV)
+    far = [wide.as_strided(t.shape, (pitch, D, 1), at) for t, at in ((q, 0), (k, 4096), (v, 8192))]
+    for dst, src in zip(far, (q, k, v)):
+        dst.copy_(src)
+    for a, b in zip(exactkv.rotate_prompt(far[0], far[1], cos, sin, _cu([n])), exactkv.rotate_prompt(q, k, cos, sin, _cu([n]))):
+        assert same_bits(a, b)
+    pair = [[exactkv.CompressedKV(n, 16, Hkv, D) for _ in range(2)] for _ in range(2)]
+    assert same_bits(exactkv.rope_append(*far, cos, sin, *pair[0]), exactkv.rope_append(q, k, v, cos, sin, *pair[1]))
+    for a, b in zip(*pair):
+        _same_cache(a, b)
+
+
 def test_positions_and_offsets_out_of_range_are_reported():
     g = torch.Generator(device=DEV).manual_seed(2)
     q, k = _rows(g, 40, 4, 128), _rows(g, 40, 2, 128)

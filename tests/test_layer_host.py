@@ -26,6 +26,7 @@ def _prompt(**kw):
     (dict(N=-1), "bad shape"), (dict(q=None), "null pointer"), (dict(v=None), "null pointer"), (dict(q=24), "aligned"),
     (dict(sk_h=100), "aligned"), (dict(sq_t=-8), "aligned"), (dict(sk_t=64), "elements apart"),
     (dict(sv_t=1 << 24), "elements apart"), (dict(N=1 << 30, Hq=64), "too many rows"), (dict(S=1 << 30), "too many rows"),
+    (dict(NK=1 << 30), "too many rows"),
 ], ids=str)
 def test_prompt_attention_arguments(kw, words):
     _fails("exkv_prompt_attention", _prompt(**kw), words)
