@@ -72,6 +72,7 @@ struct PromptArgs {
     int turn;                          // tiles from here on are taken in reverse
     float* part_o;                     // [split, N * Hq, D]
     float2* part_ml;                   // [split, N * Hq]: running maximum (log2 units), sum
+    int32_t* part_n;                   // [N * Hq]: the row's parts
 };
 
 // Two values to bf16 (nearest even): one v_cvt_pk_bf16_f32. Converted one by one they take three
@@ -166,13 +167,13 @@ __device__ inline void sequence_of(const int32_t* cu, int s, int rows, int& begi
     bad = begin != a || end != b || (s == 0 && a != 0);
 }
 
-// The tile to take `t`-th: every wavefront finds it by itself from the offsets. ORDERED: the tiles with
-// the most keys first, over up to 64 sequences (a lane each); beyond, and without, sequence by
-// sequence, each one's last tile first. The longest tiles must not start last: twelve prompts of 0 to
+// The tile to take `t`-th: every wavefront finds it by itself from the offsets. The tiles with the most
+// keys come first, over up to 64 sequences (a lane each); beyond, sequence by sequence, each one's last
+// tile first. The longest tiles must not start last: twelve prompts of 0 to
 // 1,500 tokens at 28q/4kv in their order / ordered 64.3 / 61.5 us, three at 14q/2kv with head dim 64
 // and a window of 1,024 34.9 / 31.6. `before`: the tiles of all sequences,
 // where t is past them (then false), `end` their rows' end.
-template <int ROWS, int KEYS, bool ORDERED>
+template <int ROWS, int KEYS>
 __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, int& before, int& end) {
     const int lane = threadIdx.x & 63;
     before = 0;
@@ -190,7 +191,7 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, i
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (t < before + total) {
             int l, index;
-            if (ORDERED && a.S > 1 && a.S <= 64) {
+            if (a.S > 1 && a.S <= 64) {
                 // the sequence's tiles that walk at least x key tiles: row r does if its token's key,
                 // r / G + Lk - Lq, is at least (x - 1) KEYS, and a tile if its last row does
                 auto at_least = [&](int x) {
@@ -324,12 +325,13 @@ __device__ inline void key_tiles(const PromptArgs& a, const PromptTile& tile, in
 
 // Key tiles of a part, where the keys are split: of the ways to cut the longest tile into 1 to
 // `split` parts, the one that a model of the time finds best. Lane k - 1 takes k parts; every
-// wavefront of both kernels computes it from the offsets. In steps of one tile (1.07 us with one
+// wavefront computes it from the offsets. In steps of one tile (1.07 us with one
 // workgroup on a CU): with r workgroups on every CU a step takes 0.8 r; the parts' results, written
 // and read, cost 0.04 a part at head dim 128 (64 KB each) and the second launch 3. The tiles' lengths ascend
 // evenly within a sequence, from n0 to n1, so its tiles have on average
 // (F(n1 / most) - F(n0 / most)) / (n1 / most - n0 / most) parts, F the integral of ceil.
-// Measured against no split (us): 68 rows on 32K keys 489 -> 52, 512 rows on 16K 255 -> 140.
+// Measured without / with split (us), 32q/8kv, head dim 128: 17 tokens on 32K keys 489 / 40, 512 on
+// 16K 255 / 137, 128 on 8K 128 / 38.
 __device__ inline float ceil_integral(float x) {
     const float f = floorf(x);
     return 0.5f * f * (f + 1.f) + (x - f) * (f + 1.f);
@@ -418,7 +420,7 @@ prompt_kernel(PromptArgs a, int tiles) {
     if (t >= a.turn) t = tiles - 1 - (t - a.turn);
     PromptTile tile;
     int before, end;
-    if (!find_tile<ROWS, KEYS, true>(a, t, tile, before, end)) {
+    if (!find_tile<ROWS, KEYS>(a, t, tile, before, end)) {
         if (a.zero_tail && end < a.N)
             zero_rows<D, 64 * NW>(a, end, (part * (tiles - before) + t - before) * a.Hkv + hk, (tiles - before) * a.split * a.Hkv);
         return;
@@ -436,6 +438,7 @@ prompt_kernel(PromptArgs a, int tiles) {
     key_tiles<ROWS, KEYS>(a, tile, first, last);
     const int parts = parts_of<D, ROWS, KEYS>(a, first, last);
     if (part >= parts) return;
+    if (a.split > 1 && part == 0 && half == 0 && wrow0 + col < nrows) a.part_n[(int64_t)(tile.q0 + tok) * a.Hq + hq] = parts;
     if (parts > 1) {
         const int per = (last - first + parts) / parts;
         first += part * per;
@@ -509,7 +512,6 @@ prompt_kernel(PromptArgs a, int tiles) {
     auto hide = [&](f32x16 (&sc)[KB], int it) {
         const int j0 = it * KEYS;
         if (j0 + KEYS - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window)) return;   // uniform: all seen
-        asm volatile("");
         const int rel = pos - j0 - 4 * half;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -733,67 +735,64 @@ prompt_kernel(PromptArgs a, int tiles) {
 
 // The parts of a split joined: with M the largest of a row's maxima m_i,
 //     out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
-// kMergeShare workgroups take a tile of prompt_kernel's rows. D / 4 lanes hold a row, four channels each,
-// and at first a part's maximum and sum each (hence no more parts than that); then every part's
-// factor goes to all of them, and the parts' loads do not wait for one another.
-constexpr int kMergeShare = 16;
+// D / 4 lanes hold a row, four channels each, and at first a part's maximum and sum each (hence no more
+// parts than that); then every part's factor goes to all of them, and the parts' loads do not wait for
+// one another. Rows of one part are done. Bound by the parts' reads, which the other launch has just
+// written: 813 tokens of two continued prompts 7.0 us (joined by a workgroup per four rows of a tile,
+// a row after the other, 12.5), 17 tokens on 32K keys 40 us in all (45).
 template <int D, int NW, int KEYS>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
-    constexpr int ROWS = 32 * NW, LPR = D / 4, RPW = 64 / LPR, PER = ROWS / kMergeShare;
-    const int sub = (int)blockIdx.x % kMergeShare, hk = (int)blockIdx.x / kMergeShare % a.Hkv;
-    const int t = (int)blockIdx.x / kMergeShare / a.Hkv;
+    constexpr int ROWS = 32 * NW, LPR = D / 4, RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane % LPR;
-    PromptTile tile;
-    int before, end;
-    if (!find_tile<ROWS, KEYS, false>(a, t, tile, before, end)) return;
-    int first, last;
-    key_tiles<ROWS, KEYS>(a, tile, first, last);
-    const int parts = parts_of<D, ROWS, KEYS>(a, first, last);
-    if (parts == 1) return;
-    const int nrows = tile.Lq * a.G, shift = tile.Lk - tile.Lq, row0 = tile.row0 + PER * sub, stop = min(row0 + PER, nrows);
+    const int rows = min(max(a.cu_q[a.S], 0), a.N) * a.Hq;       // of sequences
+    const int row = ((int)blockIdx.x * 4 + w) * RPW + lane / LPR, at = min(row, rows - 1);
+    const int parts = row < rows ? min(a.part_n[at], a.split) : 0;
+    if (__ballot(parts > 1) == 0) return;
     const int64_t stride = (int64_t)a.N * a.Hq;
-    uint32_t empty = 0, odd = 0;                       // bit c: row row0 + c
-    for (int r0 = row0 + w * RPW; r0 < stop; r0 += 4 * RPW) {
-        const int r = r0 + lane / LPR, rc = min(r, stop - 1), tok = rc / a.G;
-        const int64_t row = (int64_t)(tile.q0 + tok) * a.Hq + hk * a.G + rc % a.G;
-        const float2 ml = j < parts ? a.part_ml[j * stride + row] : make_float2(kLowest, 0.f);
-        float M = ml.x;
+    const float2 ml = j < parts ? a.part_ml[j * stride + at] : make_float2(kLowest, 0.f);
+    float M = ml.x;
 #pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-        const float f = exp2_fast(ml.x - M);
-        float l = ml.y * f;
+    for (int d = 1; d < LPR; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+    const float f = exp2_fast(ml.x - M);
+    float l = ml.y * f;
 #pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float* po = a.part_o + row * D + 4 * j;
+    for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* po = a.part_o + (int64_t)at * D + 4 * j;
 #pragma unroll 8
-        for (int i = 0; i < parts; ++i) {
-            const float4 x = *reinterpret_cast<const float4*>(po + i * stride * D);
-            const float fi = __shfl(f, i, LPR);
-            o.x = fmaf(x.x, fi, o.x);
-            o.y = fmaf(x.y, fi, o.y);
-            o.z = fmaf(x.z, fi, o.z);
-            o.w = fmaf(x.w, fi, o.w);
-        }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-        const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
-        if (r < stop)
-            *reinterpret_cast<uint2*>(a.out + row * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-        const uint64_t none = __ballot(r < stop && tok + shift >= 0 && l == 0.f);
-        const uint64_t bad = __ballot(r < stop && tok + shift >= 0 && finite != finite);
-#pragma unroll
-        for (int i = 0; i < RPW; ++i) {
-            const uint64_t lanes = (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull) << (i * LPR);
-            if ((none & lanes) != 0) empty |= 1u << (r0 + i - row0);
-            if ((bad & lanes) != 0) odd |= 1u << (r0 + i - row0);
-        }
+    for (int i = 0; i < parts; ++i) {                  // the lanes of a row stay together
+        const float4 x = *reinterpret_cast<const float4*>(po + i * stride * D);
+        const float fi = __shfl(f, i, LPR);
+        o.x = fmaf(x.x, fi, o.x);
+        o.y = fmaf(x.y, fi, o.y);
+        o.z = fmaf(x.z, fi, o.z);
+        o.w = fmaf(x.w, fi, o.w);
     }
-    uint32_t again = __builtin_amdgcn_readfirstlane(empty);
-    if (odd != 0 && hidden_values_bad<D, KEYS>(a, tile, hk, row0 / a.G + shift, (stop - 1) / a.G + shift, first, last)) again |= odd;
-    if (again != 0) {                                  // uniform over the wavefront
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        careful_rows<D>(a, tile, row0, hk, again);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
+    if (parts > 1)
+        *reinterpret_cast<uint2*>(a.out + (int64_t)at * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    uint64_t odd = __ballot(parts > 1 && (finite != finite || l == 0.f));
+    if (odd == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int i = 0; i < RPW; ++i) {                    // rows to look at again, one by one (uniform)
+        const uint64_t lanes = (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull) << (i * LPR);
+        if ((odd & lanes) == 0) continue;
+        const int r = __builtin_amdgcn_readlane(at, i * LPR), t = r / a.Hq, hq = r % a.Hq, hk = hq / a.G;
+        int s = 0;                                     // the sequence that holds row t
+        while (s + 1 < a.S && a.cu_q[s + 1] <= t) ++s;
+        PromptTile tile{};
+        bool bad;
+        sequence_of(a.cu_q, s, a.N, tile.q0, tile.Lq, bad);
+        sequence_of(a.cu_k, s, a.NK, tile.k0, tile.Lk, bad);
+        const int tok = t - tile.q0, p = tok + tile.Lk - tile.Lq, own = tok * a.G + hq % a.G;
+        if (tok < 0 || tok >= tile.Lq || p < 0) continue;
+        int first, last;
+        tile.row0 = own / ROWS * ROWS;
+        key_tiles<ROWS, KEYS>(a, tile, first, last);
+        const bool none = __builtin_amdgcn_readlane(__float_as_int(l), i * LPR) == 0;
+        if (none || hidden_values_bad<D, KEYS>(a, tile, hk, p, p, first, last)) careful_rows<D>(a, tile, own, hk, 1u);
     }
 }
 
@@ -803,7 +802,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
 constexpr int kRows = 128, kWaves = 4;
 constexpr int keys_per_tile(int D) { return D == 256 ? 32 : 64; }
 // Two workgroups a CU in one go: the second ones in reverse, so that a CU's two tiles add up to about
-// the same.
+// the same (one prompt of 1,500 tokens 32.7 us without, 31.4 so; of 2,048 no difference).
 struct PromptPlan {
     int64_t tiles;                     // row tiles, at most
     int split, slots, turn;
@@ -817,6 +816,7 @@ static PromptPlan plan_prompt(int64_t N, int64_t NK, int64_t S, int64_t Hq, int6
         if (units > 256 && units <= 512) p.turn = (int)((256 + Hkv - 1) / Hkv);
         return p;
     }
+    if (S == 0) return p;
     int64_t split = 2 * p.slots / units;
     if (split > D / 4) split = D / 4;
     if (split > keys / kLeast) split = keys / kLeast;
@@ -824,13 +824,21 @@ static PromptPlan plan_prompt(int64_t N, int64_t NK, int64_t S, int64_t Hq, int6
     return p;
 }
 
+static int64_t workspace_bytes(const PromptPlan& p, int64_t N, int64_t Hq, int64_t D) {
+    return (p.split * (D + 2) + 1) * N * Hq * 4;
+}
+
+// WPE wavefronts a SIMD, PIPE the next tile's scores beside this tile's weights. At head dim 64 four and
+// no PIPE (8K tokens, 32q/8kv: 287 us; two and no PIPE 330), at 128 the registers of the second scores
+// leave two (500 us; without PIPE 533), at 256 they would not fit.
 template <int D, int WPE, bool PIPE>
 static void launch_prompt(const PromptArgs& a, int64_t tiles, hipStream_t stream) {
     constexpr int KEYS = keys_per_tile(D);
     hipLaunchKernelGGL((prompt_kernel<D, kWaves, KEYS, WPE, PIPE>), dim3((unsigned)(tiles * a.split * a.Hkv)), dim3(64 * kWaves), 0,
                        stream, a, (int)tiles);
     if (a.split > 1)
-        hipLaunchKernelGGL((prompt_merge_kernel<D, kWaves, KEYS>), dim3((unsigned)(kMergeShare * tiles * a.Hkv)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((prompt_merge_kernel<D, kWaves, KEYS>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
+                           0, stream, a);
 }
 
 hipError_t fetch_errors_prompt(uint32_t* out, int first, int clear, hipStream_t stream) {
@@ -848,7 +856,7 @@ static bool rows_ok(const void* p, int64_t s_t, int64_t s_h) {
 extern "C" int64_t exkv_prompt_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window) {
     if (!head_dim_ok(D) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || S < 0 || N <= 0 || NK <= 0 || window < 0) return 0;
     const PromptPlan p = plan_prompt(N, NK, S, Hq, Hkv, D, window);
-    return p.split > 1 ? (int64_t)p.split * N * Hq * (D + 2) * 4 : 0;
+    return p.split > 1 ? workspace_bytes(p, N, Hq, D) : 0;
 }
 
 extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
@@ -874,16 +882,17 @@ extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, 
                      ((int64_t)N * G / kRows + S + 1) * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX,
                  "prompt_attention: too many rows (N=%d, NK=%d, %d heads per KV head, %d KV heads, S=%d)", N, NK, (int)G, Hkv, S);
     PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_t, sq_h, sk_t, sk_h,
-                 sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale, 1, 0, INT32_MAX, nullptr, nullptr};
+                 sv_t, sv_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, zero_tail, qk_scale, 1, 0, INT32_MAX, nullptr, nullptr, nullptr};
     PromptPlan p = plan_prompt(N, NK, S, Hq, Hkv, D, window);
     if (ws != nullptr && p.split > 1) {
-        const int64_t rows = (int64_t)p.split * N * Hq;
-        EXKV_REQUIRE((uintptr_t)ws % 16 == 0 && ws_bytes >= rows * (D + 2) * 4, "prompt_attention: workspace of %lld bytes, %lld needed",
-                     (long long)ws_bytes, (long long)(rows * (D + 2) * 4));
+        const int64_t rows = (int64_t)p.split * N * Hq, need = workspace_bytes(p, N, Hq, D);
+        EXKV_REQUIRE((uintptr_t)ws % 16 == 0 && ws_bytes >= need, "prompt_attention: workspace of %lld bytes, %lld needed",
+                     (long long)ws_bytes, (long long)need);
         a.split = p.split;
         a.slots = p.slots;
         a.part_o = (float*)ws;
         a.part_ml = (float2*)((float*)ws + rows * D);
+        a.part_n = (int32_t*)(a.part_ml + rows);
     }
     a.turn = p.turn;
     if (D == 64)

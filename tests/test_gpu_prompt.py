@@ -150,6 +150,16 @@ def test_split_rows_with_bad_values(D):
     assert (err[~seen] <= 0).all()
 
 
+def test_split_rows_without_a_finite_score():
+    q, k, v = _inputs([5], [2000], 1, 1, 64, 44)
+    q[:] = 1.0
+    k[:] = -math.inf
+    assert exactkv.prompt_attention(q, k, v, _cu([5]), cu_seqlens_k=_cu([2000])).isnan().all()
+    k[1997] = 0.25                                     # the third query's own token
+    got = exactkv.prompt_attention(q, k, v, _cu([5]), cu_seqlens_k=_cu([2000]))
+    assert got[:2].isnan().all() and same_bits(got[2:], v[1997:1998].expand(3, 1, 64).contiguous())
+
+
 def test_no_keys_at_all_and_the_widest_windows():
     q, k, v = _inputs([9], [9], 8, 2, 128, 45)
     got = exactkv.prompt_attention(q, k[:0], v[:0], _cu([4, 5]), cu_seqlens_k=_cu([0, 0]))
