@@ -8,9 +8,14 @@
 // bf16 rows in and out, fp32 between; h and y are rounded once each (y from the unrounded h).
 // No kernel of the reference (its model's own modules do this, engine.py:75-91).
 //
-// Bound by HBM: x, r and a row-wise gate are read once, h and y written once. One workgroup of
-// 64 WAVES threads holds a row in registers, eight channels a thread and piece, CH pieces; the
-// two sums go through the wavefront's lanes and, with several wavefronts, through LDS.
+// Bound by HBM: x, r and a row-wise gate are read once, h and y written once (8191 rows of 3584 with a
+// norm behind the block and a gate as large: 56 us, 5.2 TB/s; 8191 of 4,096 with neither 40 us, 6.7 TB/s;
+// 621 4.9; one 2.7, which is the launch and one round trip).
+// One workgroup of 64 WAVES threads holds a row in registers, eight channels a thread and piece, CH
+// pieces; the two sums go through the wavefront's lanes and, with several wavefronts, through LDS.
+// Rows that do not lie at whole 16 bytes (V16 false) go by the same pieces wherever they lie, as the
+// hardware allows, but for a partial last one: 8191 rows of 4,096 41 us (channel by channel 134), of
+// 4,095 57.
 #include "rope.hpp"
 #include "../../include/exactkv.h"
 
@@ -42,13 +47,16 @@ __device__ inline float block_total(float x, float* s) {
     return x;
 }
 
-// Eight channels of a row from channel c0 on (V16: one 16-byte piece, all of it in the row; else
-// one by one, those past C as zeros).
+// Eight channels of a row from channel c0 on: one 16-byte piece, which need not lie at 16 bytes unless
+// V16; then a row's last piece may be partial as well, and goes one by one, channels past C as zeros.
 template <bool V16>
 __device__ inline void load8(const uint16_t* row, int c0, int C, float (&v)[8]) {
-    if constexpr (V16) {
+    if (V16 || c0 + 8 <= C) {
         uint32_t u[4];
-        ld_words<4>(row + c0, u);
+        if constexpr (V16)
+            ld_words<4>(row + c0, u);
+        else
+            __builtin_memcpy(u, row + c0, 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[2 * i] = lo_float(u[i]);
@@ -61,11 +69,14 @@ __device__ inline void load8(const uint16_t* row, int c0, int C, float (&v)[8]) 
 }
 template <bool V16>
 __device__ inline void store8(uint16_t* row, int c0, int C, const float (&v)[8]) {
-    if constexpr (V16) {
+    if (V16 || c0 + 8 <= C) {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-        st_words<4>(row + c0, u);
+        if constexpr (V16)
+            st_words<4>(row + c0, u);
+        else
+            __builtin_memcpy(row + c0, u, 16);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -165,17 +176,21 @@ extern "C" int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t s
                      (const uint16_t*)gate, sx, r ? sr : 0, gate ? sg : 0, (uint16_t*)h, (uint16_t*)y, eps, scale, N, C};
     const bool v16 = (((uintptr_t)x | (uintptr_t)r | (uintptr_t)w | (uintptr_t)post_w | (uintptr_t)gate | (uintptr_t)h |
                        (uintptr_t)y) % 16 == 0) && C % 8 == 0 && sx % 8 == 0 && a.sr % 8 == 0 && a.sg % 8 == 0;
+    // one piece a thread while a workgroup's 1024 threads can hold the row so; us for 1, 621 and 8191
+    // rows, this / half the wavefronts with two pieces: 1,024 channels 2.1, 2.7, 11.9 / 2.6, 3.3, 10.7;
+    // 4,096 2.3, 4.6, 39.5 / 2.9, 5.0, 40.4; 8,192 2.6, 7.7, 91.0 / 3.1, 7.3, 94.7; 16,384 (two pieces
+    // / four) 3.6, 14.3, 182 / 4.4, 13.9, 197
     if (C <= 512)
         launch_norm<1, 1>(a, v16, stream);
     else if (C <= 1024)
-        launch_norm<1, 2>(a, v16, stream);
+        launch_norm<2, 1>(a, v16, stream);
     else if (C <= 2048)
         launch_norm<4, 1>(a, v16, stream);
     else if (C <= 4096)
-        launch_norm<4, 2>(a, v16, stream);
+        launch_norm<8, 1>(a, v16, stream);
     else if (C <= 8192)
-        launch_norm<4, 4>(a, v16, stream);
+        launch_norm<16, 1>(a, v16, stream);
     else
-        launch_norm<8, 4>(a, v16, stream);
+        launch_norm<16, 2>(a, v16, stream);
     return hip_status(hipGetLastError(), "add_norm");
 }
