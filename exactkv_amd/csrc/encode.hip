@@ -1341,7 +1341,8 @@ __global__ void __launch_bounds__(256) paged_bf16_append_kernel(PagedAppendArgs 
 // those of the two appends above given the rotated keys.
 //
 // D / 16 lanes hold a row and a thread takes at most a few rows, so an ordinary step is one round
-// trip (length, table row and token rows) and its stores: bound by those and the launch.
+// trip (length, table row and token rows) and its stores: bound by those and the launch. 32q/8kv, head
+// dim 128: one token 2.6 us, 128 into compressed pages 5.1, into bf16 pages 2.6 (launch after launch).
 //
 // Compressed caches at a page end: a block stores its rows, key and value rows of tokens that
 // fill a page device-coherently, waits for them, and its wavefronts encode those units' pages (all
@@ -1392,6 +1393,8 @@ __device__ inline void store_row16_dev(uint16_t* row, int g, const uint32_t (&u)
     }
 }
 
+// bf16 pages want no block that waits for others: us for 1, 128 and 512 tokens with 64 / 256 / 1024
+// threads 2.1, 2.5, 3.7 / 2.1, 2.6, 3.6 / 2.3, 3.2, 3.9. The others share the append's block.
 constexpr int kRopeBf16Threads = 256;
 constexpr int rope_threads(int kind) { return kind == kPagedBf16 ? kRopeBf16Threads : kAppendThreads; }
 
