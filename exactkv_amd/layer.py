@@ -12,7 +12,8 @@ way into the caches, and the residual stream with its norms.
 No counterpart in the reference, whose engine leaves all of this to the model's own modules
 (exactkv/engine.py:42-49,75-91). Everything is bf16 in and out and fp32 inside, rounded once.
 The tensors of a call are on one GPU; the work goes to that GPU's current stream, allocates
-nothing but the outputs, waits for nothing, and can be captured in a HIP graph.
+nothing but the outputs (and a split prompt's partial results), waits for nothing, and can be
+captured in a HIP graph. No gradients are recorded.
 """
 import operator
 
