@@ -58,6 +58,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -1e30f;      // the running maximum before any key, in log2 units
+constexpr int kRows = 128, kWaves = 4;   // query rows and wavefronts of a workgroup
 constexpr float kRaise = 8.f;          // a score this far above the running maximum raises it
 
 struct PromptArgs {
@@ -171,13 +172,11 @@ __device__ inline void sequence_of(const int32_t* cu, int s, int rows, int& begi
 // keys come first, over up to 64 sequences (a lane each); beyond, sequence by sequence, each one's last
 // tile first. The longest tiles must not start last: twelve prompts of 0 to
 // 1,500 tokens at 28q/4kv in their order / ordered 64.3 / 61.5 us, three at 14q/2kv with head dim 64
-// and a window of 1,024 34.9 / 31.6. `before`: the tiles of all sequences,
-// where t is past them (then false), `end` their rows' end.
+// and a window of 1,024 34.9 / 31.6. False where t is past the tiles of all sequences.
 template <int ROWS, int KEYS>
-__device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, int& before, int& end) {
+__device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile) {
     const int lane = threadIdx.x & 63;
-    before = 0;
-    end = 0;
+    int before = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         int begin = 0, len = 0, begin_k = 0, len_k = 0;
         bool bad = false, bad_k = false;
@@ -222,7 +221,6 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile, i
             return true;
         }
         before += total;
-        end = __builtin_amdgcn_readlane(begin + len, min(63, a.S - 1 - s0));
     }
     return false;
 }
@@ -323,20 +321,24 @@ __device__ inline void key_tiles(const PromptArgs& a, const PromptTile& tile, in
     last = k_hi < 0 ? first - 1 : k_hi / KEYS;
 }
 
-// Key tiles of a part, where the keys are split: of the ways to cut the longest tile into 1 to
-// `split` parts, the one that a model of the time finds best. Lane k - 1 takes k parts; every
-// wavefront computes it from the offsets. In steps of one tile (1.07 us with one
-// workgroup on a CU): with r workgroups on every CU a step takes 0.8 r; the parts' results, written
-// and read, cost 0.04 a part at head dim 128 (64 KB each) and the second launch 3. The tiles' lengths ascend
-// evenly within a sequence, from n0 to n1, so its tiles have on average
-// (F(n1 / most) - F(n0 / most)) / (n1 / most - n0 / most) parts, F the integral of ceil.
-// Measured without / with split (us), 32q/8kv, head dim 128: 17 tokens on 32K keys 489 / 40, 512 on
-// 16K 255 / 137, 128 on 8K 128 / 38.
+// Which row tile and part of its keys a workgroup takes where the keys are split (t: the workgroup's
+// number of its KV head). Of the ways to cut the longest row tile into 1 to `split` parts it takes the
+// one that a model of the time finds best, and `most` are then the key tiles of a part; a row tile of n
+// key tiles has ceil(n / most). Lane k - 1 models k parts, in steps of one key tile (1.07 us with one
+// workgroup on a CU): with r workgroups on every CU a step takes 0.8 r; parts that find no place at once
+// wait for half a part on average; a part's results, written and read, cost 0.02 and 0.02 more per 128
+// channels, and the second launch 3. The tiles' lengths ascend evenly within a sequence, from n0 to n1,
+// so its tiles have on average (F(n1 / most) - F(n0 / most)) / (n1 / most - n0 / most) parts, F the
+// integral of ceil. Every wavefront computes this from the offsets. Then lane p counts the row tiles that
+// have a part p, exactly: all first parts come first, then all second ones and so on, without gaps, since
+// workgroups that have nothing to do take every second CU's place, or half the XCDs, from those that do
+// (128 tokens on 8K keys 37.7 us with gaps, 31.5 so).
+// Measured without / with split (us), 32q/8kv, head dim 128: 17 tokens on 32K keys 489 / 36, 512 on
+// 16K 255 / 141, 128 on 8K 128 / 31.5.
 __device__ inline float ceil_integral(float x) {
     const float f = floorf(x);
     return 0.5f * f * (f + 1.f) + (x - f) * (f + 1.f);
 }
-constexpr int kLeast = 8;                              // tiles of keys a split call has, per part
 template <int N>
 __device__ inline float ror(float x) {                 // lane i of a 16-lane row: lane (i - N) % 16 of it
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, false));
@@ -352,60 +354,68 @@ __device__ inline float wave_least(float x) {
     return fminf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 template <int D, int ROWS, int KEYS>
-__device__ inline int tiles_per_part(const PromptArgs& a) {
+__device__ inline bool find_part(const PromptArgs& a, int limit, int& t, int& part, int& most) {
     const int lane = threadIdx.x & 63, k = lane + 1, span = (ROWS - 1) / a.G;
-    // lane's sequence: its row tiles, key tiles of the first and of the last one
-    auto lengths = [&](int s, int& tiles, int& n0, int& n1) {
-        int q0, k0, Lq = 0, Lk = 0;
-        bool bad;
-        if (s < a.S) {
-            sequence_of(a.cu_q, s, a.N, q0, Lq, bad);
-            sequence_of(a.cu_k, s, a.NK, k0, Lk, bad);
-        }
-        tiles = (Lq * a.G + ROWS - 1) / ROWS;
-        auto walked = [&](int t_hi) {
-            const int keys = max(0, t_hi + Lk - Lq + 1), window = a.window > 0 ? min(a.window, a.NK) + span : keys;
-            return (min(keys, window) + KEYS - 1) / KEYS;
-        };
-        n0 = walked(min(span, Lq - 1));
-        n1 = walked(Lq - 1);
+    // the lane's sequence (there are at most 64): its row tiles, key tiles of the first and of the last one
+    int q0, k0, Lq = 0, Lk = 0;
+    bool bad = false, bad_k = false;
+    if (lane < a.S) {
+        sequence_of(a.cu_q, lane, a.N, q0, Lq, bad);
+        sequence_of(a.cu_k, lane, a.NK, k0, Lk, bad_k);
+    }
+    if (bad || bad_k) report_error(kErrOffsets);
+    const int tiles = (Lq * a.G + ROWS - 1) / ROWS;
+    auto walked = [&](int t_hi) {                      // at most (a window may begin and end within a tile)
+        const int keys = max(0, t_hi + Lk - Lq + 1), n = (keys + KEYS - 1) / KEYS;
+        return a.window > 0 ? min(n, (a.window + span + 2 * KEYS - 2) / KEYS) : n;
     };
-    int tiles, n0, n1;
-    float far = 1.f;
-    for (int s0 = 0; s0 < a.S; s0 += 64) {
-        lengths(s0 + lane, tiles, n0, n1);
-        far = fmaxf(far, tiles > 0 ? (float)max(n0, n1) : 0.f);
-    }
-    const int longest = (int)-wave_least(-far), most = (longest + k - 1) / k;
+    const int n0 = walked(min(span, Lq - 1)), n1 = walked(Lq - 1);
+    const float far = -wave_least(-(tiles > 0 ? (float)max(1, max(n0, n1)) : 1.f));
+    const int longest = __builtin_amdgcn_readfirstlane((int)far);
+    most = (longest + k - 1) / k;
     const float per = 1.f / (float)most;
-    float parts = 0.f;
-    for (int s0 = 0; s0 < a.S; s0 += 64) {
-        if (a.S > 64) lengths(s0 + lane, tiles, n0, n1);
-        for (int i = 0; i < min(64, a.S - s0); ++i) {
-            const int t = __builtin_amdgcn_readlane(tiles, i), m0 = __builtin_amdgcn_readlane(n0, i), m1 = __builtin_amdgcn_readlane(n1, i);
-            const float x0 = (float)min(m0, m1) * per, x1 = (float)max(m0, m1) * per;
-            parts += (float)t * (x1 - x0 < 0.01f ? ceilf(x1 - 1e-4f) : (ceil_integral(x1) - ceil_integral(x0)) / (x1 - x0));
-        }
+    float model = 0.f, steps = 0.f;
+    for (int i = 0; i < a.S; ++i) {
+        const int n = __builtin_amdgcn_readlane(tiles, i), m0 = __builtin_amdgcn_readlane(n0, i), m1 = __builtin_amdgcn_readlane(n1, i);
+        const float x0 = (float)min(m0, m1) * per, x1 = (float)max(m0, m1) * per;
+        steps += 0.5f * (float)n * (float)(m0 + m1);
+        model += (float)n * (x1 - x0 < 0.01f ? ceilf(x1 - 1e-4f) : (ceil_integral(x1) - ceil_integral(x0)) / (x1 - x0));
     }
-    parts = ceilf(parts - 0.01f) * (float)a.Hkv;
-    const float slots = (float)a.slots, side = ceilf(fminf(parts, slots) * (1.f / 256.f));
-    float time = ceilf(parts / slots) * (float)most * (side <= 1.f ? 1.07f : 0.8f * side);
-    if (k > 1) time += 3.f + 0.04f / 128.f * D * parts;
-    if (k > a.split) time = INFINITY;
-    return __builtin_amdgcn_readlane(most, __builtin_ctzll(__ballot(time == wave_least(time))));
-}
-
-// Into how many parts the key tiles first .. last are split.
-template <int D, int ROWS, int KEYS>
-__device__ inline int parts_of(const PromptArgs& a, int first, int last) {
-    if (a.split == 1) return 1;                        // uniform
-    const int most = tiles_per_part<D, ROWS, KEYS>(a);
-    return max(1, (last - first + most) / most);
+    model = ceilf(model - 0.01f) * (float)a.Hkv;
+    const float slots = (float)a.slots, side = ceilf(fminf(model, slots) * (1.f / 256.f));
+    float time = (float)most;
+    if (model > slots + 1.f) time = fmaxf(time, steps * (float)a.Hkv / slots + 0.5f * time);
+    time *= side <= 1.f ? 1.07f : 0.8f * side;
+    if (k > 1) time += 3.f + (0.02f + 0.02f / 128.f * D) * model;
+    if (k > a.split || (k > 1 && model > (float)(limit * a.Hkv))) time = INFINITY;
+    most = __builtin_amdgcn_readlane(most, __builtin_ctzll(__ballot(time == wave_least(time))));
+    // row tiles with a part `lane`: with a window all of them, where any has (some parts are then empty)
+    int all = 0, count = 0;
+    for (int i = 0; i < a.S; ++i) {
+        const int n = __builtin_amdgcn_readlane(tiles, i), lq = __builtin_amdgcn_readlane(Lq, i), lk = __builtin_amdgcn_readlane(Lk, i);
+        // the first row whose key lies in that part
+        const int64_t row = ((int64_t)lane * most * KEYS - (lk - lq)) * a.G;
+        count += row >= (int64_t)lq * a.G ? 0 : n - (row > 0 ? (int)(row / ROWS) : 0);
+        all += n;
+    }
+    if (lane == 0 || (a.window > 0 && lane < (longest + most - 1) / most)) count = all;
+    else if (a.window > 0) count = 0;
+    int upto = wave_incl_scan(count);
+    if (__builtin_amdgcn_readlane(upto, 63) > limit) { // more than the model thought: no split
+        most = longest;
+        count = lane == 0 ? all : 0;
+        upto = all;
+    }
+    if (t >= __builtin_amdgcn_readlane(upto, 63)) return false;
+    part = __builtin_ctzll(__ballot(upto > t));
+    t -= __builtin_amdgcn_readlane(upto - count, part);
+    return true;
 }
 
 template <int D, int NW, int KEYS, int WPE, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 prompt_kernel(PromptArgs a, int tiles) {
+    constexpr bool CUTS = D < 256 || PIPE;                       // (the other instance never splits keys)
     constexpr int KB = KEYS / 32;                                // 32-key blocks of a tile
     constexpr int ROWS = 32 * NW, KS = D / 16, NB = D / 32;      // rows, score k-steps, 32-channel blocks
     constexpr int PIECES = D / 8, RPI = 64 / PIECES;             // 16-byte pieces of a row, rows per load
@@ -413,18 +423,20 @@ prompt_kernel(PromptArgs a, int tiles) {
     static_assert(TILE % (1024 * NW) == 0, "whole loads");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];     // two key stages, then two value stages
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    // first parts first: a tile that has fewer leaves workgroups that end at once, and between the
-    // others those would take every second CU's slot as the grid is handed out
-    const int hk = (int)blockIdx.x % a.Hkv, part = (int)blockIdx.x / a.Hkv / tiles;
-    int t = (int)blockIdx.x / a.Hkv % tiles;
-    if (t >= a.turn) t = tiles - 1 - (t - a.turn);
+    const int hk = (int)blockIdx.x % a.Hkv;
+    int t = (int)blockIdx.x / a.Hkv, part = 0, most = 0;
+    bool found = true;
+    if (CUTS && a.split > 1)                           // uniform
+        found = find_part<D, ROWS, KEYS>(a, (int)gridDim.x / a.Hkv, t, part, most);
+    else if (t >= a.turn)
+        t = tiles - 1 - (t - a.turn);
     PromptTile tile;
-    int before, end;
-    if (!find_tile<ROWS, KEYS>(a, t, tile, before, end)) {
-        if (a.zero_tail && end < a.N)
-            zero_rows<D, 64 * NW>(a, end, (part * (tiles - before) + t - before) * a.Hkv + hk, (tiles - before) * a.split * a.Hkv);
-        return;
+    found = found && find_tile<ROWS, KEYS>(a, t, tile);
+    if (a.zero_tail) {
+        const int end = a.S > 0 ? min(max(a.cu_q[a.S], 0), a.N) : 0;
+        if (end < a.N) zero_rows<D, 64 * NW>(a, end, (int)blockIdx.x, (int)gridDim.x);
     }
+    if (!found) return;
     // the lane's row
     const int col = lane & 31, half = lane >> 5, G = a.G, nrows = tile.Lq * G;
     const int wrow0 = tile.row0 + 32 * w, row = min(wrow0 + col, nrows - 1);
@@ -436,9 +448,9 @@ prompt_kernel(PromptArgs a, int tiles) {
     const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
     int first, last;
     key_tiles<ROWS, KEYS>(a, tile, first, last);
-    const int parts = parts_of<D, ROWS, KEYS>(a, first, last);
+    const int parts = CUTS && a.split > 1 ? max(1, (last - first + most) / most) : 1;
     if (part >= parts) return;
-    if (a.split > 1 && part == 0 && half == 0 && wrow0 + col < nrows) a.part_n[(int64_t)(tile.q0 + tok) * a.Hq + hq] = parts;
+    if (CUTS && a.split > 1 && part == 0 && half == 0 && wrow0 + col < nrows) a.part_n[(int64_t)(tile.q0 + tok) * a.Hq + hq] = parts;
     if (parts > 1) {
         const int per = (last - first + parts) / parts;
         first += part * per;
@@ -739,7 +751,7 @@ prompt_kernel(PromptArgs a, int tiles) {
 // parts than that); then every part's factor goes to all of them, and the parts' loads do not wait for
 // one another. Rows of one part are done. Bound by the parts' reads, which the other launch has just
 // written: 813 tokens of two continued prompts 7.0 us (joined by a workgroup per four rows of a tile,
-// a row after the other, 12.5), 17 tokens on 32K keys 40 us in all (45).
+// a row after the other, 12.5).
 template <int D, int NW, int KEYS>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     constexpr int ROWS = 32 * NW, LPR = D / 4, RPW = 64 / LPR;
@@ -796,31 +808,43 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     }
 }
 
-// How a call is laid out. Keys are split where the row tiles give no CU two workgroups, the number
-// that it runs at a time at least: into up to twice the parts that fill the slots (a call's tiles
-// differ in length; tiles_per_part says how many are used).
-constexpr int kRows = 128, kWaves = 4;
+// How a call is laid out. `slots` workgroups run at a time: two a CU (four at head dim 64). Keys are
+// split where the row tiles leave CUs free and are long enough for what the parts' results cost.
+//
+// Head dim 256 has two instances: one workgroup a CU, with the next tile's scores beside this tile's
+// weights (1.05 us a step), and two without (1.35 us alone, 0.96 together). The former where no CU gets
+// more than two: one / two a CU, 16q/4kv, 2K tokens 72 / 92 us, 3,000 101 / 131, 4K 155 / 190, but 6,000
+// 337 / 312, 8K 563 / 491.
 constexpr int keys_per_tile(int D) { return D == 256 ? 32 : 64; }
-// Two workgroups a CU in one go: the second ones in reverse, so that a CU's two tiles add up to about
-// the same (one prompt of 1,500 tokens 32.7 us without, 31.4 so; of 2,048 no difference).
+constexpr int kLeast = 8;              // key tiles of the longest row tile, per part, at least
 struct PromptPlan {
     int64_t tiles;                     // row tiles, at most
-    int split, slots, turn;
+    int split, slots;
+    int turn;                          // two workgroups a CU in one go: the second ones in reverse, so that a
+                                       // CU's two tiles add up to about the same (one prompt of 1,500
+                                       // tokens 32.7 us without, 31.4 so; of 2,048 no difference)
+    bool alone;                        // head dim 256: one workgroup a CU
+    int64_t blocks;                    // workgroups of a KV head
 };
 static PromptPlan plan_prompt(int64_t N, int64_t NK, int64_t S, int64_t Hq, int64_t Hkv, int D, int64_t window) {
-    // every sequence's last tile may be partial, and one more for rows behind the last sequence
-    PromptPlan p{N * (Hq / Hkv) / kRows + S + 1, 1, D == 64 ? 1024 : 512, INT32_MAX};
+    // every sequence's last tile may be partial
+    const int64_t tiles = (N * (Hq / Hkv) + S * (kRows - 1)) / kRows, units = (tiles > 0 ? tiles : 1) * Hkv;
+    PromptPlan p{units / Hkv, 1, D == 64 ? 1024 : 512, INT32_MAX, D == 256 && units <= 512, units / Hkv};
+    if (p.alone) p.slots = 256;
     const int64_t reach = window > 0 && window + kRows < NK ? window + kRows : NK;
-    const int64_t keys = (reach + keys_per_tile(D) - 1) / keys_per_tile(D), units = p.tiles * Hkv;
-    if (2 * units > p.slots) {
-        if (units > 256 && units <= 512) p.turn = (int)((256 + Hkv - 1) / Hkv);
+    const int64_t keys = (reach + keys_per_tile(D) - 1) / keys_per_tile(D), few = D == 64 ? 512 : 256;
+    if (units >= few || S > 64 || S == 0 || 25 * keys < 150 + units * D / 64) {
+        if (!p.alone && units > 256 && units <= 512) p.turn = (int)((256 + Hkv - 1) / Hkv);
         return p;
     }
-    if (S == 0) return p;
-    int64_t split = 2 * p.slots / units;
+    int64_t split = 4 * few / units;
     if (split > D / 4) split = D / 4;
     if (split > keys / kLeast) split = keys / kLeast;
-    if (split > 1) p.split = (int)split;
+    if (split > 1) {
+        const int64_t most = (p.slots + p.slots / (p.alone ? 2 : 8)) / Hkv;
+        p.split = (int)split;
+        p.blocks = p.tiles * split < most ? p.tiles * split : most > p.tiles ? most : p.tiles;
+    }
     return p;
 }
 
@@ -830,12 +854,13 @@ static int64_t workspace_bytes(const PromptPlan& p, int64_t N, int64_t Hq, int64
 
 // WPE wavefronts a SIMD, PIPE the next tile's scores beside this tile's weights. At head dim 64 four and
 // no PIPE (8K tokens, 32q/8kv: 287 us; two and no PIPE 330), at 128 the registers of the second scores
-// leave two (500 us; without PIPE 533), at 256 they would not fit.
+// leave two (500 us; without PIPE 533), at 256 one (PromptPlan).
 template <int D, int WPE, bool PIPE>
-static void launch_prompt(const PromptArgs& a, int64_t tiles, hipStream_t stream) {
+static void launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t stream) {
     constexpr int KEYS = keys_per_tile(D);
-    hipLaunchKernelGGL((prompt_kernel<D, kWaves, KEYS, WPE, PIPE>), dim3((unsigned)(tiles * a.split * a.Hkv)), dim3(64 * kWaves), 0,
-                       stream, a, (int)tiles);
+    const int64_t blocks = a.split > 1 ? p.blocks : p.tiles;
+    hipLaunchKernelGGL((prompt_kernel<D, kWaves, KEYS, WPE, PIPE>), dim3((unsigned)(blocks * a.Hkv)), dim3(64 * kWaves), 0, stream, a,
+                       (int)p.tiles);
     if (a.split > 1)
         hipLaunchKernelGGL((prompt_merge_kernel<D, kWaves, KEYS>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
                            0, stream, a);
@@ -896,10 +921,12 @@ extern "C" int exkv_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, 
     }
     a.turn = p.turn;
     if (D == 64)
-        launch_prompt<64, 4, false>(a, p.tiles, stream);
+        launch_prompt<64, 4, false>(a, p, stream);
     else if (D == 128)
-        launch_prompt<128, 2, true>(a, p.tiles, stream);
+        launch_prompt<128, 2, true>(a, p, stream);
+    else if (p.alone)
+        launch_prompt<256, 1, true>(a, p, stream);
     else
-        launch_prompt<256, 2, false>(a, p.tiles, stream);
+        launch_prompt<256, 2, false>(a, p, stream);
     return hip_status(hipGetLastError(), "prompt_attention");
 }

@@ -135,6 +135,28 @@ def test_few_rows_split_their_keys(lens, keys, Hq, Hkv, window, D):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (2, 2)])
+@pytest.mark.parametrize("window", [897, 961, 993, 1024, 1090, 1921, 2017])
+def test_split_windows_that_begin_within_a_tile(window, Hq, Hkv, D):
+    """A window of a whole number of key tiles that begins within one reaches into one more."""
+    _run([64, 5, 33], Hq, Hkv, D, window=window, keys=[3001, 2500, 1800], seed=45)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,keys,Hq,Hkv", [([700, 1, 300], [700, 3000, 1999], 8, 4), ([1] * 40, [1500] * 40, 8, 2),
+                                              ([513], [4000], 16, 4), ([2051, 90], [2051, 1500], 8, 1),
+                                              ([1] * 64, list(range(900, 964)), 4, 1)], ids=lambda x: str(x)[:24])
+def test_split_tiles_of_many_lengths(lens, keys, Hq, Hkv, D):
+    _run(lens, Hq, Hkv, D, keys=keys, seed=46)
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv", [([2048], 16, 4), ([1000, 900, 1100, 17], 16, 4), ([600] * 7, 4, 4), ([2500], 16, 8)],
+                         ids=lambda x: str(x)[:24])
+def test_head_dim_256_at_one_and_two_workgroups_a_cu(lens, Hq, Hkv):
+    _run(lens, Hq, Hkv, 256, seed=47)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_split_rows_with_bad_values(D):
     """The joined result of split keys is checked for the rows that must not see a bad value, too."""
     lens, keys = [30], [2000]
@@ -286,6 +308,21 @@ def test_offsets_out_of_range_are_clamped_and_reported():
     for cu in ([0, 20, 90], [0, 30, 10, 50], [-4, 50], [3, 50]):
         exactkv.prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=DEV))
         assert kernels.error_bits() == 0x20, cu
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_split_offsets_out_of_range_are_clamped_and_reported(D):
+    """A split call's too; sequences that are sound keep their rows."""
+    q, k, v = _inputs([50], [3000], 8, 2, D, 48)
+    want = exactkv.prompt_attention(q[:20], k[:1500], v[:1500], _cu([20]), cu_seqlens_k=_cu([1500])).double()
+    for cu, cu_k in (([0, 20, 90], [0, 1500, 3000]), ([0, 20, 50], [0, 1500, 9000]), ([0, 20, 10, 50], [0, 1500, 1500, 3000]),
+                     ([3, 50], [0, 3000]), ([5, 5], [0, 3000]), ([0, 50], [-7, 3000]), ([0, 20, 50], [0, 1500, -5])):
+        print("[case]", D, cu, cu_k, flush=True)
+        got = exactkv.prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=DEV),
+                                       cu_seqlens_k=torch.tensor(cu_k, dtype=torch.int32, device=DEV))
+        assert kernels.error_bits() == 0x20, (cu, cu_k)
+        if cu[1] == 20 and cu[2] >= 50:
+            assert (got[:20].double() - want).norm() <= 2.0 ** -7 * want.norm()
 
 
 def test_captured_and_replayed():
