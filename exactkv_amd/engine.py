@@ -419,7 +419,7 @@ class PagedEngine:
     def add_many(self, prompts):
         """Prefill several prompts (1-D token ids of any lengths) into new sequence slots, packed:
         one pass over the model's layers for about 16K tokens of them. Returns (slots, the greedy
-        next tokens [len(prompts)]). Where a prompt does not fit, none is added."""
+        next tokens [len(prompts)]). Where a prompt does not fit, or the model refuses one, none is added."""
         if self._layers is None:
             self._layers = _LayerKernels(self, self._positions)
         prompts = list(prompts)
@@ -429,11 +429,11 @@ class PagedEngine:
         try:
             for p in prompts:
                 slots.append(self.table.add(int(p.numel())))
-        except (RuntimeError, ValueError):
+            hidden = self._layers.prompts(prompts, slots)
+        except Exception:                       # no room, or no prompts the model takes
             for s in slots:
                 self.table.release(s)
             raise
-        hidden = self._layers.prompts(prompts, slots)
         return slots, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)
 
     @torch.no_grad()
@@ -444,7 +444,11 @@ class PagedEngine:
             if ids.numel() == 0:
                 raise ValueError("a prompt of no tokens")
             s = self.table.add(int(ids.numel()), slot)
-            hidden = self._layers.prompts([ids.view(-1)], [s])
+            try:
+                hidden = self._layers.prompts([ids.view(-1)], [s])
+            except Exception:
+                self.table.release(s)
+                raise
             return s, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)[0]
         s = self.table.add(int(ids.numel()), slot)
         with _fused_sdpa():

@@ -155,6 +155,19 @@ def test_add_many_adds_all_or_none():
     assert eng.table.live_slots() == []
 
 
+def test_prompts_that_the_model_refuses_leave_no_slot():
+    eng = exactkv.PagedEngine(_model("llama"), 4, 64, layer_kernels=True)
+    free = eng.table.free_pages()
+    with pytest.raises(RuntimeError):
+        eng.add_many([_ids(1, 30)[0].cpu(), _ids(1, 20)[0].cpu()])
+    with pytest.raises(RuntimeError):
+        eng.add(_ids(1, 30)[0].cpu())
+    assert eng.table.free_pages() == free and eng.table.live_slots() == []
+    slot, tok = eng.add(_ids(1, 30)[0])
+    (again,), (tok2,) = eng.add_many([_ids(1, 30)[0]])
+    assert tok == tok2 and eng.table.live_slots() == sorted([slot, again])
+
+
 def test_engines_refuse_what_the_kernels_do_not_do():
     m = _model("llama")
     with pytest.raises(AssertionError, match="bf16"):
