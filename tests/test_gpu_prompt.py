@@ -156,6 +156,23 @@ def test_head_dim_256_at_one_and_two_workgroups_a_cu(lens, Hq, Hkv):
     _run(lens, Hq, Hkv, 256, seed=47)
 
 
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("lens", [[1100], [500, 1, 0, 620]], ids=str)
+def test_head_dim_256_two_workgroups_a_cu(lens, window):
+    """Calls of many row tiles take the other instance; a bad value reaches the rows that see it."""
+    _run(lens, 64, 64, 256, window=window, seed=49)
+    q, k, v = _inputs(lens, lens, 64, 64, 256, 49)
+    at = lens[0] - 40
+    v[at, 3] = math.nan
+    got = exactkv.prompt_attention(q, k, v, _cu(lens), window=window)
+    assert got[at:lens[0], 3].isnan().all()
+    got[at:lens[0], 3] = 0
+    v[at, 3] = 0
+    want, mag = _formula(q, k, v, lens, lens, window)
+    want[at:lens[0], 3] = 0
+    _check(got, want, mag)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_split_rows_with_bad_values(D):
     """The joined result of split keys is checked for the rows that must not see a bad value, too."""
