@@ -355,7 +355,7 @@ __device__ inline float wave_least(float x) {
 }
 template <int D, int ROWS, int KEYS>
 __device__ inline bool find_part(const PromptArgs& a, int limit, int& t, int& part, int& most) {
-    const int lane = threadIdx.x & 63, k = lane + 1, span = (ROWS - 1) / a.G;
+    const int lane = threadIdx.x & 63, k = lane + 1;
     // the lane's sequence (there are at most 64): its row tiles, key tiles of the first and of the last one
     int q0, k0, Lq = 0, Lk = 0;
     bool bad = false, bad_k = false;
@@ -365,11 +365,14 @@ __device__ inline bool find_part(const PromptArgs& a, int limit, int& t, int& pa
     }
     if (bad || bad_k) report_error(kErrOffsets);
     const int tiles = (Lq * a.G + ROWS - 1) / ROWS;
-    auto walked = [&](int t_hi) {                      // at most (a window may begin and end within a tile)
+    // key tiles at most: a row tile's tokens, which may begin and end within a group, are up to `span`
+    // apart, and c keys in a row, which may begin and end within a tile, lie in (c - 2) / KEYS + 2
+    const int span = (ROWS - 1 + a.G - 1) / a.G;
+    auto walked = [&](int t_hi) {
         const int keys = max(0, t_hi + Lk - Lq + 1), n = (keys + KEYS - 1) / KEYS;
         return a.window > 0 ? min(n, (a.window + span + 2 * KEYS - 2) / KEYS) : n;
     };
-    const int n0 = walked(min(span, Lq - 1)), n1 = walked(Lq - 1);
+    const int n0 = walked(min((ROWS - 1) / a.G, Lq - 1)), n1 = walked(Lq - 1);
     const float far = -wave_least(-(tiles > 0 ? (float)max(1, max(n0, n1)) : 1.f));
     const int longest = __builtin_amdgcn_readfirstlane((int)far);
     most = (longest + k - 1) / k;

@@ -143,6 +143,15 @@ def test_split_windows_that_begin_within_a_tile(window, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq", [3, 5, 7])
+@pytest.mark.parametrize("extra", [0, 24, 40, 56])
+def test_split_windows_where_groups_begin_within_a_tile(extra, Hq, D):
+    """Row tiles of 128 rows hold parts of a token's heads at both ends, one token more than whole ones."""
+    _run([37, 28, 280], Hq, 1, D, window=432 + extra, keys=[37, 14, 709], seed=50)
+    _run([37, 28, 280], Hq, 1, D, window=1008 + extra, keys=[37, 14, 2709], seed=51)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("lens,keys,Hq,Hkv", [([700, 1, 300], [700, 3000, 1999], 8, 4), ([1] * 40, [1500] * 40, 8, 2),
                                               ([513], [4000], 16, 4), ([2051, 90], [2051, 1500], 8, 1),
                                               ([1] * 64, list(range(900, 964)), 4, 1)], ids=lambda x: str(x)[:24])
