@@ -192,9 +192,10 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile) {
             int l, index;
             if (a.S > 1 && a.S <= 64) {
                 // the sequence's tiles that walk at least x key tiles: row r does if its token's key,
-                // r / G + Lk - Lq, is at least (x - 1) KEYS, and a tile if its last row does
+                // r / G + Lk - Lq, is at least (x - 1) KEYS, and a tile if its last row does; all walk 0
+                // (tokens may stand far before the first key)
                 auto at_least = [&](int x) {
-                    const int64_t row = (int64_t)((x - 1) * KEYS - (len_k - len)) * a.G;
+                    const int64_t row = x == 0 ? 0 : (int64_t)((x - 1) * KEYS - (len_k - len)) * a.G;
                     return row > (int64_t)len * a.G - 1 ? 0 : n - (row > 0 ? (int)(row / ROWS) : 0);
                 };
                 // the most key tiles that more than t tiles walk at least
@@ -734,7 +735,7 @@ prompt_kernel(PromptArgs a, int tiles) {
             float x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[j] = o[nb][i + j] * inv;
+                x[j] = l == 0.f ? 0.f : o[nb][i + j] * inv;     // no key seen: 0, whatever the hidden values are
                 finite = fmaf(x[j], 0.f, finite);
             }
             if (live) *reinterpret_cast<uint2*>(op + 32 * nb + 2 * i) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
@@ -785,6 +786,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);  // no key seen: 0, whatever the hidden values are
     const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
     if (parts > 1)
         *reinterpret_cast<uint2*>(a.out + (int64_t)at * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));

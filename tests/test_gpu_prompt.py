@@ -198,6 +198,31 @@ def test_split_rows_with_bad_values(D):
     assert (err[~seen] <= 0).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("lens,keys", [([300, 40], [200, 25]), ([700, 33, 500], [0, 33, 100]), ([257] * 5, [1, 257, 0, 300, 60]),
+                                       ([900, 5], [100, 4000])], ids=str)
+def test_many_more_queries_than_keys(lens, keys, window, D):
+    """Whole row tiles that see no key are taken like the others."""
+    _run(lens, 8, 2, D, window=window, keys=keys, seed=53)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("lens,keys", [([35], [26]), ([300, 40], [200, 25]), ([70, 5], [20, 2500])], ids=str)
+def test_bad_values_do_not_reach_rows_that_see_no_key(lens, keys, bad, D):
+    q, k, v = _inputs(lens, keys, 8, 2, D, 52)
+    want, mag = _formula(q, k, v, lens, keys, 0)
+    v[3] = bad                                         # key 3 of the first sequence
+    k[7] = math.nan
+    got = exactkv.prompt_attention(q, k, v, _cu(lens), cu_seqlens_k=_cu(keys))
+    none = lens[0] - keys[0]
+    assert (got[:none] == 0).all()
+    _check(got[none:none + 3], want[none:none + 3], mag[none:none + 3])
+    assert got[none + 7:lens[0]].isnan().all()
+    _check(got[lens[0]:], want[lens[0]:], mag[lens[0]:])
+
+
 def test_split_rows_without_a_finite_score():
     q, k, v = _inputs([5], [2000], 1, 1, 64, 44)
     q[:] = 1.0
