@@ -576,9 +576,11 @@ prompt_kernel(PromptArgs a, int tiles) {
         const u32x4 u = {pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
         return __builtin_bit_cast(bf16x8, u);
     };
-    // every load so far has landed, and every wavefront is done with the stages loaded into next
+    // every load so far has landed, and every wavefront is done with the stages loaded into next: its LDS
+    // reads have returned (the products that use them may be placed behind the barrier, and the wait for
+    // a read with them)
     auto next_stage = [&] {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
