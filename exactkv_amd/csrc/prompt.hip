@@ -43,6 +43,7 @@
 // finite computes the rows in question again over their visible keys alone (careful_rows); so do rows
 // whose weights are all zero. What the formula gives then stands; finite results pay for none of it.
 #include "errors.hpp"
+#include "prompt_tiles.hpp"
 #include "tile.hpp"
 #include "../../include/exactkv.h"
 
@@ -58,7 +59,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -1e30f;      // the running maximum before any key, in log2 units
-constexpr int kRows = 128, kWaves = 4;   // query rows and wavefronts of a workgroup
 constexpr float kRaise = 8.f;          // a score this far above the running maximum raises it
 
 struct PromptArgs {
@@ -131,11 +131,6 @@ __host__ __device__ constexpr int key_swizzle(int r) { return D == 64 ? (r >> 1)
 template <int D>
 __host__ __device__ constexpr int value_swizzle(int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; }
 
-// One sequence's share of a workgroup: rows row0 .. of its Lq * G, key rows k0 .. k0 + Lk - 1.
-struct PromptTile {
-    int q0, Lq, k0, Lk, row0;
-};
-
 // The descriptor of a tile of KEYS key or value rows of one sequence and head (wave-uniform), and of
 // the next ones. Rows behind the sequence's end lie past its size.
 template <int D, int KEYS>
@@ -159,13 +154,23 @@ struct Stream {
     }
 };
 
-// The offsets of sequence s, made fit for use where they are not: 0 <= begin <= end <= rows.
-__device__ inline void sequence_of(const int32_t* cu, int s, int rows, int& begin, int& len, bool& bad) {
-    const int a = cu[s], b = cu[s + 1];
-    begin = min(max(a, 0), rows);
-    const int end = min(max(b, begin), rows);
-    len = end - begin;
-    bad = begin != a || end != b || (s == 0 && a != 0);
+// A wavefront's lane operations, for the searches.
+struct DeviceWave {
+    typedef int Int;
+    template <class F, class... X>
+    __device__ auto map(F f, X... x) const { return f(x...); }
+    __device__ int lane() const { return threadIdx.x & 63; }
+    __device__ int scan(int x) const { return wave_incl_scan(x); }
+    __device__ int read(int x, int lane) const { return __builtin_amdgcn_readlane(x, lane); }
+    __device__ uint64_t ballot(int x) const { return __ballot(x); }
+};
+
+// Begin and length of sequence s's queries and keys; offsets that do not ascend from 0 are reported (once
+// both are read: they arrive together).
+__device__ inline void sequence_of(const PromptArgs& a, int s, int& q0, int& Lq, int& k0, int& Lk) {
+    const bool bad = clip_sequence(a.cu_q[s], a.cu_q[s + 1], s == 0, a.N, q0, Lq);
+    const bool bad_k = clip_sequence(a.cu_k[s], a.cu_k[s + 1], s == 0, a.NK, k0, Lk);
+    if (bad | bad_k) report_error(kErrOffsets);
 }
 
 // The tile to take `t`-th: every wavefront finds it by itself from the offsets. The tiles with the most
@@ -173,55 +178,27 @@ __device__ inline void sequence_of(const int32_t* cu, int s, int rows, int& begi
 // tile first. The longest tiles must not start last: twelve prompts of 0 to
 // 1,500 tokens at 28q/4kv in their order / ordered 64.3 / 61.5 us, three at 14q/2kv with head dim 64
 // and a window of 1,024 34.9 / 31.6. False where t is past the tiles of all sequences.
-template <int ROWS, int KEYS>
+template <int KEYS>
 __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         int begin = 0, len = 0, begin_k = 0, len_k = 0;
-        bool bad = false, bad_k = false;
-        if (s0 + lane < a.S) {
-            sequence_of(a.cu_q, s0 + lane, a.N, begin, len, bad);
-            sequence_of(a.cu_k, s0 + lane, a.NK, begin_k, len_k, bad_k);
-        }
-        if (bad || bad_k) report_error(kErrOffsets);
-        const int n = (int)(((int64_t)len * a.G + ROWS - 1) / ROWS);
-        const int incl = wave_incl_scan(n);
-        const int total = __builtin_amdgcn_readlane(incl, 63);
-        if (t < before + total) {
+        if (s0 + lane < a.S) sequence_of(a, s0 + lane, begin, len, begin_k, len_k);
+        const int n = row_tiles(len, a.G), incl = wave_incl_scan(n), total = __builtin_amdgcn_readlane(incl, 63);
+        if (t < total) {
             int l, index;
-            if (a.S > 1 && a.S <= 64) {
-                // the sequence's tiles that walk at least x key tiles: row r does if its token's key,
-                // r / G + Lk - Lq, is at least (x - 1) KEYS, and a tile if its last row does; all walk 0
-                // (tokens may stand far before the first key)
-                auto at_least = [&](int x) {
-                    const int64_t row = x == 0 ? 0 : (int64_t)((x - 1) * KEYS - (len_k - len)) * a.G;
-                    return row > (int64_t)len * a.G - 1 ? 0 : n - (row > 0 ? (int)(row / ROWS) : 0);
-                };
-                // the most key tiles that more than t tiles walk at least
-                int lo = 0, hi = a.NK / KEYS + 2;      // all tiles walk 0; none walks hi
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    const int c = __builtin_amdgcn_readlane(wave_incl_scan(at_least(mid)), 63);
-                    if (c > t) lo = mid; else hi = mid;
-                }
-                const int more = at_least(lo + 1), same = at_least(lo) - more;
-                const int rank = t - __builtin_amdgcn_readlane(wave_incl_scan(more), 63);
-                const int upto = wave_incl_scan(same);
-                l = __builtin_ctzll(__ballot(upto > rank));
-                index = __builtin_amdgcn_readlane(n - more, l) - 1 - (rank - __builtin_amdgcn_readlane(upto - same, l));
-            } else {
-                l = __builtin_ctzll(__ballot(incl > t - before));
-                index = __builtin_amdgcn_readlane(incl, l) - 1 - (t - before);
+            if (!nth_tile<KEYS>(DeviceWave(), a.S, a.G, a.NK, t, len, len_k, n, incl, l, index)) {
+                report_error(kErrOffsets);
+                return false;
             }
             tile.q0 = __builtin_amdgcn_readlane(begin, l);
             tile.Lq = __builtin_amdgcn_readlane(len, l);
-            tile.row0 = index * ROWS;
+            tile.row0 = index * kRows;
             tile.k0 = __builtin_amdgcn_readlane(begin_k, l);
             tile.Lk = __builtin_amdgcn_readlane(len_k, l);
             return true;
         }
-        before += total;
+        t -= total;
     }
     return false;
 }
@@ -312,16 +289,6 @@ __device__ inline void zero_rows(const PromptArgs& a, int64_t end, int part, int
         out[i] = make_uint4(0, 0, 0, 0);
 }
 
-// Key tiles that row tile `row0` of a sequence walks: first .. last.
-template <int ROWS, int KEYS>
-__device__ inline void key_tiles(const PromptArgs& a, const PromptTile& tile, int& first, int& last) {
-    const int shift = tile.Lk - tile.Lq, nrows = tile.Lq * a.G;
-    const int t_lo = tile.row0 / a.G, t_hi = min(tile.row0 + ROWS - 1, nrows - 1) / a.G;
-    const int k_lo = a.window > 0 ? max(0, t_lo + shift - a.window + 1) : 0, k_hi = t_hi + shift;
-    first = k_lo / KEYS;
-    last = k_hi < 0 ? first - 1 : k_hi / KEYS;
-}
-
 // Which row tile and part of its keys a workgroup takes where the keys are split (t: the workgroup's
 // number of its KV head). Of the ways to cut the longest row tile into 1 to `split` parts it takes the
 // one that a model of the time finds best, and `most` are then the key tiles of a part; a row tile of n
@@ -330,10 +297,9 @@ __device__ inline void key_tiles(const PromptArgs& a, const PromptTile& tile, in
 // wait for half a part on average; a part's results, written and read, cost 0.02 and 0.02 more per 128
 // channels, and the second launch 3. The tiles' lengths ascend evenly within a sequence, from n0 to n1,
 // so its tiles have on average (F(n1 / most) - F(n0 / most)) / (n1 / most - n0 / most) parts, F the
-// integral of ceil. Every wavefront computes this from the offsets. Then lane p counts the row tiles that
-// have a part p, exactly: all first parts come first, then all second ones and so on, without gaps, since
-// workgroups that have nothing to do take every second CU's place, or half the XCDs, from those that do
-// (128 tokens on 8K keys 37.7 us with gaps, 31.5 so).
+// integral of ceil. Every wavefront computes this from the offsets. Parts are then handed out without gaps
+// (nth_part), since workgroups that have nothing to do take every second CU's place, or half the XCDs, from
+// those that do (128 tokens on 8K keys 37.7 us with gaps, 31.5 so).
 // Measured without / with split (us), 32q/8kv, head dim 128: 17 tokens on 32K keys 489 / 36, 512 on
 // 16K 255 / 141, 128 on 8K 128 / 31.5.
 __device__ inline float ceil_integral(float x) {
@@ -354,26 +320,15 @@ __device__ inline float wave_least(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fminf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-template <int D, int ROWS, int KEYS>
+template <int D, int KEYS>
 __device__ inline bool find_part(const PromptArgs& a, int limit, int& t, int& part, int& most) {
     const int lane = threadIdx.x & 63, k = lane + 1;
     // the lane's sequence (there are at most 64): its row tiles, key tiles of the first and of the last one
     int q0, k0, Lq = 0, Lk = 0;
-    bool bad = false, bad_k = false;
-    if (lane < a.S) {
-        sequence_of(a.cu_q, lane, a.N, q0, Lq, bad);
-        sequence_of(a.cu_k, lane, a.NK, k0, Lk, bad_k);
-    }
-    if (bad || bad_k) report_error(kErrOffsets);
-    const int tiles = (Lq * a.G + ROWS - 1) / ROWS;
-    // key tiles at most: a row tile's tokens, which may begin and end within a group, are up to `span`
-    // apart, and c keys in a row, which may begin and end within a tile, lie in (c - 2) / KEYS + 2
-    const int span = (ROWS - 1 + a.G - 1) / a.G;
-    auto walked = [&](int t_hi) {
-        const int keys = max(0, t_hi + Lk - Lq + 1), n = (keys + KEYS - 1) / KEYS;
-        return a.window > 0 ? min(n, (a.window + span + 2 * KEYS - 2) / KEYS) : n;
-    };
-    const int n0 = walked(min((ROWS - 1) / a.G, Lq - 1)), n1 = walked(Lq - 1);
+    if (lane < a.S) sequence_of(a, lane, q0, Lq, k0, Lk);
+    const int tiles = row_tiles(Lq, a.G);
+    const int n0 = key_tiles_most<KEYS>(min((kRows - 1) / a.G, Lq - 1), Lq, Lk, a.G, a.window);
+    const int n1 = key_tiles_most<KEYS>(Lq - 1, Lq, Lk, a.G, a.window);
     const float far = -wave_least(-(tiles > 0 ? (float)max(1, max(n0, n1)) : 1.f));
     const int longest = __builtin_amdgcn_readfirstlane((int)far);
     most = (longest + k - 1) / k;
@@ -392,36 +347,16 @@ __device__ inline bool find_part(const PromptArgs& a, int limit, int& t, int& pa
     time *= side <= 1.f ? 1.07f : 0.8f * side;
     if (k > 1) time += 3.f + (0.02f + 0.02f / 128.f * D) * model;
     if (k > a.split || (k > 1 && model > (float)(limit * a.Hkv))) time = INFINITY;
-    most = __builtin_amdgcn_readlane(most, __builtin_ctzll(__ballot(time == wave_least(time))));
-    // row tiles with a part `lane`: with a window all of them, where any has (some parts are then empty)
-    int all = 0, count = 0;
-    for (int i = 0; i < a.S; ++i) {
-        const int n = __builtin_amdgcn_readlane(tiles, i), lq = __builtin_amdgcn_readlane(Lq, i), lk = __builtin_amdgcn_readlane(Lk, i);
-        // the first row whose key lies in that part
-        const int64_t row = ((int64_t)lane * most * KEYS - (lk - lq)) * a.G;
-        count += row >= (int64_t)lq * a.G ? 0 : n - (row > 0 ? (int)(row / ROWS) : 0);
-        all += n;
-    }
-    if (lane == 0 || (a.window > 0 && lane < (longest + most - 1) / most)) count = all;
-    else if (a.window > 0) count = 0;
-    int upto = wave_incl_scan(count);
-    if (__builtin_amdgcn_readlane(upto, 63) > limit) { // more than the model thought: no split
-        most = longest;
-        count = lane == 0 ? all : 0;
-        upto = all;
-    }
-    if (t >= __builtin_amdgcn_readlane(upto, 63)) return false;
-    part = __builtin_ctzll(__ballot(upto > t));
-    t -= __builtin_amdgcn_readlane(upto - count, part);
-    return true;
+    most = __builtin_amdgcn_readlane(most, max(0, first_lane(__ballot(time == wave_least(time)))));
+    return nth_part<KEYS>(DeviceWave(), a.S, a.G, a.window, longest, limit, tiles, Lq, Lk, t, part, most);
 }
 
-template <int D, int NW, int KEYS, int WPE, bool PIPE>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+template <int D, int KEYS, int WPE, bool PIPE>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 prompt_kernel(PromptArgs a, int tiles) {
     constexpr bool CUTS = D < 256 || PIPE;                       // (the other instance never splits keys)
     constexpr int KB = KEYS / 32;                                // 32-key blocks of a tile
-    constexpr int ROWS = 32 * NW, KS = D / 16, NB = D / 32;      // rows, score k-steps, 32-channel blocks
+    constexpr int NW = kWaves, KS = D / 16, NB = D / 32;         // wavefronts, score k-steps, 32-channel blocks
     constexpr int PIECES = D / 8, RPI = 64 / PIECES;             // 16-byte pieces of a row, rows per load
     constexpr int TILE = KEYS * 2 * D, LOADS = TILE / 1024 / NW;
     static_assert(TILE % (1024 * NW) == 0, "whole loads");
@@ -431,11 +366,11 @@ prompt_kernel(PromptArgs a, int tiles) {
     int t = (int)blockIdx.x / a.Hkv, part = 0, most = 0;
     bool found = true;
     if (CUTS && a.split > 1)                           // uniform
-        found = find_part<D, ROWS, KEYS>(a, (int)gridDim.x / a.Hkv, t, part, most);
+        found = find_part<D, KEYS>(a, (int)gridDim.x / a.Hkv, t, part, most);
     else if (t >= a.turn)
         t = tiles - 1 - (t - a.turn);
     PromptTile tile;
-    found = found && find_tile<ROWS, KEYS>(a, t, tile);
+    found = found && find_tile<KEYS>(a, t, tile);
     if (a.zero_tail) {
         const int end = a.S > 0 ? min(max(a.cu_q[a.S], 0), a.N) : 0;
         if (end < a.N) zero_rows<D, 64 * NW>(a, end, (int)blockIdx.x, (int)gridDim.x);
@@ -451,15 +386,11 @@ prompt_kernel(PromptArgs a, int tiles) {
     const bool wave_on = wrow0 < nrows;
     const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
     int first, last;
-    key_tiles<ROWS, KEYS>(a, tile, first, last);
-    const int parts = CUTS && a.split > 1 ? max(1, (last - first + most) / most) : 1;
+    key_tiles<KEYS>(tile, G, a.window, first, last);
+    const int parts = CUTS && a.split > 1 ? parts_of(first, last, most) : 1;
     if (part >= parts) return;
     if (CUTS && a.split > 1 && part == 0 && half == 0 && wrow0 + col < nrows) a.part_n[(int64_t)(tile.q0 + tok) * a.Hq + hq] = parts;
-    if (parts > 1) {
-        const int per = (last - first + parts) / parts;
-        first += part * per;
-        last = min(last, first + per - 1);
-    }
+    if (parts > 1) part_tiles(part, parts, first, last);
 
     bf16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)(tile.q0 + tok) * a.sq_t + hq * a.sq_h + 8 * half;
@@ -758,9 +689,9 @@ prompt_kernel(PromptArgs a, int tiles) {
 // one another. Rows of one part are done. Bound by the parts' reads, which the other launch has just
 // written: 813 tokens of two continued prompts 7.0 us (joined by a workgroup per four rows of a tile,
 // a row after the other, 12.5).
-template <int D, int NW, int KEYS>
+template <int D, int KEYS>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
-    constexpr int ROWS = 32 * NW, LPR = D / 4, RPW = 64 / LPR;
+    constexpr int LPR = D / 4, RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane % LPR;
     const int rows = min(max(a.cu_q[a.S], 0), a.N) * a.Hq;       // of sequences
     const int row = ((int)blockIdx.x * 4 + w) * RPW + lane / LPR, at = min(row, rows - 1);
@@ -802,57 +733,15 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
         int s = 0;                                     // the sequence that holds row t
         while (s + 1 < a.S && a.cu_q[s + 1] <= t) ++s;
         PromptTile tile{};
-        bool bad;
-        sequence_of(a.cu_q, s, a.N, tile.q0, tile.Lq, bad);
-        sequence_of(a.cu_k, s, a.NK, tile.k0, tile.Lk, bad);
+        sequence_of(a, s, tile.q0, tile.Lq, tile.k0, tile.Lk);
         const int tok = t - tile.q0, p = tok + tile.Lk - tile.Lq, own = tok * a.G + hq % a.G;
         if (tok < 0 || tok >= tile.Lq || p < 0) continue;
         int first, last;
-        tile.row0 = own / ROWS * ROWS;
-        key_tiles<ROWS, KEYS>(a, tile, first, last);
+        tile.row0 = own / kRows * kRows;
+        key_tiles<KEYS>(tile, a.G, a.window, first, last);
         const bool none = __builtin_amdgcn_readlane(__float_as_int(l), i * LPR) == 0;
         if (none || hidden_values_bad<D, KEYS>(a, tile, hk, p, p, first, last)) careful_rows<D>(a, tile, own, hk, 1u);
     }
-}
-
-// How a call is laid out. `slots` workgroups run at a time: two a CU (four at head dim 64). Keys are
-// split where the row tiles leave CUs free and are long enough for what the parts' results cost.
-//
-// Head dim 256 has two instances: one workgroup a CU, with the next tile's scores beside this tile's
-// weights (1.05 us a step), and two without (1.35 us alone, 0.96 together). The former where no CU gets
-// more than two: one / two a CU, 16q/4kv, 2K tokens 72 / 92 us, 3,000 101 / 131, 4K 155 / 190, but 6,000
-// 337 / 312, 8K 563 / 491.
-constexpr int keys_per_tile(int D) { return D == 256 ? 32 : 64; }
-constexpr int kLeast = 8;              // key tiles of the longest row tile, per part, at least
-struct PromptPlan {
-    int64_t tiles;                     // row tiles, at most
-    int split, slots;
-    int turn;                          // two workgroups a CU in one go: the second ones in reverse, so that a
-                                       // CU's two tiles add up to about the same (one prompt of 1,500
-                                       // tokens 32.7 us without, 31.4 so; of 2,048 no difference)
-    bool alone;                        // head dim 256: one workgroup a CU
-    int64_t blocks;                    // workgroups of a KV head
-};
-static PromptPlan plan_prompt(int64_t N, int64_t NK, int64_t S, int64_t Hq, int64_t Hkv, int D, int64_t window) {
-    // every sequence's last tile may be partial
-    const int64_t tiles = (N * (Hq / Hkv) + S * (kRows - 1)) / kRows, units = (tiles > 0 ? tiles : 1) * Hkv;
-    PromptPlan p{units / Hkv, 1, D == 64 ? 1024 : 512, INT32_MAX, D == 256 && units <= 512, units / Hkv};
-    if (p.alone) p.slots = 256;
-    const int64_t reach = window > 0 && window + kRows < NK ? window + kRows : NK;
-    const int64_t keys = (reach + keys_per_tile(D) - 1) / keys_per_tile(D), few = D == 64 ? 512 : 256;
-    if (units >= few || S > 64 || S == 0 || 25 * keys < 150 + units * D / 64) {
-        if (!p.alone && units > 256 && units <= 512) p.turn = (int)((256 + Hkv - 1) / Hkv);
-        return p;
-    }
-    int64_t split = 4 * few / units;
-    if (split > D / 4) split = D / 4;
-    if (split > keys / kLeast) split = keys / kLeast;
-    if (split > 1) {
-        const int64_t most = (p.slots + p.slots / (p.alone ? 2 : 8)) / Hkv;
-        p.split = (int)split;
-        p.blocks = p.tiles * split < most ? p.tiles * split : most > p.tiles ? most : p.tiles;
-    }
-    return p;
 }
 
 static int64_t workspace_bytes(const PromptPlan& p, int64_t N, int64_t Hq, int64_t D) {
@@ -866,10 +755,10 @@ template <int D, int WPE, bool PIPE>
 static void launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t stream) {
     constexpr int KEYS = keys_per_tile(D);
     const int64_t blocks = a.split > 1 ? p.blocks : p.tiles;
-    hipLaunchKernelGGL((prompt_kernel<D, kWaves, KEYS, WPE, PIPE>), dim3((unsigned)(blocks * a.Hkv)), dim3(64 * kWaves), 0, stream, a,
+    hipLaunchKernelGGL((prompt_kernel<D, KEYS, WPE, PIPE>), dim3((unsigned)(blocks * a.Hkv)), dim3(64 * kWaves), 0, stream, a,
                        (int)p.tiles);
     if (a.split > 1)
-        hipLaunchKernelGGL((prompt_merge_kernel<D, kWaves, KEYS>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
+        hipLaunchKernelGGL((prompt_merge_kernel<D, KEYS>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
                            0, stream, a);
 }
 

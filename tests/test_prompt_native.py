@@ -1,5 +1,5 @@
 """Prompt attention's kernel, checked without a GPU: the waits in the code that the compiler makes of
-it.
+it, and the search of its tiles.
 
 No counterpart in the reference (its prefill is the model's own forward pass, engine.py:42-49)."""
 import os
@@ -37,3 +37,15 @@ def test_barriers_wait_for_lds_reads(tmp_path):
     for i in at:
         wait = lines[i - 1].split()
         assert wait[0] == "s_waitcnt" and "vmcnt(0)" in wait and "lgkmcnt(0)" in wait, lines[i - 4:i + 1]
+
+
+def test_every_tile_and_part_is_taken_once(tmp_path):
+    """The search of a workgroup's row tile and part of its keys (csrc/prompt_tiles.hpp), which the
+    addresses of its reads follow from, over random offsets, sound and broken, and every number of
+    parts (tests/native/tiles_check.cpp)."""
+    exe = tmp_path / "tiles_check"
+    subprocess.run([_hipcc(), "-O2", "-o", str(exe), os.path.join(ROOT, "tests", "native", "tiles_check.cpp")],
+                   check=True, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    r = subprocess.run([str(exe)], stdout=subprocess.PIPE, text=True)
+    assert r.returncode == 0, r.stdout
+    assert " 0 failures" in r.stdout
