@@ -215,16 +215,26 @@ def _token_rows(q, k, v, cos, sin, q_norm, k_norm, eps, out, dev):
 
 
 _ARRAYS = operator.itemgetter("sm", "code", "base", "rowmask", "rowoff", "raw")
+_WORDS = operator.itemgetter("cnt", "before", "cap", "TS")
 
 
 def _pool_args(buf, H, D, dev, what):
-    """A paged compressed cache's arrays and counters (its encoder view) as a call takes them, its
-    cap, raw rows and pages, checked."""
+    """A paged compressed cache's arrays and counters (its encoder view) as a call takes them, with the
+    arrival word last if it has one, its cap, raw rows and pages, checked: the kernel writes them by
+    address."""
     arrays = sm, code, base, rowmask, rowoff, raw = _ARRAYS(buf)
-    pages, units = buf["TS"] // P, buf["TS"] // P * H
-    if buf["H"] != H or buf["D"] != D or raw.shape[-1] != D:
-        raise ValueError(f"{what} holds {buf['H']} heads of {buf['D']}, the rows {H} of {D}")
-    if (sm.numel() != units * P * D or code.numel() * 2 != units * P * D or base.numel() != units * D
+    cnt, before, cap, TS = _WORDS(buf)
+    arrivals = buf.get("arrivals")                     # (the keys' serves both)
+    u8, i32 = torch.uint8, torch.int32
+    if (sm.dtype is not u8 or code.dtype is not u8 or base.dtype is not u8 or rowmask.dtype is not i32
+            or rowoff.dtype is not i32 or raw.dtype is not BF16):
+        raise ValueError(f"{what}: sm, code and base must be uint8, rowmask and rowoff int32, raw bfloat16")
+    shape = raw.shape
+    if len(shape) != 2 or shape[1] != D or buf["H"] != H or buf["D"] != D:
+        raise ValueError(f"{what} holds {buf['H']} heads of {buf['D']} and raw rows {tuple(shape)}, the rows {H} of {D}")
+    pages = TS // P
+    units = pages * H
+    if (TS % P or cap < 0 or sm.numel() != units * P * D or code.numel() * 2 != units * P * D or base.numel() != units * D
             or rowmask.numel() != units or rowoff.numel() != units):
         raise ValueError(f"{what}: the arrays are not those of {pages} pages")
     low, ptrs = 0, []
@@ -234,15 +244,15 @@ def _pool_args(buf, H, D, dev, what):
         p = t.data_ptr()
         low |= p
         ptrs.append(p)
-    for t in (buf["cnt"], buf["before"]):
-        if t.get_device() != dev:
-            raise ValueError(f"{what}: the counters must be on the rows' GPU")
+    for t in (cnt, before) if arrivals is None else (cnt, before, arrivals):
+        if t.dtype is not i32 or t.get_device() != dev or t.numel() < 1:
+            raise ValueError(f"{what}: cnt, before and arrivals must be int32 words on the rows' GPU")
         p = t.data_ptr()
         low |= p << 2
         ptrs.append(p)
     if low & 15:
         raise ValueError(f"{what}: the arrays must be 16-byte aligned, the counters 4-byte")
-    return ptrs, int(buf["cap"]), raw.shape[0], pages
+    return ptrs, int(cap), shape[0], pages
 
 
 def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=None, *, q_norm=None, k_norm=None,
@@ -279,13 +289,11 @@ def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=No
     if isinstance(kbuf, dict):
         kp, kcap, krows, pages = _pool_args(kbuf, H, D, dev, "kbuf")
         vp, vcap, vrows, vpages = _pool_args(vbuf, H, D, dev, "vbuf")
-        arrivals = kbuf.get("arrivals")
-        if arrivals is None:
+        if len(kp) < 9:
             raise ValueError("kbuf has no arrival word ('arrivals', int32, zero between calls)")
         if vpages != pages:
             raise ValueError("kbuf and vbuf must be pools of as many pages")
-        _lib.call("exkv_rope_append_paged", *rows, *kp, _lib.ptr(arrivals, 4, "arrivals"), kcap, krows, *vp, vcap, vrows,
-                  *table, pages, D, st)
+        _lib.call("exkv_rope_append_paged", *rows, *kp, kcap, krows, *vp[:8], vcap, vrows, *table, pages, D, st)
         return out
     shape = kbuf.shape
     for t in (kbuf, vbuf):
