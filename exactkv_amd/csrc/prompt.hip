@@ -38,10 +38,12 @@
 // by 2^8 (the accumulator is then rescaled), so they stay below 256.
 //
 // Values that a row does not attend to must not reach it, also where they are infinite or NaN,
-// but the matrix product multiplies them by a weight of zero. A wavefront whose result is not finite
-// therefore looks through the values that some of its rows do not see, and where one of those is not
-// finite computes the rows in question again over their visible keys alone (careful_rows); so do rows
-// whose weights are all zero. What the formula gives then stands; finite results pay for none of it.
+// but the matrix product multiplies them by a weight of zero. And the accumulator, which is divided by the
+// sum at the end only, overflows where values are finite but large (from about 2^128 / 2^8 / keys on).
+// A wavefront whose result is not finite, or large, therefore looks through the values of its tiles, and where one that
+// some of its rows do not see is not finite, or one is that large, computes the rows in question again over
+// their visible keys alone (careful_rows; of split keys the part looks and the join computes); so do rows
+// whose weights are all zero. What the formula gives then stands; other results pay for none of it.
 #include "errors.hpp"
 #include "prompt_tiles.hpp"
 #include "tile.hpp"
@@ -55,11 +57,14 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -1e30f;      // the running maximum before any key, in log2 units
 constexpr float kRaise = 8.f;          // a score this far above the running maximum raises it
+constexpr float kLarge = 0x1p120f;     // results from here on are looked at again: the weights' rounding, or a sum of
+                                       // parts, may leave the range
 
 struct PromptArgs {
     const uint16_t *q, *k, *v;         // rows of D channels, element strides below
@@ -72,7 +77,7 @@ struct PromptArgs {
     int split, slots;
     int turn;                          // tiles from here on are taken in reverse
     float* part_o;                     // [split, N * Hq, D]
-    float2* part_ml;                   // [split, N * Hq]: running maximum (log2 units), sum
+    float2* part_ml;                   // [split, N * Hq]: running maximum (log2 units), sum (or its negative)
     int32_t* part_n;                   // [N * Hq]: the row's parts
 };
 
@@ -203,29 +208,43 @@ __device__ inline bool find_tile(const PromptArgs& a, int t, PromptTile& tile) {
     return false;
 }
 
-// Whether a value that some row standing at keys p_lo .. p_hi does not see, of the key tiles first ..
-// last that they walk, is infinite or NaN: only such values can have reached a row wrongly.
+// Of the key tiles first .. last that rows standing at keys p_lo .. p_hi walk: whether a value that some of
+// these rows does not see is infinite or NaN, or any value so large that finite ones overflow a row's
+// accumulator (N < 2^31 keys with weights up to 2^8: from 2^88 on). Otherwise a result that is not finite is
+// what the formula gives (2,048 such tokens at 8q/8kv, head dim 128: 53 us, 32 else).
+constexpr uint32_t kLargeBits = (127 + 88) << 7;
 template <int D, int KEYS>
-__device__ inline bool hidden_values_bad(const PromptArgs& a, const PromptTile& tile, int hk, int p_lo, int p_hi, int first, int last) {
-    constexpr int PIECES = D / 8;
-    const int lane = threadIdx.x & 63;
-    bool bad = false;
-    auto scan = [&](int from, int to) {                // keys from .. to - 1
-        for (int i = lane; i < (to - from) * PIECES; i += 64) {
-            const uint4 x = ld16(a.v + (int64_t)(tile.k0 + from + i / PIECES) * a.sv_t + hk * a.sv_h + i % PIECES * 8);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+__device__ inline bool values_suspect(const PromptArgs& a, const PromptTile& tile, int hk, int p_lo, int p_hi, int first, int last) {
+    constexpr int PIECES = D / 8, BATCH = 8;           // 16-byte pieces of a row; loads in flight
+    const int lane = threadIdx.x & 63, from = first * KEYS;
+    const int64_t n = (int64_t)(min((last + 1) * KEYS, tile.Lk) - from) * PIECES;
+    // the largest exponent field + 1 of either half of a dword, where bit 15 says infinite or NaN
+    u16x2 top = {0, 0};
+    for (int64_t i0 = lane; i0 < n; i0 += 64 * BATCH) {
+        uint4 x[BATCH];
+        int j[BATCH];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bad |= (~xs[j] & 0x7F80u) == 0 || (~xs[j] & 0x7F800000u) == 0;
+        for (int u = 0; u < BATCH; ++u) {
+            const int64_t i = min(i0 + 64 * u, n - 1);  // the last piece once more where there is none
+            j[u] = from + (int)(i / PIECES);
+            x[u] = ld16(a.v + (int64_t)(tile.k0 + j[u]) * a.sv_t + hk * a.sv_h + i % PIECES * 8);
         }
-    };
-    scan(max(0, p_lo + 1), min((last + 1) * KEYS, tile.Lk));
-    if (a.window > 0) scan(first * KEYS, min(p_hi - a.window + 1, tile.Lk));
-    return __ballot(bad) != 0;
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const uint32_t keep = j[u] > p_lo || (a.window > 0 && j[u] <= p_hi - a.window) ? ~0u : 0x7FFF7FFFu;
+            const uint32_t xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, ((xs[c] & 0x7F807F80u) + 0x00800080u) & keep));
+        }
+    }
+    return __ballot(max(top.x, top.y) >= kLargeBits + 0x80) != 0;
 }
 
 // Rows (bit c of `rows`: row wrow0 + c) computed again from their visible keys alone, one row at a
-// time: 64 scores at once, a lane each, for the maximum and again for the weights, then the values
-// with D / 64 channels a lane. About 1,500 cycles a row and 64 keys.
+// time: 64 scores at once, a lane each, for the maximum, again for the sum and again for the weights, which
+// are divided by the sum first, so that finite values cannot overflow; then the values with D / 64 channels
+// a lane. 2,048 tokens at 8q/8kv, head dim 128, every row so: 10 ms (32 us else).
 template <int D>
 __device__ __attribute__((always_inline)) inline void careful_rows(const PromptArgs& a, const PromptTile& tile, int wrow0, int hk,
                                                                    uint32_t rows) {
@@ -263,10 +282,14 @@ __device__ __attribute__((always_inline)) inline void careful_rows(const PromptA
         if (__ballot(nan) != 0) m = NAN;
         for (int c = 0; c < C; ++c) o[c] = 0.f;
         // (every weight is NaN where a score is: the first keys say so)
-        for (int j0 = first; j0 <= (m != m ? first : p); j0 += 64) {
+        const int end = m != m ? first : p;
+        auto weight = [&](int j) { return j <= p ? exp2_fast(score(min(j, p)) - m) : 0.f; };
+        for (int j0 = first; j0 <= end; j0 += 64) l += weight(j0 + lane);
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+        const float inv = 1.f / l;
+        for (int j0 = first; j0 <= end; j0 += 64) {
             const int n = min(64, p - j0 + 1);
-            const float w = lane < n ? exp2_fast(score(min(j0 + lane, p)) - m) : 0.f;
-            l += w;
+            const float w = weight(j0 + lane) * inv;
             const uint16_t* v = a.v + (int64_t)(tile.k0 + j0) * a.sv_t + hk * a.sv_h + C * lane;
 #pragma unroll 4
             for (int i = 0; i < n; ++i) {
@@ -274,9 +297,8 @@ __device__ __attribute__((always_inline)) inline void careful_rows(const PromptA
                 for (int c = 0; c < C; ++c) o[c] = fmaf(wi, bf16_float(v[i * a.sv_t + c]), o[c]);
             }
         }
-        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
         uint16_t* out = a.out + ((int64_t)(tile.q0 + t) * a.Hq + h) * D + C * lane;
-        for (int c = 0; c < C; ++c) out[c] = __builtin_bit_cast(uint16_t, (__bf16)(p < first ? 0.f : o[c] / l));
+        for (int c = 0; c < C; ++c) out[c] = __builtin_bit_cast(uint16_t, (__bf16)o[c]);
     }
 }
 
@@ -648,8 +670,16 @@ prompt_kernel(PromptArgs a, int tiles) {
     const bool live = wrow0 + col < nrows, seen = pos >= 0;
     if (parts > 1) {
         const int64_t row_out = (int64_t)part * a.N * a.Hq + (int64_t)(tile.q0 + tok) * a.Hq + hq;
+        // the join adds up to 64 parts; what it cannot see, suspect values among this part's, is the sum's sign
+        float size = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) size += fabsf(o[nb][i]);
+        const bool suspect = __ballot(live && l == l && !(size < kLarge)) != 0 &&
+                             values_suspect<D, KEYS>(a, tile, hk, w_lo, w_hi, first, last);
         if (!live) return;
-        if (half == 0) a.part_ml[row_out] = make_float2(m, l);
+        if (half == 0) a.part_ml[row_out] = make_float2(m, suspect ? -l : l);
         float* op = a.part_o + row_out * D + 4 * half;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -659,7 +689,7 @@ prompt_kernel(PromptArgs a, int tiles) {
         return;
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    float finite = 0.f;                                // NaN once a value is not finite
+    float size = 0.f;                                  // not below kLarge once a value is not, or not finite
     uint16_t* op = a.out + ((int64_t)(tile.q0 + tok) * a.Hq + hq) * D + 4 * half;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -669,13 +699,14 @@ prompt_kernel(PromptArgs a, int tiles) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[j] = l == 0.f ? 0.f : o[nb][i + j] * inv;     // no key seen: 0, whatever the hidden values are
-                finite = fmaf(x[j], 0.f, finite);
+                size += fabsf(x[j]);
             }
             if (live) *reinterpret_cast<uint2*>(op + 32 * nb + 2 * i) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
-    const uint64_t empty = __ballot(live && seen && l == 0.f), odd = __ballot(live && seen && finite != finite);
+    // (l is NaN where a score the row sees is infinite or NaN: so is the row)
+    const uint64_t empty = __ballot(live && seen && l == 0.f), odd = __ballot(live && seen && l == l && !(size < kLarge));
     uint64_t again = empty;
-    if (odd != 0 && hidden_values_bad<D, KEYS>(a, tile, hk, w_lo, w_hi, first, last)) again |= odd;
+    if (odd != 0 && values_suspect<D, KEYS>(a, tile, hk, w_lo, w_hi, first, last)) again |= odd;
     if (again != 0) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // these rows' stores come first
         careful_rows<D>(a, tile, wrow0, hk, (uint32_t)again | (uint32_t)(again >> 32));
@@ -689,7 +720,7 @@ prompt_kernel(PromptArgs a, int tiles) {
 // one another. Rows of one part are done. Bound by the parts' reads, which the other launch has just
 // written: 813 tokens of two continued prompts 7.0 us (joined by a workgroup per four rows of a tile,
 // a row after the other, 12.5).
-template <int D, int KEYS>
+template <int D>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     constexpr int LPR = D / 4, RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane % LPR;
@@ -703,7 +734,8 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
 #pragma unroll
     for (int d = 1; d < LPR; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
     const float f = exp2_fast(ml.x - M);
-    float l = ml.y * f;
+    const uint64_t suspect = __ballot(__float_as_int(ml.y) < 0);
+    float l = fabsf(ml.y) * f;
 #pragma unroll
     for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -720,15 +752,16 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
     if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);  // no key seen: 0, whatever the hidden values are
-    const float finite = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
+    const float size = fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w);
     if (parts > 1)
         *reinterpret_cast<uint2*>(a.out + (int64_t)at * D + 4 * j) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-    uint64_t odd = __ballot(parts > 1 && (finite != finite || l == 0.f));
+    uint64_t odd = __ballot(parts > 1 && l == l && (!(size < kLarge) || l == 0.f));
     if (odd == 0) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    for (int i = 0; i < RPW; ++i) {                    // rows to look at again, one by one (uniform)
+    for (int i = 0; i < RPW; ++i) {                    // rows to compute again, one by one (uniform)
         const uint64_t lanes = (LPR == 64 ? ~0ull : (1ull << LPR) - 1ull) << (i * LPR);
-        if ((odd & lanes) == 0) continue;
+        const bool none = __builtin_amdgcn_readlane(__float_as_int(l), i * LPR) == 0;
+        if ((odd & lanes) == 0 || (!none && (suspect & lanes) == 0)) continue;
         const int r = __builtin_amdgcn_readlane(at, i * LPR), t = r / a.Hq, hq = r % a.Hq, hk = hq / a.G;
         int s = 0;                                     // the sequence that holds row t
         while (s + 1 < a.S && a.cu_q[s + 1] <= t) ++s;
@@ -736,11 +769,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(PromptArgs a) {
         sequence_of(a, s, tile.q0, tile.Lq, tile.k0, tile.Lk);
         const int tok = t - tile.q0, p = tok + tile.Lk - tile.Lq, own = tok * a.G + hq % a.G;
         if (tok < 0 || tok >= tile.Lq || p < 0) continue;
-        int first, last;
-        tile.row0 = own / kRows * kRows;
-        key_tiles<KEYS>(tile, a.G, a.window, first, last);
-        const bool none = __builtin_amdgcn_readlane(__float_as_int(l), i * LPR) == 0;
-        if (none || hidden_values_bad<D, KEYS>(a, tile, hk, p, p, first, last)) careful_rows<D>(a, tile, own, hk, 1u);
+        careful_rows<D>(a, tile, own, hk, 1u);
     }
 }
 
@@ -758,7 +787,7 @@ static void launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t 
     hipLaunchKernelGGL((prompt_kernel<D, KEYS, WPE, PIPE>), dim3((unsigned)(blocks * a.Hkv)), dim3(64 * kWaves), 0, stream, a,
                        (int)p.tiles);
     if (a.split > 1)
-        hipLaunchKernelGGL((prompt_merge_kernel<D, KEYS>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
+        hipLaunchKernelGGL((prompt_merge_kernel<D>), dim3((unsigned)(((int64_t)a.N * a.Hq * (D / 4) + 255) / 256)), dim3(256),
                            0, stream, a);
 }
 
