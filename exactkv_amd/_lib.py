@@ -144,6 +144,7 @@ ERROR_BITS = {
     0x10: "wire pack: a raw row's pool slot lay outside the pool (clamped)",
     0x20: "packed prompts: sequence offsets that do not ascend from 0 within the rows (clamped)",
     0x40: "rotation: a position outside the cosine and sine tables (clamped)",
+    0x80: "rotated paged append: the table entry behind a page that a token filled lies outside the pool (no page opened)",
 }
 
 

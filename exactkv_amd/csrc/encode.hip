@@ -1510,7 +1510,16 @@ __global__ void __launch_bounds__(rope_threads(KIND)) rope_append_kernel(RopeRow
                         if (tok < 0 || tok % kPage != kPage - 1) continue;
                         const int64_t pidx = paged_pidx(a, slot, tok / kPage);
                         const int64_t tail_row = a.cap + ((int64_t)slot * a.H + h) * kPage;
-                        const int64_t next = tok / kPage + 1 < a.max_pages ? paged_pidx(a, slot, tok / kPage + 1) * a.H + h : -1;
+                        // the page that the next token opens; an entry that names none of the pool is not
+                        // taken for its last one, which another sequence may hold
+                        int64_t next = -1;
+                        if (tok / kPage + 1 < a.max_pages) {
+                            const int32_t entry = a.bt[slot * a.bt_stride + tok / kPage + 1];
+                            if ((uint32_t)entry < (uint32_t)a.pool_pages)
+                                next = (int64_t)entry * a.H + h;
+                            else if (lane == 0)
+                                report_error(kErrPage);
+                        }
                         encode_unit<D>(a, a.raw + tail_row * D, pidx * a.H + h, pidx * kPage * a.H + h, lane, next, tail_row);
                     } else {
                         const AppendArgs& a = isv ? c.v : c.k;

@@ -25,6 +25,7 @@ enum : uint32_t {
     kErrWire = 1u << 4,      // wire unpack / pack: a raw row's pool slot fell outside the pool
     kErrOffsets = 1u << 5,   // packed prompts: sequence offsets that do not ascend from 0 within the rows
     kErrPosition = 1u << 6,  // rotation: a position outside the cosine / sine tables
+    kErrPage = 1u << 7,      // rotated paged append: the table entry behind a page that a token filled names no page
 };
 
 static __device__ uint32_t file_error_word;

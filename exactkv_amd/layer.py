@@ -264,7 +264,15 @@ def rope_append_paged(q, k, v, cos, sin, kbuf, vbuf, lens, block_table, slots=No
     its page block_table[slot, position // 16] (int32). kbuf, vbuf: bf16 pools [1, 16 * pages,
     Hkv, D], or the encoder views of two compressed caches (PagedCompressedKV._buf()). Norms as in
     rotate_prompt. Returns the rotated queries [n, Hq, D], ready for decode_attention; everything
-    in one launch. A slot whose lens is 0 or past the table is left alone.
+    in one launch.
+
+    In compressed pools a token that fills its page (position % 16 == 15) also opens the next one in
+    both caches, so entry position // 16 + 1, where the table has it, must be the slot's own by then
+    (PageTable.begin_step claims it). An entry outside the pool opens nothing and sets an error bit
+    (kernels.check_errors).
+
+    A slot whose lens is 0 or past the table appends nothing and its pages stay as they are; its query
+    row is written, rotated at position 0, and an error bit is set.
 
     This is rope_append on tensors: it changes no host state."""
     dev = q.get_device()

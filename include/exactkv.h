@@ -57,6 +57,7 @@ int exkv_abi_version(void);
 #define EXKV_ERR_WIRE 0x10u     /* wire pack: a raw row's pool slot lay outside the pool */
 #define EXKV_ERR_OFFSETS 0x20u  /* packed prompts: sequence offsets that do not ascend from 0 within the rows */
 #define EXKV_ERR_POSITION 0x40u /* rotation: a position outside the cosine and sine tables (clamped) */
+#define EXKV_ERR_PAGE 0x80u     /* rotated paged append: the table entry behind a filled page lies outside the pool (no page opened) */
 
 /* out (a device uint32 on the GPU of `stream`) = the OR of the error words of that GPU, in
  * stream order (a small kernel for each; nothing synchronizes, nothing is allocated); clear != 0
@@ -503,7 +504,11 @@ int exkv_rope_append_bf16(const void* q, int64_t sq_n, int64_t sq_h, const void*
                           hipStream_t stream);
 
 /* The same into paged compressed caches (exkv_cache_append_paged_counted: slots, lens counting the
- * new token, block table, and one arrival word, zero between calls, for both caches). */
+ * new token, block table, and one arrival word, zero between calls, for both caches). As there, a
+ * token that fills page pg opens table entry pg + 1 in both caches, which the caller has claimed for
+ * this slot before the call (if pg + 1 < max_pages; an entry outside the pool opens nothing and is
+ * reported, EXKV_ERR_PAGE). A slot with lens 0 or past the table appends nothing; its query row is
+ * written, rotated at position 0, and reported (EXKV_ERR_POSITION). */
 int exkv_rope_append_paged(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v,
                            int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int32_t table_rows,
                            const void* q_norm, const void* k_norm, float eps, void* q_out, int32_t n, int32_t Hq, int32_t Hkv,
