@@ -151,12 +151,22 @@ __global__ void __launch_bounds__(64 * WAVES) norm_kernel(NormArgs a) {
     }
 }
 
+// A grid holds fewer than 2^32 threads: as many rows a launch.
 template <int WAVES, int CH>
-static void launch_norm(const NormArgs& a, bool v16, hipStream_t stream) {
-    if (v16)
-        hipLaunchKernelGGL((norm_kernel<WAVES, CH, true>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
-    else
-        hipLaunchKernelGGL((norm_kernel<WAVES, CH, false>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
+static void launch_norm(NormArgs a, bool v16, hipStream_t stream) {
+    constexpr int kMost = UINT32_MAX / (64 * WAVES);
+    for (int left = a.N; left > 0; left -= kMost) {
+        a.N = left < kMost ? left : kMost;
+        if (v16)
+            hipLaunchKernelGGL((norm_kernel<WAVES, CH, true>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
+        else
+            hipLaunchKernelGGL((norm_kernel<WAVES, CH, false>), dim3((unsigned)a.N), dim3(64 * WAVES), 0, stream, a);
+        a.x += a.N * a.sx;
+        if (a.r) a.r += a.N * a.sr;
+        if (a.gate) a.gate += a.N * a.sg;
+        if (a.h) a.h += (int64_t)a.N * a.C;
+        a.y += (int64_t)a.N * a.C;
+    }
 }
 
 }  // namespace exkv

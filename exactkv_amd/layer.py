@@ -390,7 +390,7 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, *, q_norm=None, k_norm=None
 def add_norm(x, residual, weight, *, eps=1e-6, post_weight=None, gate=None, scale=1.0):
     """The residual stream between two blocks: a block's output x onto it, and the RMS norm that
     feeds the next block. x bf16 [..., C] (C up to 16384); residual of x's shape, or None (the
-    stream starts with x); weight bf16 [C]. Returns (h, y), contiguous, of x's shape:
+    stream starts with x; fewer than 2^31 rows); weight bf16 [C]. Returns (h, y), contiguous, of x's shape:
 
         u = x, or x rsqrt(mean(x^2) + eps) post_weight     (post_weight: a norm behind the block)
         u = u gate                                         (gate: bf16 [C], or of x's shape)
@@ -413,6 +413,8 @@ def add_norm(x, residual, weight, *, eps=1e-6, post_weight=None, gate=None, scal
     if wp is None:
         raise ValueError("add_norm needs the norm's weight")
     xp, N, sx = _row_view(x, shape, dev, "x")
+    if N > 0x7FFFFFFF:
+        raise ValueError(f"add_norm takes fewer than 2^31 rows (got {N})")
     rp = gp = None
     sr = sg = 0
     if residual is not None:

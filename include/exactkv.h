@@ -532,7 +532,7 @@ int exkv_rope_append_paged_bf16(const void* q, int64_t sq_n, int64_t sq_h, const
  * times gate if given; h = r + scale u (r NULL: scale u); y = h rsqrt(mean(h^2) + eps) w. bf16
  * rows of C (1 to 16384) channels, x, r and gate with row strides sx, sr, sg in elements (sg 0: one
  * gate row for all), w and post_w [C], h (may be NULL) and y [N, C] contiguous; fp32 inside, h and y
- * rounded once each. One launch.
+ * rounded once each. One launch for each 2^22 rows (2^26 of up to 512 channels).
  * Replaces: engine.py:75-91 (the residual adds and norms of the model's own modules). */
 int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t sr, const void* w, const void* post_w,
                   const void* gate, int64_t sg, float scale, float eps, void* h, void* y, int32_t N, int32_t C,
