@@ -12,7 +12,7 @@
 // head r % G of token r / G: the G query heads of a KV head share its key and value tiles, and a tile
 // of rows spans few tokens, so little of it lies beyond the causal edge, at any G. Each wavefront owns
 // 32 rows and walks the visible keys 64 at a time (32 at head dim 256, whose registers then hold two
-// wavefronts a SIMD: 8K tokens at 16q/4kv 677 -> 546 us):
+// wavefronts a SIMD: 8K tokens at 16q/4kv 491 to 508 us):
 //   S^T = K Q^T   v_mfma_f32_32x32x16_bf16, keys as rows, the wavefront's rows as columns, so a
 //                 lane holds one column (row of the tile) and half of its 64 scores: maximum and
 //                 sum are in-lane plus one exchange between the two halves of the wavefront;
@@ -25,8 +25,9 @@
 // a row are XOR-swizzled so that the reads of one piece over 16 or 32 rows hit every bank (no bank
 // conflict counted).
 //
-// What bounds it: at 8K tokens, 32q/8kv, head dim 128, 490 us = 1,120 TFLOP/s, 0.85 of what a large
-// library product reaches here; both are held by power (1.76 GHz; the same call on zeros takes 359 us).
+// What bounds it: at 8K tokens, 32q/8kv, head dim 128, 485 to 501 us on several cards = 1,100 to 1,130
+// TFLOP/s, 0.83 to 0.86 of what a large library product reaches here; both are held by power (1.76 GHz; the
+// same call on zeros takes 359 us).
 // Two workgroups a CU (four at head dim 64) overlap one's matrix products with the other's
 // exponentials; one of eight wavefronts does so less (mixed prompts 79 / 68 us), three stages of keys
 // with a second barrier a tile cost more than they hide (continued prompts 78 / 93). A workgroup alone

@@ -10,7 +10,9 @@ way into the caches, and the residual stream with its norms.
   add_norm            a block's output onto the residual stream, and the next block's norm
 
 No counterpart in the reference, whose engine leaves all of this to the model's own modules
-(exactkv/engine.py:42-49,75-91). Everything is bf16 in and out and fp32 inside, rounded once.
+(exactkv/engine.py:42-49,75-91). Everything is bf16 in and out and fp32 inside, rounded once, but
+for the weights of prompt_attention's softmax, which are rounded to bf16 for the matrix product with
+the values (at most 2^-8 of each; the sum they are divided by is not).
 The tensors of a call are on one GPU; the work goes to that GPU's current stream, allocates
 nothing but the outputs (and a split prompt's partial results), waits for nothing, and can be
 captured in a HIP graph. No gradients are recorded.
