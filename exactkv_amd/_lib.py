@@ -13,7 +13,7 @@ _PATH = os.environ.get("EXACTKV_LIB") or os.path.join(os.path.dirname(os.path.ab
 # EXACTKV_CHECK_ERRORS=1: after every kernel-launching call, wait for its stream and raise if
 # a kernel set a sticky error bit (exkv_error_bits); slow, for debugging
 _CHECK = os.environ.get("EXACTKV_CHECK_ERRORS", "") not in ("", "0")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _p, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -95,6 +95,19 @@ SIGNATURES.update({
                                             _i32, _i32, _p],
     "exkv_rope_append_paged_bf16": _ROPE_ROWS + [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
     "exkv_add_norm": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _f32, _f32, _p, _p, _i32, _i32, _p],
+    "exkv_sample": [_p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _f32, _i32, _f32, _f32, _p, _p, _p],
+    "exkv_mass_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32],
+    "exkv_attention_mass": [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64,
+                            _i32, _f32, _p, _p, _i32, _p, _i64, _p],
+    "exkv_attention_mass_bf16": [_p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i32, _f32, _p, _p, _i32,
+                                 _p, _i64, _p],
+    "exkv_prompt_mass_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
+    "exkv_prompt_mass": [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p, _p,
+                         _i64, _p],
+    "exkv_select_tokens": [_p, _i64, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p, _p],
+    "exkv_gather_tokens": [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32,
+                           _p, _i32, _p, _p, _p],
+    "exkv_gather_tokens_bf16": [_p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i32, _p, _p, _p],
 })
 
 _lib = None
@@ -119,6 +132,7 @@ def load():
         f.argtypes = args
         f.restype = {"exkv_last_error": ctypes.c_char_p, "exkv_wire_bytes": ctypes.c_int64,
                      "exkv_noalloc_scratch_bytes": ctypes.c_int64, "exkv_prompt_workspace": ctypes.c_int64,
+                     "exkv_mass_workspace": ctypes.c_int64, "exkv_prompt_mass_workspace": ctypes.c_int64,
                      "exkv_merge_counters": ctypes.c_int64}.get(name, ctypes.c_int)
     v = lib.exkv_abi_version()
     if v != ABI_VERSION:
@@ -131,7 +145,7 @@ def load():
 
 
 # entry points that take no stream (host-only, or hooks)
-_NO_STREAM = {"exkv_wire_bytes", "exkv_prompt_workspace", "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
+_NO_STREAM = {"exkv_wire_bytes", "exkv_prompt_workspace", "exkv_mass_workspace", "exkv_prompt_mass_workspace", "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
               "exkv_plan_splits", "exkv_plan_splits_hd", "exkv_abi_version", "exkv_last_error", "exkv_error_bits",
               "exkv_set_wait_limit"}
 
@@ -145,6 +159,8 @@ ERROR_BITS = {
     0x20: "packed prompts: sequence offsets that do not ascend from 0 within the rows (clamped)",
     0x40: "rotation: a position outside the cosine and sine tables (clamped)",
     0x80: "rotated paged append: the table entry behind a page that a token filled lies outside the pool (no page opened)",
+    0x200: "gathered tokens: an index that is neither -1 nor a token of the cache (taken as -1)",
+    0x400: "sampling: a row without a logit that can be drawn (token 0)",
 }
 
 

@@ -1,0 +1,235 @@
+"""Caches that hold no more than a budget of tokens: the attention that cached tokens receive, and the eviction of those
+that receive the least.
+
+  attention_mass   a decode step's attention weights over its cached keys, added to what they had
+  prompt_mass      the same for the queries of packed prompts
+  select_tokens    which tokens of each KV head a budget keeps
+  gather_tokens    their keys and values out of a pair of caches
+  evict            the three parts of an eviction in place: selected, gathered, encoded again
+
+No counterpart in the reference, whose caches keep every token (exactkv/cache.py). Keys are cached with their rotation, so
+tokens that stay keep their positions wherever they are stored, and each KV head keeps its own. The tensors of a call are
+on one GPU; but for evict, the work goes to that GPU's current stream, waits for nothing and can be captured in a HIP
+graph."""
+import torch
+
+from . import _lib
+from .cache import BF16KV, CompressedKV
+from .kernels import _QK_SCALE, P, _block_table_arg, _cache_args, _cache_dim, _check_q, _lens_arg, _window_arg
+from .layer import _check_heads, _offsets, _on, _overlap, _rows
+from .paged import PagedBF16KV, PagedCompressedKV
+
+F32 = torch.float32
+
+
+def _is_bf16(c):
+    return isinstance(c, (BF16KV, PagedBF16KV, torch.Tensor))
+
+
+def _bf16_rows(c, dev, what):
+    """The tensor [B, TS, H, D] of a bf16 cache."""
+    t = c if isinstance(c, torch.Tensor) else c.buf
+    if t.dtype is not torch.bfloat16 or t.dim() != 4 or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what} must be a contiguous bf16 [B, TS, H, D] tensor on the call's GPU")
+    _lib.ptr(t, what=what)
+    return t
+
+
+def _compressed(c, dev, what):
+    """(pointers and raw rows, TS, H, B, D) of a compressed cache on GPU `dev`."""
+    args, TS, H, B = _cache_args(c)
+    raw = c["raw"] if isinstance(c, dict) else c.raw
+    if raw.get_device() != dev:
+        raise ValueError(f"{what} must be on the call's GPU")
+    return args, TS, H, B, _cache_dim(c)
+
+
+def _table(block_table, B, dev):
+    """(pointer, stride, capacity) of a block table, or (None, 0, None)."""
+    if block_table is None:
+        return None, 0, None
+    if block_table.get_device() != dev:
+        raise ValueError("block_table must be on the call's GPU")
+    return _block_table_arg(block_table, B)
+
+
+def _lens_on(lens, B, dev):
+    if lens is not None and lens.get_device() != dev:
+        raise ValueError("lens must be on the call's GPU")
+    return _lens_arg(lens, B)
+
+
+def _tokens(T, TS, lens, what):
+    """The token count of a call without lens."""
+    if lens is not None:
+        return TS
+    if T is None:
+        raise ValueError(f"{what} needs T or lens")
+    if not 0 <= int(T) <= TS:
+        raise ValueError(f"{int(T)} tokens of a capacity of {TS}")
+    return int(T)
+
+
+def _mass_rows(t, shape, dev, what):
+    if t.dtype is not F32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous fp32 {list(shape)} tensor on the call's GPU")
+    return t.data_ptr()
+
+
+def attention_mass(q, k_cache, T=None, *, mass=None, lens=None, block_table=None, window=0, out=None):
+    """The attention that cached tokens receive from one query token of each sequence, added to what they had:
+
+        out[b, h, j] = mass[b, h, j] + sum of softmax_j(q[b, g] . k[b, j, h] / sqrt(D)) over the query heads g of KV head h
+
+    q bf16 [B, Hq, D] as decode_attention takes it. k_cache: the keys' cache, any of the four kinds (paged: rows as in
+    decode_attention's current step), or a buffers() dict, or a bf16 tensor [B, TS, Hkv, D]; T, lens (int32, one entry or one
+    per sequence), block_table and window as in attention_compressed. The softmax is over the tokens the window admits; the
+    others get nothing. mass: fp32 [B, Hkv, TS], TS the cache's capacity in tokens (16 per entry of a block table's row), or
+    None for 0. Returns out, new, or the one given, which may be mass itself; its entries behind a sequence's tokens are
+    left as they are (0 in a new one)."""
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return attention_mass(q, k_cache, T, mass=mass, lens=lens, block_table=block_table, window=window, out=out)
+    B, Hq, D = _check_q(q)
+    if isinstance(k_cache, (PagedCompressedKV, PagedBF16KV)) and block_table is None:
+        _, block_table, lens = k_cache.table.step_rows()
+    elif T is None and lens is None and isinstance(k_cache, (CompressedKV, BF16KV)):
+        T = k_cache.T
+    bt, stride, capacity = _table(block_table, B, dev)
+    if _is_bf16(k_cache):
+        t = _bf16_rows(k_cache, dev, "k_cache")
+        held, TS, Hkv, Dk = t.shape
+        name, cache = "exkv_attention_mass_bf16", (t.data_ptr(),)
+    else:
+        cache, TS, Hkv, held, Dk = _compressed(k_cache, dev, "k_cache")
+        name = "exkv_attention_mass"
+    _check_heads(Hq, Hkv, D)
+    if Dk != D:
+        raise ValueError(f"cache head dim {Dk} differs from q's {D}")
+    if block_table is None:
+        if held < B:
+            raise ValueError(f"the cache holds {held} sequences, q {B}")
+        pages = 0
+    else:
+        pages, TS = held * TS // P, capacity
+    T = _tokens(T, TS, lens, "attention_mass")
+    lp, lstride = _lens_on(lens, B, dev)
+    window = _window_arg(window)
+    if window > 0x7FFFFFFF:
+        raise ValueError(f"window must be >= 0 (got {window})")
+    shape = (B, Hkv, TS)
+    mp = None if mass is None else _mass_rows(mass, shape, dev, "mass")
+    fresh = out is None
+    if fresh:
+        out = torch.empty(shape, dtype=F32, device=q.device)
+        op = out.data_ptr()
+    else:
+        op = _mass_rows(out, shape, dev, "out")
+        if mass is not None and op != mp and _overlap(out, mass):
+            raise ValueError("out overlaps mass")
+    need = _lib.load().exkv_mass_workspace(B, Hq, Hkv, T, TS, lens is not None, window)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    _lib.call(name, q.data_ptr(), *cache, bt, stride, pages, B, Hq, Hkv, D, T, TS, lp, lstride, window, _QK_SCALE[D], mp, op, fresh,
+              ws.data_ptr(), need, _lib.stream(dev))
+    return out
+
+
+def prompt_mass(q, k, cu_seqlens, *, cu_seqlens_k=None, window=0, last=0):
+    """The attention that the keys of packed prompts receive from their queries: q, k, cu_seqlens, cu_seqlens_k and window
+    as in prompt_attention. Returns fp32 [Hkv, NK]: for each key and KV head the sum of the weights (softmax over the
+    keys each query sees) of its sequence's queries, or with last > 0 of its last `last` ones, over the query heads of the
+    KV head; 0 for keys that no sequence holds. A query that sees no key gives nothing."""
+    dev = q.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return prompt_mass(q, k, cu_seqlens, cu_seqlens_k=cu_seqlens_k, window=window, last=last)
+    N, Hq, D, sq_t, sq_h = _rows(q, dev, "q")
+    NK, Hkv, Dk, sk_t, sk_h = _rows(k, dev, "k")
+    _check_heads(Hq, Hkv, D)
+    if Dk != D:
+        raise ValueError(f"k must be [keys, heads, {D}] (got {tuple(k.shape)})")
+    cu, S = _offsets(cu_seqlens, dev, "cu_seqlens")
+    if cu_seqlens_k is None:
+        cu_k = cu
+        if NK != N:
+            raise ValueError(f"{NK} keys for {N} queries: give cu_seqlens_k")
+    else:
+        cu_k, Sk = _offsets(cu_seqlens_k, dev, "cu_seqlens_k")
+        if Sk != S:
+            raise ValueError("cu_seqlens and cu_seqlens_k must hold as many sequences")
+    window, last = int(window or 0), int(last or 0)
+    if not 0 <= window <= 0x7FFFFFFF or not 0 <= last <= 0x7FFFFFFF:
+        raise ValueError(f"window and last must be >= 0 (got {window}, {last})")
+    out = torch.empty(Hkv, NK, dtype=F32, device=q.device)
+    need = _lib.load().exkv_prompt_mass_workspace(S, N, NK, Hq, Hkv, D, window, last)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    _lib.call("exkv_prompt_mass", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, cu, cu_k, S, N, NK, Hq, Hkv, D, window, last,
+              _QK_SCALE[D], out.data_ptr(), ws.data_ptr(), need, _lib.stream(dev))
+    return out
+
+
+def select_tokens(mass, keep, T=None, *, lens=None, sinks=0, recent=0):
+    """Which `keep` tokens each KV head of each sequence keeps, by mass fp32 [B, H, TS] (rows contiguous): the first `sinks`,
+    the latest `recent`, and of those between the ones with the most mass, of equal ones the first (NaN counts as
+    the least). A sequence has T tokens, or lens[b] (int32, one entry or one per sequence). Returns (index int32 [B, H,
+    keep], their mass fp32 [B, H, keep]), tokens ascending; of a sequence of fewer tokens all, then -1 and 0."""
+    dev = mass.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return select_tokens(mass, keep, T, lens=lens, sinks=sinks, recent=recent)
+    if mass.dtype is not F32 or mass.dim() != 3 or dev < 0:
+        raise ValueError("mass must be an fp32 [B, H, TS] GPU tensor")
+    B, H, TS = mass.shape
+    if TS > 1 and mass.stride(2) != 1:
+        raise ValueError("mass: rows (the last axis) must be contiguous")
+    keep, sinks, recent = int(keep), int(sinks), int(recent)
+    if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"{sinks} first and {recent} latest tokens of {keep} kept")
+    T = _tokens(T, TS, lens, "select_tokens")
+    lp, lstride = _lens_on(lens, B, dev)
+    index = torch.empty(B, H, keep, dtype=torch.int32, device=mass.device)
+    kept = torch.empty(B, H, keep, dtype=F32, device=mass.device)
+    _lib.call("exkv_select_tokens", mass.data_ptr(), mass.stride(0) if B > 1 else 0, mass.stride(1) if H > 1 else 0, lp, lstride, T, B, H,
+              TS, keep, sinks, recent, index.data_ptr(), kept.data_ptr(), _lib.stream(dev))
+    return index, kept
+
+
+def gather_tokens(k_cache, v_cache, index, *, block_table=None):
+    """Tokens of each KV head out of a pair of caches of one kind (cache objects, buffers() dicts, or bf16 tensors [B, TS, H,
+    D]): row i of head h of sequence b is token index[b, h, i] (int32 [B, H, n]). block_table: the caches are pools of pages,
+    as in attention_compressed (of paged cache objects their table's, a row for each slot, where none is given). Returns
+    two bf16 tensors [B, n, H, D], with zeros where the index is -1; any other index outside the cache counts as -1 and sets
+    an error bit (kernels.check_errors)."""
+    dev = index.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return gather_tokens(k_cache, v_cache, index, block_table=block_table)
+    if index.dtype is not torch.int32 or index.dim() != 3 or not index.is_contiguous() or dev < 0:
+        raise ValueError("index must be a contiguous int32 [B, H, n] GPU tensor")
+    B, H, n = index.shape
+    if block_table is None and isinstance(k_cache, (PagedCompressedKV, PagedBF16KV)):
+        block_table = k_cache.table.block_table
+    bt, stride, capacity = _table(block_table, B, dev)
+    if _is_bf16(k_cache) != _is_bf16(v_cache):
+        raise ValueError("k_cache and v_cache must be of one kind")
+    if _is_bf16(k_cache):
+        k, v = _bf16_rows(k_cache, dev, "k_cache"), _bf16_rows(v_cache, dev, "v_cache")
+        held, TS, Hc, D = k.shape
+        other = v.shape
+        name, caches = "exkv_gather_tokens_bf16", (k.data_ptr(), v.data_ptr())
+    else:
+        ka, TS, Hc, held, D = _compressed(k_cache, dev, "k_cache")
+        va, *other = _compressed(v_cache, dev, "v_cache")
+        other = (other[2], other[0], other[1], other[3])
+        name, caches = "exkv_gather_tokens", (*ka, *va)
+    if tuple(other) != (held, TS, Hc, D):
+        raise ValueError(f"the caches differ in shape ({(held, TS, Hc, D)} and {tuple(other)})")
+    if Hc != H or (block_table is None and held < B):
+        raise ValueError(f"index is for {B} sequences of {H} heads, the caches hold {held} of {Hc}")
+    pages = 0
+    if block_table is not None:
+        pages, TS = held * TS // P, capacity
+    out = [torch.empty(B, n, H, D, dtype=torch.bfloat16, device=index.device) for _ in range(2)]
+    _lib.call(name, *caches, bt, stride, pages, B, H, TS, D, index.data_ptr(), n, out[0].data_ptr(), out[1].data_ptr(), _lib.stream(dev))
+    return tuple(out)

@@ -125,6 +125,10 @@ hipError_t fetch_errors_encode(uint32_t* out, int first, int clear, hipStream_t 
 hipError_t fetch_errors_wire(uint32_t* out, int first, int clear, hipStream_t stream);
 hipError_t fetch_errors_prompt(uint32_t* out, int first, int clear, hipStream_t stream);
 hipError_t fetch_errors_rope(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_mass(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_evict(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_sample(uint32_t* out, int first, int clear, hipStream_t stream);
+hipError_t fetch_errors_prompt_mass(uint32_t* out, int first, int clear, hipStream_t stream);
 }  // namespace exkv
 
 #define EXKV_OK 0

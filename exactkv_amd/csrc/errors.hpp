@@ -26,6 +26,8 @@ enum : uint32_t {
     kErrOffsets = 1u << 5,   // packed prompts: sequence offsets that do not ascend from 0 within the rows
     kErrPosition = 1u << 6,  // rotation: a position outside the cosine / sine tables
     kErrPage = 1u << 7,      // rotated paged append: the table entry behind a page that a token filled names no page
+    kErrIndex = 1u << 9,     // gathered tokens: an index that is neither -1 nor a token of the cache
+    kErrLogits = 1u << 10,   // sampling: a row without a logit that can be drawn
 };
 
 static __device__ uint32_t file_error_word;

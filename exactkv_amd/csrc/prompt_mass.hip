@@ -1,0 +1,477 @@
+// The attention that a packed prompt's keys receive from its queries, for gfx950 (no counterpart in the reference): with
+// sequences, positions and visible keys as in prompt attention, for key j of KV head h
+//     out[h, j] = sum over the queries t (of each sequence the last `last`, or all) and the query heads g of h of
+//                 softmax_j(q[t, g] . k[j, h] / sqrt(D)),
+// 0 for keys that no sequence holds.
+//
+// Two passes over the products, since a weight needs its row's sum first. In both, one side of the product stands in
+// registers, the other comes through LDS in two stages of 64 rows (32 at head dim 256), brought by direct loads, and
+// S^T = K Q^T is made by v_mfma_f32_32x32x16_bf16 with keys as rows, so that a lane holds one query row (column) of 32
+// and 16 keys of each block:
+//   rows     a wavefront holds 64 query rows (row r of a sequence is query head r % G of token r / G) and walks the
+//            keys they see: log2 of each row's sum of 2^s (s the score in log2 units), relative to the largest score of
+//            the first tile with a visible key. Later scores need no maximum: fp32 holds sums of weights up to 2^127,
+//            smaller ones lose nothing, and a sum that leaves the range is made again with a running maximum.
+//   columns  a wavefront holds 64 keys and walks the tokens that see them, one query head after the other, adding up
+//            2^(s - log2 sum) of each key; the 32 lanes of a key are added at the end.
+// Both are cut into parts where there are few tiles; parts are joined in order, so a call's bits do not change.
+#include "errors.hpp"
+#include "prompt_stage.hpp"
+#include "../../include/exactkv.h"
+
+namespace exkv {
+
+constexpr float kLowest = -1e30f;      // a maximum before any key, in log2 units
+constexpr int kTile = 256;             // rows, or keys, of a workgroup: 64 a wavefront
+
+struct PromptMassArgs {
+    const uint16_t *q, *k;             // rows of D channels, element strides below
+    int64_t sq_t, sq_h, sk_t, sk_h;
+    const int32_t *cu_q, *cu_k;        // [S + 1]
+    int S, N, NK, Hq, Hkv, G, window, last;
+    float qk_scale;                    // log2(e) / sqrt(D)
+    int row_parts, col_parts;
+    float2* part;                      // [row_parts, Hq, N]: maximum, sum
+    float* lse;                        // [Hq, N]: log2 of a row's sum; infinity where it sees no key
+    float* sums;                       // [col_parts, Hkv, NK]
+    float* out;                        // [Hkv, NK]
+};
+
+// Sequence s's queries that count, and its keys.
+__device__ inline void counted_sequence(const PromptMassArgs& a, int s, int& q0, int& Lq, int& k0, int& Lk) {
+    const bool bad = clip_sequence(a.cu_q[s], a.cu_q[s + 1], s == 0, a.N, q0, Lq);
+    const bool bad_k = clip_sequence(a.cu_k[s], a.cu_k[s + 1], s == 0, a.NK, k0, Lk);
+    if (bad | bad_k) report_error(kErrOffsets);
+    if (a.last > 0 && Lq > a.last) {
+        q0 += Lq - a.last;
+        Lq = a.last;
+    }
+}
+
+// The tile to take `t`-th, of kTile rows or keys: sequence by sequence, the tiles with the most to walk first (a
+// sequence's last rows, its first keys). row0 counts rows, or keys. False where t is past them all.
+template <bool ROWS>
+__device__ inline bool tile_at(const PromptMassArgs& a, int t, PromptTile& tile) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        int q0 = 0, Lq = 0, k0 = 0, Lk = 0;
+        if (s0 + lane < a.S) counted_sequence(a, s0 + lane, q0, Lq, k0, Lk);
+        const int n = (int)(((ROWS ? (int64_t)Lq * a.G : (int64_t)Lk) + kTile - 1) / kTile);
+        const int incl = wave_incl_scan(n), total = __builtin_amdgcn_readlane(incl, 63);
+        if (t < total) {
+            const int l = max(0, first_lane(__ballot(incl > t)));
+            const int end = __builtin_amdgcn_readlane(incl, l), count = __builtin_amdgcn_readlane(n, l);
+            const int index = ROWS ? end - 1 - t : t - (end - count);
+            tile.q0 = __builtin_amdgcn_readlane(q0, l);
+            tile.Lq = __builtin_amdgcn_readlane(Lq, l);
+            tile.k0 = __builtin_amdgcn_readlane(k0, l);
+            tile.Lk = __builtin_amdgcn_readlane(Lk, l);
+            tile.row0 = index * kTile;
+            return index >= 0 && index < count;
+        }
+        t -= total;
+    }
+    return false;
+}
+
+// Every load so far has landed, and every wavefront's LDS reads of the stage loaded into next have returned.
+__device__ inline void next_stage() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A stage's geometry: SR rows of D channels.
+template <int D>
+struct Stage {
+    static constexpr int SR = keys_per_tile(D), SB = SR / 32, KS = D / 16, BYTES = SR * 2 * D;
+    static constexpr int PIECES = D / 8, RPI = 64 / PIECES, LOADS = BYTES / 1024 / kWaves;
+    // lane's byte offsets of the wavefront's loads, row pitch s_t elements
+    __device__ static void offsets(int w, int lane, int64_t s_t, uint32_t (&off)[LOADS]) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (w * LOADS + i) * RPI + lane / PIECES, c = lane % PIECES;
+            off[i] = (uint32_t)(r * (int)s_t * 2 + (c ^ key_swizzle<D>(r)) * 16 - i * 1024);
+        }
+    }
+    // the operand piece of block b, k-step s
+    __device__ static bf16x8 piece(const uint8_t* lds, int st, int rd, int b, int s) {
+        return *(const EXKV_LDS bf16x8*)((const EXKV_LDS uint8_t*)lds + st * BYTES + (rd ^ ((s & 7) << 5)) + (s >> 3) * 256 +
+                                         b * 32 * 2 * D);
+    }
+    __device__ static int read_at(int col, int half) { return col * 2 * D + (half ^ key_swizzle<D>(col)) * 16; }
+};
+
+template <int D>
+__global__ void __launch_bounds__(64 * kWaves) mass_rows_kernel(PromptMassArgs a) {
+    typedef Stage<D> St;
+    constexpr int KS = St::KS, SR = St::SR, SB = St::SB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * St::BYTES];
+    __shared__ int s_again;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
+    const int part = rest % a.row_parts;
+    PromptTile tile;
+    if (!tile_at<true>(a, rest / a.row_parts, tile)) return;
+    const int col = lane & 31, half = lane >> 5, G = a.G, nrows = tile.Lq * G, shift = tile.Lk - tile.Lq;
+    const int wrow0 = tile.row0 + 64 * w;
+    const bool wave_on = wrow0 < nrows;
+    const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
+    int tok[2], hq[2], pos[2];
+    bf16x8 qf[2][KS];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+        const int row = min(wrow0 + 32 * rb + col, nrows - 1);
+        tok[rb] = row / G;
+        hq[rb] = hk * G + row % G;
+        pos[rb] = tok[rb] + shift;
+        const uint16_t* qp = a.q + (int64_t)(tile.q0 + tok[rb]) * a.sq_t + hq[rb] * a.sq_h + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[rb][s] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * s));
+    }
+    const int w_lo = __builtin_amdgcn_readfirstlane(pos[0]), w_hi = __builtin_amdgcn_readlane(pos[1], 31);
+    int first, last;
+    {
+        const int t_lo = tile.row0 / G, t_hi = min(tile.row0 + kTile - 1, nrows - 1) / G;
+        const int k_lo = a.window > 0 ? max(0, t_lo + shift - a.window + 1) : 0, k_hi = t_hi + shift;
+        first = k_lo / SR;
+        last = k_hi < 0 ? first - 1 : k_hi / SR;
+        const int per = (last - first + a.row_parts) / a.row_parts;
+        first += part * per;
+        last = min(last, first + per - 1);
+    }
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(EXKV_LDS uint8_t*)lds) + w * St::LOADS * 1024;
+    uint32_t off[St::LOADS];
+    St::offsets(w, lane, a.sk_t, off);
+    const int rd = St::read_at(col, half);
+    float m[2], l[2];
+    auto walk = [&](auto safe) {
+        constexpr bool SAFE = decltype(safe)::value;
+        m[0] = m[1] = kLowest;
+        l[0] = l[1] = 0.f;
+        if (first > last) return;
+        Stream<D, SR> keys(a.k, a.sk_t, hk * a.sk_h, tile, first * SR);
+        auto load = [&](int st) {
+            each<St::LOADS>([&](auto i) { load_piece<i.value>(keys.buf, off[i.value], lds0 + st * St::BYTES); });
+            keys.next();
+        };
+        load(0);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[rb][s]));
+        for (int it = first; it <= last; ++it) {
+            const int st = (it - first) & 1, j0 = it * SR;
+            next_stage();
+            if (it < last) load(st ^ 1);
+            if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + SR - 1 <= w_lo - a.window)) continue;   // uniform: none seen
+            const bool all = j0 + SR - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window);
+#pragma unroll
+            for (int kb = 0; kb < SB; ++kb) {
+                f32x16 sc[2];
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[rb][i] = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const bf16x8 kf = St::piece(lds, st, rd, kb, s);
+#pragma unroll
+                    for (int rb = 0; rb < 2; ++rb) sc[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rb][s], sc[rb], 0, 0, 0);
+                }
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    if (!all) {
+                        const int rel = pos[rb] - j0 - 4 * half;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) sc[rb][i] = -INFINITY;
+                    }
+                    if (SAFE || __ballot(m[rb] == kLowest) != 0) {
+                        float mx = sc[rb][0];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[rb][i]);
+                        mx = fmaxf(mx * a.qk_scale, kLowest);
+                        if (SAFE ? mx > m[rb] : m[rb] == kLowest) {
+                            l[rb] *= exp2_fast(m[rb] - mx);
+                            m[rb] = mx;
+                        }
+                    }
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[i & 1] += exp2_fast(fmaf(sc[rb][i], a.qk_scale, -m[rb]));
+                    l[rb] += sum[0] + sum[1];
+                }
+            }
+        }
+    };
+    if (threadIdx.x == 0) s_again = 0;
+    walk(std::false_type{});
+    __syncthreads();
+    if (!(l[0] < INFINITY) || !(l[1] < INFINITY)) s_again = 1;
+    __syncthreads();
+    if (s_again != 0) walk(std::true_type{});          // uniform
+    if (!wave_on) return;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+        const float m2 = __shfl_xor(m[rb], 32), l2 = __shfl_xor(l[rb], 32), M = fmaxf(m[rb], m2);
+        const float sum = l[rb] * exp2_fast(m[rb] - M) + l2 * exp2_fast(m2 - M);
+        if (half != 0 || wrow0 + 32 * rb + col >= nrows) continue;
+        const int64_t at = (int64_t)hq[rb] * a.N + tile.q0 + tok[rb];
+        if (a.row_parts > 1)
+            a.part[(int64_t)part * a.Hq * a.N + at] = make_float2(M, sum);
+        else
+            a.lse[at] = sum == 0.f ? INFINITY : M + __builtin_amdgcn_logf(sum);
+    }
+}
+
+// The parts of every row joined.
+__global__ void __launch_bounds__(256) mass_rows_join_kernel(PromptMassArgs a) {
+    const int64_t n = (int64_t)a.Hq * a.N, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n) return;
+    float M = kLowest, l = 0.f;
+    for (int i = 0; i < a.row_parts; ++i) {
+        const float2 x = a.part[i * n + at];
+        const float m = fmaxf(M, x.x);
+        l = l * exp2_fast(M - m) + x.y * exp2_fast(x.x - m);
+        M = m;
+    }
+    a.lse[at] = l == 0.f ? INFINITY : M + __builtin_amdgcn_logf(l);
+}
+
+template <int D>
+__global__ void __launch_bounds__(64 * kWaves) mass_columns_kernel(PromptMassArgs a) {
+    typedef Stage<D> St;
+    constexpr int KS = St::KS, SR = St::SR, SB = St::SB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * St::BYTES];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
+    const int part = rest % a.col_parts;
+    PromptTile tile;
+    if (!tile_at<false>(a, rest / a.col_parts, tile)) return;
+    const int col = lane & 31, half = lane >> 5, G = a.G, shift = tile.Lk - tile.Lq;
+    const int key0 = tile.row0, wkey0 = key0 + 64 * w;
+    const bool wave_on = wkey0 < tile.Lk;
+    const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7FFFFFFFu;
+    bf16x8 kf[2][KS];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const uint16_t* kp = a.k + (int64_t)(tile.k0 + min(wkey0 + 32 * kb + col, tile.Lk - 1)) * a.sk_t + hk * a.sk_h + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[kb][s] = __builtin_bit_cast(bf16x8, ld16(kp + 16 * s));
+    }
+    // tokens that see one of the workgroup's keys, in tiles of SR
+    const int key_hi = min(key0 + kTile, tile.Lk) - 1;
+    const int t_lo = max(0, key0 - shift), t_hi = a.window > 0 ? (int)min((int64_t)tile.Lq - 1, (int64_t)key_hi - shift + a.window - 1) : tile.Lq - 1;
+    const int first = t_lo / SR, tiles = t_hi < t_lo ? 0 : t_hi / SR - first + 1;
+    const int64_t steps = (int64_t)G * tiles, per = (steps + a.col_parts - 1) / a.col_parts;
+    const int64_t begin = min(steps, part * per), end = min(steps, begin + per);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(EXKV_LDS uint8_t*)lds) + w * St::LOADS * 1024;
+    uint32_t off[St::LOADS];
+    St::offsets(w, lane, a.sq_t, off);
+    const int rd = St::read_at(col, half);
+    f32x16 acc[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[kb][i] = 0.f;
+    // rows are tokens of one query head at a time: a "sequence" of Lq rows at the head's channels
+    PromptTile rows = tile;
+    rows.k0 = tile.q0;
+    rows.Lk = tile.Lq;
+    int g = tiles > 0 ? (int)(begin / tiles) : 0, t = tiles > 0 ? (int)(begin % tiles) : 0;
+    float next_lse[SB];
+    int gl = g, tl = t;                                // of the loads
+    auto load = [&](int st) {
+        Stream<D, SR> s(a.q, a.sq_t, (hk * G + gl) * a.sq_h, rows, (first + tl) * SR);
+        each<St::LOADS>([&](auto i) { load_piece<i.value>(s.buf, off[i.value], lds0 + st * St::BYTES); });
+#pragma unroll
+        for (int rb = 0; rb < SB; ++rb) {
+            const int tok = (first + tl) * SR + 32 * rb + col;
+            next_lse[rb] = tok < tile.Lq ? a.lse[(int64_t)(hk * G + gl) * a.N + tile.q0 + tok] : INFINITY;
+        }
+        if (++tl == tiles) {
+            tl = 0;
+            ++gl;
+        }
+    };
+    if (begin < end) load(0);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(kf[kb][s]));
+    for (int64_t step = begin; step < end; ++step) {
+        const int st = (int)(step - begin) & 1, t0 = (first + t) * SR;
+        next_stage();
+        float lse[SB];
+#pragma unroll
+        for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
+        if (step + 1 < end) load(st ^ 1);
+        if (++t == tiles) t = 0;
+        const int p_lo = t0 + shift, p_hi = p_lo + SR - 1;
+        if (!wave_on || p_hi < wkey0 || (a.window > 0 && p_lo - (wkey0 + 63) >= a.window)) continue;   // uniform: none sees
+        const bool all = p_lo >= wkey0 + 63 && (a.window == 0 || p_hi - wkey0 < a.window);
+#pragma unroll
+        for (int rb = 0; rb < SB; ++rb) {
+            f32x16 sc[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const bf16x8 qf = St::piece(lds, st, rd, rb, s);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][s], qf, sc[kb], 0, 0, 0);
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int rel = p_lo + 32 * rb + col - wkey0 - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = exp2_fast(fmaf(sc[kb][i], a.qk_scale, -lse[rb]));
+                    // (after the exponential: a row's sum may be NaN)
+                    if (!all && (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) x = 0.f;
+                    acc[kb][i] += x;
+                }
+            }
+        }
+    }
+    if (!wave_on) return;
+    // over the 32 lanes of a key: halving the values with the lanes, so that lane c of a half ends up with value
+    // c >> 1 of a block, which is key 8 (c >> 3) + 4 half + (c >> 1 & 3)
+    float* out = a.sums + ((int64_t)part * a.Hkv + hk) * a.NK + tile.k0;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[kb][i];
+#pragma unroll
+        for (int n = 8, d = 16; n > 0; n >>= 1, d >>= 1) {
+            const bool upper = (lane & d) != 0;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const float send = upper ? v[i] : v[i + n], keep = upper ? v[i + n] : v[i];
+                v[i] = keep + __shfl_xor(send, d);
+            }
+        }
+        v[0] += __shfl_xor(v[0], 1);
+        const int i = col >> 1, key = wkey0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
+        if ((col & 1) == 0 && key < tile.Lk) out[key] = v[0];
+    }
+}
+
+// The parts of every key added up; 0 behind the last sequence.
+__global__ void __launch_bounds__(256) mass_columns_join_kernel(PromptMassArgs a) {
+    const int64_t n = (int64_t)a.Hkv * a.NK, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n) return;
+    const int end = a.S > 0 ? min(max(a.cu_k[a.S], 0), a.NK) : 0;
+    float sum = 0.f;
+    if ((int)(at % a.NK) < end)
+        for (int i = 0; i < a.col_parts; ++i) sum += a.sums[i * n + at];
+    a.out[at] = sum;
+}
+
+hipError_t fetch_errors_prompt_mass(uint32_t* out, int first, int clear, hipStream_t stream) {
+    return fetch_file_errors(out, first, clear, stream);
+}
+
+// How a call is laid out: tiles at most (every sequence's last may be partial), and the parts of each, so that there
+// are about 1,024 workgroups with a few steps each.
+struct MassPlan {
+    int64_t row_tiles, col_tiles;
+    int row_parts, col_parts;
+    int64_t part_bytes, lse_bytes, sum_bytes;
+};
+static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t Hkv, int D, int64_t window, int64_t last) {
+    MassPlan p{};
+    const int64_t G = Hq / Hkv, SR = keys_per_tile(D);
+    const int64_t rows = last > 0 && S < N / last + 1 && S * last < N ? S * last : N;
+    p.row_tiles = (rows * G + S * (kTile - 1)) / kTile;
+    p.col_tiles = (NK + S * (kTile - 1)) / kTile;
+    const int64_t reach = window > 0 && window + kTile < NK ? window + kTile : NK;
+    auto cut = [&](int64_t units, int64_t steps) {
+        int64_t parts = units > 0 ? 1024 / units : 1;
+        if (parts > steps / 8) parts = steps / 8;
+        if (parts > 64) parts = 64;
+        return (int)(parts < 1 ? 1 : parts);
+    };
+    p.row_parts = cut(p.row_tiles * Hkv, (reach + SR - 1) / SR);
+    const int64_t most = last > 0 && last < N ? last : N, seen = window > 0 && window + kTile < most ? window + kTile : most;
+    p.col_parts = cut(p.col_tiles * Hkv, (seen + SR - 1) / SR * G);
+    p.part_bytes = p.row_parts > 1 ? p.row_parts * Hq * N * 8 : 0;
+    p.lse_bytes = (Hq * N * 4 + 15) / 16 * 16;
+    p.sum_bytes = (p.col_parts * Hkv * NK * 4 + 15) / 16 * 16;
+    return p;
+}
+
+template <int D>
+static void launch_prompt_mass(const PromptMassArgs& a, const MassPlan& p, hipStream_t stream) {
+    const dim3 block(64 * kWaves);
+    hipLaunchKernelGGL((mass_rows_kernel<D>), dim3((unsigned)(p.row_tiles * a.Hkv * a.row_parts)), block, 0, stream, a);
+    if (a.row_parts > 1)
+        hipLaunchKernelGGL(mass_rows_join_kernel, dim3((unsigned)(((int64_t)a.Hq * a.N + 255) / 256)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((mass_columns_kernel<D>), dim3((unsigned)(p.col_tiles * a.Hkv * a.col_parts)), block, 0, stream, a);
+}
+
+}  // namespace exkv
+
+using namespace exkv;
+
+static bool rows_ok(const void* p, int64_t s_t, int64_t s_h) {
+    return (uintptr_t)p % 16 == 0 && s_t % 8 == 0 && s_h % 8 == 0 && s_t >= 0 && s_h >= 0;
+}
+
+extern "C" int64_t exkv_prompt_mass_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window,
+                                              int32_t last) {
+    if (!head_dim_ok(D) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || S < 0 || N <= 0 || NK <= 0 || window < 0 || last < 0) return 0;
+    const MassPlan p = plan_mass(S, N, NK, Hq, Hkv, D, window, last);
+    return p.part_bytes + p.lse_bytes + p.sum_bytes;
+}
+
+extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                                const int32_t* cu_q, const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv,
+                                int32_t D, int32_t window, int32_t last, float qk_scale, float* out, void* ws, int64_t ws_bytes,
+                                hipStream_t stream) {
+    EXKV_REQUIRE(head_dim_ok(D), "prompt_mass: head dim must be 64, 128 or 256 (got %d)", D);
+    EXKV_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "prompt_mass: %d query heads over %d KV heads", Hq, Hkv);
+    EXKV_REQUIRE(S >= 0 && N >= 0 && NK >= 0 && window >= 0 && last >= 0, "prompt_mass: bad shape S=%d N=%d NK=%d window=%d last=%d", S, N,
+                 NK, window, last);
+    if (NK == 0) return EXKV_OK;
+    EXKV_REQUIRE(out && cu_q && cu_k && k && (q || N == 0), "prompt_mass: null pointer");
+    EXKV_REQUIRE((N == 0 || rows_ok(q, sq_t, sq_h)) && rows_ok(k, sk_t, sk_h),
+                 "prompt_mass: rows must be 16-byte aligned, with strides of whole 16 bytes");
+    // a stage of rows is one 32-bit window whose rows lie at least a row apart
+    EXKV_REQUIRE(sk_t >= D && sk_t <= (1 << 23) && (N == 0 || (sq_t >= D && sq_t <= (1 << 23))),
+                 "prompt_mass: query and key rows must lie %d to %d elements apart", D, 1 << 23);
+    const int64_t G = Hq / Hkv;
+    if (window > NK) window = NK;                      // no sequence is longer; sums of positions stay in 32 bits
+    if (last > N) last = N;
+    EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 && (int64_t)N + 2 * (int64_t)NK < INT32_MAX - 1024,
+                 "prompt_mass: too many rows (N=%d, NK=%d, %d heads per KV head)", N, NK, (int)G);
+    const MassPlan p = plan_mass(S, N, NK, Hq, Hkv, D, window, last);
+    EXKV_REQUIRE(p.row_tiles * p.row_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX &&
+                     p.col_tiles * p.col_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX &&
+                     (int64_t)Hq * N <= (int64_t)UINT32_MAX && (int64_t)Hkv * NK <= (int64_t)UINT32_MAX,
+                 "prompt_mass: too many rows (N=%d, NK=%d, %d query heads, %d KV heads, S=%d)", N, NK, Hq, Hkv, S);
+    PromptMassArgs a{(const uint16_t*)q, (const uint16_t*)k, sq_t, sq_h, sk_t, sk_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, last,
+                     qk_scale, p.row_parts, p.col_parts, nullptr, nullptr, nullptr, out};
+    if (N > 0 && S > 0) {
+        const int64_t need = p.part_bytes + p.lse_bytes + p.sum_bytes;
+        EXKV_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "prompt_mass: workspace of %lld bytes, %lld needed",
+                     (long long)ws_bytes, (long long)need);
+        a.lse = (float*)ws;
+        a.sums = (float*)((uint8_t*)ws + p.lse_bytes);
+        a.part = (float2*)((uint8_t*)ws + p.lse_bytes + p.sum_bytes);
+        if (D == 64)
+            launch_prompt_mass<64>(a, p, stream);
+        else if (D == 128)
+            launch_prompt_mass<128>(a, p, stream);
+        else
+            launch_prompt_mass<256>(a, p, stream);
+    } else {
+        a.S = 0;                                       // no query: zeros
+    }
+    hipLaunchKernelGGL(mass_columns_join_kernel, dim3((unsigned)(((int64_t)Hkv * NK + 255) / 256)), dim3(256), 0, stream, a);
+    return hip_status(hipGetLastError(), "prompt_mass");
+}

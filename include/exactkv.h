@@ -40,7 +40,8 @@ typedef struct ihipStream_t* hipStream_t;
 
 /* ABI version of the library (2: the encoders take a scan workspace; 3: head dims 64 and
  * 256 and exkv_plan_splits_hd; 4: exkv_error_bits and exkv_set_wait_limit; 5: the operators of a
- * decoder layer around the caches, exkv_prompt_attention and below). */
+ * decoder layer around the caches, exkv_prompt_attention and below; 6: sampling and eviction,
+ * exkv_sample and below). */
 int exkv_abi_version(void);
 
 /* Sticky error bits of the kernels. A kernel that gives up a bounded wait (a correct call
@@ -58,6 +59,8 @@ int exkv_abi_version(void);
 #define EXKV_ERR_OFFSETS 0x20u  /* packed prompts: sequence offsets that do not ascend from 0 within the rows */
 #define EXKV_ERR_POSITION 0x40u /* rotation: a position outside the cosine and sine tables (clamped) */
 #define EXKV_ERR_PAGE 0x80u     /* rotated paged append: the table entry behind a filled page lies outside the pool (no page opened) */
+#define EXKV_ERR_INDEX 0x200u   /* gathered tokens: an index that is neither -1 nor a token of the cache (taken as -1) */
+#define EXKV_ERR_LOGITS 0x400u  /* sampling: a row without a logit that can be drawn (token 0) */
 
 /* out (a device uint32 on the GPU of `stream`) = the OR of the error words of that GPU, in
  * stream order (a small kernel for each; nothing synchronizes, nothing is allocated); clear != 0
@@ -537,6 +540,77 @@ int exkv_rope_append_paged_bf16(const void* q, int64_t sq_n, int64_t sq_h, const
 int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t sr, const void* w, const void* post_w,
                   const void* gate, int64_t sg, float scale, float eps, void* h, void* y, int32_t N, int32_t C,
                   hipStream_t stream);
+
+/* One token a row of logits [B, V] (row stride in elements; type 0 bf16, 1 fp16, 2 fp32; V up to 2^19): with M the row's
+ * largest logit and w = exp((l - M) / temperature), tokens ordered by logit, equal ones by index, the ones with w >= min_p
+ * stay, of them the first top_k (0 or less: all), of these the ones before whose weights add up to less than top_p of all
+ * (1 or more: all; the first always stays); of what stays, S its sum, token[b] is the first one with which the running sum
+ * passes u[b] S, and logprob[b] (may be NULL) log(w / S). temperature not above 0: the largest logit, the first of equal
+ * ones. u: [0, 1) (clamped). temperature, top_k, top_p, min_p: [B], or NULL for the value of the same name with 0 for every
+ * row. NaN and -infinity are never drawn; a row of nothing else gives token 0, log-probability -infinity, and is reported
+ * (EXKV_ERR_LOGITS). Weights are fp64, rounded to multiples of 2^-43. One launch.
+ * No counterpart in the reference, which decodes greedily (engine.py:93-95). */
+int exkv_sample(const void* logits, int64_t stride, int32_t type, int32_t B, int32_t V, const float* u, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p, float temperature0, int32_t top_k0, float top_p0,
+                float min_p0, int64_t* token, float* logprob, hipStream_t stream);
+
+/* Bytes of the workspace that exkv_attention_mass needs (has_lens: lens is given). */
+int64_t exkv_mass_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t TS, int32_t has_lens, int32_t window);
+
+/* The attention that cached tokens receive from one query token of each sequence: q [B, Hq, D] over the keys of a
+ * compressed cache (arguments, block table, lens and window as in exkv_attn_compressed and its paged form; TS the
+ * capacity), for the tokens j of each sequence
+ *   out[b, h, j] = mass[b, h, j] + sum over the query heads g of KV head h of softmax_j(q[b, g] . k[b, j, h] / sqrt(D))
+ * (the softmax over the tokens the window admits; 0 for the others). mass (may be NULL: 0) and out: fp32 [B, Hkv, TS], which
+ * may be the same; out's entries behind a sequence's tokens are left, or 0 with fresh. ws (16-byte aligned) is the
+ * call's own while it runs. Two launches.
+ * No counterpart in the reference, which keeps every token. */
+int exkv_attention_mass(const void* q, const void* sm, const void* code, const void* base, const int32_t* rowmask,
+                        const int32_t* rowoff, const void* raw, int64_t raw_rows, const int32_t* block_table,
+                        int64_t table_stride, int64_t pool_pages, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t T,
+                        int32_t TS, const int32_t* lens, int64_t lens_stride, int32_t window, float qk_scale, const float* mass,
+                        float* out, int32_t fresh, void* ws, int64_t ws_bytes, hipStream_t stream);
+
+/* The same over bf16 keys [B, TS, Hkv, D], or a pool of pages of them. */
+int exkv_attention_mass_bf16(const void* q, const void* k, const int32_t* block_table, int64_t table_stride, int64_t pool_pages,
+                             int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t T, int32_t TS, const int32_t* lens,
+                             int64_t lens_stride, int32_t window, float qk_scale, const float* mass, float* out, int32_t fresh,
+                             void* ws, int64_t ws_bytes, hipStream_t stream);
+
+/* Bytes of the workspace that exkv_prompt_mass needs. */
+int64_t exkv_prompt_mass_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window, int32_t last);
+
+/* The attention that the keys of packed prompts receive (q, k, offsets and window as in exkv_prompt_attention): for key j of
+ * KV head h, the sum of the weights that each sequence's queries, or its last `last` ones (last > 0), give it, over the query
+ * heads of h. out: fp32 [Hkv, NK], 0 for keys that no sequence holds. ws as above. Three to five launches.
+ * No counterpart in the reference. */
+int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h, const int32_t* cu_q,
+                     const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window,
+                     int32_t last, float qk_scale, float* out, void* ws, int64_t ws_bytes, hipStream_t stream);
+
+/* The `keep` tokens that each (sequence, KV head) keeps of its n (lens[b * lens_stride], or T where lens is NULL): the first
+ * `sinks`, the last `recent`, and of those between the ones with the most mass, of equal ones the first (NaN counts as the
+ * least). mass: fp32 [B, H, TS], element strides s_b and s_h. index [B, H, keep]: their numbers, ascending, and kept their
+ * mass; where n < keep the rest is -1 and 0. One launch.
+ * No counterpart in the reference. */
+int exkv_select_tokens(const float* mass, int64_t s_b, int64_t s_h, const int32_t* lens, int64_t lens_stride, int32_t T, int32_t B,
+                       int32_t H, int32_t TS, int32_t keep, int32_t sinks, int32_t recent, int32_t* index, float* kept,
+                       hipStream_t stream);
+
+/* Rows out of two compressed caches (keys and values; contiguous [B, TS, H, D], or pools of pages through one block table as
+ * in exkv_attn_compressed_paged): k_out[b, i, h] = token index[b, h, i] of head h, bf16 [B, keep, H, D], zeros where the index
+ * is -1. Other indices outside the cache count as -1 and are reported (EXKV_ERR_INDEX). One launch.
+ * No counterpart in the reference (codec.py:58-73 decodes every row). */
+int exkv_gather_tokens(const void* k_sm, const void* k_code, const void* k_base, const int32_t* k_rowmask, const int32_t* k_rowoff,
+                       const void* k_raw, int64_t k_raw_rows, const void* v_sm, const void* v_code, const void* v_base,
+                       const int32_t* v_rowmask, const int32_t* v_rowoff, const void* v_raw, int64_t v_raw_rows,
+                       const int32_t* block_table, int64_t table_stride, int64_t pool_pages, int32_t B, int32_t H, int32_t TS,
+                       int32_t D, const int32_t* index, int32_t keep, void* k_out, void* v_out, hipStream_t stream);
+
+/* The same out of two bf16 caches. */
+int exkv_gather_tokens_bf16(const void* k, const void* v, const int32_t* block_table, int64_t table_stride, int64_t pool_pages,
+                            int32_t B, int32_t H, int32_t TS, int32_t D, const int32_t* index, int32_t keep, void* k_out,
+                            void* v_out, hipStream_t stream);
 
 #ifdef __cplusplus
 }
