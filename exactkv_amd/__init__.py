@@ -11,8 +11,8 @@ from .paged import PageTable, PagedCompressedKV, PagedBF16KV
 from .codec import encode_reference, decode_reference, bits_per_value
 from .kernels import attention_compressed, attention_reference, decode_to_bf16, encode_pages
 from .layer import prompt_attention, rotate_prompt, rope_append, rope_append_paged, add_norm
-from .budget import attention_mass, prompt_mass, select_tokens, gather_tokens
-from .sampling import sample
+from .budget import attention_mass, prompt_mass, select_tokens, gather_tokens, evict, Budget
+from .sampling import sample, Sampler
 
 
 def __getattr__(name):
@@ -28,4 +28,4 @@ __all__ = ["CompressedKV", "BF16KV", "check_overflow", "decode_attention", "Engi
            "attention_compressed", "attention_reference", "decode_to_bf16", "encode_pages",
            "PageTable", "PagedCompressedKV", "PagedBF16KV", "PagedEngine",
            "prompt_attention", "rotate_prompt", "rope_append", "rope_append_paged", "add_norm",
-           "attention_mass", "prompt_mass", "select_tokens", "gather_tokens", "sample"]
+           "attention_mass", "prompt_mass", "select_tokens", "gather_tokens", "evict", "Budget", "sample", "Sampler"]

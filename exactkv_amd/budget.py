@@ -233,3 +233,77 @@ def gather_tokens(k_cache, v_cache, index, *, block_table=None):
     out = [torch.empty(B, n, H, D, dtype=torch.bfloat16, device=index.device) for _ in range(2)]
     _lib.call(name, *caches, bt, stride, pages, B, H, TS, D, index.data_ptr(), n, out[0].data_ptr(), out[1].data_ptr(), _lib.stream(dev))
     return tuple(out)
+
+
+class Budget:
+    """How many tokens each KV head keeps, and which (Engine's budget=): the first `sinks`, the latest `recent` (default:
+    a quarter of keep) and otherwise those that have received the most attention. last: of a prompt's queries only the last
+    `last` count (0: all)."""
+
+    def __init__(self, keep, sinks=4, recent=None, last=0):
+        recent = keep // 4 if recent is None else recent
+        if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep or last < 0:
+            raise ValueError(f"{sinks} first and {recent} latest tokens of {keep} kept, last {last}")
+        self.keep, self.sinks, self.recent, self.last = int(keep), int(sinks), int(recent), int(last)
+
+
+def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
+    """An eviction in place: of each KV head of each sequence the `keep` tokens that select_tokens chooses by mass stay, in
+    their order, and are stored as the caches' first ones; their mass moves with them and what is behind them is 0. Caches
+    of one kind that hold the same tokens:
+
+      * contiguous ones: mass fp32 [B, H, TS]; the cache's token count becomes keep;
+      * paged ones of one PageTable: mass fp32 [max_seqs, H, capacity], a row for each slot; slots (host ints, default all
+        live ones) are cut, the pages behind go back to the pool (raw rows stay until compact()), and begin_step comes
+        before the next step.
+
+    Sequences of at most `keep` tokens stay as they are. Returns the index that select_tokens gave, a row for each sequence
+    (slot). Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is not captured. The next
+    token's position is what the caller counts, not the cache's length."""
+    if type(k_cache) is not type(v_cache) or not isinstance(k_cache, (CompressedKV, BF16KV, PagedCompressedKV, PagedBF16KV)):
+        raise TypeError(f"evict takes two caches of one kind (got {type(k_cache).__name__}, {type(v_cache).__name__})")
+    if k_cache is v_cache:
+        raise ValueError("keys and values need a cache each")
+    if getattr(k_cache, "_pending", None) is not None or getattr(v_cache, "_pending", None) is not None:
+        raise RuntimeError("a page filled: call check_overflow() before evict()")
+    H, D = k_cache.H, k_cache.D
+    dev = mass.get_device()
+    if dev >= 0 and dev != _lib.current_device():
+        with _on(dev):
+            return evict(k_cache, v_cache, mass, keep, sinks=sinks, recent=recent, slots=slots)
+    if isinstance(k_cache, (CompressedKV, BF16KV)):
+        B, TS, T = k_cache.B, k_cache.TS, k_cache.T
+        if slots is not None:
+            raise ValueError("contiguous caches are cut as a whole (slots are of paged ones)")
+        if (v_cache.B, v_cache.TS, v_cache.H, v_cache.D, v_cache.T) != (B, TS, H, D, T):
+            raise ValueError("k and v caches differ in shape or in the tokens they hold")
+        _mass_rows(mass, (B, H, TS), dev, "mass")
+        index, kept = select_tokens(mass, keep, T, sinks=sinks, recent=recent)
+        if T > keep:
+            k, v = gather_tokens(k_cache, v_cache, index)
+            k_cache.replace(k)
+            v_cache.replace(v)
+            mass[..., :keep] = kept
+            mass[..., keep:] = 0
+        return index
+    table = k_cache.table
+    if v_cache.table is not table or (v_cache.H, v_cache.D) != (H, D):
+        raise ValueError("k and v caches differ in shape or belong to two page tables")
+    _mass_rows(mass, (table.max_seqs, H, table.capacity), dev, "mass")
+    slots = table.live_slots() if slots is None else [int(s) for s in slots]
+    if len(set(slots)) != len(slots) or any(not 0 <= s < table.max_seqs or table._pages[s] is None for s in slots):
+        raise ValueError(f"slots must be distinct and in use (got {slots})")
+    at = torch.tensor(slots, dtype=torch.int64).to(mass.device)
+    index, kept = select_tokens(mass[at], keep, lens=table.lens[at], sinks=sinks, recent=recent)
+    long = [i for i, s in enumerate(slots) if table.length(s) > keep]
+    if not long:
+        return index
+    rows = torch.tensor(long, dtype=torch.int64).to(mass.device)
+    k, v = gather_tokens(k_cache, v_cache, index[rows], block_table=table.block_table[at[rows]])
+    for j, i in enumerate(long):
+        table.truncate(slots[i], keep)
+        k_cache.prefill(slots[i], k[j:j + 1])
+        v_cache.prefill(slots[i], v[j:j + 1])
+    mass[at[rows], :, :keep] = kept[rows]
+    mass[at[rows], :, keep:] = 0
+    return index

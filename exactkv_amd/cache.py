@@ -159,6 +159,32 @@ class CompressedKV:
             self._open_rows()[b, :, : T - full].copy_(x[0, full:].transpose(0, 1))
         self._keep_headroom(int(self.cnt.item()) if used is None else used)
 
+    def replace(self, x):
+        """x: [B, T, H, D] bf16, all that the cache holds from now on, of every sequence; what it held is gone, its raw
+        rows too (no counterpart in the reference, whose caches only grow)."""
+        if x.dim() != 4 or x.shape[0] != self.B or x.shape[2:] != (self.H, self.D) or x.dtype != torch.bfloat16 or x.stride(3) != 1:
+            raise ValueError(f"replace expects a bf16 [{self.B}, T, {self.H}, {self.D}] tensor with contiguous rows")
+        T = x.shape[1]
+        if T > self.TS:
+            raise AssertionError(f"{T} tokens do not fit a cache of {self.TS}")
+        if x.device != self.sm.device:
+            raise ValueError(f"replace expects a tensor on {self.sm.device}")
+        full = T - T % P
+        self.T, self._pending = T, None
+        self.state[0] = T
+        self.cnt.zero_()
+        used = 0
+        if full:
+            strides = (x.stride(0), P * x.stride(1), x.stride(1), x.stride(2))
+            encode_pages(x, strides, self._buf(), 0, 0, self.B, full // P)
+            used = int(self.cnt.item())
+            if used > self.cap:
+                used = self._refit(lambda: (x, strides), 0, 0, self.B, full // P)
+        self._open_page()
+        if T > full:
+            self._open_rows()[:, :, : T - full].copy_(x[:, full:].transpose(1, 2))
+        self._keep_headroom(used)
+
     def append(self, x):
         """x: [B, H, D] bf16, the next token of every sequence."""
         self._check_can_append()
@@ -227,6 +253,17 @@ class BF16KV:
     def prefill_slot(self, b, x):
         n = x.shape[1]
         self.buf[b].narrow(0, 0, n).copy_(x[0])
+        self.T = n
+        self.state[0] = n
+
+    def replace(self, x):
+        """CompressedKV.replace on plain rows."""
+        if x.dim() != 4 or x.shape[0] != self.B or x.shape[2:] != (self.H, self.D) or x.dtype != torch.bfloat16:
+            raise ValueError(f"replace expects a bf16 [{self.B}, T, {self.H}, {self.D}] tensor")
+        n = x.shape[1]
+        if n > self.TS:
+            raise AssertionError(f"{n} tokens do not fit a cache of {self.TS}")
+        self.buf[:, :n].copy_(x)
         self.T = n
         self.state[0] = n
 

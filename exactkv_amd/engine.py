@@ -18,7 +18,9 @@ MI355X specifics:
     package's kernels between the model's projections: rotation and appends in one launch, each
     residual add with the norm behind it in one, and prompts packed, several sequences in one
     pass of prompt attention. It rounds less often than the model's modules (once per kernel),
-    so its logits are near theirs, not their bits; the two caches agree bit for bit either way.
+    so its logits are near theirs, not their bits; the two caches agree bit for bit either way;
+  * budget= (with layer_kernels) lets a generation run past the caches: each step adds its attention weights to what the
+    cached tokens of each KV head have received, and full caches are cut to those with the most.
 """
 import importlib
 
@@ -27,6 +29,7 @@ import torch
 from .cache import BF16KV, CompressedKV, check_overflow
 from .attention import decode_attention
 from .kernels import HEAD_DIMS, attention_compressed, attention_reference, P
+from .budget import attention_mass, evict, gather_tokens, prompt_mass, select_tokens
 from .layer import add_norm, launch_rope_append, prompt_attention, rope_append, rotate_prompt
 
 BACKENDS = {"exactkv": CompressedKV, "bf16": BF16KV}
@@ -100,6 +103,16 @@ class _LayerKernels:
         if cos.shape[-1] != eng.D or not torch.equal(cos[..., :half], cos[..., half:]):
             raise AssertionError("layer kernels rotate half-split over the whole head")
         self.cos, self.sin = (t[0, :, :half].float().contiguous() for t in (cos, sin))
+        self.step_cos, self.step_sin = self.cos, self.sin     # of a step: by its place in the caches
+
+    def move(self, dropped, rows):
+        """Steps stand `dropped` positions behind their place in caches of `rows` tokens: tables of their own, rewritten in
+        place, so that a captured step follows."""
+        if self.step_cos is self.cos:
+            self.step_cos, self.step_sin = torch.zeros_like(self.cos[:rows]), torch.zeros_like(self.sin[:rows])
+        n = min(rows, self.cos.shape[0] - dropped)
+        self.step_cos[:n].copy_(self.cos[dropped:dropped + n])
+        self.step_sin[:n].copy_(self.sin[dropped:dropped + n])
 
     def _norm(self, x, residual, norm):
         return add_norm(x, residual, norm.weight, eps=norm.variance_epsilon)
@@ -131,7 +144,7 @@ class _LayerKernels:
         append = launch_rope_append if device_only else rope_append
 
         def layer(i, q, k, v, norms):
-            return attend(i, append(q, k, v, self.cos, self.sin, *self.eng.kv[i], **norms))
+            return attend(i, append(q, k, v, self.step_cos, self.step_sin, *self.eng.kv[i], **norms))
         return self.eng.m.lm_head(self._walk(tok, layer))
 
     def prompts(self, prompts, slots):
@@ -151,6 +164,9 @@ class _LayerKernels:
             def layer(li, q, k, v, norms):
                 q, k = rotate_prompt(q, k, self.cos, self.sin, cu, **norms)
                 kc, vc = eng.kv[li]
+                if getattr(eng, "budget", None) is not None:
+                    eng._keep_prompts(li, q, k, v, cu, slots[i:j])
+                    return prompt_attention(q, k, v, cu, window=eng.windows[li])
                 for slot, a, e in zip(slots[i:j], ends, ends[1:]):
                     kc.prefill_slot(slot, k[None, a:e])
                     vc.prefill_slot(slot, v[None, a:e])
@@ -196,13 +212,17 @@ def _layer_kv(pkv, i):
 
 class Engine:
     def __init__(self, model, B, T_max, backend="exactkv", attn=None, before_step=None, graph=True,
-                 layer_kernels=False):
+                 layer_kernels=False, budget=None):
         """backend: 'exactkv' / 'bf16', or a cache class with the same interface.
         attn(q, k_cache, v_cache) and before_step(engine, T) let benchmarks plug in other
         kernels (reference engine.py:30-33); with either plug-in the step runs eagerly.
         graph: capture the decode step in a HIP graph (default).
         layer_kernels: rotation, norms and prompt attention by this package's kernels (its own
-        caches only)."""
+        caches only).
+        budget (with layer_kernels, no sliding layers): a Budget of fewer than T_max tokens. The caches then hold T_max
+        tokens at most, prompt and generation may be longer (up to the model's positions): a prompt that does not
+        fit, and full caches before a step, are cut to the budget's tokens by the attention that each has received
+        in its KV head. self.dropped: tokens cut so far."""
         # sliding-window layers: decode attention reads each sequence's last `window` tokens,
         # the keys the model's own mask admits (positions > p - window)
         _describe(self, model)
@@ -218,7 +238,19 @@ class Engine:
         ours = isinstance(cls, type) and issubclass(cls, (CompressedKV, BF16KV))
         if layer_kernels and not ours:
             raise AssertionError("layer kernels append to this package's caches only")
-        self._layers = _LayerKernels(self, self.TS) if layer_kernels else None
+        self.budget, self.dropped, self.mass = budget, 0, None
+        if budget is not None:
+            if not layer_kernels or any(self.windows):
+                raise AssertionError("a budget needs layer_kernels and no sliding-window layer")
+            if attn is not None or before_step is not None:
+                raise AssertionError("a budget takes no plug-ins")
+            if budget.keep >= self.TS:
+                raise AssertionError(f"a budget of {budget.keep} tokens needs caches of more (T_max rounds to {self.TS})")
+            self.mass = [torch.zeros(B, self.Hkv, self.TS, dtype=torch.float32, device=self.dev) for _ in range(self.L)]
+        positions = self.TS if budget is None else max(self.TS, int(model.config.max_position_embeddings))
+        self._layers = _LayerKernels(self, positions) if layer_kernels else None
+        if budget is not None:
+            self._layers.move(0, self.TS)
         self.use_graph = bool(graph) and attn is None and before_step is None and ours
         self._stream = torch.cuda.Stream(device=self.dev) if self.use_graph else None
         self._graph = None
@@ -231,8 +263,9 @@ class Engine:
 
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
-    def prefill(self, ids, b0=0, fused=True):
+    def prefill(self, ids, b0=0, fused=True, choose=None):
         """ids: [B, T] token ids. Returns the greedy next token of each sequence, [B].
+        choose (additive): the next tokens [n] from logits [n, vocab] instead (a Sampler).
         b0 (additive): fill sequence slots b0.. with ids' rows, so a long prefill can be
         done in pieces (slot 0 first).
         fused (additive): each layer's RoPE'd keys and values go straight from the
@@ -243,12 +276,15 @@ class Engine:
         pass ends); both give the same cache bytes.
         With layer_kernels the prompts go through packed, several at a time (fused is not used)."""
         if self._layers is not None:
-            if ids.shape[1] == 0 or b0 + ids.shape[0] > self.B or ids.shape[1] > self.TS:
+            room = self.TS if self.budget is None else self._layers.cos.shape[0]
+            if ids.shape[1] == 0 or b0 + ids.shape[0] > self.B or ids.shape[1] > room:
                 raise AssertionError(f"{ids.shape[0]} prompts of {ids.shape[1]} tokens do not fit slots {b0} to {self.B - 1} "
-                                     f"of {self.TS}")
+                                     f"of {room}")
             hidden = self._layers.prompts(list(ids), list(range(b0, b0 + ids.shape[0])))
             self._graph = None                  # buffers may have grown
-            return self._prefill_next(hidden[:, None])
+            if self.budget is not None:
+                self._drop(ids.shape[1] - self.kv[0][0].T)
+            return self._prefill_next(hidden[:, None], choose)
         nxt = []
         with _fused_sdpa():
             for i0 in range(ids.shape[0]):
@@ -263,17 +299,57 @@ class Engine:
                         kc.prefill_slot(b, keys.transpose(1, 2))
                         vc.prefill_slot(b, values.transpose(1, 2))
                     del pkv
-                nxt.append(self._prefill_next(out.last_hidden_state))
+                nxt.append(self._prefill_next(out.last_hidden_state, choose))
                 del out
         self._graph = None                      # buffers may have grown
         return torch.cat(nxt)
 
-    def _prefill_next(self, hidden):
-        """Greedy next token from the prompt's last hidden state. The final norm is applied
+    def _prefill_next(self, hidden, choose=None):
+        """Greedy (or chosen) next token from the prompt's last hidden state. The final norm is applied
         to the model's output once more, as the reference prefill does (engine.py:50), so
         both backends and the reference pick the same first token."""
-        last = self.m.model.norm(hidden[:, -1])
-        return self.m.lm_head(last).argmax(dim=-1)
+        logits = self.m.lm_head(self.m.model.norm(hidden[:, -1]))
+        return logits.argmax(dim=-1) if choose is None else choose(logits)
+
+    # ---------------------------------------------------------------- budget
+    def _keep_prompts(self, i, q, k, v, cu, slots):
+        """Layer i's keys and values of packed prompts of one length (rotated) into slots, with the attention that each has
+        received; of prompts that the caches do not hold, the budget's tokens."""
+        n, b = len(slots), self.budget
+        T = k.shape[0] // n
+        got = prompt_mass(q, k, cu, last=b.last).view(self.Hkv, n, T).transpose(0, 1).contiguous()
+        k, v = k.view(n, T, self.Hkv, self.D), v.reshape(n, T, self.Hkv, self.D)
+        if T > self.TS:
+            index, got = select_tokens(got, b.keep, T, sinks=b.sinks, recent=b.recent)
+            k, v = gather_tokens(k, v, index)
+        kc, vc = self.kv[i]
+        for j, slot in enumerate(slots):
+            kc.prefill_slot(slot, k[j:j + 1])
+            vc.prefill_slot(slot, v[j:j + 1])
+            self.mass[i][slot, :, : got.shape[2]] = got[j]
+            self.mass[i][slot, :, got.shape[2]:] = 0
+
+    def _drop(self, dropped):
+        self.dropped = dropped
+        self._layers.move(dropped, self.TS)
+
+    def _make_room(self):
+        """Full caches cut to the budget before a step."""
+        b, T, positions = self.budget, self.kv[0][0].T, self._layers.cos.shape[0]
+        if self.dropped + T >= positions:
+            raise RuntimeError(f"position {self.dropped + T} is outside the model's {positions}")
+        if T < self.TS:
+            return
+        for (kc, vc), mass in zip(self.kv, self.mass):
+            evict(kc, vc, mass, b.keep, sinks=b.sinks, recent=b.recent)
+        self._drop(self.dropped + self.TS - b.keep)
+
+    def _attend_kept(self, i, q):
+        """Layer i's attention in a step, its weights added to what the cached tokens have received."""
+        kc, vc = self.kv[i]
+        out = self._attend(q, kc, vc)
+        attention_mass(q, kc, lens=kc.state[:1], mass=self.mass[i], out=self.mass[i])
+        return out
 
     def _caches(self):
         return [c for pair in self.kv for c in pair]
@@ -294,6 +370,8 @@ class Engine:
         advances its cache's host count, as the reference does, so an attention plug-in
         sees the current length."""
         m, B, Hq, Hkv, D = self.m, self.B, self.Hq, self.Hkv, self.D
+        if self.budget is not None:
+            return self._layers.step(tok, self._attend_kept, device_only)
         if self._layers is not None:
             return self._layers.step(tok, lambda i, q: self._attend(q, *self.kv[i], self.windows[i]), device_only)
         h = m.model.embed_tokens(tok.view(B, 1))
@@ -331,6 +409,8 @@ class Engine:
     @torch.no_grad()
     def step(self, tok):
         """tok: [B] current tokens. Returns logits [B, vocab] (bf16) for the next token."""
+        if self.budget is not None:
+            self._make_room()
         T = self.kv[0][0].T
         if self.use_graph:
             for kv in self.kv:
@@ -365,14 +445,15 @@ class Engine:
         return logits
 
     @torch.no_grad()
-    def generate(self, ids, n_new):
+    def generate(self, ids, n_new, choose=None):
         """Greedy decoding of n_new tokens per sequence, the first from the prefill: returns
-        (tokens [B, n_new], the logits of the n_new - 1 decode steps [B, n_new - 1, vocab])."""
-        tokens = [self.prefill(ids)]
+        (tokens [B, n_new], the logits of the n_new - 1 decode steps [B, n_new - 1, vocab]).
+        choose (additive): the next tokens [B] from logits [B, vocab] instead, e.g. Sampler(0.7, top_p=0.9)."""
+        tokens = [self.prefill(ids, choose=choose)]
         step_logits = []
         while len(tokens) < n_new:
             step_logits.append(self.step(tokens[-1]))
-            tokens.append(step_logits[-1].argmax(dim=-1))
+            tokens.append(step_logits[-1].argmax(dim=-1) if choose is None else choose(step_logits[-1]))
         return torch.stack(tokens, dim=1), torch.stack(step_logits, dim=1)
 
     def kv_bytes(self):
@@ -416,10 +497,11 @@ class PagedEngine:
         self._layers = _LayerKernels(self, self._positions) if layer_kernels else None
 
     @torch.no_grad()
-    def add_many(self, prompts):
+    def add_many(self, prompts, choose=None):
         """Prefill several prompts (1-D token ids of any lengths) into new sequence slots, packed:
         one pass over the model's layers for about 16K tokens of them. Returns (slots, the greedy
-        next tokens [len(prompts)]). Where a prompt does not fit, or the model refuses one, none is added."""
+        next tokens [len(prompts)], or those that choose takes from their logits, e.g. a Sampler). Where a prompt does not
+        fit, or the model refuses one, none is added."""
         if self._layers is None:
             self._layers = _LayerKernels(self, self._positions)
         prompts = list(prompts)
@@ -434,12 +516,17 @@ class PagedEngine:
             for s in slots:
                 self.table.release(s)
             raise
-        return slots, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)
+        return slots, self._next(hidden, choose)
+
+    def _next(self, hidden, choose):
+        """The next tokens from the prompts' last hidden states [n, C]."""
+        logits = self.m.lm_head(self.m.model.norm(hidden))
+        return logits.argmax(-1) if choose is None else choose(logits)
 
     @torch.no_grad()
-    def add(self, ids, slot=None):
+    def add(self, ids, slot=None, choose=None):
         """Prefill one prompt (1-D token ids) into a new sequence slot. Returns (slot, the
-        greedy next token)."""
+        greedy next token, or the one that choose takes from logits [1, vocab])."""
         if self._own_layers:
             if ids.numel() == 0:
                 raise ValueError("a prompt of no tokens")
@@ -449,11 +536,11 @@ class PagedEngine:
             except Exception:
                 self.table.release(s)
                 raise
-            return s, self.m.lm_head(self.m.model.norm(hidden)).argmax(-1)[0]
+            return s, self._next(hidden, choose)[0]
         s = self.table.add(int(ids.numel()), slot)
         with _fused_sdpa():
             out = self.m.model(ids.view(1, -1), use_cache=True, past_key_values=_write_through(self, s))
-        return s, self.m.lm_head(self.m.model.norm(out.last_hidden_state[:, -1])).argmax(-1)[0]
+        return s, self._next(out.last_hidden_state[:, -1], choose)[0]
 
     def release(self, slot):
         self.table.release(slot)

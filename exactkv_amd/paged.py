@@ -105,6 +105,20 @@ class PageTable:
         self.lens[slot] = 0
         self._rows = None
 
+    def truncate(self, slot, T):
+        """A slot's sequence has T tokens from now on, no more than it had: the pages behind its open one go back to the
+        pool (the caches' rows follow, see budget.evict)."""
+        if self._pages[slot] is None:
+            raise ValueError(f"slot {slot} is not in use")
+        if not 0 <= T <= self._len[slot]:
+            raise ValueError(f"{T} tokens of a sequence of {self._len[slot]}")
+        n = self._npages(T)
+        self._free.extend(reversed(self._pages[slot][n:]))
+        del self._pages[slot][n:]
+        self._len[slot] = T
+        self._write([slot], [T], [], [])
+        self._rows = None
+
     def begin_step(self, slots=None):
         """One more token for each slot in `slots` (host ints, all live and distinct; None: every
         live slot, in order). Batch row i of the step's appends and attention is slots[i]."""

@@ -66,3 +66,16 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob
     _lib.call("exkv_sample", logits.data_ptr(), logits.stride(0) if B > 1 else V, kind, B, V, u.data_ptr(), tp, kp, pp, mp, t, k, p, m,
               token.data_ptr(), lp.data_ptr() if logprob else None, _lib.stream(dev))
     return (token, lp) if logprob else token
+
+
+class Sampler:
+    """sample() with its settings and a random generator: logits [B, V] -> tokens [B], as the engines' choose= takes it. The
+    settings are numbers, or tensors with one entry for each row that is then asked for."""
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):
+        self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self.generator = generator
+
+    def __call__(self, logits):
+        u = torch.rand(logits.shape[0], generator=self.generator, device=logits.device)
+        return sample(logits, u, **self.settings)

@@ -144,3 +144,33 @@ def test_tensors_must_be_on_a_gpu():
         exactkv.select_tokens(z(1, 2, 16), 4, 16)
     with pytest.raises(ValueError, match="GPU"):
         exactkv.gather_tokens(z(1, 16, 2, 64, dtype=torch.bfloat16), z(1, 16, 2, 64, dtype=torch.bfloat16), z(1, 2, 4, dtype=torch.int32))
+
+
+def test_truncated_sequences_give_their_pages_back():
+    t = exactkv.PageTable(20, 2, 10, device="cpu")
+    a, b = t.add(100), t.add(40)
+    held, free = t.pages(a), t.free_pages()
+    t.truncate(a, 33)
+    assert t.length(a) == 33 and t.pages(a) == held[:3] and t.free_pages() == free + 4 and int(t.lens[a]) == 33
+    t.truncate(a, 32)                                  # its open page, the third, stays
+    assert t.pages(a) == held[:3]
+    with pytest.raises(RuntimeError):
+        t.step_rows()
+    t.begin_step([a, b])
+    assert t.length(a) == 33
+    t.truncate(a, 0)
+    assert t.pages(a) == held[:1]
+    for slot, T in ((a, 1), (b, -1), (b, 100)):
+        with pytest.raises(ValueError):
+            t.truncate(slot, T)
+    t.release(b)
+    with pytest.raises(ValueError):
+        t.truncate(b, 0)
+
+
+def test_budgets():
+    b = exactkv.Budget(100)
+    assert (b.keep, b.sinks, b.recent, b.last) == (100, 4, 25, 0)
+    for a in ((0,), (10, 11), (10, 4, 7), (10, -1), (10, 0, -1), (10, 0, 0, -1)):
+        with pytest.raises(ValueError):
+            exactkv.Budget(*a)
