@@ -95,7 +95,8 @@ SIGNATURES.update({
                                             _i32, _i32, _p],
     "exkv_rope_append_paged_bf16": _ROPE_ROWS + [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
     "exkv_add_norm": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _f32, _f32, _p, _p, _i32, _i32, _p],
-    "exkv_sample": [_p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _f32, _i32, _f32, _f32, _p, _p, _p],
+    "exkv_sample": [_p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _f32, _i32, _f32, _f32, _p, _p, _p, _i64, _p],
+    "exkv_sample_workspace": [_i32, _i32],
     "exkv_mass_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32],
     "exkv_attention_mass": [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64,
                             _i32, _f32, _p, _p, _i32, _p, _i64, _p],
@@ -132,7 +133,7 @@ def load():
         f.argtypes = args
         f.restype = {"exkv_last_error": ctypes.c_char_p, "exkv_wire_bytes": ctypes.c_int64,
                      "exkv_noalloc_scratch_bytes": ctypes.c_int64, "exkv_prompt_workspace": ctypes.c_int64,
-                     "exkv_mass_workspace": ctypes.c_int64, "exkv_prompt_mass_workspace": ctypes.c_int64,
+                     "exkv_mass_workspace": ctypes.c_int64, "exkv_sample_workspace": ctypes.c_int64, "exkv_prompt_mass_workspace": ctypes.c_int64,
                      "exkv_merge_counters": ctypes.c_int64}.get(name, ctypes.c_int)
     v = lib.exkv_abi_version()
     if v != ABI_VERSION:
@@ -145,7 +146,8 @@ def load():
 
 
 # entry points that take no stream (host-only, or hooks)
-_NO_STREAM = {"exkv_wire_bytes", "exkv_prompt_workspace", "exkv_mass_workspace", "exkv_prompt_mass_workspace", "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
+_NO_STREAM = {"exkv_wire_bytes", "exkv_prompt_workspace", "exkv_mass_workspace", "exkv_prompt_mass_workspace", "exkv_sample_workspace",
+              "exkv_time_next_split", "exkv_merge_counters", "exkv_noalloc_scratch_bytes",
               "exkv_plan_splits", "exkv_plan_splits_hd", "exkv_abi_version", "exkv_last_error", "exkv_error_bits",
               "exkv_set_wait_limit"}
 

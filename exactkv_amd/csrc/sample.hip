@@ -7,22 +7,25 @@
 // is the first one with which the running sum passes u S.
 //
 // Every cut is thus a place in one order, the first where a running count or sum passes a bound, and is found without
-// a sort of the row: weights are counted and added up in 2,048 bins of (M - l) / t, 1/64 wide; the bin in which
-// the bound is passed is known from the bins' sums; its tokens alone are collected, sorted and added up one by one.
-// With top_k up to 2,048 all tokens down to the k-th's bin are collected at once and no other weight is computed.
+// a sort of the row: with y = 32 log2(1 / w), weights are counted and added up in bins of one y; the bin in which a bound
+// is passed is known from the bins' sums (to a few bins, where the bound depends on a sum that is known to a bin); the
+// tokens of these bins alone are collected, sorted and added up one by one. With top_k up to 2,048 all tokens down to the
+// k-th's bin are collected at once, and no other weight is computed.
 //
-// Weights are fp64 exponentials rounded to multiples of 2^-43 and held as whole numbers, so sums do not depend on
-// the order in which they are taken and a cut falls where the formula in 64 bits has it; weights below 2^-44
-// (all of a vocabulary of 2^19 add up to less than 2^-25 of the sum) are 0.
+// Weights are fp64, to 2^-51 of each: w = 2^-(i / 32) 2^-(f / 32) with i and f the whole and the rest of y, the second factor
+// a polynomial (fifth degree, through 1 at f = 0), rounded to whole multiples of 2^-43 and added up as whole numbers, so that
+// sums do not depend on the order in which they are taken, and a bin's factor is applied to its sum. Cuts fall where the
+// formula in 64 bits has them. Weights below 2^-44 (all of a vocabulary of 2^19 add up to less than 2^-25 of the sum) are 0.
 #include "errors.hpp"
 #include "common.hpp"
 #include "../../include/exactkv.h"
 
 namespace exkv {
 
-constexpr int kThreads = 1024, kBins = 2048, kList = 4096;
-constexpr float kPerNat = 64.f;        // bins of width 1 in (M - l) / t
-constexpr double kOne = 8796093022208.0;   // 2^43: a weight of 1
+constexpr int kThreads = 1024, kList = 4096;
+constexpr int kPerOctave = 32, kReach = 44 * kPerOctave;   // bins of a factor of 2; weights from bin kReach on are 0
+constexpr int kBins = 2048;                                // places for them, two a thread
+constexpr double kOne = 0x1p43;                            // a weight of 1
 
 struct SampleArgs {
     const void* logits;                // [B, V], row stride in elements
@@ -34,6 +37,11 @@ struct SampleArgs {
     int k0;
     int64_t* token;
     float* logprob;                    // may be nullptr
+    // rows cut into `pieces` of `per` logits: their maxima [B, pieces] (order << 32 | ~index), a row's bins [B, kReach],
+    // what is collected of it [B, kList], and how much [B]
+    int pieces, per;
+    uint64_t *best, *mass, *list;
+    uint32_t *count, *n;
 };
 
 // A logit's place in the order of all; -0 as 0. NaN: 0. kMinusInf: the least that can be drawn is above it.
@@ -43,6 +51,9 @@ __device__ inline uint32_t order_of(float x) {
     return x != x ? 0u : (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 __device__ inline float of_order(uint32_t k) { return __uint_as_float((k & 0x80000000u) != 0 ? k & 0x7FFFFFFFu : ~k); }
+// A token as one number: ascending in the order of the tokens.
+__device__ inline uint64_t token_of(float l, int j) { return (uint64_t)~order_of(l) << 32 | (uint32_t)j; }
+__device__ inline float logit_of(uint64_t token) { return of_order(~(uint32_t)(token >> 32)); }
 
 enum LogitType { kBf16 = 0, kFp16 = 1, kFp32 = 2 };
 template <int TYPE>
@@ -63,19 +74,66 @@ struct Logits {
     }
 };
 
-// A row's settings and its weights.
+// 2^-(j / 32)
+__constant__ double kOctave[kPerOctave] = {
+    0x1.0000000000000p+0, 0x1.f50765b6e4540p-1, 0x1.ea4afa2a490dap-1, 0x1.dfc97337b9b5fp-1, 0x1.d5818dcfba487p-1, 0x1.cb720dcef9069p-1,
+    0x1.c199bdd85529cp-1, 0x1.b7f76f2fb5e47p-1, 0x1.ae89f995ad3adp-1, 0x1.a5503b23e255dp-1, 0x1.9c49182a3f090p-1, 0x1.93737b0cdc5e5p-1,
+    0x1.8ace5422aa0dbp-1, 0x1.82589994cce13p-1, 0x1.7a11473eb0187p-1, 0x1.71f75e8ec5f74p-1, 0x1.6a09e667f3bcdp-1, 0x1.6247eb03a5585p-1,
+    0x1.5ab07dd485429p-1, 0x1.5342b569d4f82p-1, 0x1.4bfdad5362a27p-1, 0x1.44e086061892dp-1, 0x1.3dea64c123422p-1, 0x1.371a7373aa9cbp-1,
+    0x1.306fe0a31b715p-1, 0x1.29e9df51fdee1p-1, 0x1.2387a6e756238p-1, 0x1.1d4873168b9aap-1, 0x1.172b83c7d517bp-1, 0x1.11301d0125b51p-1,
+    0x1.0b5586cf9890fp-1, 0x1.059b0d3158574p-1};
+
+// 2^-(f / 32) for 0 <= f < 1 in multiples of 2^-43: 1 + f q(f), q through (2^-(f / 32) - 1) / f at the five Chebyshev
+// nodes of the interval (2^-51.6 off at most). The last step adds 2^52 as well, so that it rounds to a whole number,
+// which the low bits then hold.
+__device__ inline uint64_t part_of(double f) {
+    double x = -0x1.5a647394e5de0p-35 * kOne;
+    x = fma(x, f, 0x1.3b27f90273e58p-27 * kOne);
+    x = fma(x, f, -0x1.c6b08b7b3d765p-20 * kOne);
+    x = fma(x, f, 0x1.ebfbdff7af203p-13 * kOne);
+    x = fma(x, f, -0x1.62e42fefa399fp-6 * kOne);
+    x = fma(x, f, kOne + 0x1p52);
+    return (uint64_t)__double_as_longlong(x) & 0xFFFFFFFFFFFFFull;
+}
+// A sum of such parts in bin i, in weights.
+__device__ inline uint64_t in_bin(uint64_t parts, int i, double octave) {
+    return (uint64_t)rint(__builtin_amdgcn_ldexp((double)parts * octave, -(i / kPerOctave)));
+}
+
+// A row's settings.
 struct Row {
-    float top, inv_bins;               // M; 64 / t
-    double inv_t, min_p;
-    __device__ int bin(float l) const {
-        const float z = (top - l) * inv_bins;
-        return l == top ? 0 : z < (float)(kBins - 1) ? (int)z : kBins - 1;   // (ascends as l falls; NaN: the last)
+    double top, per_bin, limit;        // the largest logit; bins of a logit; the last y that counts
+    float top32, p, u0;
+    int k;
+    bool none, greedy, odd, few;       // odd: the largest is infinite; few: collected by counts alone
+    __device__ Row(const SampleArgs& a, int b, uint64_t best) {
+        const float t = a.t != nullptr ? a.t[b] : a.t0, m = a.m != nullptr ? a.m[b] : a.m0;
+        p = a.p != nullptr ? a.p[b] : a.p0;
+        k = a.k != nullptr ? a.k[b] : a.k0;
+        u0 = a.u[b];
+        none = (uint32_t)(best >> 32) <= kMinusInf;
+        greedy = none || !(t > 0.f);
+        few = k > 0 && k <= kList / 2;
+        top32 = of_order((uint32_t)(best >> 32));
+        odd = top32 == INFINITY;
+        top = (double)top32;
+        per_bin = kPerOctave * 1.4426950408889634 / (double)t;
+        limit = kReach - 0x1p-40;
+        if (!(m <= 0.f)) limit = fmin(limit, m < 1.f ? -(double)kPerOctave * log2((double)m) : 0.0);
     }
-    // of a logit above -inf
+    __device__ double u() const { return u0 > 0.f ? fmin((double)u0, 1.0 - 0x1p-24) : 0.0; }
+    // y: ascends as l falls; not within the limit (NaN too): a weight of 0
+    __device__ double place(float l) const { return (top - (double)l) * per_bin; }
+    __device__ double any_place(float l) const { return l == top32 ? 0.0 : place(l); }
+    __device__ int bin(float l) const {
+        const double y = any_place(l);
+        return y <= limit ? (int)y : kReach;
+    }
     __device__ uint64_t weight(float l) const {
-        if (l == top) return (uint64_t)kOne;
-        const double w = exp(((double)l - (double)top) * inv_t);
-        return w >= min_p ? (uint64_t)__double2ll_rn(w * kOne) : 0;
+        const double y = any_place(l);
+        if (!(y <= limit)) return 0;
+        const int i = (int)y;
+        return in_bin(part_of(y - (double)i), i, kOctave[i & (kPerOctave - 1)]);
     }
 };
 
@@ -89,128 +147,133 @@ __device__ inline uint64_t wave_incl_sum(uint64_t x) {
     return x;
 }
 
-// Shared memory of a workgroup.
+// Shared memory of a row's workgroup.
 struct Shared {
-    uint64_t mass[kBins];              // then inclusive sums
-    uint64_t list[kList];              // tokens: ~order << 32 | index, ascending once sorted
+    uint64_t mass[kBins];              // bins, then their running sums
+    uint64_t list[kList];              // tokens
     uint32_t count[kBins];
     uint64_t wave_mass[16];
     uint32_t wave_count[16];
-    uint64_t lo, hi;                   // composite values
+    uint64_t lo, hi;                   // tokens
     uint32_t n;
-    int found;
+    int found, at[2];
     uint32_t found_count;
     uint64_t found_mass;
 };
 
-// Exclusive sums over the workgroup's threads of (c, m); totals in the last two.
-__device__ inline void block_excl(Shared& s, uint32_t& c, uint64_t& m, uint32_t& c_all, uint64_t& m_all) {
+// Exclusive sums over the workgroup's threads of (c, m).
+template <int WAVES>
+__device__ inline void block_excl(uint32_t& c, uint64_t& m, uint32_t* sc, uint64_t* sm) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint32_t ci = (uint32_t)wave_incl_scan((int)c);
     const uint64_t mi = wave_incl_sum(m);
     __syncthreads();
     if (lane == 63) {
-        s.wave_count[w] = ci;
-        s.wave_mass[w] = mi;
+        sc[w] = ci;
+        sm[w] = mi;
     }
     __syncthreads();
-    uint32_t cb = 0;
-    uint64_t mb = 0;
-    c_all = 0;
-    m_all = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (i == w) {
-            cb = c_all;
-            mb = m_all;
-        }
-        c_all += s.wave_count[i];
-        m_all += s.wave_mass[i];
+    c = ci - c;
+    m = mi - m;
+    for (int i = 0; i < w; ++i) {
+        c += sc[i];
+        m += sm[i];
     }
-    c = cb + ci - c;
-    m = mb + mi - m;
+}
+template <int WAVES>
+__device__ inline uint64_t block_largest(uint64_t best, uint64_t* s) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) best = max(best, s[i]);
+    return best;
 }
 
-// A bound on the running count or sum, which the first element that satisfies it passes.
+// A bound on the running count or sum, which the first token that satisfies it passes.
 struct Bound {
-    enum { kRank, kReach, kPass } kind;
+    enum { kRank, kReaches, kPasses } kind;
     uint32_t rank;
     double x;
     __device__ bool passed(uint32_t c, uint64_t m) const {
-        return kind == kRank ? c >= rank : kind == kReach ? (double)m >= x : (double)m > x;
+        return kind == kRank ? c >= rank : kind == kReaches ? (double)m >= x : (double)m > x;
     }
 };
 
-// The passes over a row: f(logit, index) of every one.
-template <int TYPE>
+// Logits from .. to - 1 of a row: f(logit, index) of every one that this thread of THREADS looks at, ascending. Two
+// 16-byte pieces at a time; the code of f stands here three times.
+template <int TYPE, int THREADS>
 struct MemoryRow {
     const uint8_t* p;
-    int V;
+    int from, to;
+    __device__ MemoryRow(const SampleArgs& a, int b, int f, int t)
+        : p((const uint8_t*)a.logits + b * a.stride * Logits<TYPE>::SIZE), from(f), to(t) {}
     template <class F>
     __device__ void each(F f) const {
-        constexpr int N = Logits<TYPE>::N, SIZE = Logits<TYPE>::SIZE;
-        for (int j = (int)threadIdx.x * N; j < V; j += kThreads * N) {
-            if (j + N <= V) {
-                uint32_t x[4];
-                __builtin_memcpy(x, p + (int64_t)j * SIZE, 16);
+        constexpr int N = Logits<TYPE>::N, SIZE = Logits<TYPE>::SIZE, STEP = THREADS * N;
+        int j = from + (int)threadIdx.x * N;
+#pragma unroll 1
+        for (; j + STEP + N <= to; j += 2 * STEP) {
+            uint32_t x[4], y[4];
+            __builtin_memcpy(x, p + (int64_t)j * SIZE, 16);
+            __builtin_memcpy(y, p + (int64_t)(j + STEP) * SIZE, 16);
 #pragma unroll
-                for (int i = 0; i < N; ++i) f(Logits<TYPE>::at(x, i), j + i);
-            } else {
-                for (int i = j; i < V; ++i) f(Logits<TYPE>::one(p + (int64_t)i * SIZE), i);
-            }
+            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(x, e), j + e);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(y, e), j + STEP + e);
         }
+#pragma unroll 1
+        for (; j < to; j += STEP) {
+            const int end = min(j + N, to);
+#pragma unroll 1
+            for (int e = j; e < end; ++e) f(Logits<TYPE>::one(p + (int64_t)e * SIZE), e);
+        }
+    }
+    // the largest logit of this thread's and the first place of it: order << 32 | ~index
+    __device__ uint64_t largest() const {
+        float top = -INFINITY;
+        int at = -1;
+        each([&](float l, int j) {
+            if (l > top) {
+                top = l;
+                at = j;
+            }
+        });
+        return at < 0 ? 0 : (uint64_t)order_of(top) << 32 | ~(uint32_t)at;
     }
 };
 
-// Bins cleared, filled by `fill`, turned into running sums (bins ascending). Returns the totals.
-template <class F>
-__device__ inline void fill_bins(Shared& s, uint32_t& c_all, uint64_t& m_all, F fill) {
-    const int tid = threadIdx.x;
-    __syncthreads();
-    s.count[tid] = s.count[tid + kThreads] = 0;
-    s.mass[tid] = s.mass[tid + kThreads] = 0;
-    __syncthreads();
-    fill();
-    __syncthreads();
-    const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-    const uint64_t m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-    uint32_t c = c0 + c1;
-    uint64_t m = m0 + m1;
-    block_excl(s, c, m, c_all, m_all);
-    s.count[2 * tid] = c + c0;
-    s.count[2 * tid + 1] = c + c0 + c1;
-    s.mass[2 * tid] = m + m0;
-    s.mass[2 * tid + 1] = m + m0 + m1;
-    __syncthreads();
+// A row that needs no draw: its largest logit, or nothing to draw at all.
+__device__ inline void take_largest(const SampleArgs& a, int b, const Row& row, uint64_t best) {
+    if (threadIdx.x != 0) return;
+    a.token[b] = row.none ? 0 : (int64_t)~(uint32_t)best;
+    if (a.logprob != nullptr) a.logprob[b] = row.none ? -INFINITY : 0.f;
+    if (row.none) report_error(kErrLogits);
+}
+__device__ inline void take(const SampleArgs& a, int b, const Row& row, uint64_t token, uint64_t S) {
+    if (threadIdx.x != 0) return;
+    a.token[b] = (int64_t)(uint32_t)token;
+    if (a.logprob != nullptr) a.logprob[b] = (float)log((double)row.weight(logit_of(token)) / (double)S);
 }
 
-// The first bin in which `b` is passed, `c` and `m` being what comes before the bins (then before that bin), and
-// its count.
-__device__ inline int find_bin(Shared& s, const Bound& b, uint32_t& c, uint64_t& m, uint32_t& in) {
-    const int tid = threadIdx.x;
-    if (tid == 0) s.found = kBins;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int j = 2 * tid + i;
-        const uint32_t cp = j > 0 ? s.count[j - 1] : 0;
-        const uint64_t mp = j > 0 ? s.mass[j - 1] : 0;
-        if (s.count[j] > cp && b.passed(c + s.count[j], m + s.mass[j]) && (cp == 0 || !b.passed(c + cp, m + mp))) s.found = j;
-    }
-    __syncthreads();
-    const int j = min(s.found, kBins - 1);
-    const uint32_t cp = j > 0 ? s.count[j - 1] : 0;
-    const uint64_t mp = j > 0 ? s.mass[j - 1] : 0;
-    in = s.count[j] - cp;
-    c += cp;
-    m += mp;
-    return j;
-}
-
-// The list's n tokens in order.
+// The list's n tokens in order: up to 256 by counting, for each, those before it; more by a bitonic sort, whose exchanges
+// within 128 neighbours are one wavefront's own and need no barrier.
 __device__ inline void sort_list(Shared& s, int n) {
     const int tid = threadIdx.x;
-    int size = 64;
+    __syncthreads();
+    if (n <= 256) {                                    // uniform
+        const uint64_t x = tid < n ? s.list[tid] : 0;
+        int at = 0;
+        if (tid < n)
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) at += s.list[i] < x;
+        __syncthreads();
+        if (tid < n) s.list[at] = x;
+        __syncthreads();
+        return;
+    }
+    int size = 512;
     while (size < n) size <<= 1;
     for (int i = n + tid; i < size; i += kThreads) s.list[i] = ~0ull;
     __syncthreads();
@@ -224,18 +287,75 @@ __device__ inline void sort_list(Shared& s, int n) {
                     s.list[b] = x;
                 }
             }
-            __syncthreads();
+            if (d > 64 || (d == 1 && k >= 128))        // (the next exchange is over more than 128 neighbours, or was)
+                __syncthreads();
+            else
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+    __syncthreads();
 }
 
-// What a bound finds: the token that passes it, and the count and sum up to it.
+// ---------------------------------------------------------------- a whole row by one workgroup
+
+// Bins cleared, filled by `fill`, their masses turned into weights by `weigh`, then into running sums. Returns the totals.
+template <class F, class G>
+__device__ inline void fill_bins(Shared& s, uint32_t& c_all, uint64_t& m_all, F fill, G weigh) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    s.count[tid] = s.count[tid + kThreads] = 0;
+    s.mass[tid] = s.mass[tid + kThreads] = 0;
+    __syncthreads();
+    fill();
+    __syncthreads();
+    const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+    const uint64_t m0 = weigh(s.mass[2 * tid], 2 * tid), m1 = weigh(s.mass[2 * tid + 1], 2 * tid + 1);
+    uint32_t c = c0 + c1;
+    uint64_t m = m0 + m1;
+    block_excl<16>(c, m, s.wave_count, s.wave_mass);
+    s.count[2 * tid] = c + c0;
+    s.count[2 * tid + 1] = c + c0 + c1;
+    s.mass[2 * tid] = m + m0;
+    s.mass[2 * tid + 1] = m + m0 + m1;
+    __syncthreads();
+    c_all = s.count[kBins - 1];
+    m_all = s.mass[kBins - 1];
+}
+
+// The first bin in which `b` is passed (the last one with a token where none is), `c` and `m` being what comes before the
+// bins (then before that bin), and its count.
+__device__ inline int find_bin(Shared& s, const Bound& b, uint32_t& c, uint64_t& m, uint32_t& in) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) {
+        s.found = kBins;
+        s.at[0] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = 2 * tid + i;
+        const uint32_t cp = j > 0 ? s.count[j - 1] : 0;
+        if (s.count[j] > cp) {
+            if (b.passed(c + s.count[j], m + s.mass[j])) atomicMin(&s.found, j);
+            if (s.count[j] == s.count[kBins - 1]) s.at[0] = j;
+        }
+    }
+    __syncthreads();
+    const int j = s.found < kBins ? s.found : s.at[0];
+    const uint32_t cp = j > 0 ? s.count[j - 1] : 0;
+    const uint64_t mp = j > 0 ? s.mass[j - 1] : 0;
+    in = s.count[j] - cp;
+    c += cp;
+    m += mp;
+    return j;
+}
+
+// What a bound finds: the token that passes it, and the sum up to it.
 struct Found {
-    uint64_t token;                    // ~order << 32 | index
-    uint32_t count;
-    uint64_t mass;
+    uint64_t token, mass;
 };
 
-// In the sorted list of n tokens, with c and m before it; weights of tokens past `limit` in all count as none.
+// In the sorted list of n tokens, with c and m before it (the last one with a weight where none passes it).
 __device__ inline Found find_token(Shared& s, const Row& row, const Bound& b, int n, uint32_t c, uint64_t m) {
     constexpr int E = kList / kThreads;
     const int tid = threadIdx.x;
@@ -244,39 +364,38 @@ __device__ inline Found find_token(Shared& s, const Row& row, const Bound& b, in
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const int j = tid * E + i;
-        w[i] = j < n ? row.weight(of_order(~(uint32_t)(s.list[j] >> 32))) : 0;
+        w[i] = j < n ? row.weight(logit_of(s.list[j])) : 0;
         k += w[i] > 0;
         sum += w[i];
     }
-    uint32_t c_all;
-    uint64_t m_all;
-    block_excl(s, k, sum, c_all, m_all);
+    block_excl<16>(k, sum, s.wave_count, s.wave_mass);
     k += c;
     sum += m;
-    if (tid == 0) s.found = -1;
+    if (tid == 0) {
+        s.found = kList;
+        s.at[0] = 0;
+    }
     __syncthreads();
-    bool before = k > 0 && b.passed(k, sum);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         if (w[i] == 0) continue;
         ++k;
-        sum += w[i];
-        const bool now = b.passed(k, sum);
-        // (the last one where none passes it)
-        if ((now && !before) || (!now && k == c + c_all)) {
-            s.found = tid * E + i;
-            s.found_count = k;
-            s.found_mass = sum;
-        }
-        before = now;
+        w[i] = sum += w[i];
+        if (b.passed(k, sum)) atomicMin(&s.found, tid * E + i);
+        atomicMax(&s.at[0], tid * E + i);
     }
     __syncthreads();
-    const Found f{s.list[max(s.found, 0)], s.found_count, s.found_mass};
+    const int found = s.found < kList ? s.found : s.at[0];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (found == tid * E + i) s.found_mass = w[i];
+    __syncthreads();
+    const Found f{s.list[found], s.found_mass};
     __syncthreads();
     return f;
 }
 
-// The token that passes `b` among those of z-bin `bin`, c and m before it, `in` of them.
+// The token that passes `b` among those of bin `bin`, c and m before it, `in` of them.
 template <class R>
 __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const Bound& b, int bin, uint32_t c, uint64_t m,
                                     uint32_t in) {
@@ -284,9 +403,8 @@ __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const
     uint64_t lo = 0, hi = ~0ull;
     auto each = [&](auto f) {
         r.each([&](float l, int j) {
-            const uint32_t o = order_of(l);
-            if (o <= kMinusInf || row.bin(l) != bin) return;
-            const uint64_t x = (uint64_t)~o << 32 | (uint32_t)j;
+            if (order_of(l) <= kMinusInf || row.bin(l) != bin) return;
+            const uint64_t x = token_of(l, j);
             if (x >= lo && x <= hi) f(x, l);
         });
     };
@@ -297,8 +415,7 @@ __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const
         }
         __syncthreads();
         uint64_t a = ~0ull, z = 0;
-        each([&](uint64_t x, float l) {
-            if (row.weight(l) == 0) return;
+        each([&](uint64_t x, float) {
             a = min(a, x);
             z = max(z, x);
         });
@@ -314,13 +431,11 @@ __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const
             uint64_t m_all;
             fill_bins(s, c_all, m_all, [&] {
                 each([&](uint64_t x, float l) {
-                    const uint64_t w = row.weight(l);
-                    if (w == 0) return;
                     const int i = (int)((x - lo) >> shift);
                     atomicAdd(&s.count[i], 1u);
-                    atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)w);
+                    atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)row.weight(l));
                 });
-            });
+            }, [](uint64_t mass, int) { return mass; });
             const int i = find_bin(s, b, c, m, in);
             lo += (uint64_t)i << shift;
             hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
@@ -329,8 +444,7 @@ __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const
     __syncthreads();
     if (tid == 0) s.n = 0;
     __syncthreads();
-    each([&](uint64_t x, float l) {
-        if (row.weight(l) == 0) return;                // (below min_p: not counted either)
+    each([&](uint64_t x, float) {
         const uint32_t at = atomicAdd(&s.n, 1u);
         if (at < (uint32_t)kList) s.list[at] = x;
     });
@@ -341,57 +455,27 @@ __device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const
 }
 
 template <class R>
-__device__ inline void sample_row(Shared& s, const SampleArgs& a, const R& r, int b) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    // the largest logit, the first of equal ones
-    uint64_t best = 0;
-    r.each([&](float l, int j) { best = max(best, (uint64_t)order_of(l) << 32 | ~(uint32_t)j); });
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
-    if (lane == 0) s.wave_mass[w] = best;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) best = max(best, s.wave_mass[i]);
-    const float t = a.t != nullptr ? a.t[b] : a.t0, p = a.p != nullptr ? a.p[b] : a.p0, m = a.m != nullptr ? a.m[b] : a.m0;
-    const int k = a.k != nullptr ? a.k[b] : a.k0;
-    const uint32_t top = (uint32_t)(best >> 32);
-    if (top <= kMinusInf || !(t > 0.f)) {              // uniform
-        if (tid == 0) {
-            const bool none = top <= kMinusInf;
-            a.token[b] = none ? 0 : (int64_t)~(uint32_t)best;
-            if (a.logprob != nullptr) a.logprob[b] = none ? -INFINITY : 0.f;
-            if (none) report_error(kErrLogits);
-        }
-        return;
-    }
-    Row row;
-    row.top = of_order(top);
-    row.inv_bins = kPerNat / t;
-    row.inv_t = 1.0 / (double)t;
-    row.min_p = fmin((double)m, 1.0);
-    const float u0 = a.u[b];
-    const double u = u0 > 0.f ? fmin((double)u0, 1.0 - 0x1p-24) : 0.0;
+__device__ __attribute__((noinline)) void sample_row(Shared& s, const SampleArgs& a, const R& r, const Row& row, int b) {
+    const int tid = threadIdx.x;
     uint32_t c_all;
     uint64_t m_all;
-    const bool few = k > 0 && k <= kBins;
-    fill_bins(s, c_all, m_all, [&] {
-        r.each([&](float l, int) {
-            if (order_of(l) <= kMinusInf) return;
-            const int i = row.bin(l);
-            if (i == kBins - 1) return;                // (weights of 0)
-            if (few) {
+    auto fill = [&] {
+        fill_bins(s, c_all, m_all, [&] {
+            r.each([&](float l, int) {
+                if (order_of(l) <= kMinusInf) return;
+                const double y = row.any_place(l);
+                if (!(y <= row.limit)) return;
+                const int i = (int)y;
                 atomicAdd(&s.count[i], 1u);
-                return;
-            }
-            const uint64_t x = row.weight(l);
-            if (x == 0) return;
-            atomicAdd(&s.count[i], 1u);
-            atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)x);
-        });
-    });
-    bool listed = false;
+                atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)part_of(y - (double)i));
+            });
+        }, [](uint64_t parts, int i) { return parts == 0 ? 0 : in_bin(parts, i, kOctave[i & (kPerOctave - 1)]); });
+    };
+    fill();
+    bool listed = false, filled = true;
     int n = 0;
-    if (few) {                                         // uniform
-        const Bound rank{Bound::kRank, min((uint32_t)k, c_all), 0.0};
+    if (row.few) {                                     // uniform
+        const Bound rank{Bound::kRank, min((uint32_t)row.k, c_all), 0.0};
         uint32_t c = 0, in;
         uint64_t none = 0;
         const int last = find_bin(s, rank, c, none, in);
@@ -401,71 +485,336 @@ __device__ inline void sample_row(Shared& s, const SampleArgs& a, const R& r, in
             if (tid == 0) s.n = 0;
             __syncthreads();
             r.each([&](float l, int j) {
-                const uint32_t o = order_of(l);
-                if (o <= kMinusInf || row.bin(l) > last) return;
+                if (order_of(l) <= kMinusInf || row.bin(l) > last) return;
                 const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < (uint32_t)kList) s.list[at] = (uint64_t)~o << 32 | (uint32_t)j;
+                if (at < (uint32_t)kList) s.list[at] = token_of(l, j);
             });
             __syncthreads();
             n = min((int)s.n, kList);
             sort_list(s, n);
-        } else {
-            fill_bins(s, c_all, m_all, [&] {
-                r.each([&](float l, int) {
-                    if (order_of(l) <= kMinusInf) return;
-                    const int i = row.bin(l);
-                    const uint64_t x = i == kBins - 1 ? 0 : row.weight(l);
-                    if (x == 0) return;
-                    atomicAdd(&s.count[i], 1u);
-                    atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)x);
-                });
-            });
         }
     }
     auto find = [&](const Bound& bound) {
         if (listed) return find_token(s, row, bound, n, 0, 0);
         uint32_t c = 0, in;
         uint64_t mass = 0;
+        if (!filled) fill();
         const int bin = find_bin(s, bound, c, mass, in);
-        // (the bins are overwritten where a bin is cut further: they are filled again for the next bound)
+        filled = in <= (uint32_t)kList;                // cut further, the bins are overwritten
         return find_in_bin(s, r, row, bound, bin, c, mass, in);
     };
-    auto refill = [&] {
-        if (listed) return;
-        fill_bins(s, c_all, m_all, [&] {
-            r.each([&](float l, int) {
-                if (order_of(l) <= kMinusInf) return;
-                const int i = row.bin(l);
-                const uint64_t x = i == kBins - 1 ? 0 : row.weight(l);
-                if (x == 0) return;
-                atomicAdd(&s.count[i], 1u);
-                atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)x);
-            });
-        });
-    };
     uint64_t S = m_all;
-    if (k > 0 && (listed || (uint32_t)k < c_all)) {
-        S = find(Bound{Bound::kRank, (uint32_t)k, 0.0}).mass;
-        refill();
+    if (row.k > 0 && (listed || (uint32_t)row.k < c_all)) S = find(Bound{Bound::kRank, (uint32_t)row.k, 0.0}).mass;
+    if (row.p < 1.f) S = find(Bound{Bound::kReaches, 0, (double)row.p * (double)S}).mass;
+    take(a, b, row, find(Bound{Bound::kPasses, 0, row.u() * (double)S}).token, S);
+}
+
+// One launch, a workgroup a row: short rows.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs a) {
+    __shared__ Shared s;
+    const int b = blockIdx.x;
+    const MemoryRow<TYPE, kThreads> r(a, b, 0, a.V);
+    const uint64_t best = block_largest<16>(r.largest(), s.wave_mass);
+    const Row row(a, b, best);
+    __syncthreads();
+    if (row.greedy)                                    // uniform
+        take_largest(a, b, row, best);
+    else
+        sample_row(s, a, r, row, b);
+}
+
+// ---------------------------------------------------------------- a row in pieces
+//
+// Four launches, pieces of a row a workgroup for the first three: the largest logit of a piece; the row's bins; the
+// tokens of the bins in question; and what they say.
+constexpr int kPiece = 256;            // threads of a piece's workgroup
+constexpr int kLocal = 1024;           // tokens that a piece collects at most
+
+template <int TYPE>
+__global__ void __launch_bounds__(kPiece) sample_largest_kernel(SampleArgs a) {
+    __shared__ uint64_t s[kPiece / 64];
+    const int b = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), from = piece * a.per;
+    const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
+    for (int i = piece * kPiece + (int)threadIdx.x; i < kReach; i += a.pieces * kPiece) {
+        a.mass[(int64_t)b * kReach + i] = 0;
+        a.count[(int64_t)b * kReach + i] = 0;
     }
-    if (p < 1.f) {
-        S = find(Bound{Bound::kReach, 0, (double)p * (double)S}).mass;
-        refill();
-    }
-    const Found f = find(Bound{Bound::kPass, 0, u * (double)S});
-    if (tid == 0) {
-        const float l = of_order(~(uint32_t)(f.token >> 32));
-        a.token[b] = (int64_t)(uint32_t)f.token;
-        if (a.logprob != nullptr) a.logprob[b] = (float)log((double)row.weight(l) / (double)S);
-    }
+    if (piece == 0 && threadIdx.x == 0) a.n[b] = 0;
+    const uint64_t best = block_largest<kPiece / 64>(r.largest(), s);
+    if (threadIdx.x == 0) a.best[(int64_t)b * a.pieces + piece] = best;
+}
+
+// The largest of the row's pieces.
+template <int WAVES>
+__device__ inline uint64_t row_largest(const SampleArgs& a, int b, uint64_t* s) {
+    uint64_t best = 0;
+    for (int i = threadIdx.x; i < a.pieces; i += 64 * WAVES) best = max(best, a.best[(int64_t)b * a.pieces + i]);
+    return block_largest<WAVES>(best, s);
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kPiece) sample_bins_kernel(SampleArgs a) {
+    __shared__ uint64_t mass[kReach];
+    __shared__ uint32_t count[kReach];
+    __shared__ uint64_t s[kPiece / 64];
+    const int b = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), from = piece * a.per;
+    for (int i = threadIdx.x; i < kReach; i += kPiece) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
+    const Row row(a, b, row_largest<kPiece / 64>(a, b, s));
+    __syncthreads();
+    if (row.greedy || row.odd) return;                 // uniform
+    const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
+    if (row.few) {                                     // uniform
+        r.each([&](float l, int) {
+            const double y = row.place(l);
+            if (y <= row.limit) atomicAdd(&count[(int)y], 1u);
+        });
+    } else {
+        const bool counts = row.k > 0;
+        r.each([&](float l, int) {
+            const double y = row.place(l);
+            if (!(y <= row.limit)) return;
+            const int i = (int)y;
+            atomicAdd((unsigned long long*)&mass[i], (unsigned long long)part_of(__builtin_amdgcn_fract(y)));
+            if (counts) atomicAdd(&count[i], 1u);
+        });
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kReach; i += kPiece) {
+        if (mass[i] != 0) atomicAdd((unsigned long long*)&a.mass[(int64_t)b * kReach + i], (unsigned long long)mass[i]);
+        if (count[i] != 0) atomicAdd(&a.count[(int64_t)b * kReach + i], count[i]);
+    }
+}
+
+// Which bins the row's bounds are in: ranges that ascend and lie apart (empty ones: last below first), and the count and
+// sum that a token in one has before it less those of the collected tokens before it.
+struct Range {
+    int first = 1, last = 0;
+    uint32_t count = 0;
+    uint64_t mass = 0;
+};
+struct Ranges {
+    Range r[3];
+    bool cut;                          // top_k cuts
+    uint64_t all;                      // the sum of all weights
+    __device__ bool hold(int bin) const {
+        bool in = false;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) in |= bin >= r[i].first && bin <= r[i].last;
+        return in;
+    }
+    __device__ void before(int bin, uint32_t& c, uint64_t& m) const {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (bin >= r[i].first && bin <= r[i].last) {
+                c += r[i].count;
+                m += r[i].mass;
+            }
+    }
+};
+
+// A row's bins as loaded, E neighbouring ones a thread of kBins / E.
+template <int E>
+struct Bins {
+    uint64_t m[E];
+    uint32_t c[E];
+    __device__ Bins(const SampleArgs& a, int b) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = (int)threadIdx.x * E + i;
+            m[i] = j < kReach ? a.mass[(int64_t)b * kReach + j] : 0;
+            c[i] = j < kReach ? a.count[(int64_t)b * kReach + j] : 0;
+        }
+    }
+};
+
+// The row's bins as running sums in `mass` and `count` [kBins], and the ranges of its bounds; sc, sm, at: scratch. All
+// threads get the same.
+template <int THREADS>
+__device__ inline Ranges find_ranges(const Row& row, const Bins<kBins / THREADS>& bins, uint64_t* mass, uint32_t* count, int* at,
+                                     uint32_t* sc, uint64_t* sm) {
+    constexpr int E = kBins / THREADS;
+    const int j0 = (int)threadIdx.x * E;
+    const bool counts = row.k > 0;
+    uint64_t m[E], ms = 0;
+    uint32_t c[E], cs = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        c[i] = bins.c[i];
+        m[i] = bins.m[i] == 0 ? 0 : in_bin(bins.m[i], j0 + i, kOctave[(j0 + i) & (kPerOctave - 1)]);
+        ms += m[i];
+        cs += c[i];
+    }
+    block_excl<THREADS / 64>(cs, ms, sc, sm);
+    const uint64_t m0 = ms;
+    const uint32_t c0 = cs;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        m[i] = mass[j0 + i] = ms += m[i];
+        c[i] = count[j0 + i] = cs += c[i];
+    }
+    // the first bins that satisfy two bounds (the last bin where none does)
+    auto find = [&](auto passed0, auto passed1, int& x, int& y) {
+        __syncthreads();
+        if (threadIdx.x == 0) at[0] = at[1] = kReach - 1;
+        __syncthreads();
+        uint32_t cb = c0;
+        uint64_t mb = m0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (passed0(c[i], m[i]) && (j0 + i == 0 || !passed0(cb, mb))) at[0] = j0 + i;
+            if (passed1(c[i], m[i]) && (j0 + i == 0 || !passed1(cb, mb))) at[1] = j0 + i;
+            cb = c[i];
+            mb = m[i];
+        }
+        __syncthreads();
+        x = at[0];
+        y = at[1];
+    };
+    Ranges r;
+    __syncthreads();
+    r.all = mass[kBins - 1];
+    const uint32_t c_all = count[kBins - 1];
+    r.cut = counts && (row.few || (uint32_t)row.k < c_all);
+    int x, y;
+    double s0 = (double)r.all, s1 = s0;                // the sums that are known to a bin, from and to
+    if (r.cut) {                                       // uniform
+        const uint32_t k = min((uint32_t)row.k, c_all);
+        auto reach = [&](uint32_t n, uint64_t) { return n >= k; };
+        find(reach, reach, x, y);
+        r.r[2].first = row.few ? 0 : x;
+        r.r[2].last = x;
+        s0 = x > 0 ? (double)mass[x - 1] : 0.0;
+        s1 = (double)mass[x];
+    }
+    if (row.few) return r;
+    if (row.p < 1.f) {                                 // uniform
+        const double p0 = (double)row.p * s0, p1 = (double)row.p * s1;
+        find([&](uint32_t, uint64_t f) { return (double)f >= p0; }, [&](uint32_t, uint64_t f) { return (double)f >= p1; }, x, y);
+        r.r[1].first = x;
+        r.r[1].last = y;
+        s0 = x > 0 ? (double)mass[x - 1] : 0.0;
+        s1 = (double)mass[y];
+    }
+    const double u0 = row.u() * s0, u1 = row.u() * s1;
+    find([&](uint32_t, uint64_t f) { return (double)f > u0; }, [&](uint32_t, uint64_t f) { return (double)f > u1; }, x, y);
+    r.r[0].first = x;
+    r.r[0].last = y;
+    // (each bound lies at or before the next range's)
+    r.r[1].first = max(r.r[1].first, y + 1);
+    r.r[2].first = max(r.r[2].first, max(y, r.r[1].last) + 1);
+    uint64_t took_m = 0;
+    uint32_t took_c = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (r.r[i].last < r.r[i].first) continue;
+        const int f = r.r[i].first;
+        const uint64_t before_m = f > 0 ? mass[f - 1] : 0;
+        const uint32_t before_c = f > 0 ? count[f - 1] : 0;
+        r.r[i].mass = before_m - took_m;
+        r.r[i].count = before_c - took_c;
+        took_m += mass[r.r[i].last] - before_m;
+        took_c += count[r.r[i].last] - before_c;
+    }
+    return r;
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
+    __shared__ uint64_t mass[kBins], list[kLocal];
+    __shared__ uint32_t count[kBins];
+    __shared__ uint64_t s[kPiece / 64], sm[kPiece / 64];
+    __shared__ uint32_t sc[kPiece / 64], n, base;
+    __shared__ int at[2];
+    const int b = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), from = piece * a.per;
+    const Bins<kBins / kPiece> bins(a, b);
+    const Row row(a, b, row_largest<kPiece / 64>(a, b, s));
+    if (threadIdx.x == 0) n = 0;
+    if (row.greedy || row.odd) return;                 // uniform
+    const Ranges ranges = find_ranges<kPiece>(row, bins, mass, count, at, sc, sm);
+    const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
+    r.each([&](float l, int j) {
+        const double y = row.place(l);
+        if (!(y <= row.limit) || !ranges.hold((int)y)) return;
+        const uint32_t i = atomicAdd(&n, 1u);
+        if (i < (uint32_t)kLocal) list[i] = token_of(l, j);
+    });
+    __syncthreads();
+    if (n == 0) return;                                // uniform
+    if (threadIdx.x == 0) base = atomicAdd(&a.n[b], n <= (uint32_t)kLocal ? n : (uint32_t)kList + 1);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(n, (uint32_t)kLocal); i += kPiece)
+        if (base + i < (uint32_t)kList) a.list[(int64_t)b * kList + base + i] = list[i];
+}
+
+// The collected tokens sorted, and the row's bounds found among them one after the other.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
     __shared__ Shared s;
-    const int b = blockIdx.x;
-    const MemoryRow<TYPE> r{(const uint8_t*)a.logits + b * a.stride * Logits<TYPE>::SIZE, a.V};
-    sample_row(s, a, r, b);
+    constexpr int E = kList / kThreads;
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const Bins<kBins / kThreads> bins(a, b);
+    const uint32_t n_all = a.n[b];
+    const uint64_t early = a.list[(int64_t)b * kList + tid];
+    const uint64_t best = row_largest<16>(a, b, s.wave_mass);
+    const Row row(a, b, best);
+    __syncthreads();
+    if (row.greedy) return take_largest(a, b, row, best);   // uniform
+    if (row.odd || n_all > (uint32_t)kList) {          // uniform: more equal or near ones than the list holds
+        sample_row(s, a, MemoryRow<TYPE, kThreads>(a, b, 0, a.V), row, b);
+        return;
+    }
+    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
+    const int n = (int)n_all;
+    if (tid < n) s.list[tid] = early;
+    for (int i = tid + kThreads; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
+    sort_list(s, n);
+    // each token's running count and sum over the row
+    uint64_t w[E], F[E], m = 0;
+    uint32_t K[E], c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int j = tid * E + i;
+        w[i] = 0;
+        F[i] = 0;
+        K[i] = 0;
+        if (j < n) {
+            const float l = logit_of(s.list[j]);
+            w[i] = row.weight(l);
+            ranges.before(row.bin(l), K[i], F[i]);
+            ++c;
+            m += w[i];
+        }
+    }
+    block_excl<16>(c, m, s.wave_count, s.wave_mass);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        F[i] += m += w[i];
+        K[i] += ++c;
+    }
+    // the first token that satisfies a bound, or the last one
+    auto find = [&](const Bound& bound) {
+        if (tid == 0) s.found = n - 1;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (tid * E + i < n && bound.passed(K[i], F[i])) atomicMin(&s.found, tid * E + i);
+        __syncthreads();
+        const int found = s.found;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (found == tid * E + i) s.found_mass = F[i];
+        __syncthreads();
+        return s.found_mass;
+    };
+    uint64_t S = ranges.all;
+    if (ranges.cut) S = find(Bound{Bound::kRank, (uint32_t)row.k, 0.0});
+    if (row.p < 1.f) S = find(Bound{Bound::kReaches, 0, (double)row.p * (double)S});
+    find(Bound{Bound::kPasses, 0, row.u() * (double)S});
+    take(a, b, row, s.list[s.found], S);
 }
 
 hipError_t fetch_errors_sample(uint32_t* out, int first, int clear, hipStream_t stream) {
@@ -476,22 +825,66 @@ hipError_t fetch_errors_sample(uint32_t* out, int first, int clear, hipStream_t 
 
 using namespace exkv;
 
+// Rows of up to this many logits go by one workgroup each.
+constexpr int kShort = 8192;
+
+struct SamplePlan {
+    int pieces, per;
+    int64_t best, mass, list, count, n, bytes;         // offsets in the workspace
+};
+static SamplePlan plan_sample(int64_t B, int64_t V) {
+    SamplePlan p{};
+    if (V <= kShort || B == 0) return p;
+    // pieces of whole 2,048 logits, of 4,096 at least, about 1,024 workgroups in all
+    int64_t pieces = (1024 + B - 1) / B;
+    if (pieces > V / 4096) pieces = V / 4096;
+    p.per = (int)(((V + pieces - 1) / pieces + 2047) / 2048 * 2048);
+    p.pieces = (int)((V + p.per - 1) / p.per);
+    p.mass = B * p.pieces * 8;
+    p.list = p.mass + B * kReach * 8;
+    p.count = p.list + B * kList * 8;
+    p.n = p.count + B * kReach * 4;
+    p.bytes = p.n + B * 4;
+    return p;
+}
+
+template <int TYPE>
+static void launch_sample(const SampleArgs& a, hipStream_t stream) {
+    if (a.pieces == 0) {
+        hipLaunchKernelGGL((sample_row_kernel<TYPE>), dim3((unsigned)a.B), dim3(kThreads), 0, stream, a);
+        return;
+    }
+    const dim3 grid((unsigned)((int64_t)a.B * a.pieces)), block(kPiece);
+    hipLaunchKernelGGL((sample_largest_kernel<TYPE>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sample_bins_kernel<TYPE>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sample_collect_kernel<TYPE>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sample_take_kernel<TYPE>), dim3((unsigned)a.B), dim3(kThreads), 0, stream, a);
+}
+
+extern "C" int64_t exkv_sample_workspace(int32_t B, int32_t V) { return B <= 0 || V <= 0 ? 0 : plan_sample(B, V).bytes; }
+
 extern "C" int exkv_sample(const void* logits, int64_t stride, int32_t type, int32_t B, int32_t V, const float* u, const float* temperature,
                            const int32_t* top_k, const float* top_p, const float* min_p, float temperature0, int32_t top_k0,
-                           float top_p0, float min_p0, int64_t* token, float* logprob, hipStream_t stream) {
+                           float top_p0, float min_p0, int64_t* token, float* logprob, void* ws, int64_t ws_bytes, hipStream_t stream) {
     EXKV_REQUIRE(type >= 0 && type <= 2, "sample: logits of type %d", type);
     EXKV_REQUIRE(B >= 0 && V > 0 && V <= (1 << 19) && stride >= 0, "sample: bad shape B=%d V=%d (up to %d)", B, V, 1 << 19);
-    EXKV_REQUIRE((int64_t)B * kThreads <= (int64_t)UINT32_MAX, "sample: too many rows (%d)", B);
     if (B == 0) return EXKV_OK;
+    const SamplePlan p = plan_sample(B, V);
+    EXKV_REQUIRE((int64_t)B * kThreads <= (int64_t)UINT32_MAX && (int64_t)B * p.pieces * kPiece <= (int64_t)UINT32_MAX,
+                 "sample: too many rows (%d)", B);
     EXKV_REQUIRE(logits && u && token, "sample: null pointer");
     EXKV_REQUIRE((uintptr_t)logits % (type == kFp32 ? 4 : 2) == 0, "sample: logits must be aligned to their size");
-    const SampleArgs a{logits, stride, B, V, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, token, logprob};
-    const dim3 grid((unsigned)B), block(kThreads);
+    EXKV_REQUIRE(p.bytes == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.bytes), "sample: workspace of %lld bytes, %lld needed",
+                 (long long)ws_bytes, (long long)p.bytes);
+    uint8_t* w = (uint8_t*)ws;
+    const SampleArgs a{logits, stride, B, V, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, token, logprob,
+                       p.pieces, p.per, (uint64_t*)w, (uint64_t*)(w + p.mass), (uint64_t*)(w + p.list), (uint32_t*)(w + p.count),
+                       (uint32_t*)(w + p.n)};
     if (type == kBf16)
-        hipLaunchKernelGGL((sample_kernel<kBf16>), grid, block, 0, stream, a);
+        launch_sample<kBf16>(a, stream);
     else if (type == kFp16)
-        hipLaunchKernelGGL((sample_kernel<kFp16>), grid, block, 0, stream, a);
+        launch_sample<kFp16>(a, stream);
     else
-        hipLaunchKernelGGL((sample_kernel<kFp32>), grid, block, 0, stream, a);
+        launch_sample<kFp32>(a, stream);
     return hip_status(hipGetLastError(), "sample");
 }

@@ -63,8 +63,11 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob
                          f"{top_k!r}, {top_p!r}, {min_p!r})")
     token = torch.empty(B, dtype=torch.int64, device=logits.device)
     lp = torch.empty(B, dtype=f32, device=logits.device) if logprob else None
+    need = _lib.load().exkv_sample_workspace(B, V)
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     _lib.call("exkv_sample", logits.data_ptr(), logits.stride(0) if B > 1 else V, kind, B, V, u.data_ptr(), tp, kp, pp, mp, t, k, p, m,
-              token.data_ptr(), lp.data_ptr() if logprob else None, _lib.stream(dev))
+              token.data_ptr(), lp.data_ptr() if logprob else None, ws.data_ptr() if need else None, need,
+              _lib.stream(dev))
     return (token, lp) if logprob else token
 
 

@@ -14,7 +14,8 @@ def _fails(name, args, words):
 
 
 def _sample(**kw):
-    a = dict(logits=16, stride=100, type=0, B=4, V=100, u=16, t=None, k=None, p=None, m=None, t0=1.0, k0=0, p0=1.0, m0=0.0, token=16, lp=None)
+    a = dict(logits=16, stride=100, type=0, B=4, V=100, u=16, t=None, k=None, p=None, m=None, t0=1.0, k0=0, p0=1.0, m0=0.0, token=16, lp=None, ws=None,
+             wsb=0)
     a.update(kw)
     return (*a.values(), None)
 
@@ -22,7 +23,8 @@ def _sample(**kw):
 @pytest.mark.parametrize("kw,words", [
     (dict(type=3), "type"), (dict(type=-1), "type"), (dict(V=0), "bad shape"), (dict(V=2 ** 19 + 1), "bad shape"), (dict(B=-1), "bad shape"),
     (dict(stride=-1), "bad shape"), (dict(B=2 ** 23), "too many rows"), (dict(logits=None), "null pointer"), (dict(u=None), "null pointer"),
-    (dict(token=None), "null pointer"), (dict(logits=17), "aligned"), (dict(type=2, logits=18), "aligned"),
+    (dict(token=None), "null pointer"), (dict(logits=17), "aligned"), (dict(type=2, logits=18), "aligned"), (dict(V=9000), "workspace"),
+    (dict(V=9000, ws=16, wsb=100), "workspace"), (dict(V=9000, ws=24, wsb=1 << 30), "workspace"),
 ], ids=str)
 def test_sample_arguments(kw, words):
     _fails("exkv_sample", _sample(**kw), words)
