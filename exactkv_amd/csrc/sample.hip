@@ -100,20 +100,25 @@ __device__ inline uint64_t in_bin(uint64_t parts, int i, double octave) {
     return (uint64_t)rint(__builtin_amdgcn_ldexp((double)parts * octave, -(i / kPerOctave)));
 }
 
-// A row's settings.
+// A row's settings, and with its largest logit what its weights go by.
+struct Settings {
+    float t, p, m, u;
+    int k;
+    __device__ Settings(const SampleArgs& a, int b)
+        : t(a.t != nullptr ? a.t[b] : a.t0), p(a.p != nullptr ? a.p[b] : a.p0), m(a.m != nullptr ? a.m[b] : a.m0), u(a.u[b]),
+          k(a.k != nullptr ? a.k[b] : a.k0) {}
+    __device__ bool few() const { return k > 0 && k <= kList / 2; }     // collected by counts alone
+};
 struct Row {
     double top, per_bin, limit;        // the largest logit; bins of a logit; the last y that counts
+    const double* octave;              // kOctave in LDS
     float top32, p, u0;
     int k;
-    bool none, greedy, odd, few;       // odd: the largest is infinite; few: collected by counts alone
-    __device__ Row(const SampleArgs& a, int b, uint64_t best) {
-        const float t = a.t != nullptr ? a.t[b] : a.t0, m = a.m != nullptr ? a.m[b] : a.m0;
-        p = a.p != nullptr ? a.p[b] : a.p0;
-        k = a.k != nullptr ? a.k[b] : a.k0;
-        u0 = a.u[b];
+    bool none, greedy, odd, few;       // odd: the largest is infinite
+    __device__ Row(const Settings& set, uint64_t best, const double* table) : octave(table), p(set.p), u0(set.u), k(set.k), few(set.few()) {
+        const float t = set.t, m = set.m;
         none = (uint32_t)(best >> 32) <= kMinusInf;
         greedy = none || !(t > 0.f);
-        few = k > 0 && k <= kList / 2;
         top32 = of_order((uint32_t)(best >> 32));
         odd = top32 == INFINITY;
         top = (double)top32;
@@ -133,22 +138,38 @@ struct Row {
         const double y = any_place(l);
         if (!(y <= limit)) return 0;
         const int i = (int)y;
-        return in_bin(part_of(y - (double)i), i, kOctave[i & (kPerOctave - 1)]);
+        return in_bin(part_of(y - (double)i), i, octave[i & (kPerOctave - 1)]);
     }
 };
 
+// Inclusive sums across the lanes of a wavefront, by the steps of wave_incl_scan.
+template <int CTRL, int ROWS>
+__device__ inline uint64_t moved(uint64_t x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
 __device__ inline uint64_t wave_incl_sum(uint64_t x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)x, d);
-        if (lane >= d) x += y;
-    }
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);
+    x += moved<0x143, 0xc>(x);
     return x;
+}
+// The first of the wavefronts' lowest values, `none` where a lane has none: to *at, one atomic a wavefront. (A lane's value
+// lies below those of the lanes behind it.)
+__device__ inline void first_of(int x, int none, int* at) {
+    const uint64_t lanes = __ballot(x != none);
+    if (lanes == 0) return;
+    const int first = __builtin_amdgcn_readlane(x, __builtin_ctzll(lanes));
+    if ((threadIdx.x & 63) == 0) atomicMin(at, first);
 }
 
 // Shared memory of a row's workgroup.
 struct Shared {
+    double octave[kPerOctave];
     uint64_t mass[kBins];              // bins, then their running sums
     uint64_t list[kList];              // tokens
     uint32_t count[kBins];
@@ -202,7 +223,7 @@ struct Bound {
 };
 
 // Logits from .. to - 1 of a row: f(logit, index) of every one that this thread of THREADS looks at, ascending. Two
-// 16-byte pieces at a time; the code of f stands here three times.
+// 16-byte pieces at a time, the next two already on their way; the code of f stands here three times.
 template <int TYPE, int THREADS>
 struct MemoryRow {
     const uint8_t* p;
@@ -213,15 +234,27 @@ struct MemoryRow {
     __device__ void each(F f) const {
         constexpr int N = Logits<TYPE>::N, SIZE = Logits<TYPE>::SIZE, STEP = THREADS * N;
         int j = from + (int)threadIdx.x * N;
+        uint32_t x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+        auto load = [&](int at) {
+            if (at + STEP + N <= to) {
+                __builtin_memcpy(x, p + (int64_t)at * SIZE, 16);
+                __builtin_memcpy(y, p + (int64_t)(at + STEP) * SIZE, 16);
+            }
+        };
+        load(j);
 #pragma unroll 1
         for (; j + STEP + N <= to; j += 2 * STEP) {
-            uint32_t x[4], y[4];
-            __builtin_memcpy(x, p + (int64_t)j * SIZE, 16);
-            __builtin_memcpy(y, p + (int64_t)(j + STEP) * SIZE, 16);
+            uint32_t u[4], v[4];
 #pragma unroll
-            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(x, e), j + e);
+            for (int i = 0; i < 4; ++i) {
+                u[i] = x[i];
+                v[i] = y[i];
+            }
+            load(j + 2 * STEP);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(y, e), j + STEP + e);
+            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(u, e), j + e);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(v, e), j + STEP + e);
         }
 #pragma unroll 1
         for (; j < to; j += STEP) {
@@ -369,6 +402,8 @@ __device__ inline Found find_token(Shared& s, const Row& row, const Bound& b, in
         sum += w[i];
     }
     block_excl<16>(k, sum, s.wave_count, s.wave_mass);
+    uint32_t k_all = 0;
+    for (int i = 0; i < 16; ++i) k_all += s.wave_count[i];
     k += c;
     sum += m;
     if (tid == 0) {
@@ -376,14 +411,16 @@ __device__ inline Found find_token(Shared& s, const Row& row, const Bound& b, in
         s.at[0] = 0;
     }
     __syncthreads();
+    int first = kList;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         if (w[i] == 0) continue;
         ++k;
         w[i] = sum += w[i];
-        if (b.passed(k, sum)) atomicMin(&s.found, tid * E + i);
-        atomicMax(&s.at[0], tid * E + i);
+        if (first == kList && b.passed(k, sum)) first = tid * E + i;
+        if (k == c + k_all) s.at[0] = tid * E + i;
     }
+    first_of(first, kList, &s.found);
     __syncthreads();
     const int found = s.found < kList ? s.found : s.at[0];
 #pragma unroll
@@ -469,7 +506,7 @@ __device__ __attribute__((noinline)) void sample_row(Shared& s, const SampleArgs
                 atomicAdd(&s.count[i], 1u);
                 atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)part_of(y - (double)i));
             });
-        }, [](uint64_t parts, int i) { return parts == 0 ? 0 : in_bin(parts, i, kOctave[i & (kPerOctave - 1)]); });
+        }, [&](uint64_t parts, int i) { return parts == 0 ? 0 : in_bin(parts, i, row.octave[i & (kPerOctave - 1)]); });
     };
     fill();
     bool listed = false, filled = true;
@@ -515,8 +552,10 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs a) {
     __shared__ Shared s;
     const int b = blockIdx.x;
     const MemoryRow<TYPE, kThreads> r(a, b, 0, a.V);
+    const Settings set(a, b);
+    if (threadIdx.x < kPerOctave) s.octave[threadIdx.x] = kOctave[threadIdx.x];
     const uint64_t best = block_largest<16>(r.largest(), s.wave_mass);
-    const Row row(a, b, best);
+    const Row row(set, best, s.octave);
     __syncthreads();
     if (row.greedy)                                    // uniform
         take_largest(a, b, row, best);
@@ -563,7 +602,8 @@ __global__ void __launch_bounds__(kPiece) sample_bins_kernel(SampleArgs a) {
         mass[i] = 0;
         count[i] = 0;
     }
-    const Row row(a, b, row_largest<kPiece / 64>(a, b, s));
+    const Settings set(a, b);
+    const Row row(set, row_largest<kPiece / 64>(a, b, s), nullptr);
     __syncthreads();
     if (row.greedy || row.odd) return;                 // uniform
     const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
@@ -621,12 +661,13 @@ template <int E>
 struct Bins {
     uint64_t m[E];
     uint32_t c[E];
-    __device__ Bins(const SampleArgs& a, int b) {
+    __device__ Bins(const SampleArgs& a, const Settings& set, int b) {
+        const bool masses = !set.few(), counts = set.k > 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const int j = (int)threadIdx.x * E + i;
-            m[i] = j < kReach ? a.mass[(int64_t)b * kReach + j] : 0;
-            c[i] = j < kReach ? a.count[(int64_t)b * kReach + j] : 0;
+            m[i] = j < kReach && masses ? a.mass[(int64_t)b * kReach + j] : 0;
+            c[i] = j < kReach && counts ? a.count[(int64_t)b * kReach + j] : 0;
         }
     }
 };
@@ -644,7 +685,7 @@ __device__ inline Ranges find_ranges(const Row& row, const Bins<kBins / THREADS>
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         c[i] = bins.c[i];
-        m[i] = bins.m[i] == 0 ? 0 : in_bin(bins.m[i], j0 + i, kOctave[(j0 + i) & (kPerOctave - 1)]);
+        m[i] = bins.m[i] == 0 ? 0 : in_bin(bins.m[i], j0 + i, row.octave[(j0 + i) & (kPerOctave - 1)]);
         ms += m[i];
         cs += c[i];
     }
@@ -726,12 +767,15 @@ template <int TYPE>
 __global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
     __shared__ uint64_t mass[kBins], list[kLocal];
     __shared__ uint32_t count[kBins];
+    __shared__ double octave[kPerOctave];
     __shared__ uint64_t s[kPiece / 64], sm[kPiece / 64];
     __shared__ uint32_t sc[kPiece / 64], n, base;
     __shared__ int at[2];
     const int b = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), from = piece * a.per;
-    const Bins<kBins / kPiece> bins(a, b);
-    const Row row(a, b, row_largest<kPiece / 64>(a, b, s));
+    const Settings set(a, b);
+    if (threadIdx.x < kPerOctave) octave[threadIdx.x] = kOctave[threadIdx.x];
+    const Bins<kBins / kPiece> bins(a, set, b);
+    const Row row(set, row_largest<kPiece / 64>(a, b, s), octave);
     if (threadIdx.x == 0) n = 0;
     if (row.greedy || row.odd) return;                 // uniform
     const Ranges ranges = find_ranges<kPiece>(row, bins, mass, count, at, sc, sm);
@@ -756,21 +800,21 @@ __global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
     __shared__ Shared s;
     constexpr int E = kList / kThreads;
     const int b = blockIdx.x, tid = threadIdx.x;
-    const Bins<kBins / kThreads> bins(a, b);
+    const Settings set(a, b);
     const uint32_t n_all = a.n[b];
-    const uint64_t early = a.list[(int64_t)b * kList + tid];
+    if (tid < kPerOctave) s.octave[tid] = kOctave[tid];
+    const Bins<kBins / kThreads> bins(a, set, b);
     const uint64_t best = row_largest<16>(a, b, s.wave_mass);
-    const Row row(a, b, best);
+    const Row row(set, best, s.octave);
     __syncthreads();
     if (row.greedy) return take_largest(a, b, row, best);   // uniform
     if (row.odd || n_all > (uint32_t)kList) {          // uniform: more equal or near ones than the list holds
         sample_row(s, a, MemoryRow<TYPE, kThreads>(a, b, 0, a.V), row, b);
         return;
     }
-    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
     const int n = (int)n_all;
-    if (tid < n) s.list[tid] = early;
-    for (int i = tid + kThreads; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
+    for (int i = tid; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
+    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
     sort_list(s, n);
     // each token's running count and sum over the row
     uint64_t w[E], F[E], m = 0;
@@ -799,9 +843,11 @@ __global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
     auto find = [&](const Bound& bound) {
         if (tid == 0) s.found = n - 1;
         __syncthreads();
+        int first = kList;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (tid * E + i < n && bound.passed(K[i], F[i])) atomicMin(&s.found, tid * E + i);
+        for (int i = E - 1; i >= 0; --i)
+            if (tid * E + i < n && bound.passed(K[i], F[i])) first = tid * E + i;
+        first_of(first, kList, &s.found);
         __syncthreads();
         const int found = s.found;
 #pragma unroll
