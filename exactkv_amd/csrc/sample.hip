@@ -95,6 +95,13 @@ __device__ inline uint64_t part_of(double f) {
     x = fma(x, f, kOne + 0x1p52);
     return (uint64_t)__double_as_longlong(x) & 0xFFFFFFFFFFFFFull;
 }
+// The whole and the rest of y, from kBase + y.
+constexpr double kBase = 2048.0;
+static_assert(kReach < 2048, "y below kBase");
+__device__ inline int whole_of(double y) { return (int)((uint32_t)(__double_as_longlong(y) >> 41) & 0x7FFu); }
+__device__ inline double rest_of(double y) {
+    return __longlong_as_double((__double_as_longlong(y) & 0x1FFFFFFFFFFll) | 0x40A0000000000000ll) - kBase;
+}
 // A sum of such parts in bin i, in weights.
 __device__ inline uint64_t in_bin(uint64_t parts, int i, double octave) {
     return (uint64_t)rint(__builtin_amdgcn_ldexp((double)parts * octave, -(i / kPerOctave)));
@@ -115,7 +122,7 @@ struct Row {
     float top32, p, u0;
     int k;
     bool none, greedy, odd, few;       // odd: the largest is infinite
-    __device__ Row(const Settings& set, uint64_t best, const double* table) : octave(table), p(set.p), u0(set.u), k(set.k), few(set.few()) {
+    __device__ __attribute__((always_inline)) Row(const Settings& set, uint64_t best, const double* table) : octave(table), p(set.p), u0(set.u), k(set.k), few(set.few()) {
         const float t = set.t, m = set.m;
         none = (uint32_t)(best >> 32) <= kMinusInf;
         greedy = none || !(t > 0.f);
@@ -123,22 +130,23 @@ struct Row {
         odd = top32 == INFINITY;
         top = (double)top32;
         per_bin = kPerOctave * 1.4426950408889634 / (double)t;
-        limit = kReach - 0x1p-40;
-        if (!(m <= 0.f)) limit = fmin(limit, m < 1.f ? -(double)kPerOctave * log2((double)m) : 0.0);
+        limit = kBase + kReach - 0x1p-40;
+        if (!(m <= 0.f)) limit = fmin(limit, m < 1.f ? kBase - (double)kPerOctave * log2((double)m) : kBase);
     }
     __device__ double u() const { return u0 > 0.f ? fmin((double)u0, 1.0 - 0x1p-24) : 0.0; }
-    // y: ascends as l falls; not within the limit (NaN too): a weight of 0
-    __device__ double place(float l) const { return (top - (double)l) * per_bin; }
-    __device__ double any_place(float l) const { return l == top32 ? 0.0 : place(l); }
+    // 2^11 + y, rounded to 41 bits behind the point, so that its bits hold y's whole and its rest: ascends as l falls; not
+    // within the limit (NaN too): a weight of 0.
+    __device__ double place(float l) const { return fma(top - (double)l, per_bin, kBase); }
+    __device__ double any_place(float l) const { return l == top32 ? kBase : place(l); }
     __device__ int bin(float l) const {
         const double y = any_place(l);
-        return y <= limit ? (int)y : kReach;
+        return y <= limit ? whole_of(y) : kReach;
     }
     __device__ uint64_t weight(float l) const {
         const double y = any_place(l);
         if (!(y <= limit)) return 0;
-        const int i = (int)y;
-        return in_bin(part_of(y - (double)i), i, octave[i & (kPerOctave - 1)]);
+        const int i = whole_of(y);
+        return in_bin(part_of(rest_of(y)), i, octave[i & (kPerOctave - 1)]);
     }
 };
 
@@ -222,26 +230,47 @@ struct Bound {
     }
 };
 
-// Logits from .. to - 1 of a row: f(logit, index) of every one that this thread of THREADS looks at, ascending. Two
-// 16-byte pieces at a time, the next two already on their way; the code of f stands here three times.
+// Logits from .. to - 1 of a row, as a workgroup of THREADS looks at them: 16-byte pieces wherever they lie, ascending for a
+// thread, what is behind the end as -infinity.
 template <int TYPE, int THREADS>
 struct MemoryRow {
+    static constexpr int N = Logits<TYPE>::N, SIZE = Logits<TYPE>::SIZE, STEP = THREADS * N;
     const uint8_t* p;
     int from, to;
-    __device__ MemoryRow(const SampleArgs& a, int b, int f, int t)
-        : p((const uint8_t*)a.logits + b * a.stride * Logits<TYPE>::SIZE), from(f), to(t) {}
+    __device__ MemoryRow(const SampleArgs& a, int b, int f, int t) : p((const uint8_t*)a.logits + b * a.stride * SIZE), from(f), to(t) {}
+    __device__ float one(int j) const { return Logits<TYPE>::one(p + (int64_t)j * SIZE); }
+    __device__ void load(int j, uint32_t (&x)[4]) const {
+        if (j + N <= to) {
+            __builtin_memcpy(x, p + (int64_t)j * SIZE, 16);
+            return;
+        }
+        constexpr uint32_t NONE = TYPE == kFp32 ? 0xFF800000u : TYPE == kBf16 ? 0xFF80FF80u : 0xFC00FC00u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = NONE;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if (j + e >= to) continue;
+            const uint8_t* at = p + (int64_t)(j + e) * SIZE;
+            if constexpr (SIZE == 4) {
+                x[e] = *reinterpret_cast<const uint32_t*>(at);
+            } else {
+                const uint32_t v = *reinterpret_cast<const uint16_t*>(at);
+                x[e / 2] = e % 2 != 0 ? (x[e / 2] & 0xFFFFu) | v << 16 : (x[e / 2] & 0xFFFF0000u) | v;
+            }
+        }
+    }
+    // f(piece, index of its first logit): two at a time, the next two on their way; the code of f stands here three times
     template <class F>
-    __device__ void each(F f) const {
-        constexpr int N = Logits<TYPE>::N, SIZE = Logits<TYPE>::SIZE, STEP = THREADS * N;
+    __device__ void pieces(F f) const {
         int j = from + (int)threadIdx.x * N;
         uint32_t x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
-        auto load = [&](int at) {
+        auto ahead = [&](int at) {
             if (at + STEP + N <= to) {
                 __builtin_memcpy(x, p + (int64_t)at * SIZE, 16);
                 __builtin_memcpy(y, p + (int64_t)(at + STEP) * SIZE, 16);
             }
         };
-        load(j);
+        ahead(j);
 #pragma unroll 1
         for (; j + STEP + N <= to; j += 2 * STEP) {
             uint32_t u[4], v[4];
@@ -250,30 +279,44 @@ struct MemoryRow {
                 u[i] = x[i];
                 v[i] = y[i];
             }
-            load(j + 2 * STEP);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(u, e), j + e);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f(Logits<TYPE>::at(v, e), j + STEP + e);
+            ahead(j + 2 * STEP);
+            f(u, j);
+            f(v, j + STEP);
         }
 #pragma unroll 1
         for (; j < to; j += STEP) {
-            const int end = min(j + N, to);
+            load(j, x);
+            f(x, j);
+        }
+    }
+    // f(logit, index): less code
+    template <class F>
+    __device__ void each(F f) const {
 #pragma unroll 1
-            for (int e = j; e < end; ++e) f(Logits<TYPE>::one(p + (int64_t)e * SIZE), e);
+        for (int j = from + (int)threadIdx.x * N; j < to; j += STEP) {
+            uint32_t x[4];
+            load(j, x);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (j + e < to) f(Logits<TYPE>::at(x, e), j + e);
         }
     }
     // the largest logit of this thread's and the first place of it: order << 32 | ~index
     __device__ uint64_t largest() const {
         float top = -INFINITY;
         int at = -1;
-        each([&](float l, int j) {
-            if (l > top) {
-                top = l;
+        pieces([&](const uint32_t (&x)[4], int j) {
+            float m = Logits<TYPE>::at(x, 0);
+#pragma unroll
+            for (int e = 1; e < N; ++e) m = fmaxf(m, Logits<TYPE>::at(x, e));
+            if (m > top) {
+                top = m;
                 at = j;
             }
         });
-        return at < 0 ? 0 : (uint64_t)order_of(top) << 32 | ~(uint32_t)at;
+        if (at < 0) return 0;
+        while (!(one(at) == top)) ++at;
+        return (uint64_t)order_of(top) << 32 | ~(uint32_t)at;
     }
 };
 
@@ -432,118 +475,95 @@ __device__ inline Found find_token(Shared& s, const Row& row, const Bound& b, in
     return f;
 }
 
-// The token that passes `b` among those of bin `bin`, c and m before it, `in` of them.
+// A row's bounds one after the other: the bin that each is in, and the token among those of the bin, which are cut further
+// by value and then by index while they are more than the list holds.
 template <class R>
-__device__ inline Found find_in_bin(Shared& s, const R& r, const Row& row, const Bound& b, int bin, uint32_t c, uint64_t m,
-                                    uint32_t in) {
+__device__ inline void sample_row(Shared& s, const SampleArgs& a, const R& r, const Row& row, int b) {
     const int tid = threadIdx.x;
-    uint64_t lo = 0, hi = ~0ull;
-    auto each = [&](auto f) {
-        r.each([&](float l, int j) {
-            if (order_of(l) <= kMinusInf || row.bin(l) != bin) return;
-            const uint64_t x = token_of(l, j);
-            if (x >= lo && x <= hi) f(x, l);
-        });
-    };
-    if (in > kList) {                                  // uniform: cut further, by value and then by index
-        if (tid == 0) {
-            s.lo = ~0ull;
-            s.hi = 0;
+    uint32_t c_all = 0;
+    uint64_t m_all = 0, S = 0;
+    bool filled = false;
+#pragma unroll 1
+    for (int step = 0;; ++step) {                      // top_k, top_p, the draw
+        if (!filled)
+            fill_bins(s, c_all, m_all, [&] {
+                r.each([&](float l, int) {
+                    if (order_of(l) <= kMinusInf) return;
+                    const double y = row.any_place(l);
+                    if (!(y <= row.limit)) return;
+                    const int i = whole_of(y);
+                    atomicAdd(&s.count[i], 1u);
+                    atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)part_of(rest_of(y)));
+                });
+            }, [&](uint64_t parts, int i) { return parts == 0 ? 0 : in_bin(parts, i, row.octave[i & (kPerOctave - 1)]); });
+        filled = true;
+        if (step == 0) S = m_all;
+        if (step == 0 ? row.k <= 0 || (uint32_t)row.k >= c_all : step == 1 && !(row.p < 1.f)) continue;
+        const Bound bound = step == 0   ? Bound{Bound::kRank, (uint32_t)row.k, 0.0}
+                            : step == 1 ? Bound{Bound::kReaches, 0, (double)row.p * (double)S}
+                                        : Bound{Bound::kPasses, 0, row.u() * (double)S};
+        uint32_t c = 0, in;
+        uint64_t m = 0, lo = 0, hi = ~0ull;
+        const int bin = find_bin(s, bound, c, m, in);
+        auto each = [&](auto f) {
+            r.each([&](float l, int j) {
+                if (order_of(l) <= kMinusInf || row.bin(l) != bin) return;
+                const uint64_t x = token_of(l, j);
+                if (x >= lo && x <= hi) f(x, l);
+            });
+        };
+        if (in > kList) {                              // uniform
+            filled = false;
+            if (tid == 0) {
+                s.lo = ~0ull;
+                s.hi = 0;
+            }
+            __syncthreads();
+            uint64_t x0 = ~0ull, x1 = 0;
+            each([&](uint64_t x, float) {
+                x0 = min(x0, x);
+                x1 = max(x1, x);
+            });
+            atomicMin((unsigned long long*)&s.lo, (unsigned long long)x0);
+            atomicMax((unsigned long long*)&s.hi, (unsigned long long)x1);
+            __syncthreads();
+            lo = s.lo;
+            hi = s.hi;
         }
-        __syncthreads();
-        uint64_t a = ~0ull, z = 0;
-        each([&](uint64_t x, float) {
-            a = min(a, x);
-            z = max(z, x);
-        });
-        atomicMin((unsigned long long*)&s.lo, (unsigned long long)a);
-        atomicMax((unsigned long long*)&s.hi, (unsigned long long)z);
-        __syncthreads();
-        lo = s.lo;
-        hi = s.hi;
+#pragma unroll 1
         while (in > kList) {                           // each turn narrows hi - lo 1,024 times at least
             const uint64_t span = hi - lo;
             const int shift = span < (uint64_t)kBins ? 0 : 53 - __builtin_clzll(span);
-            uint32_t c_all;
-            uint64_t m_all;
-            fill_bins(s, c_all, m_all, [&] {
+            uint32_t c_in;
+            uint64_t m_in;
+            fill_bins(s, c_in, m_in, [&] {
                 each([&](uint64_t x, float l) {
                     const int i = (int)((x - lo) >> shift);
                     atomicAdd(&s.count[i], 1u);
                     atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)row.weight(l));
                 });
             }, [](uint64_t mass, int) { return mass; });
-            const int i = find_bin(s, b, c, m, in);
+            const int i = find_bin(s, bound, c, m, in);
             lo += (uint64_t)i << shift;
             hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
         }
-    }
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    each([&](uint64_t x, float) {
-        const uint32_t at = atomicAdd(&s.n, 1u);
-        if (at < (uint32_t)kList) s.list[at] = x;
-    });
-    __syncthreads();
-    const int n = min((int)s.n, kList);
-    sort_list(s, n);
-    return find_token(s, row, b, n, c, m);
-}
-
-template <class R>
-__device__ __attribute__((noinline)) void sample_row(Shared& s, const SampleArgs& a, const R& r, const Row& row, int b) {
-    const int tid = threadIdx.x;
-    uint32_t c_all;
-    uint64_t m_all;
-    auto fill = [&] {
-        fill_bins(s, c_all, m_all, [&] {
-            r.each([&](float l, int) {
-                if (order_of(l) <= kMinusInf) return;
-                const double y = row.any_place(l);
-                if (!(y <= row.limit)) return;
-                const int i = (int)y;
-                atomicAdd(&s.count[i], 1u);
-                atomicAdd((unsigned long long*)&s.mass[i], (unsigned long long)part_of(y - (double)i));
-            });
-        }, [&](uint64_t parts, int i) { return parts == 0 ? 0 : in_bin(parts, i, row.octave[i & (kPerOctave - 1)]); });
-    };
-    fill();
-    bool listed = false, filled = true;
-    int n = 0;
-    if (row.few) {                                     // uniform
-        const Bound rank{Bound::kRank, min((uint32_t)row.k, c_all), 0.0};
-        uint32_t c = 0, in;
-        uint64_t none = 0;
-        const int last = find_bin(s, rank, c, none, in);
-        listed = c + in <= (uint32_t)kList;
         __syncthreads();
-        if (listed) {
-            if (tid == 0) s.n = 0;
-            __syncthreads();
-            r.each([&](float l, int j) {
-                if (order_of(l) <= kMinusInf || row.bin(l) > last) return;
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < (uint32_t)kList) s.list[at] = token_of(l, j);
-            });
-            __syncthreads();
-            n = min((int)s.n, kList);
-            sort_list(s, n);
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        each([&](uint64_t x, float) {
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            if (at < (uint32_t)kList) s.list[at] = x;
+        });
+        __syncthreads();
+        const int n = min((int)s.n, kList);
+        sort_list(s, n);
+        const Found f = find_token(s, row, bound, n, c, m);
+        if (step == 2) {
+            take(a, b, row, f.token, S);
+            return;
         }
+        S = f.mass;
     }
-    auto find = [&](const Bound& bound) {
-        if (listed) return find_token(s, row, bound, n, 0, 0);
-        uint32_t c = 0, in;
-        uint64_t mass = 0;
-        if (!filled) fill();
-        const int bin = find_bin(s, bound, c, mass, in);
-        filled = in <= (uint32_t)kList;                // cut further, the bins are overwritten
-        return find_in_bin(s, r, row, bound, bin, c, mass, in);
-    };
-    uint64_t S = m_all;
-    if (row.k > 0 && (listed || (uint32_t)row.k < c_all)) S = find(Bound{Bound::kRank, (uint32_t)row.k, 0.0}).mass;
-    if (row.p < 1.f) S = find(Bound{Bound::kReaches, 0, (double)row.p * (double)S}).mass;
-    take(a, b, row, find(Bound{Bound::kPasses, 0, row.u() * (double)S}).token, S);
 }
 
 // One launch, a workgroup a row: short rows.
@@ -607,19 +627,33 @@ __global__ void __launch_bounds__(kPiece) sample_bins_kernel(SampleArgs a) {
     __syncthreads();
     if (row.greedy || row.odd) return;                 // uniform
     const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
+    // (a piece's logits side by side, without a branch before the last step)
+    constexpr int N = Logits<TYPE>::N;
     if (row.few) {                                     // uniform
-        r.each([&](float l, int) {
-            const double y = row.place(l);
-            if (y <= row.limit) atomicAdd(&count[(int)y], 1u);
+        r.pieces([&](const uint32_t (&x)[4], int) {
+            double y[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[e] = row.place(Logits<TYPE>::at(x, e));
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (y[e] <= row.limit) atomicAdd(&count[whole_of(y[e])], 1u);
         });
     } else {
         const bool counts = row.k > 0;
-        r.each([&](float l, int) {
-            const double y = row.place(l);
-            if (!(y <= row.limit)) return;
-            const int i = (int)y;
-            atomicAdd((unsigned long long*)&mass[i], (unsigned long long)part_of(__builtin_amdgcn_fract(y)));
-            if (counts) atomicAdd(&count[i], 1u);
+        r.pieces([&](const uint32_t (&x)[4], int) {
+            double y[N];
+            uint64_t part[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[e] = row.place(Logits<TYPE>::at(x, e));
+#pragma unroll
+            for (int e = 0; e < N; ++e) part[e] = part_of(rest_of(y[e]));
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (y[e] <= row.limit) atomicAdd((unsigned long long*)&mass[whole_of(y[e])], (unsigned long long)part[e]);
+            if (counts)                                // uniform
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (y[e] <= row.limit) atomicAdd(&count[whole_of(y[e])], 1u);
         });
     }
     __syncthreads();
@@ -656,12 +690,31 @@ struct Ranges {
     }
 };
 
+// Logits among which are all that the ranges hold (found in fp32, with 2^-20 of the row's reach and of the largest logit to
+// spare), and few others.
+struct Near {
+    float low[3], high[3];
+    __device__ __attribute__((always_inline)) Near(const Row& row, const Ranges& ranges) {
+        const float wide = (float)(1.0 / row.per_bin), spare = 0x1p-20f * (fabsf(row.top32) + (float)kReach * wide);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const Range& q = ranges.r[i];
+            const bool none = q.last < q.first;
+            low[i] = none ? INFINITY : row.top32 - (float)(q.last + 1) * wide - spare;
+            high[i] = none ? -INFINITY : row.top32 - (float)q.first * wide + spare;
+        }
+    }
+    __device__ bool hold(float l) const {
+        return (l >= low[0] && l <= high[0]) | (l >= low[1] && l <= high[1]) | (l >= low[2] && l <= high[2]);
+    }
+};
+
 // A row's bins as loaded, E neighbouring ones a thread of kBins / E.
 template <int E>
 struct Bins {
     uint64_t m[E];
     uint32_t c[E];
-    __device__ Bins(const SampleArgs& a, const Settings& set, int b) {
+    __device__ void read(const SampleArgs& a, const Settings& set, int b) {
         const bool masses = !set.few(), counts = set.k > 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -774,17 +827,29 @@ __global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
     const int b = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), from = piece * a.per;
     const Settings set(a, b);
     if (threadIdx.x < kPerOctave) octave[threadIdx.x] = kOctave[threadIdx.x];
-    const Bins<kBins / kPiece> bins(a, set, b);
+    Bins<kBins / kPiece> bins;
+    bins.read(a, set, b);
     const Row row(set, row_largest<kPiece / 64>(a, b, s), octave);
     if (threadIdx.x == 0) n = 0;
+    if (row.odd && piece == 0 && threadIdx.x == 0) a.n[b] = kList + 1;
     if (row.greedy || row.odd) return;                 // uniform
     const Ranges ranges = find_ranges<kPiece>(row, bins, mass, count, at, sc, sm);
     const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
-    r.each([&](float l, int j) {
-        const double y = row.place(l);
-        if (!(y <= row.limit) || !ranges.hold((int)y)) return;
-        const uint32_t i = atomicAdd(&n, 1u);
-        if (i < (uint32_t)kLocal) list[i] = token_of(l, j);
+    const Near near(row, ranges);
+    constexpr int N = Logits<TYPE>::N;
+    r.pieces([&](const uint32_t (&x)[4], int j) {
+        uint32_t found = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) found |= (uint32_t)near.hold(Logits<TYPE>::at(x, e)) << e;
+        while (found != 0) {
+            const int at = j + __builtin_ctz(found);
+            found &= found - 1;
+            const float l = r.one(at);
+            const double y = row.place(l);
+            if (!(y <= row.limit) || !ranges.hold(whole_of(y))) continue;
+            const uint32_t i = atomicAdd(&n, 1u);
+            if (i < (uint32_t)kLocal) list[i] = token_of(l, at);
+        }
     });
     __syncthreads();
     if (n == 0) return;                                // uniform
@@ -794,27 +859,10 @@ __global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
         if (base + i < (uint32_t)kList) a.list[(int64_t)b * kList + base + i] = list[i];
 }
 
-// The collected tokens sorted, and the row's bounds found among them one after the other.
-template <int TYPE>
-__global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
-    __shared__ Shared s;
+// The n collected tokens of s.list sorted, and the row's bounds found among them one after the other.
+__device__ inline void take_bounds(Shared& s, const SampleArgs& a, const Row& row, const Ranges& ranges, int n, int b) {
     constexpr int E = kList / kThreads;
-    const int b = blockIdx.x, tid = threadIdx.x;
-    const Settings set(a, b);
-    const uint32_t n_all = a.n[b];
-    if (tid < kPerOctave) s.octave[tid] = kOctave[tid];
-    const Bins<kBins / kThreads> bins(a, set, b);
-    const uint64_t best = row_largest<16>(a, b, s.wave_mass);
-    const Row row(set, best, s.octave);
-    __syncthreads();
-    if (row.greedy) return take_largest(a, b, row, best);   // uniform
-    if (row.odd || n_all > (uint32_t)kList) {          // uniform: more equal or near ones than the list holds
-        sample_row(s, a, MemoryRow<TYPE, kThreads>(a, b, 0, a.V), row, b);
-        return;
-    }
-    const int n = (int)n_all;
-    for (int i = tid; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
-    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
+    const int tid = threadIdx.x;
     sort_list(s, n);
     // each token's running count and sum over the row
     uint64_t w[E], F[E], m = 0;
@@ -863,6 +911,29 @@ __global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
     take(a, b, row, s.list[s.found], S);
 }
 
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
+    __shared__ Shared s;
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const Settings set(a, b);
+    const uint32_t n_all = a.n[b];
+    if (tid < kPerOctave) s.octave[tid] = kOctave[tid];
+    Bins<kBins / kThreads> bins;
+    bins.read(a, set, b);
+    const uint64_t best = row_largest<16>(a, b, s.wave_mass);
+    const Row row(set, best, s.octave);
+    __syncthreads();
+    if (row.greedy) return take_largest(a, b, row, best);   // uniform
+    if (n_all > (uint32_t)kList) {                     // uniform: an infinite largest logit, or more near ones than the list holds
+        sample_row(s, a, MemoryRow<TYPE, kThreads>(a, b, 0, a.V), row, b);
+        return;
+    }
+    const int n = (int)n_all;
+    for (int i = tid; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
+    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
+    take_bounds(s, a, row, ranges, n, b);
+}
+
 hipError_t fetch_errors_sample(uint32_t* out, int first, int clear, hipStream_t stream) {
     return fetch_file_errors(out, first, clear, stream);
 }
@@ -881,9 +952,12 @@ struct SamplePlan {
 static SamplePlan plan_sample(int64_t B, int64_t V) {
     SamplePlan p{};
     if (V <= kShort || B == 0) return p;
-    // pieces of whole 2,048 logits, of 4,096 at least, about 1,024 workgroups in all
+    // pieces of whole 2,048 logits, about 1,024 workgroups in all (256 x 152064, 512 / 1,024 / 2,048: 112 / 99 / 102 us; 128
+    // mixed rows 68 / 59 / 62), of 4,096 logits at least (61 x 50257, 2,048 / 4,096: 44.8 / 43.2 us), but not so few that CUs
+    // stay idle (1 x 128256: 24.7 / 27.9)
+    const int64_t least = B * (V / 4096) < 256 ? 2048 : 4096;
     int64_t pieces = (1024 + B - 1) / B;
-    if (pieces > V / 4096) pieces = V / 4096;
+    if (pieces > V / least) pieces = V / least;
     p.per = (int)(((V + pieces - 1) / pieces + 2047) / 2048 * 2048);
     p.pieces = (int)((V + p.per - 1) / p.per);
     p.mass = B * p.pieces * 8;
