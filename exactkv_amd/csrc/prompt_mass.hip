@@ -103,7 +103,7 @@ struct Stage {
 };
 
 template <int D>
-__global__ void __launch_bounds__(64 * kWaves) mass_rows_kernel(PromptMassArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) mass_rows_kernel(PromptMassArgs a) {
     typedef Stage<D> St;
     constexpr int KS = St::KS, SR = St::SR, SB = St::SB;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * St::BYTES];
@@ -145,8 +145,11 @@ __global__ void __launch_bounds__(64 * kWaves) mass_rows_kernel(PromptMassArgs a
     St::offsets(w, lane, a.sk_t, off);
     const int rd = St::read_at(col, half);
     float m[2], l[2];
+    // A unit is 32 keys of a stage and the wavefront's 64 rows. The next unit's products go among this one's exponentials,
+    // a k-step each (which take 768 cycles a unit at head dim 128, the products 512): a wavefront alone keeps both busy.
     auto walk = [&](auto safe) {
         constexpr bool SAFE = decltype(safe)::value;
+        constexpr int AHEAD = 2;                       // k-steps of keys read ahead
         m[0] = m[1] = kLowest;
         l[0] = l[1] = 0.f;
         if (first > last) return;
@@ -155,54 +158,104 @@ __global__ void __launch_bounds__(64 * kWaves) mass_rows_kernel(PromptMassArgs a
             each<St::LOADS>([&](auto i) { load_piece<i.value>(keys.buf, off[i.value], lds0 + st * St::BYTES); });
             keys.next();
         };
+        auto products = [&](int st, int kb, f32x16 (&sc)[2], auto between) {
+            bf16x8 kf[KS];
+            each<AHEAD>([&](auto s) { kf[s.value] = St::piece(lds, st, rd, kb, s.value); });
+            each<KS>([&](auto step) {
+                constexpr int s = decltype(step)::value;
+                if constexpr (s + AHEAD < KS) kf[s + AHEAD] = St::piece(lds, st, rd, kb, s + AHEAD);
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    if constexpr (s == 0)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[rb][i] = 0.f;
+                    sc[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qf[rb][s], sc[rb], 0, 0, 0);
+                }
+                between(step);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        // the maximum that a row's weights are relative to: of its first unit with a visible key (SAFE: so far)
+        auto raise = [&](const f32x16 (&sc)[2]) {
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+                if (SAFE || __ballot(m[rb] == kLowest) != 0) {
+                    float mx = sc[rb][0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[rb][i]);
+                    mx = fmaxf(mx * a.qk_scale, kLowest);
+                    if (SAFE ? mx > m[rb] : m[rb] == kLowest) {
+                        l[rb] *= exp2_fast(m[rb] - mx);
+                        m[rb] = mx;
+                    }
+                }
+        };
+        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        auto weigh = [&](const f32x16 (&sc)[2], int e) {
+            sum[e >> 4][e & 1] += exp2_fast(fmaf(sc[e >> 4][e & 15], a.qk_scale, -m[e >> 4]));
+        };
+        // this unit's weights, of keys j0 on, and the next one's scores
+        auto step = [&](int j0, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int kb) {
+            const bool all = j0 + 31 <= w_lo && (a.window == 0 || j0 > w_hi - a.window);
+            if (all && more && !SAFE) {                // uniform
+                raise(cur);
+                products(st, kb, nxt, [&](auto s) {
+#pragma unroll
+                    for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) weigh(cur, e);
+                });
+            } else {
+                if (more) products(st, kb, nxt, [](auto) {});
+                if (j0 <= w_hi && (a.window == 0 || j0 + 31 > w_lo - a.window)) {   // uniform: some key is seen
+                    if (!all)
+#pragma unroll
+                        for (int rb = 0; rb < 2; ++rb) {
+                            const int rel = pos[rb] - j0 - 4 * half;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if ((uint32_t)(rel - (8 * (i >> 2) + (i & 3))) >= span) cur[rb][i] = -INFINITY;
+                        }
+                    raise(cur);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) weigh(cur, e);
+                }
+            }
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                l[rb] += sum[rb][0] + sum[rb][1];
+                sum[rb][0] = sum[rb][1] = 0.f;
+            }
+        };
         load(0);
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[rb][s]));
-        for (int it = first; it <= last; ++it) {
-            const int st = (it - first) & 1, j0 = it * SR;
-            next_stage();
-            if (it < last) load(st ^ 1);
-            if (!wave_on || j0 > w_hi || (a.window > 0 && j0 + SR - 1 <= w_lo - a.window)) continue;   // uniform: none seen
-            const bool all = j0 + SR - 1 <= w_lo && (a.window == 0 || j0 > w_hi - a.window);
-#pragma unroll
-            for (int kb = 0; kb < SB; ++kb) {
-                f32x16 sc[2];
-#pragma unroll
-                for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[rb][i] = 0.f;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const bf16x8 kf = St::piece(lds, st, rd, kb, s);
-#pragma unroll
-                    for (int rb = 0; rb < 2; ++rb) sc[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rb][s], sc[rb], 0, 0, 0);
-                }
-#pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    if (!all) {
-                        const int rel = pos[rb] - j0 - 4 * half;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if ((uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) sc[rb][i] = -INFINITY;
-                    }
-                    if (SAFE || __ballot(m[rb] == kLowest) != 0) {
-                        float mx = sc[rb][0];
-#pragma unroll
-                        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[rb][i]);
-                        mx = fmaxf(mx * a.qk_scale, kLowest);
-                        if (SAFE ? mx > m[rb] : m[rb] == kLowest) {
-                            l[rb] *= exp2_fast(m[rb] - mx);
-                            m[rb] = mx;
-                        }
-                    }
-                    float sum[2] = {0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[i & 1] += exp2_fast(fmaf(sc[rb][i], a.qk_scale, -m[rb]));
-                    l[rb] += sum[0] + sum[1];
-                }
+        next_stage();
+        if (first < last) load(1);
+        f32x16 s0[2], s1[2];
+        if (wave_on) products(0, 0, s0, [](auto) {});
+        auto stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+            constexpr int st = decltype(parity)::value;
+            if constexpr (SB == 2)
+                if (wave_on) step(it * SR, cur, nxt, true, st, 1);
+            const bool more = it < last;
+            if (more) next_stage();
+            if (it + 1 < last) load(st);
+            if (wave_on) {
+                if constexpr (SB == 2)
+                    step(it * SR + 32, nxt, cur, more, st ^ 1, 0);
+                else
+                    step(it * SR, cur, nxt, more, st ^ 1, 0);
             }
+        };
+        // (at two units a stage, a stage ends with the scores where they began)
+        for (int it = first; it <= last; it += 2) {
+            stage(it, std::integral_constant<int, 0>{}, s0, s1);
+            if (it == last) break;
+            if constexpr (SB == 2)
+                stage(it + 1, std::integral_constant<int, 1>{}, s0, s1);
+            else
+                stage(it + 1, std::integral_constant<int, 1>{}, s1, s0);
         }
     };
     if (threadIdx.x == 0) s_again = 0;
@@ -240,7 +293,7 @@ __global__ void __launch_bounds__(256) mass_rows_join_kernel(PromptMassArgs a) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(64 * kWaves) mass_columns_kernel(PromptMassArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) mass_columns_kernel(PromptMassArgs a) {
     typedef Stage<D> St;
     constexpr int KS = St::KS, SR = St::SR, SB = St::SB;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * St::BYTES];
@@ -280,7 +333,7 @@ __global__ void __launch_bounds__(64 * kWaves) mass_columns_kernel(PromptMassArg
     rows.k0 = tile.q0;
     rows.Lk = tile.Lq;
     int g = tiles > 0 ? (int)(begin / tiles) : 0, t = tiles > 0 ? (int)(begin % tiles) : 0;
-    float next_lse[SB];
+    float lse[SB], next_lse[SB];
     int gl = g, tl = t;                                // of the loads
     auto load = [&](int st) {
         Stream<D, SR> s(a.q, a.sq_t, (hk * G + gl) * a.sq_h, rows, (first + tl) * SR);
@@ -295,46 +348,91 @@ __global__ void __launch_bounds__(64 * kWaves) mass_columns_kernel(PromptMassArg
             ++gl;
         }
     };
-    if (begin < end) load(0);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(kf[kb][s]));
-    for (int64_t step = begin; step < end; ++step) {
-        const int st = (int)(step - begin) & 1, t0 = (first + t) * SR;
-        next_stage();
-        float lse[SB];
-#pragma unroll
-        for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
-        if (step + 1 < end) load(st ^ 1);
-        if (++t == tiles) t = 0;
-        const int p_lo = t0 + shift, p_hi = p_lo + SR - 1;
-        if (!wave_on || p_hi < wkey0 || (a.window > 0 && p_lo - (wkey0 + 63) >= a.window)) continue;   // uniform: none sees
-        const bool all = p_lo >= wkey0 + 63 && (a.window == 0 || p_hi - wkey0 < a.window);
-#pragma unroll
-        for (int rb = 0; rb < SB; ++rb) {
-            f32x16 sc[2];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const bf16x8 qf = St::piece(lds, st, rd, rb, s);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][s], qf, sc[kb], 0, 0, 0);
-            }
+    // A unit is 32 tokens of a stage and the wavefront's 64 keys, walked as the other pass walks its units.
+    constexpr int AHEAD = 2;
+    auto products = [&](int st, int rb, f32x16 (&sc)[2], auto between) {
+        bf16x8 qf[KS];
+        each<AHEAD>([&](auto s) { qf[s.value] = St::piece(lds, st, rd, rb, s.value); });
+        each<KS>([&](auto step) {
+            constexpr int s = decltype(step)::value;
+            if constexpr (s + AHEAD < KS) qf[s + AHEAD] = St::piece(lds, st, rd, rb, s + AHEAD);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const int rel = p_lo + 32 * rb + col - wkey0 - 4 * half;
+                if constexpr (s == 0)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = exp2_fast(fmaf(sc[kb][i], a.qk_scale, -lse[rb]));
-                    // (after the exponential: a row's sum may be NaN)
-                    if (!all && (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) x = 0.f;
-                    acc[kb][i] += x;
-                }
+                    for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+                sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][s], qf[s], sc[kb], 0, 0, 0);
             }
+            between(step);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // this unit's weights, of tokens standing at p0 on, and the next one's scores
+    auto step = [&](int p0, float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
+        const bool all = p0 >= wkey0 + 63 && (a.window == 0 || p0 + 31 - wkey0 < a.window);
+        if (all && more) {                             // uniform
+            products(st, rb, nxt, [&](auto s) {
+#pragma unroll
+                for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e)
+                    acc[e >> 4][e & 15] += exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row_lse));
+            });
+            return;
+        }
+        if (more) products(st, rb, nxt, [](auto) {});
+        if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int rel = p0 + col - wkey0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float x = exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row_lse));
+                // (after the exponential: a row's sum may be NaN)
+                if (!all && (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) x = 0.f;
+                acc[kb][i] += x;
+            }
+        }
+    };
+    const int count = (int)(end - begin);
+    if (count > 0) {
+        load(0);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(kf[kb][s]));
+        next_stage();
+#pragma unroll
+        for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
+        if (count > 1) load(1);
+        f32x16 s0[2], s1[2];
+        if (wave_on) products(0, 0, s0, [](auto) {});
+        auto stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+            constexpr int st = decltype(parity)::value;
+            const int p0 = (first + t) * SR + shift;
+            if (++t == tiles) t = 0;
+            if constexpr (SB == 2)
+                if (wave_on) step(p0, lse[0], cur, nxt, true, st, 1);
+            const bool more = it + 1 < count;
+            const float last_lse = lse[SB - 1];
+            if (more) {
+                next_stage();
+#pragma unroll
+                for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
+            }
+            if (it + 2 < count) load(st);
+            if (wave_on) {
+                if constexpr (SB == 2)
+                    step(p0 + 32, last_lse, nxt, cur, more, st ^ 1, 0);
+                else
+                    step(p0, last_lse, cur, nxt, more, st ^ 1, 0);
+            }
+        };
+        for (int it = 0; it < count; it += 2) {
+            stage(it, std::integral_constant<int, 0>{}, s0, s1);
+            if (it + 1 == count) break;
+            if constexpr (SB == 2)
+                stage(it + 1, std::integral_constant<int, 1>{}, s0, s1);
+            else
+                stage(it + 1, std::integral_constant<int, 1>{}, s1, s0);
         }
     }
     if (!wave_on) return;
