@@ -191,71 +191,108 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                 }
         };
         float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        // (weights are made here, not sunk to the sums' use)
+        auto here = [](float (&x)[2]) { asm volatile("" : "+v"(x[0]), "+v"(x[1])); };
         auto weigh = [&](const f32x16 (&sc)[2], int e) {
             sum[e >> 4][e & 1] += exp2_fast(fmaf(sc[e >> 4][e & 15], a.qk_scale, -m[e >> 4]));
         };
-        // this unit's weights, of keys j0 on, and the next one's scores
-        auto step = [&](int j0, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int kb) {
-            const bool all = j0 + 31 <= w_lo && (a.window == 0 || j0 > w_hi - a.window);
-            if (all && more && !SAFE) {                // uniform
-                raise(cur);
-                products(st, kb, nxt, [&](auto s) {
-#pragma unroll
-                    for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) weigh(cur, e);
-                });
-            } else {
-                if (more) products(st, kb, nxt, [](auto) {});
-                if (j0 <= w_hi && (a.window == 0 || j0 + 31 > w_lo - a.window)) {   // uniform: some key is seen
-                    if (!all)
-#pragma unroll
-                        for (int rb = 0; rb < 2; ++rb) {
-                            const int rel = pos[rb] - j0 - 4 * half;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if ((uint32_t)(rel - (8 * (i >> 2) + (i & 3))) >= span) cur[rb][i] = -INFINITY;
-                        }
-                    raise(cur);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) weigh(cur, e);
-                }
-            }
+        auto settle = [&] {
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
                 l[rb] += sum[rb][0] + sum[rb][1];
                 sum[rb][0] = sum[rb][1] = 0.f;
             }
         };
+        // this unit's weights, of keys j0 on, and the next one's scores: where every row sees all of them, and otherwise
+        auto full_step = [&](f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int kb) {
+            products(st, kb, nxt, [&](auto s) {
+#pragma unroll
+                for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) weigh(cur, e);
+                here(sum[s.value * 2 / KS]);
+            });
+        };
+        auto part_step = [&](int j0, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int kb) {
+            if (more) products(st, kb, nxt, [](auto) {});
+            if (j0 > w_hi || (a.window > 0 && j0 + 31 <= w_lo - a.window)) return;   // uniform: none seen
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                const int rel = pos[rb] - j0 - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if ((uint32_t)(rel - (8 * (i >> 2) + (i & 3))) >= span) cur[rb][i] = -INFINITY;
+            }
+            raise(cur);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) weigh(cur, e);
+            settle();
+        };
         load(0);
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[rb][s]));
+        f32x16 s0[2], s1[2];
+        if constexpr (SAFE) {                          // seldom: unit by unit
+            for (int it = first; it <= last; ++it) {
+                next_stage();
+                if (it < last) load((it - first + 1) & 1);
+                if (!wave_on) continue;
+#pragma unroll 1
+                for (int kb = 0; kb < SB; ++kb) {
+                    products((it - first) & 1, kb, s0, [](auto) {});
+                    part_step(it * SR + 32 * kb, s0, s1, false, 0, 0);
+                }
+            }
+            return;
+        }
         next_stage();
         if (first < last) load(1);
-        f32x16 s0[2], s1[2];
         if (wave_on) products(0, 0, s0, [](auto) {});
-        auto stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+        auto part_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
             constexpr int st = decltype(parity)::value;
             if constexpr (SB == 2)
-                if (wave_on) step(it * SR, cur, nxt, true, st, 1);
+                if (wave_on) part_step(it * SR, cur, nxt, true, st, 1);
             const bool more = it < last;
             if (more) next_stage();
             if (it + 1 < last) load(st);
             if (wave_on) {
                 if constexpr (SB == 2)
-                    step(it * SR + 32, nxt, cur, more, st ^ 1, 0);
+                    part_step(it * SR + 32, nxt, cur, more, st ^ 1, 0);
                 else
-                    step(it * SR, cur, nxt, more, st ^ 1, 0);
+                    part_step(it * SR, cur, nxt, more, st ^ 1, 0);
             }
         };
-        // (at two units a stage, a stage ends with the scores where they began)
+        auto full_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+            constexpr int st = decltype(parity)::value;
+            if constexpr (SB == 2) full_step(cur, nxt, st, 1);
+            next_stage();
+            if (it + 1 < last) load(st);
+            if constexpr (SB == 2)
+                full_step(nxt, cur, st ^ 1, 0);
+            else
+                full_step(cur, nxt, st ^ 1, 0);
+            settle();
+        };
+        constexpr std::integral_constant<int, 0> even{};
+        constexpr std::integral_constant<int, 1> odd{};
+        // (at two units a stage, a stage ends with the scores where they began; two stages a turn, and the full ones in a loop
+        // of their own, so that registers need no copies)
         for (int it = first; it <= last; it += 2) {
-            stage(it, std::integral_constant<int, 0>{}, s0, s1);
+            const bool set = __ballot(m[0] == kLowest || m[1] == kLowest) == 0;
+            while (set && wave_on && it + 1 < last && (it + 2) * SR - 1 <= w_lo && (a.window == 0 || it * SR > w_hi - a.window)) {
+                full_stage(it, even, s0, s1);
+                if constexpr (SB == 2)
+                    full_stage(it + 1, odd, s0, s1);
+                else
+                    full_stage(it + 1, odd, s1, s0);
+                it += 2;
+            }
+            part_stage(it, even, s0, s1);
             if (it == last) break;
             if constexpr (SB == 2)
-                stage(it + 1, std::integral_constant<int, 1>{}, s0, s1);
+                part_stage(it + 1, odd, s0, s1);
             else
-                stage(it + 1, std::integral_constant<int, 1>{}, s1, s0);
+                part_stage(it + 1, odd, s1, s0);
         }
     };
     if (threadIdx.x == 0) s_again = 0;
@@ -367,17 +404,20 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    // this unit's weights, of tokens standing at p0 on, and the next one's scores
-    auto step = [&](int p0, float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
-        const bool all = p0 >= wkey0 + 63 && (a.window == 0 || p0 + 31 - wkey0 < a.window);
-        if (all && more) {                             // uniform
-            products(st, rb, nxt, [&](auto s) {
+    auto here = [](float x) {                          // made here, not sunk to its use
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    // this unit's weights, of tokens standing at p0 on, and the next one's scores: where all of them see every key, and otherwise
+    auto full_step = [&](float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int rb) {
+        products(st, rb, nxt, [&](auto s) {
 #pragma unroll
-                for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e)
-                    acc[e >> 4][e & 15] += exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row_lse));
-            });
-            return;
-        }
+            for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) {
+                acc[e >> 4][e & 15] = here(acc[e >> 4][e & 15] + exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row_lse)));
+            }
+        });
+    };
+    auto part_step = [&](int p0, float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
         if (more) products(st, rb, nxt, [](auto) {});
         if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
 #pragma unroll
@@ -385,10 +425,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             const int rel = p0 + col - wkey0 - 4 * half;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float x = exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row_lse));
+                const float x = exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row_lse));
                 // (after the exponential: a row's sum may be NaN)
-                if (!all && (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) >= span) x = 0.f;
-                acc[kb][i] += x;
+                acc[kb][i] += (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) < span ? x : 0.f;
             }
         }
     };
@@ -405,12 +444,14 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         if (count > 1) load(1);
         f32x16 s0[2], s1[2];
         if (wave_on) products(0, 0, s0, [](auto) {});
-        auto stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+        auto advance = [&] {
+            if (++t == tiles) t = 0;
+        };
+        auto part_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
             constexpr int st = decltype(parity)::value;
             const int p0 = (first + t) * SR + shift;
-            if (++t == tiles) t = 0;
             if constexpr (SB == 2)
-                if (wave_on) step(p0, lse[0], cur, nxt, true, st, 1);
+                if (wave_on) part_step(p0, lse[0], cur, nxt, true, st, 1);
             const bool more = it + 1 < count;
             const float last_lse = lse[SB - 1];
             if (more) {
@@ -421,18 +462,48 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             if (it + 2 < count) load(st);
             if (wave_on) {
                 if constexpr (SB == 2)
-                    step(p0 + 32, last_lse, nxt, cur, more, st ^ 1, 0);
+                    part_step(p0 + 32, last_lse, nxt, cur, more, st ^ 1, 0);
                 else
-                    step(p0, last_lse, cur, nxt, more, st ^ 1, 0);
+                    part_step(p0, last_lse, cur, nxt, more, st ^ 1, 0);
             }
+            advance();
         };
+        auto full_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+            constexpr int st = decltype(parity)::value;
+            if constexpr (SB == 2) full_step(lse[0], cur, nxt, st, 1);
+            const float last_lse = lse[SB - 1];
+            next_stage();
+#pragma unroll
+            for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
+            if (it + 2 < count) load(st);
+            if constexpr (SB == 2)
+                full_step(last_lse, nxt, cur, st ^ 1, 0);
+            else
+                full_step(last_lse, cur, nxt, st ^ 1, 0);
+            advance();
+        };
+        // whether all of the tile of tokens `at` see every key of the wavefront
+        auto full = [&](int at) {
+            const int p0 = (first + at) * SR + shift;
+            return p0 >= wkey0 + 63 && (a.window == 0 || p0 + SR - 1 - wkey0 < a.window);
+        };
+        constexpr std::integral_constant<int, 0> even{};
+        constexpr std::integral_constant<int, 1> odd{};
         for (int it = 0; it < count; it += 2) {
-            stage(it, std::integral_constant<int, 0>{}, s0, s1);
+            while (wave_on && it + 2 < count && full(t) && full(t + 1 == tiles ? 0 : t + 1)) {
+                full_stage(it, even, s0, s1);
+                if constexpr (SB == 2)
+                    full_stage(it + 1, odd, s0, s1);
+                else
+                    full_stage(it + 1, odd, s1, s0);
+                it += 2;
+            }
+            part_stage(it, even, s0, s1);
             if (it + 1 == count) break;
             if constexpr (SB == 2)
-                stage(it + 1, std::integral_constant<int, 1>{}, s0, s1);
+                part_stage(it + 1, odd, s0, s1);
             else
-                stage(it + 1, std::integral_constant<int, 1>{}, s1, s0);
+                part_stage(it + 1, odd, s1, s0);
         }
     }
     if (!wave_on) return;
