@@ -31,9 +31,9 @@ struct PromptMassArgs {
     int S, N, NK, Hq, Hkv, G, window, last;
     float qk_scale;                    // log2(e) / sqrt(D)
     int row_parts, col_parts;
-    float2* part;                      // [row_parts, Hq, N]: maximum, sum
+    float2* part;                      // [row tiles, Hkv, row_parts, kTile]: maximum, sum
     float* lse;                        // [Hq, N]: log2 of a row's sum; infinity where it sees no key
-    float* sums;                       // [col_parts, Hkv, NK]
+    float* sums;                       // [col_parts, Hkv, NK]; out where there is one part
     float* out;                        // [Hkv, NK]
 };
 
@@ -110,9 +110,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     __shared__ int s_again;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
-    const int part = rest % a.row_parts;
+    const int part = rest % a.row_parts, index = rest / a.row_parts;
     PromptTile tile;
-    if (!tile_at<true>(a, rest / a.row_parts, tile)) return;
+    if (!tile_at<true>(a, index, tile)) return;
     const int col = lane & 31, half = lane >> 5, G = a.G, nrows = tile.Lq * G, shift = tile.Lk - tile.Lq;
     const int wrow0 = tile.row0 + 64 * w;
     const bool wave_on = wrow0 < nrows;
@@ -307,26 +307,51 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         const float m2 = __shfl_xor(m[rb], 32), l2 = __shfl_xor(l[rb], 32), M = fmaxf(m[rb], m2);
         const float sum = l[rb] * exp2_fast(m[rb] - M) + l2 * exp2_fast(m2 - M);
         if (half != 0 || wrow0 + 32 * rb + col >= nrows) continue;
-        const int64_t at = (int64_t)hq[rb] * a.N + tile.q0 + tok[rb];
         if (a.row_parts > 1)
-            a.part[(int64_t)part * a.Hq * a.N + at] = make_float2(M, sum);
+            a.part[(((int64_t)index * a.Hkv + hk) * a.row_parts + part) * kTile + 64 * w + 32 * rb + col] = make_float2(M, sum);
         else
-            a.lse[at] = sum == 0.f ? INFINITY : M + __builtin_amdgcn_logf(sum);
+            a.lse[(int64_t)hq[rb] * a.N + tile.q0 + tok[rb]] = sum == 0.f ? INFINITY : M + __builtin_amdgcn_logf(sum);
     }
 }
 
-// The parts of every row joined.
-__global__ void __launch_bounds__(256) mass_rows_join_kernel(PromptMassArgs a) {
-    const int64_t n = (int64_t)a.Hq * a.N, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= n) return;
+// The parts of a tile's rows joined: four threads a row, a quarter of the parts each.
+__global__ void __launch_bounds__(4 * kTile) mass_rows_join_kernel(PromptMassArgs a) {
+    __shared__ float2 s[4][kTile];
+    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), index = (int)(blockIdx.x / (unsigned)a.Hkv);
+    const int r = threadIdx.x % kTile, quarter = threadIdx.x / kTile;
+    PromptTile tile;
+    if (!tile_at<true>(a, index, tile)) return;
+    const int row = tile.row0 + r;
     float M = kLowest, l = 0.f;
-    for (int i = 0; i < a.row_parts; ++i) {
-        const float2 x = a.part[i * n + at];
+    const float2* part = a.part + ((int64_t)index * a.Hkv + hk) * a.row_parts * kTile + r;
+    if (row < tile.Lq * a.G)
+#pragma unroll 8
+        for (int i = quarter; i < a.row_parts; i += 4) {
+            const float2 x = part[(int64_t)i * kTile];
+            const float m = fmaxf(M, x.x);
+            l = l * exp2_fast(M - m) + x.y * exp2_fast(x.x - m);
+            M = m;
+        }
+    s[quarter][r] = make_float2(M, l);
+    __syncthreads();
+    if (quarter != 0 || row >= tile.Lq * a.G) return;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        const float2 x = s[i][r];
         const float m = fmaxf(M, x.x);
         l = l * exp2_fast(M - m) + x.y * exp2_fast(x.x - m);
         M = m;
     }
-    a.lse[at] = l == 0.f ? INFINITY : M + __builtin_amdgcn_logf(l);
+    a.lse[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? INFINITY : M + __builtin_amdgcn_logf(l);
+}
+
+// Entries of keys that no sequence holds, from key `end` on: 0, shared by all workgroups.
+template <int THREADS>
+__device__ inline void zero_keys(const PromptMassArgs& a) {
+    const int end = a.S > 0 ? min(max(a.cu_k[a.S], 0), a.NK) : 0;
+    const int64_t n = (int64_t)(a.NK - end) * a.Hkv;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS)
+        a.out[i / (a.NK - end) * a.NK + end + i % (a.NK - end)] = 0.f;
 }
 
 template <int D>
@@ -337,6 +362,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
     const int part = rest % a.col_parts;
+    if (a.col_parts == 1) zero_keys<64 * kWaves>(a);
     PromptTile tile;
     if (!tile_at<false>(a, rest / a.col_parts, tile)) return;
     const int col = lane & 31, half = lane >> 5, G = a.G, shift = tile.Lk - tile.Lq;
@@ -537,6 +563,7 @@ __global__ void __launch_bounds__(256) mass_columns_join_kernel(PromptMassArgs a
     const int end = a.S > 0 ? min(max(a.cu_k[a.S], 0), a.NK) : 0;
     float sum = 0.f;
     if ((int)(at % a.NK) < end)
+#pragma unroll 8
         for (int i = 0; i < a.col_parts; ++i) sum += a.sums[i * n + at];
     a.out[at] = sum;
 }
@@ -561,16 +588,16 @@ static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t 
     const int64_t reach = window > 0 && window + kTile < NK ? window + kTile : NK;
     auto cut = [&](int64_t units, int64_t steps) {
         int64_t parts = units > 0 ? 1024 / units : 1;
-        if (parts > steps / 8) parts = steps / 8;
+        if (parts > steps / 4) parts = steps / 4;
         if (parts > 64) parts = 64;
         return (int)(parts < 1 ? 1 : parts);
     };
     p.row_parts = cut(p.row_tiles * Hkv, (reach + SR - 1) / SR);
     const int64_t most = last > 0 && last < N ? last : N, seen = window > 0 && window + kTile < most ? window + kTile : most;
     p.col_parts = cut(p.col_tiles * Hkv, (seen + SR - 1) / SR * G);
-    p.part_bytes = p.row_parts > 1 ? p.row_parts * Hq * N * 8 : 0;
+    p.part_bytes = p.row_parts > 1 ? p.row_tiles * Hkv * p.row_parts * kTile * 8 : 0;
     p.lse_bytes = (Hq * N * 4 + 15) / 16 * 16;
-    p.sum_bytes = (p.col_parts * Hkv * NK * 4 + 15) / 16 * 16;
+    p.sum_bytes = p.col_parts > 1 ? (p.col_parts * Hkv * NK * 4 + 15) / 16 * 16 : 0;
     return p;
 }
 
@@ -579,7 +606,7 @@ static void launch_prompt_mass(const PromptMassArgs& a, const MassPlan& p, hipSt
     const dim3 block(64 * kWaves);
     hipLaunchKernelGGL((mass_rows_kernel<D>), dim3((unsigned)(p.row_tiles * a.Hkv * a.row_parts)), block, 0, stream, a);
     if (a.row_parts > 1)
-        hipLaunchKernelGGL(mass_rows_join_kernel, dim3((unsigned)(((int64_t)a.Hq * a.N + 255) / 256)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(mass_rows_join_kernel, dim3((unsigned)(p.row_tiles * a.Hkv)), dim3(4 * kTile), 0, stream, a);
     hipLaunchKernelGGL((mass_columns_kernel<D>), dim3((unsigned)(p.col_tiles * a.Hkv * a.col_parts)), block, 0, stream, a);
 }
 
@@ -619,7 +646,7 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
     EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 && (int64_t)N + 2 * (int64_t)NK < INT32_MAX - 1024,
                  "prompt_mass: too many rows (N=%d, NK=%d, %d heads per KV head)", N, NK, (int)G);
     const MassPlan p = plan_mass(S, N, NK, Hq, Hkv, D, window, last);
-    EXKV_REQUIRE(p.row_tiles * p.row_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX &&
+    EXKV_REQUIRE(p.row_tiles * p.row_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX && p.row_tiles * Hkv * 4 * kTile <= (int64_t)UINT32_MAX &&
                      p.col_tiles * p.col_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX &&
                      (int64_t)Hq * N <= (int64_t)UINT32_MAX && (int64_t)Hkv * NK <= (int64_t)UINT32_MAX,
                  "prompt_mass: too many rows (N=%d, NK=%d, %d query heads, %d KV heads, S=%d)", N, NK, Hq, Hkv, S);
@@ -630,7 +657,7 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
         EXKV_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "prompt_mass: workspace of %lld bytes, %lld needed",
                      (long long)ws_bytes, (long long)need);
         a.lse = (float*)ws;
-        a.sums = (float*)((uint8_t*)ws + p.lse_bytes);
+        a.sums = p.col_parts > 1 ? (float*)((uint8_t*)ws + p.lse_bytes) : out;
         a.part = (float2*)((uint8_t*)ws + p.lse_bytes + p.sum_bytes);
         if (D == 64)
             launch_prompt_mass<64>(a, p, stream);
@@ -638,6 +665,7 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
             launch_prompt_mass<128>(a, p, stream);
         else
             launch_prompt_mass<256>(a, p, stream);
+        if (p.col_parts == 1) return hip_status(hipGetLastError(), "prompt_mass");
     } else {
         a.S = 0;                                       // no query: zeros
     }

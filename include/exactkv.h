@@ -586,7 +586,7 @@ int64_t exkv_prompt_mass_workspace(int32_t S, int32_t N, int32_t NK, int32_t Hq,
 
 /* The attention that the keys of packed prompts receive (q, k, offsets and window as in exkv_prompt_attention): for key j of
  * KV head h, the sum of the weights that each sequence's queries, or its last `last` ones (last > 0), give it, over the query
- * heads of h. out: fp32 [Hkv, NK], 0 for keys that no sequence holds. ws as above. Three to five launches.
+ * heads of h. out: fp32 [Hkv, NK], 0 for keys that no sequence holds. ws as above. Two to four launches.
  * No counterpart in the reference. */
 int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h, const int32_t* cu_q,
                      const int32_t* cu_k, int32_t S, int32_t N, int32_t NK, int32_t Hq, int32_t Hkv, int32_t D, int32_t window,
