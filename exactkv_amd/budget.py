@@ -11,15 +11,28 @@ No counterpart in the reference, whose caches keep every token (exactkv/cache.py
 tokens that stay keep their positions wherever they are stored, and each KV head keeps its own. The tensors of a call are
 on one GPU; but for evict, the work goes to that GPU's current stream, waits for nothing and can be captured in a HIP
 graph."""
+import functools
+
 import torch
 
 from . import _lib
 from .cache import BF16KV, CompressedKV
 from .kernels import _QK_SCALE, P, _block_table_arg, _cache_args, _cache_dim, _check_q, _lens_arg, _window_arg
-from .layer import _check_heads, _offsets, _on, _overlap, _rows
+from .layer import _check_heads, _offsets, _on, _rows
 from .paged import PagedBF16KV, PagedCompressedKV
 
 F32 = torch.float32
+
+
+# bytes of the calls' workspaces (16 at least), which the sizes alone determine
+@functools.lru_cache(maxsize=4096)
+def _mass_workspace(*sizes):
+    return max(16, _lib.load().exkv_mass_workspace(*sizes))
+
+
+@functools.lru_cache(maxsize=4096)
+def _prompt_workspace(*sizes):
+    return max(16, _lib.load().exkv_prompt_mass_workspace(*sizes))
 
 
 def _is_bf16(c):
@@ -115,9 +128,12 @@ def attention_mass(q, k_cache, T=None, *, mass=None, lens=None, block_table=None
         pages, TS = held * TS // P, capacity
     T = _tokens(T, TS, lens, "attention_mass")
     lp, lstride = _lens_on(lens, B, dev)
-    window = _window_arg(window)
-    if window > 0x7FFFFFFF:
-        raise ValueError(f"window must be >= 0 (got {window})")
+    if window:
+        window = _window_arg(window)
+        if window > 0x7FFFFFFF:
+            raise ValueError(f"window must be >= 0 (got {window})")
+    else:
+        window = 0
     shape = (B, Hkv, TS)
     mp = None if mass is None else _mass_rows(mass, shape, dev, "mass")
     fresh = out is None
@@ -126,10 +142,10 @@ def attention_mass(q, k_cache, T=None, *, mass=None, lens=None, block_table=None
         op = out.data_ptr()
     else:
         op = _mass_rows(out, shape, dev, "out")
-        if mass is not None and op != mp and _overlap(out, mass):
+        if mass is not None and op != mp and abs(op - mp) < out.numel() * 4:
             raise ValueError("out overlaps mass")
-    need = _lib.load().exkv_mass_workspace(B, Hq, Hkv, T, TS, lens is not None, window)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    need = _mass_workspace(B, Hq, Hkv, T, TS, lens is not None, window)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _lib.call(name, q.data_ptr(), *cache, bt, stride, pages, B, Hq, Hkv, D, T, TS, lp, lstride, window, _QK_SCALE[D], mp, op, fresh,
               ws.data_ptr(), need, _lib.stream(dev))
     return out
@@ -162,8 +178,8 @@ def prompt_mass(q, k, cu_seqlens, *, cu_seqlens_k=None, window=0, last=0):
     if not 0 <= window <= 0x7FFFFFFF or not 0 <= last <= 0x7FFFFFFF:
         raise ValueError(f"window and last must be >= 0 (got {window}, {last})")
     out = torch.empty(Hkv, NK, dtype=F32, device=q.device)
-    need = _lib.load().exkv_prompt_mass_workspace(S, N, NK, Hq, Hkv, D, window, last)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    need = _prompt_workspace(S, N, NK, Hq, Hkv, D, window, last)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _lib.call("exkv_prompt_mass", q.data_ptr(), sq_t, sq_h, k.data_ptr(), sk_t, sk_h, cu, cu_k, S, N, NK, Hq, Hkv, D, window, last,
               _QK_SCALE[D], out.data_ptr(), ws.data_ptr(), need, _lib.stream(dev))
     return out

@@ -80,9 +80,17 @@ __global__ void __launch_bounds__(256) mass_score_kernel(MassArgs a) {
         const uint4 x = real ? ld16(a.q + (b * a.Hq + hq) * D + ch) : make_uint4(0, 0, 0, 0);
         qf[s] = __builtin_bit_cast(bf16x8, x);
     }
+    // the run's pool pages, a lane each, 64 at a time: read one by one, each would hold up its page's loads
+    int pool = 0;
+    auto table = [&](int p) {
+        if (a.table != nullptr) pool = a.table[b * a.table_stride + min(p + lane, last - 1)];
+    };
     auto load = [&](int p, PageIn<D, COMPRESSED>& in) {
         int64_t page = p;
-        if (a.table != nullptr) page = min(max((int64_t)a.table[b * a.table_stride + p], (int64_t)0), a.pool_pages - 1);
+        if (a.table != nullptr) {                      // uniform
+            if (p > first && (p - first) % 64 == 0) table(p);
+            page = min(max((int64_t)__builtin_amdgcn_readlane(pool, (p - first) % 64), (int64_t)0), a.pool_pages - 1);
+        }
         if constexpr (COMPRESSED) {
             if (a.table == nullptr) page += b * (a.TS / kPage);
             const int64_t unit = page * a.Hkv + h;
@@ -96,7 +104,10 @@ __global__ void __launch_bounds__(256) mass_score_kernel(MassArgs a) {
     };
     float m = kLowest, l = 0.f;
     PageIn<D, COMPRESSED> in;
-    if (first < last) load(first, in);
+    if (first < last) {
+        table(first);
+        load(first, in);
+    }
     for (int p = first; p < last; ++p) {
         uint32_t x[Run<D>::V];
         if constexpr (COMPRESSED)
@@ -145,6 +156,19 @@ __global__ void __launch_bounds__(256) mass_join_kernel(MassArgs a, int tiles) {
     const int j = (tile * 256 + (int)threadIdx.x) * 4;
     if (tile * 1024 >= n && a.fresh == 0) return;
     const int64_t head = b * a.Hq + h * a.G;
+    // scores and masses are on their way while the sums are joined
+    constexpr int FIRST = 8;
+    const bool some = j < n && j + 3 >= low;
+    const int64_t at = unit * a.TS;
+    f32x4 score[FIRST];
+    float before[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < FIRST; ++g)
+        if (some && g < a.G) score[g] = *reinterpret_cast<const f32x4*>(a.score + (head + g) * a.tsw + j);
+    if (a.mass != nullptr)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (j + i < n) before[i] = a.mass[at + j + i];
     for (int g = w; g < a.G; g += 4) {
         const float2* part = a.part + (head + g) * a.runs;
         float m = kLowest, l = 0.f;
@@ -164,19 +188,23 @@ __global__ void __launch_bounds__(256) mass_join_kernel(MassArgs a, int tiles) {
     }
     __syncthreads();
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (j < n && j + 3 >= low)
-        for (int g = 0; g < a.G; ++g) {
+    if (some) {
+#pragma unroll
+        for (int g = 0; g < FIRST; ++g)
+            if (g < a.G)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(score[g][i] - s_lse[g]);
+        for (int g = FIRST; g < a.G; ++g) {
             const f32x4 s = *reinterpret_cast<const f32x4*>(a.score + (head + g) * a.tsw + j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(s[i] - s_lse[g]);
         }
-    const int64_t at = unit * a.TS;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (j + i >= (a.fresh != 0 ? a.TS : n)) break;
         const bool seen = j + i >= low && j + i < n;
-        const float before = a.mass != nullptr && j + i < n ? a.mass[at + j + i] : 0.f;
-        a.out[at + j + i] = seen ? before + sum[i] : before;
+        a.out[at + j + i] = seen ? before[i] + sum[i] : before[i];
     }
 }
 
@@ -184,7 +212,8 @@ hipError_t fetch_errors_mass(uint32_t* out, int first, int clear, hipStream_t st
     return fetch_file_errors(out, first, clear, stream);
 }
 
-// Runs of pages that each (sequence, KV head) is cut into.
+// Runs of pages that each (sequence, KV head) is cut into: about 8,192 wavefronts in all (new data each call, 4,096 / 6,144 /
+// 8,192 / 12,288: 8 x 8192 34.9 / 39.0 / 33.8 / 35.5 us, 61 x 4339 over a pool 57.3 / 56.3 / 53.3 / 51.4).
 static int mass_runs(int64_t B, int64_t Hq, int64_t Hkv, int64_t reach) {
     const int64_t G = Hq / Hkv, units = B * Hkv * ((G + 15) / 16), pages = (reach + kPage - 1) / kPage;
     int64_t runs = 8192 / units;

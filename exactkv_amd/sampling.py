@@ -3,12 +3,20 @@
 No counterpart in the reference, whose engine takes the largest logit (exactkv/engine.py:93-95). The draw is one launch
 on the logits' GPU and its current stream; it waits for nothing, keeps nothing between calls and can be captured in a HIP
 graph (with u, and settings given as tensors, rewritten between replays)."""
+import functools
+
 import torch
 
 from . import _lib
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_VOCAB = 1 << 19
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B, V):
+    """Bytes of a call's workspace, which the sizes alone determine."""
+    return _lib.load().exkv_sample_workspace(B, V)
 
 
 def _setting(v, B, dtype, dev, what, kind):
@@ -63,7 +71,7 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob
                          f"{top_k!r}, {top_p!r}, {min_p!r})")
     token = torch.empty(B, dtype=torch.int64, device=logits.device)
     lp = torch.empty(B, dtype=f32, device=logits.device) if logprob else None
-    need = _lib.load().exkv_sample_workspace(B, V)
+    need = _workspace(B, V)
     ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     _lib.call("exkv_sample", logits.data_ptr(), logits.stride(0) if B > 1 else V, kind, B, V, u.data_ptr(), tp, kp, pp, mp, t, k, p, m,
               token.data_ptr(), lp.data_ptr() if logprob else None, ws.data_ptr() if need else None, need,
