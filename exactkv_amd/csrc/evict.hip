@@ -33,7 +33,7 @@ constexpr int kBins = 2048, kNear = 512;
 // 1024 E tokens after the other, read anew by every pass. The r-th largest is found by cutting the interval of the keys
 // into 2,048 bins of one width, counting, and going on with the bin that holds it while that has more than 512 tokens;
 // among these it is the one with r - 1 before it. Keys that are all equal go by index. The tokens that stay are then
-// written in order by a scan. Bound by its steps, each a barrier or two: 64 rows of 8,192 tokens LATER us.
+// written in order by a scan. Bound by its steps, each a barrier or two: 64 rows of 8,192 tokens 9.6 us, 8 rows of 2,048 tokens 6.6 us.
 template <int E, bool WHOLE>
 __global__ void __launch_bounds__(1024) select_kernel(SelectArgs a) {
     __shared__ uint32_t hist[kBins];
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(1024) select_kernel(SelectArgs a) {
     constexpr int PIECE = 1024 * E;
     const int pieces = WHOLE ? 1 : (n + PIECE - 1) / PIECE;
     const int from = a.sinks, to = n - a.recent;       // those between; from <= to, as keep < n
+    const bool aligned = ((uintptr_t)mass & 15) == 0;
     uint32_t key[E];
     float val[E];
     auto load = [&](int p) {
@@ -61,8 +62,13 @@ __global__ void __launch_bounds__(1024) select_kernel(SelectArgs a) {
         for (int i = 0; i < E; i += 4) {
             const int j = p * PIECE + tid * E + i;
             float x[4];
+            if (aligned && j + 4 <= n) {
+                const float4 v = *reinterpret_cast<const float4*>(mass + j);
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x[c] = j + c < n ? mass[j + c] : 0.f;
+                for (int c = 0; c < 4; ++c) x[c] = j + c < n ? mass[j + c] : 0.f;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 val[i + c] = x[c];

@@ -214,12 +214,14 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         auto part_step = [&](int j0, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int kb) {
             if (more) products(st, kb, nxt, [](auto) {});
             if (j0 > w_hi || (a.window > 0 && j0 + 31 <= w_lo - a.window)) return;   // uniform: none seen
+            if (j0 + 31 > w_lo || (a.window > 0 && j0 <= w_hi - a.window)) {   // uniform: not all seen
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                const int rel = pos[rb] - j0 - 4 * half;
+                for (int rb = 0; rb < 2; ++rb) {
+                    const int rel = pos[rb] - j0 - 4 * half;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if ((uint32_t)(rel - (8 * (i >> 2) + (i & 3))) >= span) cur[rb][i] = -INFINITY;
+                    for (int i = 0; i < 16; ++i)
+                        if ((uint32_t)(rel - (8 * (i >> 2) + (i & 3))) >= span) cur[rb][i] = -INFINITY;
+                }
             }
             raise(cur);
 #pragma unroll
