@@ -16,7 +16,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLowest = -1e30f;      // a running maximum before any key, in log2 units
+constexpr float kLowest = -3.402823466e38f;   // a running maximum before any key, in log2 units
 
 struct MassArgs {
     const uint16_t* q;                 // [B, Hq, D]
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256) mass_score_kernel(MassArgs a) {
 
 // One workgroup: 1,024 tokens of one sequence and KV head, four neighbouring ones a thread.
 __global__ void __launch_bounds__(256) mass_join_kernel(MassArgs a, int tiles) {
-    extern __shared__ float s_lse[];                   // [G]: log2 of each query head's sum
+    extern __shared__ float2 s_head[];                 // [G]: each query head's maximum, 1 / sum (apart, as far scores need it)
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t unit = blockIdx.x / (unsigned)tiles, b = unit / a.Hkv;
     const int h = (int)(unit % a.Hkv), tile = (int)(blockIdx.x % (unsigned)tiles);
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(MassArgs a, int tiles) {
             l = l * exp2_fast(m - M) + l2 * exp2_fast(m2 - M);
             m = M;
         }
-        if (lane == 0) s_lse[g] = m + __builtin_amdgcn_logf(l);
+        if (lane == 0) s_head[g] = make_float2(m, 1.f / l);
     }
     __syncthreads();
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -193,11 +193,11 @@ __global__ void __launch_bounds__(256) mass_join_kernel(MassArgs a, int tiles) {
         for (int g = 0; g < FIRST; ++g)
             if (g < a.G)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(score[g][i] - s_lse[g]);
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_fast(score[g][i] - s_head[g].x), s_head[g].y, sum[i]);
         for (int g = FIRST; g < a.G; ++g) {
             const f32x4 s = *reinterpret_cast<const f32x4*>(a.score + (head + g) * a.tsw + j);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(s[i] - s_lse[g]);
+            for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_fast(s[i] - s_head[g].x), s_head[g].y, sum[i]);
         }
     }
 #pragma unroll
@@ -234,7 +234,7 @@ static int launch_mass(MassArgs a, int32_t D, void* ws, int64_t ws_bytes, hipStr
     EXKV_REQUIRE(a.q && a.out && ws, "attention_mass: null pointer");
     EXKV_REQUIRE(a.table == nullptr || (a.pool_pages > 0 && a.table_stride >= (a.TS + kPage - 1) / kPage), "attention_mass: bad page table");
     EXKV_REQUIRE((COMPRESSED || a.table) ? a.TS % kPage == 0 : true, "attention_mass: TS=%d is no multiple of %d", a.TS, kPage);
-    EXKV_REQUIRE(a.TS <= (1 << 30) && a.Hq <= 16384, "attention_mass: TS=%d, %d query heads", a.TS, a.Hq);
+    EXKV_REQUIRE(a.TS <= (1 << 30) && a.Hq <= 8192, "attention_mass: TS=%d, %d query heads", a.TS, a.Hq);
     a.G = a.Hq / a.Hkv;
     const int64_t reach = reach_of(a.lens != nullptr ? a.TS : a.T, a.window), rows = (int64_t)a.B * a.Hq;
     a.runs = mass_runs(a.B, a.Hq, a.Hkv, reach);
@@ -255,7 +255,7 @@ static int launch_mass(MassArgs a, int32_t D, void* ws, int64_t ws_bytes, hipStr
         hipLaunchKernelGGL((mass_score_kernel<128, COMPRESSED>), grid, block, 0, stream, a);
     else
         hipLaunchKernelGGL((mass_score_kernel<256, COMPRESSED>), grid, block, 0, stream, a);
-    if (tiles > 0) hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)(tiles * a.B * a.Hkv)), block, a.G * 4, stream, a, (int)tiles);
+    if (tiles > 0) hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)(tiles * a.B * a.Hkv)), block, a.G * 8, stream, a, (int)tiles);
     return hip_status(hipGetLastError(), "attention_mass");
 }
 

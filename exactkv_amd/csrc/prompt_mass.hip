@@ -9,19 +9,25 @@
 // S^T = K Q^T is made by v_mfma_f32_32x32x16_bf16 with keys as rows, so that a lane holds one query row (column) of 32
 // and 16 keys of each block:
 //   rows     a wavefront holds 64 query rows (row r of a sequence is query head r % G of token r / G) and walks the
-//            keys they see: log2 of each row's sum of 2^s (s the score in log2 units), relative to the largest score of
-//            the first tile with a visible key. Later scores need no maximum: fp32 holds sums of weights up to 2^127,
+//            keys they see: each row's sum of 2^(s - m) (s the score in log2 units), m the largest score of the
+//            first unit with a visible key. Later scores need no maximum: fp32 holds sums of weights up to 2^100,
 //            smaller ones lose nothing, and a sum that leaves the range is made again with a running maximum.
 //   columns  a wavefront holds 64 keys and walks the tokens that see them, one query head after the other, adding up
-//            2^(s - log2 sum) of each key; the 32 lanes of a key are added at the end.
+//            2^(s - m) / sum of each key; the 32 lanes of a key are added at the end.
 // Both are cut into parts where there are few tiles; parts are joined in order, so a call's bits do not change.
+//
+// Bound by the exponentials, two for each visible pair: one of 8,192 tokens, 32 query and 8 KV heads of 128, needs
+// 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); rows take 250 us,
+// columns 275 us. Prompts of few rows are bound by the latency of their few stages: 128 rows over 8,192 keys 19 + 6 + 27 us.
 #include "errors.hpp"
 #include "prompt_stage.hpp"
 #include "../../include/exactkv.h"
 
 namespace exkv {
 
-constexpr float kLowest = -1e30f;      // a maximum before any key, in log2 units
+constexpr float kLowest = -3.402823466e38f;   // a maximum before any key
+constexpr float kFar = 0x1p24f;        // log2 units from which on scores are told apart before they are scaled
+constexpr float kMost = 0x1p100f;      // a row's sum relative to its first tile's maximum
 constexpr int kTile = 256;             // rows, or keys, of a workgroup: 64 a wavefront
 
 struct PromptMassArgs {
@@ -31,11 +37,28 @@ struct PromptMassArgs {
     int S, N, NK, Hq, Hkv, G, window, last;
     float qk_scale;                    // log2(e) / sqrt(D)
     int row_parts, col_parts;
-    float2* part;                      // [row tiles, Hkv, row_parts, kTile]: maximum, sum
-    float* lse;                        // [Hq, N]: log2 of a row's sum; infinity where it sees no key
+    float2* part;                      // [row tiles, Hkv, row_parts, kTile]: m, sum
+    float2* row;                       // [Hq, N]: m, 1 / sum; infinity and 0 where the row sees no key
     float* sums;                       // [col_parts, Hkv, NK]; out where there is one part
     float* out;                        // [Hkv, NK]
 };
+
+// A row's weights are 2^((s - m) / scale) over their sum, m one of its scores. Both passes make them alike, so that a
+// row's add up to 1 however far from 0 its scores lie: as s / scale - M with M = m / scale rounded, in one instruction;
+// where M's rounding would be a bit of the exponent, from s - m.
+__device__ inline float scaled(float m, float scale) {
+#pragma clang fp contract(off)
+    return m * scale;
+}
+__device__ inline float weight_of(float s, float m, float scale) {
+    const float M = scaled(m, scale);
+    return exp2_fast(fabsf(M) > kFar ? (s - m) * scale : fmaf(s, scale, -M));
+}
+// From sums relative to m to sums relative to `to`.
+__device__ inline float rescale(float m, float to, float scale) {
+    const float a = scaled(m, scale), b = scaled(to, scale);
+    return exp2_fast(fabsf(a) > kFar || fabsf(b) > kFar ? (m - to) * scale : a - b);
+}
 
 // Sequence s's queries that count, and its keys.
 __device__ inline void counted_sequence(const PromptMassArgs& a, int s, int& q0, int& Lq, int& k0, int& Lk) {
@@ -144,13 +167,13 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     uint32_t off[St::LOADS];
     St::offsets(w, lane, a.sk_t, off);
     const int rd = St::read_at(col, half);
-    float m[2], l[2];
+    float m[2], M[2], l[2];                            // M: m scaled
     // A unit is 32 keys of a stage and the wavefront's 64 rows. The next unit's products go among this one's exponentials,
     // a k-step each (which take 768 cycles a unit at head dim 128, the products 512): a wavefront alone keeps both busy.
     auto walk = [&](auto safe) {
         constexpr bool SAFE = decltype(safe)::value;
         constexpr int AHEAD = 2;                       // k-steps of keys read ahead
-        m[0] = m[1] = kLowest;
+        m[0] = m[1] = M[0] = M[1] = kLowest;
         l[0] = l[1] = 0.f;
         if (first > last) return;
         Stream<D, SR> keys(a.k, a.sk_t, hk * a.sk_h, tile, first * SR);
@@ -183,10 +206,11 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                     float mx = sc[rb][0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[rb][i]);
-                    mx = fmaxf(mx * a.qk_scale, kLowest);
+                    mx = fmaxf(mx, kLowest);
                     if (SAFE ? mx > m[rb] : m[rb] == kLowest) {
-                        l[rb] *= exp2_fast(m[rb] - mx);
+                        if (SAFE) l[rb] *= rescale(m[rb], mx, a.qk_scale);
                         m[rb] = mx;
+                        M[rb] = scaled(mx, a.qk_scale);
                     }
                 }
         };
@@ -194,7 +218,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         // (weights are made here, not sunk to the sums' use)
         auto here = [](float (&x)[2]) { asm volatile("" : "+v"(x[0]), "+v"(x[1])); };
         auto weigh = [&](const f32x16 (&sc)[2], int e) {
-            sum[e >> 4][e & 1] += exp2_fast(fmaf(sc[e >> 4][e & 15], a.qk_scale, -m[e >> 4]));
+            sum[e >> 4][e & 1] += SAFE ? weight_of(sc[e >> 4][e & 15], m[e >> 4], a.qk_scale)
+                                       : exp2_fast(fmaf(sc[e >> 4][e & 15], a.qk_scale, -M[e >> 4]));
         };
         auto settle = [&] {
 #pragma unroll
@@ -300,19 +325,21 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     if (threadIdx.x == 0) s_again = 0;
     walk(std::false_type{});
     __syncthreads();
-    if (!(l[0] < INFINITY) || !(l[1] < INFINITY)) s_again = 1;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+        if (!(l[rb] < kMost) || (m[rb] != kLowest && fabsf(M[rb]) > kFar)) s_again = 1;
     __syncthreads();
     if (s_again != 0) walk(std::true_type{});          // uniform
     if (!wave_on) return;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
-        const float m2 = __shfl_xor(m[rb], 32), l2 = __shfl_xor(l[rb], 32), M = fmaxf(m[rb], m2);
-        const float sum = l[rb] * exp2_fast(m[rb] - M) + l2 * exp2_fast(m2 - M);
+        const float m2 = __shfl_xor(m[rb], 32), l2 = __shfl_xor(l[rb], 32), top = fmaxf(m[rb], m2);
+        const float sum = l[rb] * rescale(m[rb], top, a.qk_scale) + l2 * rescale(m2, top, a.qk_scale);
         if (half != 0 || wrow0 + 32 * rb + col >= nrows) continue;
         if (a.row_parts > 1)
-            a.part[(((int64_t)index * a.Hkv + hk) * a.row_parts + part) * kTile + 64 * w + 32 * rb + col] = make_float2(M, sum);
+            a.part[(((int64_t)index * a.Hkv + hk) * a.row_parts + part) * kTile + 64 * w + 32 * rb + col] = make_float2(top, sum);
         else
-            a.lse[(int64_t)hq[rb] * a.N + tile.q0 + tok[rb]] = sum == 0.f ? INFINITY : M + __builtin_amdgcn_logf(sum);
+            a.row[(int64_t)hq[rb] * a.N + tile.q0 + tok[rb]] = sum == 0.f ? make_float2(INFINITY, 0.f) : make_float2(top, 1.f / sum);
     }
 }
 
@@ -324,27 +351,27 @@ __global__ void __launch_bounds__(4 * kTile) mass_rows_join_kernel(PromptMassArg
     PromptTile tile;
     if (!tile_at<true>(a, index, tile)) return;
     const int row = tile.row0 + r;
-    float M = kLowest, l = 0.f;
+    float m = kLowest, l = 0.f;
     const float2* part = a.part + ((int64_t)index * a.Hkv + hk) * a.row_parts * kTile + r;
     if (row < tile.Lq * a.G)
 #pragma unroll 8
         for (int i = quarter; i < a.row_parts; i += 4) {
             const float2 x = part[(int64_t)i * kTile];
-            const float m = fmaxf(M, x.x);
-            l = l * exp2_fast(M - m) + x.y * exp2_fast(x.x - m);
-            M = m;
+            const float top = fmaxf(m, x.x);
+            l = l * rescale(m, top, a.qk_scale) + x.y * rescale(x.x, top, a.qk_scale);
+            m = top;
         }
-    s[quarter][r] = make_float2(M, l);
+    s[quarter][r] = make_float2(m, l);
     __syncthreads();
     if (quarter != 0 || row >= tile.Lq * a.G) return;
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
         const float2 x = s[i][r];
-        const float m = fmaxf(M, x.x);
-        l = l * exp2_fast(M - m) + x.y * exp2_fast(x.x - m);
-        M = m;
+        const float top = fmaxf(m, x.x);
+        l = l * rescale(m, top, a.qk_scale) + x.y * rescale(x.x, top, a.qk_scale);
+        m = top;
     }
-    a.lse[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? INFINITY : M + __builtin_amdgcn_logf(l);
+    a.row[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / l);
 }
 
 // Entries of keys that no sequence holds, from key `end` on: 0, shared by all workgroups.
@@ -389,151 +416,182 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     St::offsets(w, lane, a.sq_t, off);
     const int rd = St::read_at(col, half);
     f32x16 acc[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[kb][i] = 0.f;
     // rows are tokens of one query head at a time: a "sequence" of Lq rows at the head's channels
     PromptTile rows = tile;
     rows.k0 = tile.q0;
     rows.Lk = tile.Lq;
-    int g = tiles > 0 ? (int)(begin / tiles) : 0, t = tiles > 0 ? (int)(begin % tiles) : 0;
-    float lse[SB], next_lse[SB];
-    int gl = g, tl = t;                                // of the loads
-    auto load = [&](int st) {
-        Stream<D, SR> s(a.q, a.sq_t, (hk * G + gl) * a.sq_h, rows, (first + tl) * SR);
-        each<St::LOADS>([&](auto i) { load_piece<i.value>(s.buf, off[i.value], lds0 + st * St::BYTES); });
-#pragma unroll
-        for (int rb = 0; rb < SB; ++rb) {
-            const int tok = (first + tl) * SR + 32 * rb + col;
-            next_lse[rb] = tok < tile.Lq ? a.lse[(int64_t)(hk * G + gl) * a.N + tile.q0 + tok] : INFINITY;
-        }
-        if (++tl == tiles) {
-            tl = 0;
-            ++gl;
-        }
-    };
-    // A unit is 32 tokens of a stage and the wavefront's 64 keys, walked as the other pass walks its units.
-    constexpr int AHEAD = 2;
-    auto products = [&](int st, int rb, f32x16 (&sc)[2], auto between) {
-        bf16x8 qf[KS];
-        each<AHEAD>([&](auto s) { qf[s.value] = St::piece(lds, st, rd, rb, s.value); });
-        each<KS>([&](auto step) {
-            constexpr int s = decltype(step)::value;
-            if constexpr (s + AHEAD < KS) qf[s + AHEAD] = St::piece(lds, st, rd, rb, s + AHEAD);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                if constexpr (s == 0)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
-                sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][s], qf[s], sc[kb], 0, 0, 0);
-            }
-            between(step);
-            __builtin_amdgcn_sched_barrier(0);
-        });
-    };
-    auto here = [](float x) {                          // made here, not sunk to its use
-        asm volatile("" : "+v"(x));
-        return x;
-    };
-    // this unit's weights, of tokens standing at p0 on, and the next one's scores: where all of them see every key, and otherwise
-    auto full_step = [&](float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int rb) {
-        products(st, rb, nxt, [&](auto s) {
-#pragma unroll
-            for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) {
-                acc[e >> 4][e & 15] = here(acc[e >> 4][e & 15] + exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row_lse)));
-            }
-        });
-    };
-    auto part_step = [&](int p0, float row_lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
-        if (more) products(st, rb, nxt, [](auto) {});
-        if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int rel = p0 + col - wkey0 - 4 * half;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row_lse));
-                // (after the exponential: a row's sum may be NaN)
-                acc[kb][i] += (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) < span ? x : 0.f;
-            }
-        }
-    };
-    const int count = (int)(end - begin);
-    if (count > 0) {
-        load(0);
+    auto walk = [&](auto safe) {                       // the largest M of the rows
+        constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(kf[kb][s]));
-        next_stage();
+            for (int i = 0; i < 16; ++i) acc[kb][i] = 0.f;
+        int g = tiles > 0 ? (int)(begin / tiles) : 0, t = tiles > 0 ? (int)(begin % tiles) : 0;
+        float2 row[SB], next_row[SB];                      // m, 1 / sum
+        float far = 0.f;                                   // the largest M so far
+        int gl = g, tl = t;                                // of the loads
+        auto load = [&](int st) {
+            Stream<D, SR> s(a.q, a.sq_t, (hk * G + gl) * a.sq_h, rows, (first + tl) * SR);
+            each<St::LOADS>([&](auto i) { load_piece<i.value>(s.buf, off[i.value], lds0 + st * St::BYTES); });
 #pragma unroll
-        for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
-        if (count > 1) load(1);
-        f32x16 s0[2], s1[2];
-        if (wave_on) products(0, 0, s0, [](auto) {});
-        auto advance = [&] {
-            if (++t == tiles) t = 0;
+            for (int rb = 0; rb < SB; ++rb) {
+                const int tok = (first + tl) * SR + 32 * rb + col;
+                next_row[rb] = tok < tile.Lq ? a.row[(int64_t)(hk * G + gl) * a.N + tile.q0 + tok] : make_float2(INFINITY, 0.f);
+            }
+            if (++tl == tiles) {
+                tl = 0;
+                ++gl;
+            }
         };
-        auto part_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
-            constexpr int st = decltype(parity)::value;
-            const int p0 = (first + t) * SR + shift;
-            if constexpr (SB == 2)
-                if (wave_on) part_step(p0, lse[0], cur, nxt, true, st, 1);
-            const bool more = it + 1 < count;
-            const float last_lse = lse[SB - 1];
-            if (more) {
-                next_stage();
+        auto take = [&](int rb) {                          // the rows of the stage that has landed
+            row[rb] = next_row[rb];
+            const float M = scaled(row[rb].x, a.qk_scale);
+            far = fmaxf(far, fabsf(M) < INFINITY ? fabsf(M) : 0.f);
+            if (!SAFE) row[rb].x = M;
+        };
+        // A unit is 32 tokens of a stage and the wavefront's 64 keys, walked as the other pass walks its units.
+        constexpr int AHEAD = 2;
+        auto products = [&](int st, int rb, f32x16 (&sc)[2], auto between) {
+            bf16x8 qf[KS];
+            each<AHEAD>([&](auto s) { qf[s.value] = St::piece(lds, st, rd, rb, s.value); });
+            each<KS>([&](auto step) {
+                constexpr int s = decltype(step)::value;
+                if constexpr (s + AHEAD < KS) qf[s + AHEAD] = St::piece(lds, st, rd, rb, s + AHEAD);
 #pragma unroll
-                for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
-            }
-            if (it + 2 < count) load(st);
-            if (wave_on) {
-                if constexpr (SB == 2)
-                    part_step(p0 + 32, last_lse, nxt, cur, more, st ^ 1, 0);
-                else
-                    part_step(p0, last_lse, cur, nxt, more, st ^ 1, 0);
-            }
-            advance();
+                for (int kb = 0; kb < 2; ++kb) {
+                    if constexpr (s == 0)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+                    sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][s], qf[s], sc[kb], 0, 0, 0);
+                }
+                between(step);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         };
-        auto full_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
-            constexpr int st = decltype(parity)::value;
-            if constexpr (SB == 2) full_step(lse[0], cur, nxt, st, 1);
-            const float last_lse = lse[SB - 1];
+        auto here = [](float x) {                          // made here, not sunk to its use
+            asm volatile("" : "+v"(x));
+            return x;
+        };
+        // this unit's weights, of tokens standing at p0 on, and the next one's scores: where all of them see every key, and otherwise
+        auto full_step = [&](float2 row, f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int rb) {
+            products(st, rb, nxt, [&](auto s) {
+#pragma unroll
+                for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) {
+                    acc[e >> 4][e & 15] = here(fmaf(exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row.x)), row.y, acc[e >> 4][e & 15]));
+                }
+            });
+        };
+        auto part_step = [&](int p0, float2 row, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
+            if (more) products(st, rb, nxt, [](auto) {});
+            if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int rel = p0 + col - wkey0 - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = SAFE ? weight_of(cur[kb][i], row.x, a.qk_scale) : exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row.x));
+                    // (after the product: a row's sum may be NaN)
+                    acc[kb][i] += (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) < span ? x * row.y : 0.f;
+                }
+            }
+        };
+        const int count = (int)(end - begin);
+        if (count > 0) {
+            load(0);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(kf[kb][s]));
             next_stage();
 #pragma unroll
-            for (int rb = 0; rb < SB; ++rb) lse[rb] = next_lse[rb];
-            if (it + 2 < count) load(st);
-            if constexpr (SB == 2)
-                full_step(last_lse, nxt, cur, st ^ 1, 0);
-            else
-                full_step(last_lse, cur, nxt, st ^ 1, 0);
-            advance();
-        };
-        // whether all of the tile of tokens `at` see every key of the wavefront
-        auto full = [&](int at) {
-            const int p0 = (first + at) * SR + shift;
-            return p0 >= wkey0 + 63 && (a.window == 0 || p0 + SR - 1 - wkey0 < a.window);
-        };
-        constexpr std::integral_constant<int, 0> even{};
-        constexpr std::integral_constant<int, 1> odd{};
-        for (int it = 0; it < count; it += 2) {
-            while (wave_on && it + 2 < count && full(t) && full(t + 1 == tiles ? 0 : t + 1)) {
-                full_stage(it, even, s0, s1);
-                if constexpr (SB == 2)
-                    full_stage(it + 1, odd, s0, s1);
-                else
-                    full_stage(it + 1, odd, s1, s0);
-                it += 2;
+            for (int rb = 0; rb < SB; ++rb) take(rb);
+            if (count > 1) load(1);
+            f32x16 s0[2], s1[2];
+            if constexpr (SAFE) {                          // seldom: unit by unit
+#pragma unroll 1
+                for (int it = 0; it < count; ++it) {
+                    if (it > 0) {
+                        next_stage();
+#pragma unroll
+                        for (int rb = 0; rb < SB; ++rb) take(rb);
+                        if (it + 1 < count) load((it + 1) & 1);
+                    }
+                    if (wave_on)
+#pragma unroll 1
+                        for (int rb = 0; rb < SB; ++rb) {
+                            products(it & 1, rb, s0, [](auto) {});
+                            part_step((first + t) * SR + shift + 32 * rb, rb == 0 ? row[0] : row[SB - 1], s0, s1, false, 0, 0);
+                        }
+                    if (++t == tiles) t = 0;
+                }
+                return far;
             }
-            part_stage(it, even, s0, s1);
-            if (it + 1 == count) break;
-            if constexpr (SB == 2)
-                part_stage(it + 1, odd, s0, s1);
-            else
-                part_stage(it + 1, odd, s1, s0);
+            if (wave_on) products(0, 0, s0, [](auto) {});
+            auto advance = [&] {
+                if (++t == tiles) t = 0;
+            };
+            auto part_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+                constexpr int st = decltype(parity)::value;
+                const int p0 = (first + t) * SR + shift;
+                if constexpr (SB == 2)
+                    if (wave_on) part_step(p0, row[0], cur, nxt, true, st, 1);
+                const bool more = it + 1 < count;
+                const float2 last_row = row[SB - 1];
+                if (more) {
+                    next_stage();
+#pragma unroll
+                    for (int rb = 0; rb < SB; ++rb) take(rb);
+                }
+                if (it + 2 < count) load(st);
+                if (wave_on) {
+                    if constexpr (SB == 2)
+                        part_step(p0 + 32, last_row, nxt, cur, more, st ^ 1, 0);
+                    else
+                        part_step(p0, last_row, cur, nxt, more, st ^ 1, 0);
+                }
+                advance();
+            };
+            auto full_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+                constexpr int st = decltype(parity)::value;
+                if constexpr (SB == 2) full_step(row[0], cur, nxt, st, 1);
+                const float2 last_row = row[SB - 1];
+                next_stage();
+#pragma unroll
+                for (int rb = 0; rb < SB; ++rb) take(rb);
+                if (it + 2 < count) load(st);
+                if constexpr (SB == 2)
+                    full_step(last_row, nxt, cur, st ^ 1, 0);
+                else
+                    full_step(last_row, cur, nxt, st ^ 1, 0);
+                advance();
+            };
+            // whether all of the tile of tokens `at` see every key of the wavefront
+            auto full = [&](int at) {
+                const int p0 = (first + at) * SR + shift;
+                return p0 >= wkey0 + 63 && (a.window == 0 || p0 + SR - 1 - wkey0 < a.window);
+            };
+            constexpr std::integral_constant<int, 0> even{};
+            constexpr std::integral_constant<int, 1> odd{};
+            for (int it = 0; it < count; it += 2) {
+                while (wave_on && it + 2 < count && full(t) && full(t + 1 == tiles ? 0 : t + 1)) {
+                    full_stage(it, even, s0, s1);
+                    if constexpr (SB == 2)
+                        full_stage(it + 1, odd, s0, s1);
+                    else
+                        full_stage(it + 1, odd, s1, s0);
+                    it += 2;
+                }
+                part_stage(it, even, s0, s1);
+                if (it + 1 == count) break;
+                if constexpr (SB == 2)
+                    part_stage(it + 1, odd, s0, s1);
+                else
+                    part_stage(it + 1, odd, s1, s0);
+            }
         }
-    }
+        return far;
+    };
+    if (__syncthreads_or(walk(std::false_type{}) > kFar)) walk(std::true_type{});
     if (!wave_on) return;
     // over the 32 lanes of a key: halving the values with the lanes, so that lane c of a half ends up with value
     // c >> 1 of a block, which is key 8 (c >> 3) + 4 half + (c >> 1 & 3)
@@ -548,8 +606,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             const bool upper = (lane & d) != 0;
 #pragma unroll
             for (int i = 0; i < n; ++i) {
-                const float send = upper ? v[i] : v[i + n], keep = upper ? v[i + n] : v[i];
-                v[i] = keep + __shfl_xor(send, d);
+                const float low = v[i], high = v[i + n];
+                v[i] = (upper ? high : low) + __shfl_xor(upper ? low : high, d);
             }
         }
         v[0] += __shfl_xor(v[0], 1);
@@ -579,7 +637,7 @@ hipError_t fetch_errors_prompt_mass(uint32_t* out, int first, int clear, hipStre
 struct MassPlan {
     int64_t row_tiles, col_tiles;
     int row_parts, col_parts;
-    int64_t part_bytes, lse_bytes, sum_bytes;
+    int64_t part_bytes, row_bytes, sum_bytes;
 };
 static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t Hkv, int D, int64_t window, int64_t last) {
     MassPlan p{};
@@ -598,7 +656,7 @@ static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t 
     const int64_t most = last > 0 && last < N ? last : N, seen = window > 0 && window + kTile < most ? window + kTile : most;
     p.col_parts = cut(p.col_tiles * Hkv, (seen + SR - 1) / SR * G);
     p.part_bytes = p.row_parts > 1 ? p.row_tiles * Hkv * p.row_parts * kTile * 8 : 0;
-    p.lse_bytes = (Hq * N * 4 + 15) / 16 * 16;
+    p.row_bytes = (Hq * N * 8 + 15) / 16 * 16;
     p.sum_bytes = p.col_parts > 1 ? (p.col_parts * Hkv * NK * 4 + 15) / 16 * 16 : 0;
     return p;
 }
@@ -624,7 +682,7 @@ extern "C" int64_t exkv_prompt_mass_workspace(int32_t S, int32_t N, int32_t NK, 
                                               int32_t last) {
     if (!head_dim_ok(D) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || S < 0 || N <= 0 || NK <= 0 || window < 0 || last < 0) return 0;
     const MassPlan p = plan_mass(S, N, NK, Hq, Hkv, D, window, last);
-    return p.part_bytes + p.lse_bytes + p.sum_bytes;
+    return p.part_bytes + p.row_bytes + p.sum_bytes;
 }
 
 extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
@@ -655,12 +713,12 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
     PromptMassArgs a{(const uint16_t*)q, (const uint16_t*)k, sq_t, sq_h, sk_t, sk_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, last,
                      qk_scale, p.row_parts, p.col_parts, nullptr, nullptr, nullptr, out};
     if (N > 0 && S > 0) {
-        const int64_t need = p.part_bytes + p.lse_bytes + p.sum_bytes;
+        const int64_t need = p.part_bytes + p.row_bytes + p.sum_bytes;
         EXKV_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "prompt_mass: workspace of %lld bytes, %lld needed",
                      (long long)ws_bytes, (long long)need);
-        a.lse = (float*)ws;
-        a.sums = p.col_parts > 1 ? (float*)((uint8_t*)ws + p.lse_bytes) : out;
-        a.part = (float2*)((uint8_t*)ws + p.lse_bytes + p.sum_bytes);
+        a.row = (float2*)ws;
+        a.sums = p.col_parts > 1 ? (float*)((uint8_t*)ws + p.row_bytes) : out;
+        a.part = (float2*)((uint8_t*)ws + p.row_bytes + p.sum_bytes);
         if (D == 64)
             launch_prompt_mass<64>(a, p, stream);
         else if (D == 128)

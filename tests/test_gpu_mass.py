@@ -319,6 +319,40 @@ def test_scores_far_apart():
     _check_prompt(z, k, [400], [400])
 
 
+@pytest.mark.parametrize("scale", [0, 7, 14, 20, 40])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_equal_keys_share_alike_whatever_their_scores(D, scale):
+    """Keys that are all one row have one score each, up to about 2^(2 scale + 7) here; each row's weights are equal and
+    add up to 1. An entry sums up to n weights 1 / k that are off by the sums they were divided by (n 2^-24) and a few roundings."""
+    g = _gen(16)
+    n, Hq, Hkv = 300, 6, 2
+    q = (torch.randn(n, Hq, D, generator=g, device=DEV) * 2.0 ** scale).bfloat16()
+    row = (torch.randn(1, Hkv, D, generator=g, device=DEV) * 2.0 ** scale).bfloat16()
+    k = row.expand(n, Hkv, D).contiguous()
+    share = 3.0 / torch.arange(1, n + 1, dtype=torch.float64, device=DEV)
+    rel = 2 * n * 2.0 ** -24 + 2.0 ** -20
+    want = share.flip(0).cumsum(0).flip(0).expand(Hkv, n)
+    _near(exactkv.prompt_mass(q, k, _offsets([n])), want, want * rel)
+    _near(exactkv.prompt_mass(q[:40].contiguous(), k, _offsets([40]), cu_seqlens_k=_offsets([n]), last=1),
+          share[-1].expand(Hkv, n), share[-1] * rel)
+    _near(exactkv.attention_mass(q[:1], k[None], n), share[-1].expand(1, Hkv, n), share[-1] * rel)
+
+
+@pytest.mark.parametrize("scale", [10, 30, 55])
+def test_weights_add_up_to_one_whatever_the_scores(scale):
+    """Scores of any size, split keys and not: every row's weights add up to 1 (to the n 2^-24 of its sum and of the
+    entries', and the exponentials' 2^-22), and none is negative."""
+    g = _gen(17)
+    for n, nk, last in ((500, 500, 0), (64, 4000, 0), (700, 700, 33)):
+        q, k = _prompt(g, n, nk, 8, 2, 128)
+        q, k = (q.float() * 2.0 ** scale).bfloat16(), (k.float() * 2.0 ** scale).bfloat16()
+        got = exactkv.prompt_mass(q, k, _offsets([n]), cu_seqlens_k=_offsets([nk]), last=last)
+        rows = 4 * (last or n)
+        assert (got >= 0).all() and (got.double().sum(-1) - rows).abs().max() < rows * 2 * (nk + rows) * 2.0 ** -24
+        got = exactkv.attention_mass(q[:1], k[None], nk)
+        assert (got >= 0).all() and (got.double().sum(-1) - 4).abs().max() < 8 * nk * 2.0 ** -24
+
+
 def test_strided_views_and_streams():
     g = _gen(14)
     Hq, Hkv, D, N = 8, 2, 128, 333
