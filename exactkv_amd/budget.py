@@ -106,6 +106,8 @@ def attention_mass(q, k_cache, T=None, *, mass=None, lens=None, block_table=None
             return attention_mass(q, k_cache, T, mass=mass, lens=lens, block_table=block_table, window=window, out=out)
     B, Hq, D = _check_q(q)
     if isinstance(k_cache, (PagedCompressedKV, PagedBF16KV)) and block_table is None:
+        if lens is not None or T is not None:
+            raise ValueError("a paged cache's step has its own lengths: give block_table with T or lens")
         _, block_table, lens = k_cache.table.step_rows()
     elif T is None and lens is None and isinstance(k_cache, (CompressedKV, BF16KV)):
         T = k_cache.T
@@ -273,53 +275,83 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
         live ones) are cut, the pages behind go back to the pool (raw rows stay until compact()), and begin_step comes
         before the next step.
 
+    Of several layers, give lists of equal length: a cache pair and its mass each. Paged layers share their table's lengths,
+    so all caches of a table are cut in one call (ValueError otherwise).
+
     Sequences of at most `keep` tokens stay as they are. Returns the index that select_tokens gave, a row for each sequence
-    (slot). Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is not captured. The next
-    token's position is what the caller counts, not the cache's length."""
-    if type(k_cache) is not type(v_cache) or not isinstance(k_cache, (CompressedKV, BF16KV, PagedCompressedKV, PagedBF16KV)):
-        raise TypeError(f"evict takes two caches of one kind (got {type(k_cache).__name__}, {type(v_cache).__name__})")
-    if k_cache is v_cache:
+    (slot); of lists, a list of them. Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is
+    not captured. The next token's position is what the caller counts, not the cache's length."""
+    many = isinstance(k_cache, (list, tuple))
+    layers = list(zip(k_cache, v_cache, mass)) if many else [(k_cache, v_cache, mass)]
+    if many and not (len(k_cache) == len(v_cache) == len(mass) > 0):
+        raise ValueError(f"{len(k_cache)} key caches, {len(v_cache)} value caches and {len(mass)} masses")
+    kind = type(layers[0][0])
+    if any(type(c) is not kind for k, v, _ in layers for c in (k, v)) or not issubclass(kind, (CompressedKV, BF16KV, PagedCompressedKV,
+                                                                                               PagedBF16KV)):
+        raise TypeError(f"evict takes caches of one kind (got {', '.join(sorted({type(c).__name__ for x in layers for c in x[:2]}))})")
+    caches = [c for k, v, _ in layers for c in (k, v)]
+    if len({id(c) for c in caches}) != len(caches):
         raise ValueError("keys and values need a cache each")
-    if getattr(k_cache, "_pending", None) is not None or getattr(v_cache, "_pending", None) is not None:
+    if any(getattr(c, "_pending", None) is not None for c in caches):
         raise RuntimeError("a page filled: call check_overflow() before evict()")
-    H, D = k_cache.H, k_cache.D
-    dev = mass.get_device()
+    dev = layers[0][2].get_device()
     if dev >= 0 and dev != _lib.current_device():
         with _on(dev):
             return evict(k_cache, v_cache, mass, keep, sinks=sinks, recent=recent, slots=slots)
-    if isinstance(k_cache, (CompressedKV, BF16KV)):
-        B, TS, T = k_cache.B, k_cache.TS, k_cache.T
-        if slots is not None:
-            raise ValueError("contiguous caches are cut as a whole (slots are of paged ones)")
-        if (v_cache.B, v_cache.TS, v_cache.H, v_cache.D, v_cache.T) != (B, TS, H, D, T):
-            raise ValueError("k and v caches differ in shape or in the tokens they hold")
-        _mass_rows(mass, (B, H, TS), dev, "mass")
-        index, kept = select_tokens(mass, keep, T, sinks=sinks, recent=recent)
-        if T > keep:
-            k, v = gather_tokens(k_cache, v_cache, index)
-            k_cache.replace(k)
-            v_cache.replace(v)
-            mass[..., :keep] = kept
-            mass[..., keep:] = 0
-        return index
-    table = k_cache.table
-    if v_cache.table is not table or (v_cache.H, v_cache.D) != (H, D):
-        raise ValueError("k and v caches differ in shape or belong to two page tables")
-    _mass_rows(mass, (table.max_seqs, H, table.capacity), dev, "mass")
+    paged = issubclass(kind, (PagedCompressedKV, PagedBF16KV))
+    if slots is not None and not paged:
+        raise ValueError("contiguous caches are cut as a whole (slots are of paged ones)")
+    for k, v, m in layers:
+        if paged:
+            if any(c.table is not layers[0][0].table or (c.H, c.D) != (k.H, k.D) for c in (k, v)):
+                raise ValueError("k and v caches differ in shape or belong to two page tables")
+            shape = (k.table.max_seqs, k.H, k.table.capacity)
+        else:
+            if (v.B, v.TS, v.H, v.D, v.T) != (k.B, k.TS, k.H, k.D, k.T):
+                raise ValueError("k and v caches differ in shape or in the tokens they hold")
+            shape = (k.B, k.H, k.TS)
+        _mass_rows(m, shape, dev, "mass")
+    choice = dict(sinks=sinks, recent=recent)
+    kept = _evict_paged(layers, keep, choice, slots) if paged else [_evict_rows(*x, keep, choice) for x in layers]
+    return kept if many else kept[0]
+
+
+def _evict_rows(k_cache, v_cache, mass, keep, choice):
+    T = k_cache.T
+    index, kept = select_tokens(mass, keep, T, **choice)
+    if T > keep:
+        k, v = gather_tokens(k_cache, v_cache, index)
+        k_cache.replace(k)
+        v_cache.replace(v)
+        mass[..., :keep] = kept
+        mass[..., keep:] = 0
+    return index
+
+
+def _evict_paged(layers, keep, choice, slots):
+    table = layers[0][0].table
+    caches = {id(c) for k, v, _ in layers for c in (k, v)}
+    if any(id(c) not in caches for c in table.caches()):
+        raise ValueError("other caches share the page table and its lengths: evict from all of them in one call")
+    if table.step_open() and any(c._appended != table.step for k, v, _ in layers for c in (k, v)):
+        raise RuntimeError("the step's tokens come before evict()")
     slots = table.live_slots() if slots is None else [int(s) for s in slots]
     if len(set(slots)) != len(slots) or any(not 0 <= s < table.max_seqs or table._pages[s] is None for s in slots):
         raise ValueError(f"slots must be distinct and in use (got {slots})")
-    at = torch.tensor(slots, dtype=torch.int64).to(mass.device)
-    index, kept = select_tokens(mass[at], keep, lens=table.lens[at], sinks=sinks, recent=recent)
+    at = torch.tensor(slots, dtype=torch.int64).to(layers[0][2].device)
+    lens = table.lens[at]
+    chosen = [select_tokens(mass[at], keep, lens=lens, **choice) for _, _, mass in layers]
     long = [i for i, s in enumerate(slots) if table.length(s) > keep]
-    if not long:
-        return index
-    rows = torch.tensor(long, dtype=torch.int64).to(mass.device)
-    k, v = gather_tokens(k_cache, v_cache, index[rows], block_table=table.block_table[at[rows]])
-    for j, i in enumerate(long):
-        table.truncate(slots[i], keep)
-        k_cache.prefill(slots[i], k[j:j + 1])
-        v_cache.prefill(slots[i], v[j:j + 1])
-    mass[at[rows], :, :keep] = kept[rows]
-    mass[at[rows], :, keep:] = 0
-    return index
+    if long:
+        rows = torch.tensor(long, dtype=torch.int64).to(at.device)
+        pages = table.block_table[at[rows]]
+        tokens = [gather_tokens(k, v, index[rows], block_table=pages) for (k, v, _), (index, _) in zip(layers, chosen)]
+        for i in long:
+            table.truncate(slots[i], keep)
+        for (k_cache, v_cache, mass), (_, kept), (k, v) in zip(layers, chosen, tokens):
+            for j, i in enumerate(long):
+                k_cache.prefill(slots[i], k[j:j + 1])
+                v_cache.prefill(slots[i], v[j:j + 1])
+            mass[at[rows], :, :keep] = kept[rows]
+            mass[at[rows], :, keep:] = 0
+    return [index for index, _ in chosen]

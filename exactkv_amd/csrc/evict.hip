@@ -312,7 +312,8 @@ extern "C" int exkv_select_tokens(const float* mass, int64_t s_b, int64_t s_h, c
     EXKV_REQUIRE((int64_t)B * H * 1024 <= (int64_t)UINT32_MAX, "select_tokens: too many rows (B=%d, H=%d)", B, H);
     EXKV_REQUIRE(s_b >= 0 && s_h >= 0 && lens_stride >= 0, "select_tokens: negative stride");
     if (B == 0 || keep == 0) return EXKV_OK;
-    EXKV_REQUIRE(mass && index && kept, "select_tokens: null pointer");
+    EXKV_REQUIRE((mass || TS == 0) && index && kept, "select_tokens: null pointer");
+    EXKV_REQUIRE(TS <= (1 << 30), "select_tokens: TS=%d", TS);
     const SelectArgs a{mass, s_b, s_h, lens, lens_stride, T, H, TS, keep, sinks, recent, index, kept};
     const dim3 grid((unsigned)(B * H)), block(1024);
     const int most = lens != nullptr ? TS : T;

@@ -299,10 +299,10 @@ class Engine:
                         kc.prefill_slot(b, keys.transpose(1, 2))
                         vc.prefill_slot(b, values.transpose(1, 2))
                     del pkv
-                nxt.append(self._prefill_next(out.last_hidden_state, choose))
+                nxt.append(self._prefill_next(out.last_hidden_state, None if choose is None else lambda logits: logits))
                 del out
         self._graph = None                      # buffers may have grown
-        return torch.cat(nxt)
+        return torch.cat(nxt) if choose is None else choose(torch.cat(nxt))
 
     def _prefill_next(self, hidden, choose=None):
         """Greedy (or chosen) next token from the prompt's last hidden state. The final norm is applied
@@ -340,8 +340,7 @@ class Engine:
             raise RuntimeError(f"position {self.dropped + T} is outside the model's {positions}")
         if T < self.TS:
             return
-        for (kc, vc), mass in zip(self.kv, self.mass):
-            evict(kc, vc, mass, b.keep, sinks=b.sinks, recent=b.recent)
+        evict(*zip(*self.kv), self.mass, b.keep, sinks=b.sinks, recent=b.recent)
         self._drop(self.dropped + self.TS - b.keep)
 
     def _attend_kept(self, i, q):

@@ -22,6 +22,8 @@ A sequence's newest, partly filled page lives in its tail area at the end of the
 (all rows raw), as in CompressedKV. Raw rows of released sequences stay in the pool until
 compact().
 """
+import weakref
+
 import torch
 
 from . import _lib
@@ -43,6 +45,7 @@ class PageTable:
         self.step = 0
         self._step_slots = []
         self._rows = None                                       # (slots tensor or None, table, lens) of the step
+        self._caches = weakref.WeakSet()                        # over this table's pages
 
     @property
     def capacity(self):
@@ -56,6 +59,13 @@ class PageTable:
 
     def pages(self, slot):
         return list(self._pages[slot])
+
+    def caches(self):
+        return list(self._caches)
+
+    def step_open(self):
+        """Whether begin_step's tokens are counted and no sequence came, went or was cut since."""
+        return self._rows is not None
 
     def live_slots(self):
         return [s for s in range(self.max_seqs) if self._pages[s] is not None]
@@ -107,7 +117,7 @@ class PageTable:
 
     def truncate(self, slot, T):
         """A slot's sequence has T tokens from now on, no more than it had: the pages behind its open one go back to the
-        pool (the caches' rows follow, see budget.evict)."""
+        pool. The caches hold none of them until each is prefilled anew (budget.evict does both)."""
         if self._pages[slot] is None:
             raise ValueError(f"slot {slot} is not in use")
         if not 0 <= T <= self._len[slot]:
@@ -183,6 +193,7 @@ class PagedCompressedKV:
     def __init__(self, table, H, D=128, reserve=0.01):
         assert D in HEAD_DIMS, f"head dim must be one of {HEAD_DIMS} (got {D})"
         self.table, self.H, self.D = table, H, D
+        table._caches.add(self)
         dev = self.dev = table.dev
         NPg = table.num_pages
         self.TS = NPg * P                                      # the pool read as one [1, TS] cache
@@ -381,6 +392,7 @@ class PagedBF16KV:
 
     def __init__(self, table, H, D=128):
         self.table, self.H, self.D = table, H, D
+        table._caches.add(self)
         self.buf = torch.zeros(1, table.num_pages * P, H, D, dtype=torch.bfloat16, device=table.dev)
         self._appended = 0
         self.cnt = None

@@ -191,6 +191,66 @@ def test_evict_refusals():
             exactkv.evict(pk, pv, m, 2, slots=slots)
 
 
+@pytest.mark.parametrize("kind", ["compressed", "bf16"])
+def test_layers_of_one_table_are_cut_together(kind):
+    """Two layers over one PageTable: one of them alone is refused and left as it was; both keep what their masses say."""
+    g = _gen(10)
+    H, D, lens = 2, 64, [70, 33, 8]
+    table = exactkv.PageTable(24, 3, 8)
+    cls = exactkv.PagedCompressedKV if kind == "compressed" else exactkv.PagedBF16KV
+    layers = [(cls(table, H, D=D), cls(table, H, D=D)) for _ in range(2)]
+    for n in lens:
+        table.add(n)
+    xs = [[[_rows(g, 1, n, 8, D)[:, :, :H].contiguous() for n in lens] for _ in "kv"] for _ in layers]
+    for pair, rows in zip(layers, xs):
+        for c, r in zip(pair, rows):
+            for s, x in enumerate(r):
+                c.prefill(s, x)
+    mass = [torch.rand(3, H, 128, generator=g, device=DEV) for _ in layers]
+    before = [m.clone() for m in mass]
+    for bad in ((*layers[0], mass[0]), ([layers[0][0]], [layers[0][1]], mass[:1]), ([layers[0][0]] * 2, [p[1] for p in layers], mass),
+                ([p[0] for p in layers], [p[1] for p in layers], mass[:1])):
+        with pytest.raises(ValueError):
+            exactkv.evict(*bad, 20)
+    assert [table.length(s) for s in range(3)] == lens and all(torch.equal(m, b) for m, b in zip(mass, before))
+    index = exactkv.evict([p[0] for p in layers], [p[1] for p in layers], mass, 20, recent=4)
+    assert [table.length(s) for s in range(3)] == [20, 20, 8] and table.free_pages() == 24 - 2 - 2 - 1
+    for pair, rows, at, m, b in zip(layers, xs, index, mass, before):
+        assert torch.equal(at, exactkv.select_tokens(b, 20, lens=torch.tensor(lens, dtype=torch.int32, device=DEV), recent=4)[0])
+        want = [_padded(torch.cat([_padded(_gathered(x, at[s:s + 1, :, : min(20, n)]), 20) for s, (n, x) in enumerate(zip(lens, r))]), 128) for r in rows]
+        table.begin_step()
+        table.truncate(0, 20), table.truncate(1, 20), table.truncate(2, 8)     # (lengths only, for the comparison)
+        n = torch.tensor([20, 20, 8], dtype=torch.int32, device=DEV)
+        q = torch.randn(3, 4, D, generator=g, device=DEV).bfloat16()
+        kw = dict(lens=n, nsplit=1, split_len=128)
+        if kind == "compressed":
+            got = exactkv.attention_compressed(q, *pair, 0, block_table=table.block_table, **kw)
+        else:
+            got = exactkv.attention_reference(q, pair[0].buf, pair[1].buf, 0, block_table=table.block_table, **kw)
+        assert same_bits(got, exactkv.attention_reference(q, *want, 0, **kw))
+        for s, n in enumerate((20, 20, 8)):
+            assert torch.equal(m[s, :, :n], b[s].gather(1, at[s, :, :n].long())) and (s == 2 or (m[s, :, n:] == 0).all())
+
+
+def test_a_step_is_whole_before_an_eviction():
+    table = exactkv.PageTable(8, 2, 4)
+    k, v = exactkv.PagedBF16KV(table, 2, D=64), exactkv.PagedBF16KV(table, 2, D=64)
+    g = _gen(12)
+    table.add(30)
+    for c in (k, v):
+        c.prefill(0, _rows(g, 1, 30, 8, 64)[:, :, :2].contiguous())
+    mass = torch.rand(2, 2, 64, generator=g, device=DEV)
+    table.begin_step()
+    k.append(_rows(g, 1, 2, 64))
+    with pytest.raises(RuntimeError, match="step"):
+        exactkv.evict(k, v, mass, 8)
+    with pytest.raises(ValueError, match="lengths"):
+        exactkv.attention_mass(_rows(g, 1, 4, 64), k, lens=table.lens[:1])
+    v.append(_rows(g, 1, 2, 64))
+    exactkv.evict(k, v, mass, 8)
+    assert table.length(0) == 8
+
+
 # ---------------------------------------------------------------- engines
 
 KEEP = dict(sinks=3, recent=10)
@@ -362,3 +422,15 @@ def test_a_generation_under_a_budget_with_sampling():
         assert eng.dropped + eng.kv[0][0].T == 50 + 149 and torch.isfinite(logits.float()).all()
         out.append((tokens, logits))
     assert torch.equal(out[0][0], out[1][0]) and same_bits(out[0][1], out[1][1])
+
+
+@pytest.mark.parametrize("layer_kernels", [False, True])
+def test_settings_of_their_own_for_each_sequence(layer_kernels):
+    """A Sampler with a setting per sequence draws the prompts' tokens too: a temperature of 0 is the greedy engine's choice."""
+    m = _model("llama")
+    ids = _ids(3, 20)
+    t = torch.tensor([0.0, 1.5, 0.0], device=DEV)
+    eng = exactkv.Engine(m, 3, 48, layer_kernels=layer_kernels)
+    tokens, logits = eng.generate(ids, 12, choose=exactkv.Sampler(t, generator=_gen(3)))
+    greedy = exactkv.Engine(m, 3, 48, layer_kernels=layer_kernels).generate(ids, 12)[0]
+    assert torch.equal(tokens[::2], greedy[::2]) and not torch.equal(tokens[1], greedy[1])

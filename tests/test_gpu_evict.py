@@ -197,6 +197,12 @@ def test_selected_tokens_gathered_in_a_graph():
             assert same_bits(rows, _gathered(x, index))
 
 
+def test_rows_of_no_tokens():
+    for kw in (dict(T=0), dict(lens=torch.zeros(1, dtype=torch.int32, device="cuda"))):
+        index, kept = exactkv.select_tokens(torch.zeros(2, 3, 0, device="cuda"), 4, **kw)
+        assert (index == -1).all() and index.shape == (2, 3, 4) and (kept == 0).all()
+
+
 def test_refusals():
     mass = torch.rand(2, 2, 50, device=DEV)
     for a, kw in (((mass.double(), 5, 50), {}), ((mass[0], 5, 50), {}), ((mass, 0, 50), {}), ((mass, 5, 51), {}), ((mass, 5), {}), ((mass, 5, 50), dict(sinks=6)),
