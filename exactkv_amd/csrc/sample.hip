@@ -42,6 +42,7 @@ struct SampleArgs {
     int pieces, per;
     uint64_t *best, *mass, *list;
     uint32_t *count, *n;
+    struct Ranges* ranges;             // what a row's bins say [B]
 };
 
 // A logit's place in the order of all; -0 as 0. NaN: 0. kMinusInf: the least that can be drawn is above it.
@@ -333,23 +334,94 @@ __device__ inline void take(const SampleArgs& a, int b, const Row& row, uint64_t
     if (a.logprob != nullptr) a.logprob[b] = (float)log((double)row.weight(logit_of(token)) / (double)S);
 }
 
-// The list's n tokens in order: up to 256 by counting, for each, those before it; more by a bitonic sort, whose exchanges
-// within 128 neighbours are one wavefront's own and need no barrier.
+// x of lane ^ D.
+template <int D>
+__device__ inline uint64_t across(uint64_t x) {
+    static_assert(D < 16, "a row of lanes");
+    auto half = [](uint32_t v) -> uint32_t {
+        if constexpr (D == 4) v = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x1B, 0xf, 0xf, true);   // ^ 3, then ^ 7
+        constexpr int CTRL = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x128;
+        return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+    };
+    return (uint64_t)half((uint32_t)(x >> 32)) << 32 | half((uint32_t)x);
+}
+// The lower (or higher) of a pair of lanes' values, D apart.
+template <int D>
+__device__ inline uint64_t one_of_pair(uint64_t x, bool lower) {
+    uint64_t a = x, b;
+    if constexpr (D < 16) {
+        b = across<D>(x);
+    } else {
+        const uint32_t l = (uint32_t)x, h = (uint32_t)(x >> 32);
+        const auto pl = D == 16 ? __builtin_amdgcn_permlane16_swap(l, l, false, false) : __builtin_amdgcn_permlane32_swap(l, l, false, false);
+        const auto ph = D == 16 ? __builtin_amdgcn_permlane16_swap(h, h, false, false) : __builtin_amdgcn_permlane32_swap(h, h, false, false);
+        a = (uint64_t)ph[0] << 32 | pl[0];
+        b = (uint64_t)ph[1] << 32 | pl[1];
+    }
+    return (a < b) == lower ? a : b;
+}
+
+// The list's n tokens in order. Up to 256: by counting, for each, those before it, a quarter of them a thread. Up to 1,024:
+// by a bitonic sort of one token a thread, whose exchanges within a wavefront stay in registers (rows of up to 640:
+// 9.4 us in the last launch, with the sort below 19). More: by the same network over LDS, where those within 128 neighbours are one wavefront's own and need no barrier.
 __device__ inline void sort_list(Shared& s, int n) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (n <= 256) {                                    // uniform
-        const uint64_t x = tid < n ? s.list[tid] : 0;
-        int at = 0;
-        if (tid < n)
+        uint32_t* before = reinterpret_cast<uint32_t*>(s.list + 1024);
+        const int t = tid & 255, part = tid >> 8, per = (n + 3) / 4;
+        const uint64_t x = t < n ? s.list[t] : 0;
+        uint32_t at = 0;
+        const int end = min(n, (part + 1) * per);
+        if (t < n)
 #pragma unroll 8
-            for (int i = 0; i < n; ++i) at += s.list[i] < x;
+            for (int i = part * per; i < end; ++i) at += s.list[i] < x;
+        before[tid] = at;
         __syncthreads();
-        if (tid < n) s.list[at] = x;
+        if (tid < n) s.list[before[tid] + before[tid + 256] + before[tid + 512] + before[tid + 768]] = x;
         __syncthreads();
         return;
     }
-    int size = 512;
+    if (n <= kThreads) {                               // uniform
+        uint64_t x = tid < n ? s.list[tid] : ~0ull;
+        int side = 0;                                  // halves of the list in turn, so that an exchange takes one barrier
+        auto merge = [&](auto size) {
+            constexpr int K = decltype(size)::value;
+            const bool up = (tid & K) == 0;
+            auto far = [&](int d) {
+                side ^= 1024;
+                s.list[side + tid] = x;
+                __syncthreads();
+                const uint64_t y = s.list[side + (tid ^ d)];
+                x = (x < y) == (((tid & d) == 0) == up) ? x : y;
+            };
+            if constexpr (K >= 1024) far(512);
+            if constexpr (K >= 512) far(256);
+            if constexpr (K >= 256) far(128);
+            if constexpr (K >= 128) far(64);
+            if constexpr (K >= 64) x = one_of_pair<32>(x, ((tid & 32) == 0) == up);
+            if constexpr (K >= 32) x = one_of_pair<16>(x, ((tid & 16) == 0) == up);
+            if constexpr (K >= 16) x = one_of_pair<8>(x, ((tid & 8) == 0) == up);
+            if constexpr (K >= 8) x = one_of_pair<4>(x, ((tid & 4) == 0) == up);
+            if constexpr (K >= 4) x = one_of_pair<2>(x, ((tid & 2) == 0) == up);
+            x = one_of_pair<1>(x, ((tid & 1) == 0) == up);
+        };
+        merge(std::integral_constant<int, 2>{});
+        merge(std::integral_constant<int, 4>{});
+        merge(std::integral_constant<int, 8>{});
+        merge(std::integral_constant<int, 16>{});
+        merge(std::integral_constant<int, 32>{});
+        merge(std::integral_constant<int, 64>{});
+        merge(std::integral_constant<int, 128>{});
+        merge(std::integral_constant<int, 256>{});
+        merge(std::integral_constant<int, 512>{});
+        if (n > 512) merge(std::integral_constant<int, 1024>{});   // uniform
+        __syncthreads();
+        s.list[tid] = x;
+        __syncthreads();
+        return;
+    }
+    int size = 2048;
     while (size < n) size <<= 1;
     for (int i = n + tid; i < size; i += kThreads) s.list[i] = ~0ull;
     __syncthreads();
@@ -674,6 +746,7 @@ struct Ranges {
     Range r[3];
     bool cut;                          // top_k cuts
     uint64_t all;                      // the sum of all weights
+    uint64_t best;                     // the row's largest logit
     __device__ bool hold(int bin) const {
         bool in = false;
 #pragma unroll
@@ -829,11 +902,17 @@ __global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
     if (threadIdx.x < kPerOctave) octave[threadIdx.x] = kOctave[threadIdx.x];
     Bins<kBins / kPiece> bins;
     bins.read(a, set, b);
-    const Row row(set, row_largest<kPiece / 64>(a, b, s), octave);
+    const uint64_t best = row_largest<kPiece / 64>(a, b, s);
+    const Row row(set, best, octave);
     if (threadIdx.x == 0) n = 0;
     if (row.odd && piece == 0 && threadIdx.x == 0) a.n[b] = kList + 1;
-    if (row.greedy || row.odd) return;                 // uniform
-    const Ranges ranges = find_ranges<kPiece>(row, bins, mass, count, at, sc, sm);
+    if (row.greedy || row.odd) {                       // uniform
+        if (piece == 0 && threadIdx.x == 0) a.ranges[b].best = best;
+        return;
+    }
+    Ranges ranges = find_ranges<kPiece>(row, bins, mass, count, at, sc, sm);
+    ranges.best = best;
+    if (piece == 0 && threadIdx.x == 0) a.ranges[b] = ranges;
     const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
     const Near near(row, ranges);
     constexpr int N = Logits<TYPE>::N;
@@ -917,20 +996,23 @@ __global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
     const int b = blockIdx.x, tid = threadIdx.x;
     const Settings set(a, b);
     const uint32_t n_all = a.n[b];
+    const Ranges ranges = a.ranges[b];
+    uint64_t early[2];                                 // most rows' tokens, on their way with these
+#pragma unroll
+    for (int i = 0; i < 2; ++i) early[i] = a.list[(int64_t)b * kList + tid + i * kThreads];
     if (tid < kPerOctave) s.octave[tid] = kOctave[tid];
-    Bins<kBins / kThreads> bins;
-    bins.read(a, set, b);
-    const uint64_t best = row_largest<16>(a, b, s.wave_mass);
-    const Row row(set, best, s.octave);
+    const Row row(set, ranges.best, s.octave);
     __syncthreads();
-    if (row.greedy) return take_largest(a, b, row, best);   // uniform
+    if (row.greedy) return take_largest(a, b, row, ranges.best);   // uniform
     if (n_all > (uint32_t)kList) {                     // uniform: an infinite largest logit, or more near ones than the list holds
         sample_row(s, a, MemoryRow<TYPE, kThreads>(a, b, 0, a.V), row, b);
         return;
     }
     const int n = (int)n_all;
-    for (int i = tid; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
-    const Ranges ranges = find_ranges<kThreads>(row, bins, s.mass, s.count, s.at, s.wave_count, s.wave_mass);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (tid + i * kThreads < n) s.list[tid + i * kThreads] = early[i];
+    for (int i = tid + 2 * kThreads; i < n; i += kThreads) s.list[i] = a.list[(int64_t)b * kList + i];
     take_bounds(s, a, row, ranges, n, b);
 }
 
@@ -947,7 +1029,7 @@ constexpr int kShort = 8192;
 
 struct SamplePlan {
     int pieces, per;
-    int64_t best, mass, list, count, n, bytes;         // offsets in the workspace
+    int64_t best, mass, list, ranges, count, n, bytes;   // offsets in the workspace
 };
 static SamplePlan plan_sample(int64_t B, int64_t V) {
     SamplePlan p{};
@@ -962,7 +1044,8 @@ static SamplePlan plan_sample(int64_t B, int64_t V) {
     p.pieces = (int)((V + p.per - 1) / p.per);
     p.mass = B * p.pieces * 8;
     p.list = p.mass + B * kReach * 8;
-    p.count = p.list + B * kList * 8;
+    p.ranges = p.list + B * kList * 8;
+    p.count = p.ranges + B * (int64_t)sizeof(Ranges);
     p.n = p.count + B * kReach * 4;
     p.bytes = p.n + B * 4;
     return p;
@@ -999,7 +1082,7 @@ extern "C" int exkv_sample(const void* logits, int64_t stride, int32_t type, int
     uint8_t* w = (uint8_t*)ws;
     const SampleArgs a{logits, stride, B, V, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, token, logprob,
                        p.pieces, p.per, (uint64_t*)w, (uint64_t*)(w + p.mass), (uint64_t*)(w + p.list), (uint32_t*)(w + p.count),
-                       (uint32_t*)(w + p.n)};
+                       (uint32_t*)(w + p.n), (Ranges*)(w + p.ranges)};
     if (type == kBf16)
         launch_sample<kBf16>(a, stream);
     else if (type == kFp16)

@@ -125,6 +125,26 @@ def test_few_distinct_logits(k):
     _check(x, u, t=0.5, p=0.9, m=0.2, k=k)
 
 
+@pytest.mark.parametrize("V", [5000, 20001])
+@pytest.mark.parametrize("n", [1, 5, 63, 64, 65, 255, 256, 257, 300, 511, 512, 513, 640, 1000, 1023, 1024, 1025, 1500, 2048, 2049, 3000, 4096])
+def test_near_ones_of_every_number(V, n):
+    """n logits so near each other that no bin tells them apart, anywhere in the row and in any order; u and the cuts take
+    places all over them. (Weights within 2^-9 of each other: n <= 2^12 of them leave no sum within 2^-24 of a bound but
+    by chance, which seeds decide for both sides alike.)"""
+    print("[case]", V, n, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x = torch.full((4, V), -9.0, device=DEV)
+    at = torch.stack([torch.randperm(V, generator=g, device=DEV)[:n] for _ in range(4)])
+    near = 2.0 + torch.rand(4, n, generator=g, device=DEV) * 2.0 ** -9
+    near[2:] = (near[2:] * 2.0 ** 14).round() * 2.0 ** -14                    # 32 values: ties
+    x.scatter_(1, at, near)
+    u = torch.tensor([0.03, 0.98, 0.51, 0.7], device=DEV)
+    _check(x, u, m=0.5)
+    _check(x, u, p=0.6, m=0.5)
+    _check(x, u, k=(n + 1) // 2)
+    _check(x, u, k=n, p=0.9)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
 def test_hidden_logits(dtype):
     """Masked tokens at -infinity, the type's lowest value and NaN, most of a row or all but one."""
