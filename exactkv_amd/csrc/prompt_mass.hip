@@ -18,7 +18,7 @@
 //
 // Bound by the exponentials, two for each visible pair: one of 8,192 tokens, 32 query and 8 KV heads of 128, needs
 // 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); rows take 247 us,
-// columns 270 us. Prompts of few rows are bound by the latency of their few stages: 128 rows over 8,192 keys 20 + 6 + 27 us.
+// columns 270 us. Prompts of few rows are bound by the latency of their few stages: 64 queries of 32 heads over 16,385 keys 20 + 6 + 27 us.
 #include "errors.hpp"
 #include "prompt_stage.hpp"
 #include "../../include/exactkv.h"
