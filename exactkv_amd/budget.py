@@ -338,7 +338,10 @@ def _evict_paged(layers, keep, choice, slots):
     slots = table.live_slots() if slots is None else [int(s) for s in slots]
     if len(set(slots)) != len(slots) or any(not 0 <= s < table.max_seqs or table._pages[s] is None for s in slots):
         raise ValueError(f"slots must be distinct and in use (got {slots})")
-    at = torch.tensor(slots, dtype=torch.int64).to(layers[0][2].device)
+    dev = layers[0][2].device
+    if not slots:
+        return [torch.empty(0, k.H, int(keep), dtype=torch.int32, device=dev) for k, _, _ in layers]
+    at = torch.tensor(slots, dtype=torch.int64).to(dev)
     lens = table.lens[at]
     chosen = [select_tokens(mass[at], keep, lens=lens, **choice) for _, _, mass in layers]
     long = [i for i, s in enumerate(slots) if table.length(s) > keep]

@@ -768,18 +768,18 @@ struct Ranges {
     }
 };
 
-// Logits among which are all that the ranges hold (found in fp32, with 2^-20 of the row's reach and of the largest logit to
+// Logits among which are all that the ranges hold (compared in fp32, with 2^-20 of the row's reach and of the largest logit to
 // spare), and few others.
 struct Near {
     float low[3], high[3];
     __device__ __attribute__((always_inline)) Near(const Row& row, const Ranges& ranges) {
-        const float wide = (float)(1.0 / row.per_bin), spare = 0x1p-20f * (fabsf(row.top32) + (float)kReach * wide);
+        const double wide = 1.0 / row.per_bin, spare = 0x1p-20 * (fabs(row.top) + kReach * wide);   // (infinite at t = infinity)
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             const Range& q = ranges.r[i];
             const bool none = q.last < q.first;
-            low[i] = none ? INFINITY : row.top32 - (float)(q.last + 1) * wide - spare;
-            high[i] = none ? -INFINITY : row.top32 - (float)q.first * wide + spare;
+            low[i] = none ? INFINITY : (float)(row.top - (q.last + 1) * wide - spare);
+            high[i] = none ? -INFINITY : q.first == 0 ? row.top32 : (float)(row.top - q.first * wide + spare);
         }
     }
     __device__ bool hold(float l) const {
@@ -1014,6 +1014,7 @@ __global__ void __launch_bounds__(kThreads) sample_take_kernel(SampleArgs a) {
         return;
     }
     const int n = (int)n_all;
+    if (n == 0) return take_largest(a, b, row, ranges.best);   // uniform (the largest is always near itself)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (tid + i * kThreads < n) s.list[tid + i * kThreads] = early[i];

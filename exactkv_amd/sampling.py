@@ -1,7 +1,7 @@
 """The next token of each row of logits, drawn with given random numbers.
 
-No counterpart in the reference, whose engine takes the largest logit (exactkv/engine.py:93-95). The draw is one launch
-on the logits' GPU and its current stream; it waits for nothing, keeps nothing between calls and can be captured in a HIP
+No counterpart in the reference, whose engine takes the largest logit (exactkv/engine.py:93-95). The draw is one
+launch or four on the logits' GPU and its current stream; it waits for nothing, keeps nothing between calls and can be captured in a HIP
 graph (with u, and settings given as tensors, rewritten between replays)."""
 import functools
 

@@ -184,8 +184,10 @@ def test_evict_refusals():
     exactkv.evict(k, v, mass, 4)
     t = exactkv.PageTable(8, 2, 4)
     pk, pv = exactkv.PagedCompressedKV(t, 2, D=64), exactkv.PagedCompressedKV(t, 2, D=64)
-    t.add(5)
     m = torch.zeros(2, 2, 64, device=DEV)
+    assert exactkv.evict(pk, pv, m, 2).shape == (0, 2, 2)                      # no sequence yet
+    t.add(5)
+    assert exactkv.evict(pk, pv, m, 2, slots=[]).shape == (0, 2, 2) and t.length(0) == 5
     for slots in ([1], [0, 0], [-1], [2]):
         with pytest.raises(ValueError):
             exactkv.evict(pk, pv, m, 2, slots=slots)

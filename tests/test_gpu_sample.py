@@ -187,6 +187,27 @@ def test_far_logits_and_temperatures():
     _check(x + 1e5, u, p=0.8)
 
 
+@pytest.mark.parametrize("V", [5003, 20011])
+def test_far_logits_and_temperatures_of_every_path(V):
+    """Temperatures from fp32's least to infinity, logits up to its ends, one row's largest infinite."""
+    x, u = _logits(3, V, 15, torch.float32)
+    for t in (1e-45, 1e-30, 1e-6, 1e6, 1e30, 3e38, math.inf):
+        _check(x, u, t=t)
+        _check(x, u, t=t, p=0.7)
+        _check(x, u, t=t, k=700, p=0.9)
+    for y in (x * 1e4, x * 1e-5, x + 1e5, x * 1e-38, x * 1e37):
+        _check(y, u, p=0.9)
+        _check(y, u, k=900)
+        _check(y, u, t=1e37, p=0.6, k=3000)
+    x[0, [5, 77, V - 1]] = math.inf
+    x[1] = 3e38
+    x[1, 9] = -3e38
+    _check(x, u)
+    _check(x, u, k=2)
+    _check(x, u, t=0.0)
+    _check(x, u, t=1e38, p=0.5)
+
+
 def test_nothing_to_draw():
     x, u = _logits(3, 999, 14)
     x[1] = -math.inf
