@@ -41,7 +41,7 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob
 
     and the token is the first one with which the running sum of the weights passes u times their sum: u = 0 is the likeliest one.
     A temperature of 0 gives the largest logit (the first of equal ones) whatever u is. Each setting is a number, or a
-    tensor with one entry per row (fp32; top_k int32). Returns int64 [B], and with logprob=True also fp32 [B], the
+    tensor with one entry per row (fp32; top_k int32), where values outside a range count as its nearest one. Returns int64 [B], and with logprob=True also fp32 [B], the
     logarithm of the probability with which each token was drawn.
 
     The same inputs give the same tokens: weights are fp64 and added up as whole multiples of 2^-43. NaN and -infinity

@@ -218,6 +218,36 @@ def test_nothing_to_draw():
     assert kernels.error_bits(clear=True) == 0x400 and "logit" in _lib.describe_errors(0x400)
 
 
+@pytest.mark.parametrize("V", [999, 9000])
+def test_entries_out_of_range(V):
+    """Settings given as tensors, and u, beyond their ranges count as the nearest value in them; NaN draws some token."""
+    x, u = _logits(6, V, 16)
+
+    def row(v, dtype=torch.float32):
+        return torch.full((6,), v, device=DEV, dtype=dtype)
+    for bad, ok in ((dict(temperature=row(-1.0)), dict(temperature=0.0)), (dict(temperature=row(-math.inf)), dict(temperature=0.0)),
+                    (dict(top_k=row(-3, torch.int32)), {}), (dict(top_p=row(1.5)), {}), (dict(top_p=row(-0.5)), dict(top_p=0.0)),
+                    (dict(min_p=row(-1.0)), {}), (dict(min_p=row(7.0)), dict(min_p=1.0))):
+        got, want = (exactkv.sample(x, u, logprob=True, **kw) for kw in (bad, ok))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for name in ("temperature", "top_p", "min_p"):
+        got = exactkv.sample(x, u, **{name: row(math.nan)})
+        assert ((got >= 0) & (got < V)).all()
+    for v, w in ((-1.0, 0.0), (2.0, 1 - 2.0 ** -24), (math.inf, 1 - 2.0 ** -24)):
+        assert torch.equal(exactkv.sample(x, row(v)), exactkv.sample(x, row(w)))
+
+
+@pytest.mark.parametrize("V", [8192, 8193, 70000])
+def test_rows_with_nothing_to_draw_among_others(V):
+    x, u = _logits(4, V, 17)
+    x[1] = -math.inf
+    x[2] = math.nan
+    token, lp = exactkv.sample(x, u, logprob=True)
+    assert kernels.error_bits(clear=True) == 0x400
+    assert token[1:3].tolist() == [0, 0] and torch.isneginf(lp[1:3]).all()
+    _check(x[::3], u[::3].contiguous())
+
+
 def test_u_out_of_range_is_clamped():
     x, _ = _logits(4, 2000, 15)
     x[:] = x[0]
