@@ -265,34 +265,32 @@ struct MemoryRow {
             }
         }
     }
-    // f(piece, index of its first logit): two at a time, the next two on their way; the code of f stands here three times
-    template <class F>
+    // f(piece, index of its first logit): U at a time, the next U on their way; the code of f stands here U + 1 times
+    template <int U = 2, class F>
     __device__ void pieces(F f) const {
         int j = from + (int)threadIdx.x * N;
-        uint32_t x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+        uint32_t x[U][4] = {};
         auto ahead = [&](int at) {
-            if (at + STEP + N <= to) {
-                __builtin_memcpy(x, p + (int64_t)at * SIZE, 16);
-                __builtin_memcpy(y, p + (int64_t)(at + STEP) * SIZE, 16);
-            }
+            if (at + (U - 1) * STEP + N <= to)
+#pragma unroll
+                for (int i = 0; i < U; ++i) __builtin_memcpy(x[i], p + (int64_t)(at + i * STEP) * SIZE, 16);
         };
         ahead(j);
 #pragma unroll 1
-        for (; j + STEP + N <= to; j += 2 * STEP) {
-            uint32_t u[4], v[4];
+        for (; j + (U - 1) * STEP + N <= to; j += U * STEP) {
+            uint32_t u[U][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                u[i] = x[i];
-                v[i] = y[i];
-            }
-            ahead(j + 2 * STEP);
-            f(u, j);
-            f(v, j + STEP);
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) u[i][d] = x[i][d];
+            ahead(j + U * STEP);
+#pragma unroll
+            for (int i = 0; i < U; ++i) f(u[i], j + i * STEP);
         }
 #pragma unroll 1
         for (; j < to; j += STEP) {
-            load(j, x);
-            f(x, j);
+            load(j, x[0]);
+            f(x[0], j);
         }
     }
     // f(logit, index): less code
@@ -311,7 +309,7 @@ struct MemoryRow {
     __device__ uint64_t largest() const {
         float top = -INFINITY;
         int at = -1;
-        pieces([&](const uint32_t (&x)[4], int j) {
+        pieces<4>([&](const uint32_t (&x)[4], int j) {
             float m = Logits<TYPE>::at(x, 0);
 #pragma unroll
             for (int e = 1; e < N; ++e) m = fmaxf(m, Logits<TYPE>::at(x, e));
@@ -771,7 +769,8 @@ struct Ranges {
 // Logits among which are all that the ranges hold (compared in fp32, with 2^-20 of the row's reach and of the largest logit to
 // spare), and few others.
 struct Near {
-    float low[3], high[3];
+    float low[3], high[3], one_low, one_high;
+    int ranges = 0;
     __device__ __attribute__((always_inline)) Near(const Row& row, const Ranges& ranges) {
         const double wide = 1.0 / row.per_bin, spare = 0x1p-20 * (fabs(row.top) + kReach * wide);   // (infinite at t = infinity)
 #pragma unroll
@@ -780,8 +779,12 @@ struct Near {
             const bool none = q.last < q.first;
             low[i] = none ? INFINITY : (float)(row.top - (q.last + 1) * wide - spare);
             high[i] = none ? -INFINITY : q.first == 0 ? row.top32 : (float)(row.top - q.first * wide + spare);
+            this->ranges += !none;
         }
+        one_low = fminf(low[0], fminf(low[1], low[2]));
+        one_high = fmaxf(high[0], fmaxf(high[1], high[2]));
     }
+    __device__ bool single() const { return ranges == 1; }
     __device__ bool hold(float l) const {
         return (l >= low[0] && l <= high[0]) | (l >= low[1] && l <= high[1]) | (l >= low[2] && l <= high[2]);
     }
@@ -921,20 +924,27 @@ __global__ void __launch_bounds__(kPiece) sample_collect_kernel(SampleArgs a) {
     const MemoryRow<TYPE, kPiece> r(a, b, from, min(from + a.per, a.V));
     const Near near(row, ranges);
     constexpr int N = Logits<TYPE>::N;
-    r.pieces([&](const uint32_t (&x)[4], int j) {
-        uint32_t found = 0;
+    auto collect = [&](auto hold) {
+        r.pieces([&](const uint32_t (&x)[4], int j) {
+            uint32_t found = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) found |= (uint32_t)near.hold(Logits<TYPE>::at(x, e)) << e;
-        while (found != 0) {
-            const int at = j + __builtin_ctz(found);
-            found &= found - 1;
-            const float l = r.one(at);
-            const double y = row.place(l);
-            if (!(y <= row.limit) || !ranges.hold(whole_of(y))) continue;
-            const uint32_t i = atomicAdd(&n, 1u);
-            if (i < (uint32_t)kLocal) list[i] = token_of(l, at);
-        }
-    });
+            for (int e = 0; e < N; ++e) found |= (uint32_t)hold(Logits<TYPE>::at(x, e)) << e;
+            while (found != 0) {
+                const int at = j + __builtin_ctz(found);
+                found &= found - 1;
+                const float l = r.one(at);
+                const double y = row.place(l);
+                if (!(y <= row.limit) || !ranges.hold(whole_of(y))) continue;
+                const uint32_t i = atomicAdd(&n, 1u);
+                if (i < (uint32_t)kLocal) list[i] = token_of(l, at);
+            }
+        });
+    };
+    // rows with one range, which most settings have, look at no more
+    if (near.single())                                 // uniform
+        collect([&](float l) { return l >= near.one_low && l <= near.one_high; });
+    else
+        collect([&](float l) { return near.hold(l); });
     __syncthreads();
     if (n == 0) return;                                // uniform
     if (threadIdx.x == 0) base = atomicAdd(&a.n[b], n <= (uint32_t)kLocal ? n : (uint32_t)kList + 1);
