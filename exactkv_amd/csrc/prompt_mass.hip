@@ -18,7 +18,8 @@
 //
 // Bound by the exponentials, two for each visible pair: one of 8,192 tokens, 32 query and 8 KV heads of 128, needs
 // 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); rows take 247 us,
-// columns 270 us. Prompts of few rows are bound by the latency of their few stages: 64 queries of 32 heads over 16,385 keys 20 + 6 + 27 us.
+// columns 285 us. Prompts of few rows are bound by the latency of their few stages: 64 queries of 32 heads over 16,385 keys
+// 19 + 6 + 27 us (four stages in LDS instead of two do not shorten them: 19.6, and 8,192 tokens' rows take 267).
 #include "errors.hpp"
 #include "prompt_stage.hpp"
 #include "../../include/exactkv.h"
@@ -27,7 +28,6 @@ namespace exkv {
 
 constexpr float kLowest = -3.402823466e38f;   // a maximum before any key
 constexpr float kFar = 0x1p24f;        // log2 units from which on scores are told apart before they are scaled
-constexpr float kNearby = 0x1p10f;     // log2 units up to which a sum goes into the exponent
 constexpr float kMost = 0x1p100f;      // a row's sum relative to its first tile's maximum
 constexpr int kTile = 256;             // rows, or keys, of a workgroup: 64 a wavefront
 
@@ -40,15 +40,14 @@ struct PromptMassArgs {
     int row_parts, col_parts;
     float2* part;                      // [row tiles, Hkv, row_parts, kTile]: m, sum
     float2* row;                       // [Hq, N]: m, 1 / sum; infinity and 0 where the row sees no key
-    float* lse;                        // [Hq, N]: M + log2 of the sum
     float* sums;                       // [col_parts, Hkv, NK]; out where there is one part
     float* out;                        // [Hkv, NK]
 };
 
-// A row's weights are 2^((s - m) scale) over their sum, m one of its scores: as s scale - M with M = m scale rounded, in one
-// instruction; where M's rounding would be a bit of the exponent, from s - m. Both passes make them alike, so that a row's
-// add up to 1 however far from 0 its scores lie. Near 0 the second pass takes s scale - lse instead, with an addition a key
-// less (8,192 tokens 532 us for 550): the rounding of lse moves a row's weights by 2^-15 at most.
+// A row's weights are 2^((s - m) scale) over their sum, m one of its scores. Both passes make them alike, so that a
+// row's add up to 1 however far from 0 its scores lie: as s scale - M with M = m scale rounded, in one instruction;
+// where M's rounding would be a bit of the exponent, from s - m. (With the sum's logarithm in the exponent too, the second
+// pass adds where it now multiplies and adds: 8,192 tokens 512 to 532 us for 526 to 545, but five times the error, 2.7e-7.)
 __device__ inline float scaled(float m, float scale) {
 #pragma clang fp contract(off)
     return m * scale;
@@ -61,13 +60,6 @@ __device__ inline float weight_of(float s, float m, float scale) {
 __device__ inline float rescale(float m, float to, float scale) {
     const float a = scaled(m, scale), b = scaled(to, scale);
     return exp2_fast(fabsf(a) > kFar || fabsf(b) > kFar ? (m - to) * scale : a - b);
-}
-
-__device__ inline void put_row(const PromptMassArgs& a, int hq, int token, float m, float sum) {
-    const int64_t at = (int64_t)hq * a.N + token;
-    const bool none = sum == 0.f;
-    a.row[at] = none ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / sum);
-    a.lse[at] = none ? INFINITY : scaled(m, a.qk_scale) + __builtin_amdgcn_logf(sum);
 }
 
 // Sequence s's queries that count, and its keys.
@@ -349,7 +341,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         if (a.row_parts > 1)
             a.part[(((int64_t)index * a.Hkv + hk) * a.row_parts + part) * kTile + 64 * w + 32 * rb + col] = make_float2(top, sum);
         else
-            put_row(a, hq[rb], tile.q0 + tok[rb], top, sum);
+            a.row[(int64_t)hq[rb] * a.N + tile.q0 + tok[rb]] = sum == 0.f ? make_float2(INFINITY, 0.f) : make_float2(top, 1.f / sum);
     }
 }
 
@@ -381,7 +373,7 @@ __global__ void __launch_bounds__(4 * kTile) mass_rows_join_kernel(PromptMassArg
         l = l * rescale(m, top, a.qk_scale) + x.y * rescale(x.x, top, a.qk_scale);
         m = top;
     }
-    put_row(a, hk * a.G + row % a.G, tile.q0 + row / a.G, m, l);
+    a.row[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / l);
 }
 
 // Entries of keys that no sequence holds, from key `end` on: 0, shared by all workgroups.
@@ -430,16 +422,15 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     PromptTile rows = tile;
     rows.k0 = tile.q0;
     rows.Lk = tile.Lq;
-    auto walk = [&](auto safe) {                       // the largest |lse| of the rows
+    auto walk = [&](auto safe) {                       // the largest M of the rows
         constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[kb][i] = 0.f;
         int g = tiles > 0 ? (int)(begin / tiles) : 0, t = tiles > 0 ? (int)(begin % tiles) : 0;
-        typedef std::conditional_t<SAFE, float2, float> Sum;   // m and 1 / sum, or M + log2 of the sum
-        Sum row[SB], next_row[SB];
-        float far = 0.f;                                   // the largest |lse| so far
+        float2 row[SB], next_row[SB];                      // m, 1 / sum
+        float far = 0.f;                                   // the largest M so far
         int gl = g, tl = t;                                // of the loads
         auto load = [&](int st) {
             Stream<D, SR> s(a.q, a.sq_t, (hk * G + gl) * a.sq_h, rows, (first + tl) * SR);
@@ -447,11 +438,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
             for (int rb = 0; rb < SB; ++rb) {
                 const int tok = (first + tl) * SR + 32 * rb + col;
-                const int64_t at = (int64_t)(hk * G + gl) * a.N + tile.q0 + tok;
-                if constexpr (SAFE)
-                    next_row[rb] = tok < tile.Lq ? a.row[at] : make_float2(INFINITY, 0.f);
-                else
-                    next_row[rb] = tok < tile.Lq ? a.lse[at] : INFINITY;
+                next_row[rb] = tok < tile.Lq ? a.row[(int64_t)(hk * G + gl) * a.N + tile.q0 + tok] : make_float2(INFINITY, 0.f);
             }
             if (++tl == tiles) {
                 tl = 0;
@@ -460,7 +447,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         };
         auto take = [&](int rb) {                          // the rows of the stage that has landed
             row[rb] = next_row[rb];
-            if constexpr (!SAFE) far = fmaxf(far, fabsf(row[rb]) < INFINITY ? fabsf(row[rb]) : 0.f);
+            const float M = scaled(row[rb].x, a.qk_scale);
+            far = fmaxf(far, fabsf(M) < INFINITY ? fabsf(M) : 0.f);
+            if (!SAFE) row[rb].x = M;
         };
         // A unit is 32 tokens of a stage and the wavefront's 64 keys, walked as the other pass walks its units.
         constexpr int AHEAD = 2;
@@ -486,15 +475,15 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             return x;
         };
         // this unit's weights, of tokens standing at p0 on, and the next one's scores: where all of them see every key, and otherwise
-        auto full_step = [&](float lse, f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int rb) {
+        auto full_step = [&](float2 row, f32x16 (&cur)[2], f32x16 (&nxt)[2], int st, int rb) {
             products(st, rb, nxt, [&](auto s) {
 #pragma unroll
                 for (int e = 32 * s.value / KS; e < 32 * (s.value + 1) / KS; ++e) {
-                    acc[e >> 4][e & 15] = here(acc[e >> 4][e & 15] + exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -lse)));
+                    acc[e >> 4][e & 15] = here(fmaf(exp2_fast(fmaf(cur[e >> 4][e & 15], a.qk_scale, -row.x)), row.y, acc[e >> 4][e & 15]));
                 }
             });
         };
-        auto part_step = [&](int p0, Sum row, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
+        auto part_step = [&](int p0, float2 row, f32x16 (&cur)[2], f32x16 (&nxt)[2], bool more, int st, int rb) {
             if (more) products(st, rb, nxt, [](auto) {});
             if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
 #pragma unroll
@@ -502,13 +491,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                 const int rel = p0 + col - wkey0 - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float x;
-                    if constexpr (SAFE)
-                        x = weight_of(cur[kb][i], row.x, a.qk_scale) * row.y;
-                    else
-                        x = exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row));
-                    // (after the exponential: a row's sum may be NaN)
-                    acc[kb][i] += (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) < span ? x : 0.f;
+                    const float x = SAFE ? weight_of(cur[kb][i], row.x, a.qk_scale) : exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row.x));
+                    // (after the product: a row's sum may be NaN)
+                    acc[kb][i] += (uint32_t)(rel - (kb * 32 + 8 * (i >> 2) + (i & 3))) < span ? x * row.y : 0.f;
                 }
             }
         };
@@ -524,7 +509,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             for (int rb = 0; rb < SB; ++rb) take(rb);
             if (count > 1) load(1);
             f32x16 s0[2], s1[2];
-            if constexpr (SAFE) {                          // far ones, seldom: unit by unit
+            if constexpr (SAFE) {                          // seldom: unit by unit
 #pragma unroll 1
                 for (int it = 0; it < count; ++it) {
                     if (it > 0) {
@@ -543,7 +528,6 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                 }
                 return far;
             }
-            if constexpr (!SAFE) {
             if (wave_on) products(0, 0, s0, [](auto) {});
             auto advance = [&] {
                 if (++t == tiles) t = 0;
@@ -554,7 +538,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                 if constexpr (SB == 2)
                     if (wave_on) part_step(p0, row[0], cur, nxt, true, st, 1);
                 const bool more = it + 1 < count;
-                const Sum last_row = row[SB - 1];
+                const float2 last_row = row[SB - 1];
                 if (more) {
                     next_stage();
 #pragma unroll
@@ -572,7 +556,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             auto full_stage = [&](int it, auto parity, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
                 constexpr int st = decltype(parity)::value;
                 if constexpr (SB == 2) full_step(row[0], cur, nxt, st, 1);
-                const Sum last_row = row[SB - 1];
+                const float2 last_row = row[SB - 1];
                 next_stage();
 #pragma unroll
                 for (int rb = 0; rb < SB; ++rb) take(rb);
@@ -606,11 +590,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                 else
                     part_stage(it + 1, odd, s1, s0);
             }
-            }
         }
         return far;
     };
-    if (__syncthreads_or(walk(std::false_type{}) > kNearby)) walk(std::true_type{});
+    if (__syncthreads_or(walk(std::false_type{}) > kFar)) walk(std::true_type{});
     if (!wave_on) return;
     // over the 32 lanes of a key: halving the values with the lanes, so that lane c of a half ends up with value
     // c >> 1 of a block, which is key 8 (c >> 3) + 4 half + (c >> 1 & 3)
@@ -675,7 +658,7 @@ static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t 
     const int64_t most = last > 0 && last < N ? last : N, seen = window > 0 && window + kTile < most ? window + kTile : most;
     p.col_parts = cut(p.col_tiles * Hkv, (seen + SR - 1) / SR * G);
     p.part_bytes = p.row_parts > 1 ? p.row_tiles * Hkv * p.row_parts * kTile * 8 : 0;
-    p.row_bytes = (Hq * N * 12 + 15) / 16 * 16;
+    p.row_bytes = (Hq * N * 8 + 15) / 16 * 16;
     p.sum_bytes = p.col_parts > 1 ? (p.col_parts * Hkv * NK * 4 + 15) / 16 * 16 : 0;
     return p;
 }
@@ -730,13 +713,12 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
                      (int64_t)Hq * N <= (int64_t)UINT32_MAX && (int64_t)Hkv * NK <= (int64_t)UINT32_MAX,
                  "prompt_mass: too many rows (N=%d, NK=%d, %d query heads, %d KV heads, S=%d)", N, NK, Hq, Hkv, S);
     PromptMassArgs a{(const uint16_t*)q, (const uint16_t*)k, sq_t, sq_h, sk_t, sk_h, cu_q, cu_k, S, N, NK, Hq, Hkv, (int)G, window, last,
-                     qk_scale, p.row_parts, p.col_parts, nullptr, nullptr, nullptr, nullptr, out};
+                     qk_scale, p.row_parts, p.col_parts, nullptr, nullptr, nullptr, out};
     if (N > 0 && S > 0) {
         const int64_t need = p.part_bytes + p.row_bytes + p.sum_bytes;
         EXKV_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "prompt_mass: workspace of %lld bytes, %lld needed",
                      (long long)ws_bytes, (long long)need);
         a.row = (float2*)ws;
-        a.lse = (float*)(a.row + (int64_t)Hq * N);
         a.sums = p.col_parts > 1 ? (float*)((uint8_t*)ws + p.row_bytes) : out;
         a.part = (float2*)((uint8_t*)ws + p.row_bytes + p.sum_bytes);
         if (D == 64)

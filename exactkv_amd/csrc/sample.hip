@@ -18,8 +18,8 @@
 // formula in 64 bits has them. Weights below 2^-44 (all of a vocabulary of 2^19 add up to less than 2^-25 of the sum) are 0.
 //
 // Rows of up to 8,192 logits take one launch, a workgroup each; longer ones four, cut into pieces: largest, bins, collected,
-// taken. 256 rows of 152,064 bf16 logits (78 MB): 20, 33, 29 and 9.5 us, the second bound by its fp64 operations, the first and the
-// third by memory (2.7 to 4 TB/s); 61 of 50,257 fp32 (12 MB): 4.9, 8.1, 12 and 8.7; one of 128,256: 3.7, 4.8, 6.9
+// taken. 256 rows of 152,064 bf16 logits (78 MB): 19, 33, 25 and 9.5 us, the second bound by its fp64 operations, the first and the
+// third by memory (3.1 to 4.1 TB/s); 61 of 50,257 fp32 (12 MB): 4.9, 8.1, 12 and 8.7; one of 128,256: 3.7, 4.7, 6.1
 // and 6.6, each a chain of launches, loads and barriers.
 #include "errors.hpp"
 #include "common.hpp"
