@@ -19,7 +19,7 @@
 // Bound by the exponentials, two for each visible pair: one of 8,192 tokens, 32 query and 8 KV heads of 128, needs
 // 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); rows take 247 us,
 // columns 285 us. Prompts of few rows are bound by the latency of their few stages: 64 queries of 32 heads over 16,385 keys
-// 19 + 6 + 27 us (four stages in LDS instead of two do not shorten them: 19.6, and 8,192 tokens' rows take 267).
+// 19 + 5 + 27 us (four stages in LDS instead of two do not shorten them: 19.6, and 8,192 tokens' rows take 267).
 #include "errors.hpp"
 #include "prompt_stage.hpp"
 #include "../../include/exactkv.h"
@@ -345,34 +345,41 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     }
 }
 
-// The parts of a tile's rows joined: four threads a row, a quarter of the parts each.
-__global__ void __launch_bounds__(4 * kTile) mass_rows_join_kernel(PromptMassArgs a) {
-    __shared__ float2 s[4][kTile];
-    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), index = (int)(blockIdx.x / (unsigned)a.Hkv);
-    const int r = threadIdx.x % kTile, quarter = threadIdx.x / kTile;
+// The parts of 64 of a tile's rows joined: a thread a row and wavefront, with four parts or less each.
+constexpr int kPartsEach = 4;
+__global__ void __launch_bounds__(1024) mass_rows_join_kernel(PromptMassArgs a) {
+    __shared__ float2 s[16][64];
+    constexpr int QUARTERS = kTile / 64;
+    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv), index = rest / QUARTERS;
+    const int r = threadIdx.x % 64, w = threadIdx.x / 64, waves = blockDim.x / 64, at = rest % QUARTERS * 64 + r;
+    const float2* part = a.part + ((int64_t)index * a.Hkv + hk) * a.row_parts * kTile + at;
+    float2 x[kPartsEach];                              // on their way while the tile is found
+#pragma unroll
+    for (int i = 0; i < kPartsEach; ++i)
+        x[i] = w + waves * i < a.row_parts ? part[(int64_t)(w + waves * i) * kTile] : make_float2(kLowest, 0.f);
     PromptTile tile;
     if (!tile_at<true>(a, index, tile)) return;
-    const int row = tile.row0 + r;
+    const int row = tile.row0 + at;
+    const bool real = row < tile.Lq * a.G;             // (behind them parts were not written)
     float m = kLowest, l = 0.f;
-    const float2* part = a.part + ((int64_t)index * a.Hkv + hk) * a.row_parts * kTile + r;
-    if (row < tile.Lq * a.G)
-#pragma unroll 8
-        for (int i = quarter; i < a.row_parts; i += 4) {
-            const float2 x = part[(int64_t)i * kTile];
-            const float top = fmaxf(m, x.x);
-            l = l * rescale(m, top, a.qk_scale) + x.y * rescale(x.x, top, a.qk_scale);
+#pragma unroll
+    for (int i = 0; i < kPartsEach; ++i)
+        if (real) {
+            const float top = fmaxf(m, x[i].x);
+            l = l * rescale(m, top, a.qk_scale) + x[i].y * rescale(x[i].x, top, a.qk_scale);
             m = top;
         }
-    s[quarter][r] = make_float2(m, l);
+    s[w][r] = make_float2(m, l);
     __syncthreads();
-    if (quarter != 0 || row >= tile.Lq * a.G) return;
+    if (w != 0 || !real) return;
+    float2 all[16];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-        const float2 x = s[i][r];
-        const float top = fmaxf(m, x.x);
-        l = l * rescale(m, top, a.qk_scale) + x.y * rescale(x.x, top, a.qk_scale);
-        m = top;
-    }
+    for (int i = 0; i < 16; ++i) all[i] = i < waves ? s[i][r] : make_float2(kLowest, 0.f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, all[i].x);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) l += all[i].y * rescale(all[i].x, m, a.qk_scale);
     a.row[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / l);
 }
 
@@ -651,7 +658,7 @@ static MassPlan plan_mass(int64_t S, int64_t N, int64_t NK, int64_t Hq, int64_t 
     auto cut = [&](int64_t units, int64_t steps) {
         int64_t parts = units > 0 ? 1024 / units : 1;
         if (parts > steps / 4) parts = steps / 4;
-        if (parts > 64) parts = 64;
+        if (parts > 64) parts = 64;                    // (four for each of a workgroup's wavefronts in the rows' join)
         return (int)(parts < 1 ? 1 : parts);
     };
     p.row_parts = cut(p.row_tiles * Hkv, (reach + SR - 1) / SR);
@@ -668,7 +675,8 @@ static void launch_prompt_mass(const PromptMassArgs& a, const MassPlan& p, hipSt
     const dim3 block(64 * kWaves);
     hipLaunchKernelGGL((mass_rows_kernel<D>), dim3((unsigned)(p.row_tiles * a.Hkv * a.row_parts)), block, 0, stream, a);
     if (a.row_parts > 1)
-        hipLaunchKernelGGL(mass_rows_join_kernel, dim3((unsigned)(p.row_tiles * a.Hkv)), dim3(4 * kTile), 0, stream, a);
+        hipLaunchKernelGGL(mass_rows_join_kernel, dim3((unsigned)(p.row_tiles * a.Hkv * (kTile / 64))), dim3(64 * ((a.row_parts + kPartsEach - 1) / kPartsEach)),
+                           0, stream, a);
     hipLaunchKernelGGL((mass_columns_kernel<D>), dim3((unsigned)(p.col_tiles * a.Hkv * a.col_parts)), block, 0, stream, a);
 }
 
@@ -708,7 +716,7 @@ extern "C" int exkv_prompt_mass(const void* q, int64_t sq_t, int64_t sq_h, const
     EXKV_REQUIRE(((int64_t)N + 1) * G < INT32_MAX - 1024 && (int64_t)N + 2 * (int64_t)NK < INT32_MAX - 1024,
                  "prompt_mass: too many rows (N=%d, NK=%d, %d heads per KV head)", N, NK, (int)G);
     const MassPlan p = plan_mass(S, N, NK, Hq, Hkv, D, window, last);
-    EXKV_REQUIRE(p.row_tiles * p.row_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX && p.row_tiles * Hkv * 4 * kTile <= (int64_t)UINT32_MAX &&
+    EXKV_REQUIRE(p.row_tiles * p.row_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX && p.row_tiles * Hkv * (kTile / 64) * 1024 <= (int64_t)UINT32_MAX &&
                      p.col_tiles * p.col_parts * Hkv * 64 * kWaves <= (int64_t)UINT32_MAX &&
                      (int64_t)Hq * N <= (int64_t)UINT32_MAX && (int64_t)Hkv * NK <= (int64_t)UINT32_MAX,
                  "prompt_mass: too many rows (N=%d, NK=%d, %d query heads, %d KV heads, S=%d)", N, NK, Hq, Hkv, S);
