@@ -47,6 +47,12 @@ class PageTable:
         self._rows = None                                       # (slots tensor or None, table, lens) of the step
         self._caches = weakref.WeakSet()                        # over this table's pages
 
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_caches"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _caches=weakref.WeakSet())   # (copied caches enter by themselves)
+
     @property
     def capacity(self):
         return P * self.max_pages
@@ -187,13 +193,25 @@ def _popc16(x):
     return (x + (x >> 8)) & 0x1F
 
 
-class PagedCompressedKV:
+class _OfTable:
+    """A cache over a PageTable's pages, which the table knows of."""
+
+    def _join(self, table):
+        self.table = table
+        table._caches.add(self)
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.table._caches.add(self)
+
+
+class PagedCompressedKV(_OfTable):
     """One layer's keys (or values) for the pages of a PageTable, in the exactkv byte format."""
 
     def __init__(self, table, H, D=128, reserve=0.01):
         assert D in HEAD_DIMS, f"head dim must be one of {HEAD_DIMS} (got {D})"
-        self.table, self.H, self.D = table, H, D
-        table._caches.add(self)
+        self._join(table)
+        self.H, self.D = H, D
         dev = self.dev = table.dev
         NPg = table.num_pages
         self.TS = NPg * P                                      # the pool read as one [1, TS] cache
@@ -387,12 +405,12 @@ class PagedCompressedKV:
         return sum(t.numel() * t.element_size() for t in (self.sm, self.code, self.base, self.rowmask, self.rowoff, self.raw))
 
 
-class PagedBF16KV:
+class PagedBF16KV(_OfTable):
     """Plain bf16 pages [1, 16 * num_pages, H, D] for the same table (the reference twin)."""
 
     def __init__(self, table, H, D=128):
-        self.table, self.H, self.D = table, H, D
-        table._caches.add(self)
+        self._join(table)
+        self.H, self.D = H, D
         self.buf = torch.zeros(1, table.num_pages * P, H, D, dtype=torch.bfloat16, device=table.dev)
         self._appended = 0
         self.cnt = None

@@ -176,3 +176,20 @@ def test_budgets():
     for a in ((0,), (10, 11), (10, 4, 7), (10, -1), (10, 0, -1), (10, 0, 0, -1)):
         with pytest.raises(ValueError):
             exactkv.Budget(*a)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_of_a_page_table_and_its_caches(how):
+    """A table knows the caches over it, the copies' as well, and keeps none of them alive."""
+    import copy
+    import gc
+    import pickle
+    table = exactkv.PageTable(8, 2, 4, device="cpu")
+    k, v = exactkv.PagedBF16KV(table, 2, D=64), exactkv.PagedBF16KV(table, 2, D=64)
+    table.add(20)
+    assert {id(c) for c in table.caches()} == {id(k), id(v)}
+    t2, k2, v2 = copy.deepcopy((table, k, v)) if how == "deepcopy" else pickle.loads(pickle.dumps((table, k, v)))
+    assert k2.table is t2 and {id(c) for c in t2.caches()} == {id(k2), id(v2)} and t2.length(0) == 20 and t2.free_pages() == table.free_pages()
+    del v
+    gc.collect()
+    assert table.caches() == [k]
