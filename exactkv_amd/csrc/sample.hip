@@ -12,10 +12,12 @@
 // tokens of these bins alone are collected, sorted and added up one by one. With top_k up to 2,048 all tokens down to the
 // k-th's bin are collected at once, and no other weight is computed.
 //
-// Weights are fp64, to 2^-51 of each: w = 2^-(i / 32) 2^-(f / 32) with i and f the whole and the rest of y, the second factor
-// a polynomial (fifth degree, through 1 at f = 0), rounded to whole multiples of 2^-43 and added up as whole numbers, so that
-// sums do not depend on the order in which they are taken, and a bin's factor is applied to its sum. Cuts fall where the
-// formula in 64 bits has them. Weights below 2^-44 (all of a vocabulary of 2^19 add up to less than 2^-25 of the sum) are 0.
+// Weights are made in fp64: w = 2^-(i / 32) 2^-(f / 32) with i and f the whole and the rest of y, the second factor a polynomial
+// (fifth degree, through 1 at f = 0, to 2^-51). They are rounded to whole multiples of 2^-43 of the largest and added up as
+// whole numbers, so that sums do not depend on the order in which they are taken; a bin's factor is applied to its sum. A
+// weight in a sum is thus off by up to 2^-44 absolute, and one below 2^-44 is 0: all of a vocabulary of 2^19 together by less
+// than 2^-25 of the sum, so that cuts and draws fall where the formula in 64 bits has them but for bounds nearer to a
+// running sum than that. The log-probability that is returned takes the token's own y, which is not rounded so.
 //
 // Rows of up to 8,192 logits take one launch, a workgroup each; longer ones four, cut into pieces: largest, bins, collected,
 // taken. 256 rows of 152,064 bf16 logits (78 MB): 19, 33, 25 and 9.5 us, the second bound by its fp64 operations, the first and the
@@ -334,7 +336,10 @@ __device__ inline void take_largest(const SampleArgs& a, int b, const Row& row, 
 __device__ inline void take(const SampleArgs& a, int b, const Row& row, uint64_t token, uint64_t S) {
     if (threadIdx.x != 0) return;
     a.token[b] = (int64_t)(uint32_t)token;
-    if (a.logprob != nullptr) a.logprob[b] = (float)log((double)row.weight(logit_of(token)) / (double)S);
+    // log w - log S, w from its place and not as it is added up: of an unlikely token's few multiples of 2^-43 a logarithm
+    // would be off by up to 0.1
+    if (a.logprob != nullptr)
+        a.logprob[b] = (float)(-0.6931471805599453 / kPerOctave * (row.any_place(logit_of(token)) - kBase) - log((double)S / kOne));
 }
 
 // x of lane ^ D.

@@ -44,8 +44,9 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob
     tensor with one entry per row (fp32; top_k int32), where values outside a range count as its nearest one. Returns int64 [B], and with logprob=True also fp32 [B], the
     logarithm of the probability with which each token was drawn.
 
-    The same inputs give the same tokens: weights are fp64 and added up as whole multiples of 2^-43. NaN and -infinity
-    are never drawn; a row of nothing else gives token 0 with log-probability -infinity and sets an error bit
+    The same inputs give the same tokens: weights are made in fp64 and added up as whole multiples of 2^-43 of the largest;
+    smaller ones than half of that are never drawn. A log-probability is off by at most 2^-25 and its own rounding, however
+    unlikely its token. NaN and -infinity are never drawn; a row of nothing else gives token 0 with log-probability -infinity and sets an error bit
     (kernels.check_errors)."""
     dev = logits.get_device()
     if dev >= 0 and dev != _lib.current_device():
