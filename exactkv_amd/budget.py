@@ -280,7 +280,10 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
 
     Sequences of at most `keep` tokens stay as they are. Returns the index that select_tokens gave, a row for each sequence
     (slot); of lists, a list of them. Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is
-    not captured. The next token's position is what the caller counts, not the cache's length."""
+    not captured.
+
+    The next token's position is from then on its place plus what was cut (PageTable.dropped(slot)), and rope_append's tables
+    have to begin at that. A PagedEngine, whose slots stand at their lengths, refuses steps of slots that were cut."""
     many = isinstance(k_cache, (list, tuple))
     layers = list(zip(k_cache, v_cache, mass)) if many else [(k_cache, v_cache, mass)]
     if many and not (len(k_cache) == len(v_cache) == len(mass) > 0):
@@ -350,7 +353,7 @@ def _evict_paged(layers, keep, choice, slots):
         pages = table.block_table[at[rows]]
         tokens = [gather_tokens(k, v, index[rows], block_table=pages) for (k, v, _), (index, _) in zip(layers, chosen)]
         for i in long:
-            table.truncate(slots[i], keep)
+            table.cut(slots[i], keep)
         for (k_cache, v_cache, mass), (_, kept), (k, v) in zip(layers, chosen, tokens):
             for j, i in enumerate(long):
                 k_cache.prefill(slots[i], k[j:j + 1])

@@ -351,8 +351,10 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, *, q_norm=None, k_norm=None
 
     leaves, and the rotated queries [n, Hq, D] for decode_attention, in one launch. q bf16 [n, Hq,
     D], k and v bf16 [n, Hkv, D], not rotated (strided views allowed), one row per sequence, or per
-    slot of the current step (begin_step) for paged caches; the position of each is the number of
-    tokens its cache holds, and cos, sin (fp32 [positions, D / 2]) must reach it. k_cache, v_cache:
+    slot of the current step (begin_step) for paged caches; the row of cos and sin (fp32
+    [positions, D / 2], which must reach it) that turns each is the number of tokens its cache
+    holds. (After an eviction that is its position less the tokens cut: the tables then begin at
+    these, and slots cut by different numbers of tokens are refused.) k_cache, v_cache:
     two different caches of one kind -- CompressedKV, BF16KV, PagedCompressedKV or PagedBF16KV (of
     one PageTable) -- holding the same tokens. check_overflow follows at page ends as after append.
     q_norm, k_norm, eps: as in rotate_prompt. out: a contiguous tensor shaped like q."""
@@ -370,6 +372,8 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, *, q_norm=None, k_norm=None
             raise ValueError("k and v caches belong to two page tables")
         for c in (k_cache, v_cache):
             c._check_append(tuple(k.shape))
+        if t._cut and len({t.dropped(s) for s in t._step_slots}) > 1:
+            raise RuntimeError("the step's slots were cut by different numbers of tokens (evict): no table of angles serves them all")
         last = max((t.length(s) for s in t._step_slots), default=1) - 1
     else:
         if (k_cache.B, k_cache.TS, k_cache.T) != (v_cache.B, v_cache.TS, v_cache.T):

@@ -42,6 +42,7 @@ class PageTable:
         self._free = list(range(num_pages - 1, -1, -1))       # pop() hands out low pages first
         self._pages = [None] * max_seqs                         # pool pages of each live slot
         self._len = [0] * max_seqs
+        self._cut = {}                                          # tokens that evictions took out of a slot, where any
         self.step = 0
         self._step_slots = []
         self._rows = None                                       # (slots tensor or None, table, lens) of the step
@@ -62,6 +63,10 @@ class PageTable:
 
     def length(self, slot):
         return self._len[slot]
+
+    def dropped(self, slot):
+        """How many tokens evictions took out of a slot's sequence: its next token stands that far behind its place."""
+        return self._cut.get(slot, 0)
 
     def pages(self, slot):
         return list(self._pages[slot])
@@ -118,6 +123,7 @@ class PageTable:
         self._free.extend(reversed(self._pages[slot]))
         self._pages[slot] = None
         self._len[slot] = 0
+        self._cut.pop(slot, None)
         self.lens[slot] = 0
         self._rows = None
 
@@ -132,8 +138,17 @@ class PageTable:
         self._free.extend(reversed(self._pages[slot][n:]))
         del self._pages[slot][n:]
         self._len[slot] = T
+        if T == 0:                                              # it starts over
+            self._cut.pop(slot, None)
         self._write([slot], [T], [], [])
         self._rows = None
+
+    def cut(self, slot, T):
+        """truncate() of a sequence that keeps T tokens of its choice (an eviction): the others count as dropped."""
+        gone = self.length(slot) - T
+        self.truncate(slot, T)
+        if gone and T:
+            self._cut[slot] = self.dropped(slot) + gone
 
     def begin_step(self, slots=None):
         """One more token for each slot in `slots` (host ints, all live and distinct; None: every
