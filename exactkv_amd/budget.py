@@ -282,8 +282,8 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
     (slot); of lists, a list of them. Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is
     not captured.
 
-    The next token's position is from then on its place plus what was cut (PageTable.dropped(slot)), and rope_append's tables
-    have to begin at that. A PagedEngine, whose slots stand at their lengths, refuses steps of slots that were cut."""
+    The next token's position is from then on its place plus what was cut (the caches' dropped, PageTable.dropped(slot)), and
+    rope_append's tables have to begin at that. Engines refuse to go on from evictions that they did not make."""
     many = isinstance(k_cache, (list, tuple))
     layers = list(zip(k_cache, v_cache, mass)) if many else [(k_cache, v_cache, mass)]
     if many and not (len(k_cache) == len(v_cache) == len(mass) > 0):
@@ -324,8 +324,10 @@ def _evict_rows(k_cache, v_cache, mass, keep, choice):
     index, kept = select_tokens(mass, keep, T, **choice)
     if T > keep:
         k, v = gather_tokens(k_cache, v_cache, index)
-        k_cache.replace(k)
-        v_cache.replace(v)
+        dropped = k_cache.dropped + T - keep
+        for c, x in ((k_cache, k), (v_cache, v)):
+            c.replace(x)
+            c.dropped = dropped
         mass[..., :keep] = kept
         mass[..., keep:] = 0
     return index

@@ -38,6 +38,8 @@ def _device_words(n, dev):
 
 
 class CompressedKV:
+    dropped = 0                                        # tokens that evictions took out since the last prefill (budget.evict)
+
     def __init__(self, B, TS, H, D, device="cuda", reserve=0.01):
         """B sequences of up to TS tokens (a multiple of 16), H KV heads of dimension D (64,
         128 or 256; the reference stores 128 only, cache.py:21). reserve: escaped-row slots
@@ -136,7 +138,7 @@ class CompressedKV:
         if T > self.TS:
             raise AssertionError(f"{T} prompt tokens do not fit a cache of {self.TS}")
         full = T - T % P
-        self.T = T
+        self.T, self.dropped = T, 0
         if type(b) is int and 0 <= b < self.B and prefill_ready(x, self.sm.device, self.H, self.D):
             used = prefill_pages(x, self, b=b)
             if full and used > self.cap:
@@ -170,7 +172,7 @@ class CompressedKV:
         if x.device != self.sm.device:
             raise ValueError(f"replace expects a tensor on {self.sm.device}")
         full = T - T % P
-        self.T, self._pending = T, None
+        self.T, self.dropped, self._pending = T, 0, None
         self.state[0] = T
         self.cnt.zero_()
         used = 0
@@ -243,6 +245,8 @@ class BF16KV:
     """The uncompressed twin: a plain bf16 [B, TS, H, D] cache (buf) with the same interface;
     its appends are a device-side kernel as well (the position comes from state[0])."""
 
+    dropped = 0                                        # as CompressedKV's
+
     def __init__(self, B, TS, H, D, device="cuda"):
         self.B, self.TS, self.H, self.D = B, TS, H, D
         self.buf = torch.zeros((B, TS, H, D), dtype=torch.bfloat16, device=device)
@@ -253,7 +257,7 @@ class BF16KV:
     def prefill_slot(self, b, x):
         n = x.shape[1]
         self.buf[b].narrow(0, 0, n).copy_(x[0])
-        self.T = n
+        self.T, self.dropped = n, 0
         self.state[0] = n
 
     def replace(self, x):
@@ -264,7 +268,7 @@ class BF16KV:
         if n > self.TS:
             raise AssertionError(f"{n} tokens do not fit a cache of {self.TS}")
         self.buf[:, :n].copy_(x)
-        self.T = n
+        self.T, self.dropped = n, 0
         self.state[0] = n
 
     def append(self, x):

@@ -239,6 +239,7 @@ class Engine:
         if layer_kernels and not ours:
             raise AssertionError("layer kernels append to this package's caches only")
         self.budget, self.dropped, self.mass = budget, 0, None
+        self._prompt_cut = 0                    # of those, the prompts' (the caches count the others)
         if budget is not None:
             if not layer_kernels or any(self.windows):
                 raise AssertionError("a budget needs layer_kernels and no sliding-window layer")
@@ -283,7 +284,8 @@ class Engine:
             hidden = self._layers.prompts(list(ids), list(range(b0, b0 + ids.shape[0])))
             self._graph = None                  # buffers may have grown
             if self.budget is not None:
-                self._drop(ids.shape[1] - self.kv[0][0].T)
+                self._prompt_cut = ids.shape[1] - self.kv[0][0].T
+                self._drop(self._prompt_cut)
             return self._prefill_next(hidden[:, None], choose)
         nxt = []
         with _fused_sdpa():
@@ -408,6 +410,8 @@ class Engine:
     @torch.no_grad()
     def step(self, tok):
         """tok: [B] current tokens. Returns logits [B, vocab] (bf16) for the next token."""
+        if getattr(self.kv[0][0], "dropped", 0) != self.dropped - self._prompt_cut:
+            raise RuntimeError("the caches were cut outside the engine (evict): their places are not the tokens' positions; prefill anew")
         if self.budget is not None:
             self._make_room()
         T = self.kv[0][0].T

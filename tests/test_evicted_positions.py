@@ -86,3 +86,40 @@ def test_evicting_a_paged_engines_caches(layer_kernels):
     eng.release(slots[0])
     assert eng.add(ids[0])[0] == slots[0]
     assert eng.step(ids[:, 1]).shape == (2, 1024)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [exactkv.CompressedKV, exactkv.BF16KV])
+def test_contiguous_caches_count_what_was_cut(cls):
+    k, v = cls(1, 64, 2, 64), cls(1, 64, 2, 64)
+    x = torch.randn(1, 40, 2, 64, device=DEV).bfloat16()
+    for c in (k, v):
+        c.prefill_slot(0, x)
+        assert c.dropped == 0
+    mass = torch.rand(1, 2, 64, device=DEV)
+    exactkv.evict(k, v, mass, 30)
+    assert k.dropped == v.dropped == 10
+    for c in (k, v):
+        c.append(x[:, 0].contiguous())
+    exactkv.evict(k, v, mass, 12)
+    assert k.dropped == v.dropped == 29 and k.T == 12
+    k.replace(x)
+    v.prefill_slot(0, x)
+    assert k.dropped == v.dropped == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget", [None, exactkv.Budget(20, 2, 4)])
+def test_evicting_an_engines_caches_from_outside(budget):
+    """An Engine counts the evictions that it makes itself; of others' it says so, until the next prefill."""
+    m = _model("llama")
+    ids = _ids(2, 60)
+    eng = exactkv.Engine(m, 2, 64, layer_kernels=budget is not None, budget=budget)
+    eng.prefill(ids[:, :40])
+    mass = [torch.rand(2, 2, 64, device=DEV) for _ in eng.kv]
+    exactkv.evict(*zip(*eng.kv), mass, 30)
+    with pytest.raises(RuntimeError, match="cut"):
+        eng.step(ids[:, 40])
+    assert eng.kv[0][0].T == 30
+    eng.prefill(ids[:, :40])
+    assert eng.step(ids[:, 40]).shape == (2, 1024) and eng.kv[0][0].T == 41
