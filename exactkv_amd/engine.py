@@ -22,6 +22,8 @@ MI355X specifics:
   * budget= (with layer_kernels) lets a generation run past the caches: each step adds its attention weights to what the
     cached tokens of each KV head have received, and full caches are cut to those with the most.
 """
+import contextlib
+import gc
 import importlib
 
 import torch
@@ -40,6 +42,22 @@ def _fused_sdpa():
     instead of falling back to the unfused math path)."""
     from torch.nn.attention import SDPBackend, sdpa_kernel
     return sdpa_kernel([SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION])
+
+
+@contextlib.contextmanager
+def _captured(stream):
+    """A HIP graph of what the context launches on `stream`. Garbage is not collected meanwhile: a graph among it (of an
+    engine that went, in a cycle) waits for its GPU as it is destroyed, which a capture forbids, and that ends the
+    process."""
+    collects = gc.isenabled()
+    gc.disable()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            yield graph
+    finally:
+        if collects:
+            gc.enable()
 
 
 _WRITE_THROUGH = None
@@ -434,10 +452,10 @@ class Engine:
                 else:
                     key = self._buffers_key()
                     if self._graph is None or key != self._graph_key:
-                        self._graph = torch.cuda.CUDAGraph()
-                        with torch.cuda.graph(self._graph, stream=self._stream):
+                        self._graph = None
+                        with _captured(self._stream) as graph:
                             self._logits = self._forward(self._tok, device_only=True)
-                        self._graph_key = key
+                        self._graph, self._graph_key = graph, key
                         self.captures += 1
                     self._graph.replay()
                     logits = self._logits.clone()
@@ -596,10 +614,10 @@ class PagedEngine:
                     self._warm.add(n)
                 else:
                     if self._graph is None or key != self._graph_key:
-                        self._graph = torch.cuda.CUDAGraph()
-                        with torch.cuda.graph(self._graph, stream=self._stream):
+                        self._graph = None
+                        with _captured(self._stream) as graph:
                             self._logits = self._forward(self._tok[:n], n)
-                        self._graph_key = key
+                        self._graph, self._graph_key = graph, key
                         self.captures += 1
                     self._graph.replay()
                     logits = self._logits.clone()

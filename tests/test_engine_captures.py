@@ -1,0 +1,75 @@
+"""What must not happen while an engine captures its step: a collection of garbage, which may hold another engine's graph.
+
+No counterpart in the reference, whose steps are not captured (exactkv/engine.py:66-91)."""
+import contextlib
+import gc
+
+import pytest
+import torch
+
+import exactkv_amd as exactkv
+from exactkv_amd import engine as engines
+from tests.conftest import same_bits
+
+
+@pytest.mark.parametrize("collects", [True, False])
+def test_no_collection_in_a_capture(collects, monkeypatch):
+    """Nor is a graph kept that was not captured to its end; the collector is left as it was."""
+    seen = []
+
+    @contextlib.contextmanager
+    def graph(g, stream=None):
+        seen.append((g, stream, gc.isenabled()))
+        yield
+    monkeypatch.setattr(torch.cuda, "graph", graph)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: "graph")
+    was = gc.isenabled()
+    try:
+        (gc.enable if collects else gc.disable)()
+        with engines._captured("stream") as g:
+            assert g == "graph" and not gc.isenabled()
+        assert gc.isenabled() == collects
+        with pytest.raises(ValueError):
+            with engines._captured("stream"):
+                raise ValueError
+        assert gc.isenabled() == collects
+    finally:
+        (gc.enable if was else gc.disable)()
+    assert seen == [("graph", "stream", False)] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("paged", [False, True])
+def test_engines_that_went_while_another_captures(paged):
+    """Engines with captured steps in cycles, nobody's any more, and a collector that runs at every allocation."""
+    from tests.test_gpu_engine_layers import _ids, _model
+    m = _model("llama")
+    ids = _ids(2, 30)
+
+    def run():
+        if paged:
+            eng = exactkv.PagedEngine(m, 2, 64, layer_kernels=True)
+            eng.add_many(list(ids[:, :20]))
+        else:
+            eng = exactkv.Engine(m, 2, 64, layer_kernels=True)
+            eng.prefill(ids[:, :20])
+        out = torch.stack([eng.step(ids[:, t]) for t in range(20, 30)])
+        assert eng.captures == 1
+        return eng, out
+    was = gc.get_threshold()
+    gc.collect()
+    try:
+        gc.disable()
+        want = None
+        for _ in range(3):
+            eng, out = run()
+            eng.itself = eng                           # a cycle: only the collector finds it
+            del eng
+            assert want is None or same_bits(out, want)
+            want = out
+        gc.set_threshold(1)
+        gc.enable()
+        assert same_bits(run()[1], want)
+    finally:
+        gc.set_threshold(*was)
+        gc.enable()
