@@ -25,6 +25,7 @@ MI355X specifics:
 import contextlib
 import gc
 import importlib
+import weakref
 
 import torch
 
@@ -113,7 +114,7 @@ class _LayerKernels:
             raise AssertionError(f"layer kernels take fixed rotary tables (the model's are {kind!r})")
         if next(m.parameters()).dtype != torch.bfloat16:
             raise AssertionError("layer kernels take a bf16 model")
-        self.eng = eng
+        self.eng = weakref.proxy(eng)              # (which holds this: no cycle, so that its caches go with it)
         # the model's own tables, in fp32
         like = torch.zeros(1, dtype=torch.float32, device=eng.dev)
         cos, sin = m.rotary_emb(like, torch.arange(positions, device=eng.dev)[None])

@@ -1,8 +1,9 @@
-"""What must not happen while an engine captures its step: a collection of garbage, which may hold another engine's graph.
+"""Engines that went: their memory, and their graphs while another engine captures its step, where no garbage may be collected.
 
 No counterpart in the reference, whose steps are not captured (exactkv/engine.py:66-91)."""
 import contextlib
 import gc
+import weakref
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ import torch
 import exactkv_amd as exactkv
 from exactkv_amd import engine as engines
 from tests.conftest import same_bits
+from tests.test_engine_host import _tiny
 
 
 @pytest.mark.parametrize("collects", [True, False])
@@ -36,6 +38,23 @@ def test_no_collection_in_a_capture(collects, monkeypatch):
     finally:
         (gc.enable if was else gc.disable)()
     assert seen == [("graph", "stream", False)] * 2
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_an_engine_goes_with_its_last_name(paged):
+    """Its caches are most of a GPU's memory: they wait for no collection."""
+    m = _tiny("llama").bfloat16()
+    if paged:
+        eng = exactkv.PagedEngine(m, 2, 64, backend="bf16", graph=False, layer_kernels=True)
+    else:
+        eng = exactkv.Engine(m, 2, 64, backend="bf16", graph=False, layer_kernels=True)
+    gone = [weakref.ref(eng), weakref.ref(eng.kv[0][0])]
+    gc.disable()
+    try:
+        del eng
+        assert [r() for r in gone] == [None, None]
+    finally:
+        gc.enable()
 
 
 @pytest.mark.gpu
