@@ -278,6 +278,9 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
     Of several layers, give lists of equal length: a cache pair and its mass each. Paged layers share their table's lengths,
     so all caches of a table are cut in one call (ValueError otherwise).
 
+    Everything about the arguments is checked before the first cache changes. An eviction that fails all the same (memory runs
+    out) leaves caches of different lengths behind, which want a new prefill.
+
     Sequences of at most `keep` tokens stay as they are. Returns the index that select_tokens gave, a row for each sequence
     (slot); of lists, a list of them. Compressed caches wait for a raw-row count each (as a prefill does), so an eviction is
     not captured.
@@ -285,6 +288,7 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
     The next token's position is from then on its place plus what was cut (the caches' dropped, PageTable.dropped(slot)), and
     rope_append's tables have to begin at that. Engines refuse to go on from evictions that they did not make."""
     many = isinstance(k_cache, (list, tuple))
+    keep = int(keep)
     layers = list(zip(k_cache, v_cache, mass)) if many else [(k_cache, v_cache, mass)]
     if many and not (len(k_cache) == len(v_cache) == len(mass) > 0):
         raise ValueError(f"{len(k_cache)} key caches, {len(v_cache)} value caches and {len(mass)} masses")
@@ -314,6 +318,11 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
                 raise ValueError("k and v caches differ in shape or in the tokens they hold")
             shape = (k.B, k.H, k.TS)
         _mass_rows(m, shape, dev, "mass")
+        if any((c.buf if _is_bf16(c) else c.raw).get_device() != dev for c in (k, v)):
+            raise ValueError("the caches must be on the mass's GPU")
+    spans = sorted((m.data_ptr(), m.data_ptr() + m.nbytes) for _, _, m in layers)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("each layer needs a mass of its own")
     choice = dict(sinks=sinks, recent=recent)
     kept = _evict_paged(layers, keep, choice, slots) if paged else [_evict_rows(*x, keep, choice) for x in layers]
     return kept if many else kept[0]
@@ -345,7 +354,7 @@ def _evict_paged(layers, keep, choice, slots):
         raise ValueError(f"slots must be distinct and in use (got {slots})")
     dev = layers[0][2].device
     if not slots:
-        return [torch.empty(0, k.H, int(keep), dtype=torch.int32, device=dev) for k, _, _ in layers]
+        return [torch.empty(0, k.H, keep, dtype=torch.int32, device=dev) for k, _, _ in layers]
     at = torch.tensor(slots, dtype=torch.int64).to(dev)
     lens = table.lens[at]
     chosen = [select_tokens(mass[at], keep, lens=lens, **choice) for _, _, mass in layers]

@@ -357,6 +357,8 @@ class Engine:
     def _make_room(self):
         """Full caches cut to the budget before a step."""
         b, T, positions = self.budget, self.kv[0][0].T, self._layers.cos.shape[0]
+        if any(c.T != T or c.dropped != self.dropped - self._prompt_cut for c in self._caches()):
+            raise RuntimeError("the caches were cut unevenly (an eviction that failed halfway): prefill anew")
         if self.dropped + T >= positions:
             raise RuntimeError(f"position {self.dropped + T} is outside the model's {positions}")
         if T < self.TS:
