@@ -287,7 +287,8 @@ class Engine:
         """ids: [B, T] token ids. Returns the greedy next token of each sequence, [B].
         choose (additive): the next tokens [n] from logits [n, vocab] instead (a Sampler).
         b0 (additive): fill sequence slots b0.. with ids' rows, so a long prefill can be
-        done in pieces (slot 0 first).
+        done in pieces (slot 0 first; under a budget a piece of another length than the
+        slots before it is refused, as they then have no common position).
         fused (additive): each layer's RoPE'd keys and values go straight from the
         attention module into the page encoder, read in place through strides ([1, H, T, D]
         as a [1, T, H, D] view), so the model's DynamicCache never holds the prompt's K/V
@@ -300,6 +301,12 @@ class Engine:
             if ids.shape[1] == 0 or b0 + ids.shape[0] > self.B or ids.shape[1] > room:
                 raise AssertionError(f"{ids.shape[0]} prompts of {ids.shape[1]} tokens do not fit slots {b0} to {self.B - 1} "
                                      f"of {room}")
+            held = self.kv[0][0].T
+            if self.budget is not None and b0 > 0 and held + self.dropped > 0:
+                T = ids.shape[1] if ids.shape[1] <= self.TS else self.budget.keep
+                if (T, ids.shape[1] - T) != (held, self.dropped):
+                    raise AssertionError(f"prompts of {ids.shape[1]} tokens beside sequences that stand at position {held + self.dropped} "
+                                         f"with {self.dropped} tokens cut: an engine's sequences have one position (slot 0 comes first)")
             hidden = self._layers.prompts(list(ids), list(range(b0, b0 + ids.shape[0])))
             self._graph = None                  # buffers may have grown
             if self.budget is not None:

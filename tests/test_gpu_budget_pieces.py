@@ -1,4 +1,4 @@
-"""An Engine's budget where its work ends halfway: an eviction that fails.
+"""An Engine's budget where its work comes in pieces or ends halfway: prompts prefilled by b0=, an eviction that fails.
 
 No counterpart in the reference, whose caches end when they are full (exactkv/cache.py:102)."""
 import pytest
@@ -11,6 +11,43 @@ from tests.test_gpu_engine_layers import _ids, _model
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+@pytest.mark.parametrize("first,then", [(100, 140), (140, 100), (30, 100), (100, 30), (40, 30), (64, 65)])
+def test_pieces_of_different_lengths_are_refused(first, then):
+    """All sequences of an Engine stand at one position: a piece of another length is refused, and nothing is written. Of
+    one length, pieces give what one prefill gives."""
+    m = _model("llama")
+    ids = _ids(4, 160)
+    eng = exactkv.Engine(m, 4, 64, layer_kernels=True, budget=exactkv.Budget(30, **KEEP))
+    eng.prefill(ids[:2, :first])
+    before = [(c.T, _held(c, c.T).clone()) for c in eng._caches()]
+    mass, dropped = [x.clone() for x in eng.mass], eng.dropped
+    with pytest.raises(AssertionError, match="position"):
+        eng.prefill(ids[2:, :then], b0=2)
+    assert eng.dropped == dropped and all(torch.equal(a, b) for a, b in zip(mass, eng.mass))
+    assert all(c.T == T and same_bits(_held(c, T), x) for c, (T, x) in zip(eng._caches(), before))
+    eng.prefill(ids[2:, :first], b0=2)
+    whole = exactkv.Engine(m, 4, 64, layer_kernels=True, budget=exactkv.Budget(30, **KEEP))
+    whole.prefill(ids[:, :first])
+    rows = [c.T for c in eng._caches()]
+    assert eng.dropped == whole.dropped and rows == [c.T for c in whole._caches()]
+    for a, b in zip(eng._caches(), whole._caches()):
+        assert same_bits(_held(a, a.T), _held(b, b.T))
+    eng.prefill(ids[:2, :then])                                                # slot 0 starts over
+    eng.prefill(ids[2:, :then], b0=2)
+    assert eng.dropped + eng.kv[0][0].T == then
+
+
+def test_a_piece_after_steps_is_refused():
+    m = _model("llama")
+    ids = _ids(3, 100)
+    eng = exactkv.Engine(m, 3, 64, layer_kernels=True, budget=exactkv.Budget(30, **KEEP))
+    eng.prefill(ids[:, :40])
+    _run(eng, ids[:, :80], 40)                                                 # over an eviction
+    for n in (40, 80, eng.kv[0][0].T):
+        with pytest.raises(AssertionError, match="position"):
+            eng.prefill(ids[2:, :n], b0=2)
 
 
 @pytest.mark.parametrize("fails_at", [1, 2, 3])
