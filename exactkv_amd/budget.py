@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .cache import BF16KV, CompressedKV
-from .kernels import _QK_SCALE, P, _block_table_arg, _cache_args, _cache_dim, _check_q, _lens_arg, _window_arg
+from .kernels import _QK_SCALE, P, _block_table_arg, _cache_args, _cache_dim, _check_q, _lens_arg, _window_arg, read_words
 from .layer import _check_heads, _offsets, _on, _rows
 from .paged import PagedBF16KV, PagedCompressedKV
 
@@ -272,8 +272,8 @@ def evict(k_cache, v_cache, mass, keep, *, sinks=0, recent=0, slots=None):
 
       * contiguous ones: mass fp32 [B, H, TS]; the cache's token count becomes keep;
       * paged ones of one PageTable: mass fp32 [max_seqs, H, capacity], a row for each slot; slots (host ints, default all
-        live ones) are cut, the pages behind go back to the pool (raw rows stay until compact()), and begin_step comes
-        before the next step.
+        live ones) are cut, the pages behind go back to the pool (raw rows of evicted tokens stay in theirs until an eviction
+        finds it more than half full, or compact()), and begin_step comes before the next step.
 
     Of several layers, give lists of equal length: a cache pair and its mass each. Paged layers share their table's lengths,
     so all caches of a table are cut in one call (ValueError otherwise).
@@ -342,6 +342,17 @@ def _evict_rows(k_cache, v_cache, mass, keep, choice):
     return index
 
 
+def _drop_raw_rows(caches, cut):
+    """The raw rows of `cut` slots, which are about to be encoded again, out of pools that are more than half full: what
+    earlier evictions left in them goes as well, so that a pool grows by what its sequences hold alone."""
+    if not isinstance(caches[0], PagedCompressedKV):
+        return
+    others = [s for s in caches[0].table.live_slots() if s not in cut]
+    for c, rows in zip(caches, read_words([c.cnt for c in caches])):
+        if 2 * rows > c.cap:
+            c._pack(others)
+
+
 def _evict_paged(layers, keep, choice, slots):
     table = layers[0][0].table
     caches = {id(c) for k, v, _ in layers for c in (k, v)}
@@ -365,6 +376,7 @@ def _evict_paged(layers, keep, choice, slots):
         tokens = [gather_tokens(k, v, index[rows], block_table=pages) for (k, v, _), (index, _) in zip(layers, chosen)]
         for i in long:
             table.cut(slots[i], keep)
+        _drop_raw_rows([c for k, v, _ in layers for c in (k, v)], {slots[i] for i in long})
         for (k_cache, v_cache, mass), (_, kept), (k, v) in zip(layers, chosen, tokens):
             for j, i in enumerate(long):
                 k_cache.prefill(slots[i], k[j:j + 1])

@@ -20,7 +20,7 @@ PageTable holds the allocation, shared by every layer's K and V caches:
 PagedCompressedKV / PagedBF16KV hold one layer's keys (or values) for the table's pool.
 A sequence's newest, partly filled page lives in its tail area at the end of the raw pool
 (all rows raw), as in CompressedKV. Raw rows of released sequences stay in the pool until
-compact().
+compact(), those of evicted tokens until then or an eviction that finds the pool half full.
 """
 import weakref
 
@@ -391,8 +391,12 @@ class PagedCompressedKV(_OfTable):
         (page, head) order; returns the rows freed. Host-synchronising; not for a graph."""
         if self._pending is not None:
             raise RuntimeError("call check_overflow() before compact()")
+        return self._pack(self.table.live_slots())
+
+    def _pack(self, slots):
+        """compact(), of these slots' pages: the others' are encoded again before they are read."""
         t = self.table
-        live = sorted(p for s in t.live_slots() for p in t._pages[s][: t.length(s) // P])
+        live = sorted(p for s in slots for p in t._pages[s][: t.length(s) // P])
         old = int(self.cnt.item())
         if not live:
             self.cnt.zero_()
