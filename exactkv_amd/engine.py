@@ -532,7 +532,7 @@ class PagedEngine:
         """Prefill several prompts (1-D token ids of any lengths) into new sequence slots, packed:
         one pass over the model's layers for about 16K tokens of them. Returns (slots, the greedy
         next tokens [len(prompts)], or those that choose takes from their logits, e.g. a Sampler). Where a prompt does not
-        fit, or the model refuses one, none is added."""
+        fit, the model refuses one or choose fails, none is added."""
         if self._layers is None:
             self._layers = _LayerKernels(self, self._positions)
         prompts = list(prompts)
@@ -542,12 +542,11 @@ class PagedEngine:
         try:
             for p in prompts:
                 slots.append(self.table.add(int(p.numel())))
-            hidden = self._layers.prompts(prompts, slots)
-        except Exception:                       # no room, or no prompts the model takes
+            return slots, self._next(self._layers.prompts(prompts, slots), choose)
+        except Exception:                       # no room, no prompts the model takes, or a choice that fails
             for s in slots:
                 self.table.release(s)
             raise
-        return slots, self._next(hidden, choose)
 
     def _next(self, hidden, choose):
         """The next tokens from the prompts' last hidden states [n, C]."""
@@ -557,21 +556,22 @@ class PagedEngine:
     @torch.no_grad()
     def add(self, ids, slot=None, choose=None):
         """Prefill one prompt (1-D token ids) into a new sequence slot. Returns (slot, the
-        greedy next token, or the one that choose takes from logits [1, vocab])."""
-        if self._own_layers:
-            if ids.numel() == 0:
-                raise ValueError("a prompt of no tokens")
-            s = self.table.add(int(ids.numel()), slot)
-            try:
-                hidden = self._layers.prompts([ids.view(-1)], [s])
-            except Exception:
-                self.table.release(s)
-                raise
-            return s, self._next(hidden, choose)[0]
+        greedy next token, or the one that choose takes from logits [1, vocab]). Where one of
+        these fails, none is added."""
+        if self._own_layers and ids.numel() == 0:
+            raise ValueError("a prompt of no tokens")
         s = self.table.add(int(ids.numel()), slot)
-        with _fused_sdpa():
-            out = self.m.model(ids.view(1, -1), use_cache=True, past_key_values=_write_through(self, s))
-        return s, self._next(out.last_hidden_state[:, -1], choose)[0]
+        try:
+            if self._own_layers:
+                hidden = self._layers.prompts([ids.view(-1)], [s])
+            else:
+                with _fused_sdpa():
+                    out = self.m.model(ids.view(1, -1), use_cache=True, past_key_values=_write_through(self, s))
+                hidden = out.last_hidden_state[:, -1]
+            return s, self._next(hidden, choose)[0]
+        except Exception:                       # a prompt that the model refuses, a choice that fails
+            self.table.release(s)
+            raise
 
     def release(self, slot):
         self.table.release(slot)
