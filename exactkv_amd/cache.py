@@ -171,6 +171,8 @@ class CompressedKV:
             raise AssertionError(f"{T} tokens do not fit a cache of {self.TS}")
         if x.device != self.sm.device:
             raise ValueError(f"replace expects a tensor on {self.sm.device}")
+        if x.data_ptr() % 4 or any(n % 2 for n in x.stride()[:3]):     # (the encoder reads words)
+            x = x.clone(memory_format=torch.contiguous_format)
         full = T - T % P
         self.T, self.dropped, self._pending = T, 0, None
         self.state[0] = T
