@@ -127,6 +127,13 @@ struct Stage {
     __device__ static int read_at(int col, int half) { return col * 2 * D + (half ^ key_swizzle<D>(col)) * 16; }
 };
 
+// The second pass's sums as 0, shared by all workgroups of the first: keys that no sequence holds stay so, in front of the
+// first one and between offsets that do not ascend as well.
+__device__ inline void zero_sums(const PromptMassArgs& a) {
+    const int64_t n = (int64_t)a.col_parts * a.Hkv * a.NK;
+    for (int64_t i = (int64_t)blockIdx.x * (64 * kWaves) + threadIdx.x; i < n; i += (int64_t)gridDim.x * (64 * kWaves)) a.sums[i] = 0.f;
+}
+
 template <int D>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) mass_rows_kernel(PromptMassArgs a) {
     typedef Stage<D> St;
@@ -136,6 +143,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
     const int part = rest % a.row_parts, index = rest / a.row_parts;
+    zero_sums(a);
     PromptTile tile;
     if (!tile_at<true>(a, index, tile)) return;
     const int col = lane & 31, half = lane >> 5, G = a.G, nrows = tile.Lq * G, shift = tile.Lk - tile.Lq;
@@ -383,15 +391,6 @@ __global__ void __launch_bounds__(1024) mass_rows_join_kernel(PromptMassArgs a) 
     a.row[(int64_t)(hk * a.G + row % a.G) * a.N + tile.q0 + row / a.G] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / l);
 }
 
-// Entries of keys that no sequence holds, from key `end` on: 0, shared by all workgroups.
-template <int THREADS>
-__device__ inline void zero_keys(const PromptMassArgs& a) {
-    const int end = a.S > 0 ? min(max(a.cu_k[a.S], 0), a.NK) : 0;
-    const int64_t n = (int64_t)(a.NK - end) * a.Hkv;
-    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS)
-        a.out[i / (a.NK - end) * a.NK + end + i % (a.NK - end)] = 0.f;
-}
-
 template <int D>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) mass_columns_kernel(PromptMassArgs a) {
     typedef Stage<D> St;
@@ -400,7 +399,6 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), rest = (int)(blockIdx.x / (unsigned)a.Hkv);
     const int part = rest % a.col_parts;
-    if (a.col_parts == 1) zero_keys<64 * kWaves>(a);
     PromptTile tile;
     if (!tile_at<false>(a, rest / a.col_parts, tile)) return;
     const int col = lane & 31, half = lane >> 5, G = a.G, shift = tile.Lk - tile.Lq;
@@ -625,13 +623,12 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     }
 }
 
-// The parts of every key added up; 0 behind the last sequence.
+// The parts of every key added up; 0 where the call has no query.
 __global__ void __launch_bounds__(256) mass_columns_join_kernel(PromptMassArgs a) {
     const int64_t n = (int64_t)a.Hkv * a.NK, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= n) return;
-    const int end = a.S > 0 ? min(max(a.cu_k[a.S], 0), a.NK) : 0;
     float sum = 0.f;
-    if ((int)(at % a.NK) < end)
+    if (a.S > 0)
 #pragma unroll 8
         for (int i = 0; i < a.col_parts; ++i) sum += a.sums[i * n + at];
     a.out[at] = sum;
