@@ -493,7 +493,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             if (p0 + 31 < wkey0 || (a.window > 0 && p0 - (wkey0 + 63) >= a.window)) return;   // uniform: none sees
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const int rel = p0 + col - wkey0 - 4 * half;
+                // (rows behind the last token are zeros, and zeros times an infinite key are no weight of 0: none of them sees a key)
+                const int rel = p0 + col < tile.Lk ? p0 + col - wkey0 - 4 * half : -1;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float x = SAFE ? weight_of(cur[kb][i], row.x, a.qk_scale) : exp2_fast(fmaf(cur[kb][i], a.qk_scale, -row.x));
@@ -572,10 +573,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
                     full_step(last_row, cur, nxt, st ^ 1, 0);
                 advance();
             };
-            // whether all of the tile of tokens `at` see every key of the wavefront
+            // whether the tile of tokens `at` is whole, and all of them see every key of the wavefront
             auto full = [&](int at) {
                 const int p0 = (first + at) * SR + shift;
-                return p0 >= wkey0 + 63 && (a.window == 0 || p0 + SR - 1 - wkey0 < a.window);
+                return p0 >= wkey0 + 63 && p0 + SR <= tile.Lk && (a.window == 0 || p0 + SR - 1 - wkey0 < a.window);
             };
             constexpr std::integral_constant<int, 0> even{};
             constexpr std::integral_constant<int, 1> odd{};

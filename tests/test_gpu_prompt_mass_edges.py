@@ -55,3 +55,32 @@ def test_offsets_that_do_not_ascend(cu):
     got = _mass(q, k, _cu(*cu))
     assert kernels.error_bits(clear=True) == 0x20
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (4, 4, 64), (6, 1, 256)])
+@pytest.mark.parametrize("lens,last", [((100,), 0), ((64,), 0), ((65, 31, 300), 0), ((700,), 33), ((2001, 5), 0), ((333, 200), 100)], ids=str)
+def test_keys_whose_scores_are_all_minus_infinity(lens, last, Hq, Hkv, D):
+    """An infinite key that every query scores with -infinity gets nothing and takes nothing from the others, wherever the queries' rows end."""
+    print("[case]", lens, last, Hq, Hkv, D, flush=True)
+    g = _gen(sum(lens))
+    n = sum(lens)
+    q, k = torch.randn(n, Hq, D, generator=g, device=DEV).bfloat16(), _rows(g, n, Hkv, D)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    ends = [0]
+    far = torch.zeros(n, dtype=torch.bool, device=DEV)
+    for m in lens:
+        ends.append(ends[-1] + m)
+        far[[ends[-2] + i for i in (1, 2, m // 2, m - 2)]] = True              # (never a sequence's first key)
+    k[far, :, 3] = -math.inf
+    got = exactkv.prompt_mass(q, k, _cu(*ends), last=last)
+    want, bound = (torch.zeros(Hkv, n, dtype=torch.float64, device=DEV) for _ in range(2))
+    for a, e in zip(ends, ends[1:]):
+        keep = (~far[a:e]).nonzero()[:, 0]
+        rows = torch.arange(max(0, e - a - last) if last else 0, e - a, device=DEV)
+        # (the others' weights are those of a row without these keys: each query stands behind the kept keys up to its own)
+        pos = torch.searchsorted(keep, rows, right=True) - 1
+        w, err = _weights(q[a:e][rows], k[a:e][keep], pos, 0)
+        for x, y in ((want, w), (bound, err)):
+            x[:, a + keep] = y.view(Hkv, -1, keep.numel()).sum(1)
+    assert (got[:, far] == 0).all()
+    _near(got, want, bound)
