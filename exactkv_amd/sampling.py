@@ -25,9 +25,12 @@ def _setting(v, B, dtype, dev, what, kind):
         if v.dtype is not dtype or v.shape != (B,) or v.get_device() != dev or not v.is_contiguous():
             raise ValueError(f"{what} must be a number or a contiguous {str(dtype)[6:]} [{B}] tensor on the logits' GPU")
         return v.data_ptr(), kind(0)
-    if isinstance(v, bool) or not isinstance(v, (int, float)) or (kind is int and v != int(v)):
-        raise ValueError(f"{what} must be a number or a {str(dtype)[6:]} [{B}] tensor (got {v!r})")
-    return None, kind(v)
+    try:
+        if isinstance(v, (int, float)) and not isinstance(v, bool) and (kind is float or v == int(v)):
+            return None, kind(v)
+    except (OverflowError, ValueError):                # infinite or NaN where whole, whole past a float's range
+        pass
+    raise ValueError(f"{what} must be a number or a {str(dtype)[6:]} [{B}] tensor (got {v!r})")
 
 
 def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=False):
