@@ -99,7 +99,10 @@ def attention_mass(q, k_cache, T=None, *, mass=None, lens=None, block_table=None
     per sequence), block_table and window as in attention_compressed. The softmax is over the tokens the window admits; the
     others get nothing. mass: fp32 [B, Hkv, TS], TS the cache's capacity in tokens (16 per entry of a block table's row), or
     None for 0. Returns out, new, or the one given, which may be mass itself; its entries behind a sequence's tokens are
-    left as they are (0 in a new one)."""
+    left as they are (0 in a new one).
+
+    While it runs, the call holds 4 bytes a query head and token of workspace: T tokens a sequence, with lens as many as the
+    cache's capacity (whatever the window), since its host does not know them."""
     dev = q.get_device()
     if dev >= 0 and dev != _lib.current_device():
         with _on(dev):

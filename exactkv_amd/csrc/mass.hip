@@ -32,8 +32,8 @@ struct MassArgs {
     int64_t lens_stride;
     int B, Hq, Hkv, G, T, TS, window, runs;
     float qk_scale;                    // log2(e) / sqrt(D)
-    float* score;                      // [B * Hq, TSW], TSW = TS rounded up to 16
-    int64_t tsw;
+    float* score;                      // [B * Hq, tsw]
+    int64_t tsw;                       // T (with lens TS, as a sequence may have so many) rounded up to 16
     float2* part;                      // [B * Hq, runs]: maximum, sum
     const float* mass;                 // [B, Hkv, TS], or nullptr
     float* out;
@@ -225,6 +225,7 @@ static int mass_runs(int64_t B, int64_t Hq, int64_t Hkv, int64_t reach) {
     if (runs > pages) runs = pages;
     return runs < 1 ? 1 : (int)runs;
 }
+static int64_t score_row(int64_t T) { return (T + kPage - 1) / kPage * kPage; }
 static int64_t reach_of(int64_t T, int64_t window) { return window > 0 && window + kPage - 1 < T ? window + kPage - 1 : T; }
 
 template <bool COMPRESSED>
@@ -242,7 +243,7 @@ static int launch_mass(MassArgs a, int32_t D, void* ws, int64_t ws_bytes, hipStr
     a.G = a.Hq / a.Hkv;
     const int64_t reach = reach_of(a.lens != nullptr ? a.TS : a.T, a.window), rows = (int64_t)a.B * a.Hq;
     a.runs = mass_runs(a.B, a.Hq, a.Hkv, reach);
-    a.tsw = ((int64_t)a.TS + kPage - 1) / kPage * kPage;
+    a.tsw = score_row(a.lens != nullptr ? a.TS : a.T);
     const int64_t need = rows * (a.tsw * 4 + a.runs * 8);
     EXKV_REQUIRE((uintptr_t)ws % 16 == 0 && ws_bytes >= need, "attention_mass: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                  (long long)need);
@@ -269,8 +270,8 @@ using namespace exkv;
 
 extern "C" int64_t exkv_mass_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t TS, int32_t has_lens, int32_t window) {
     if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || TS < 0 || T < 0 || window < 0) return 0;
-    const int64_t tsw = ((int64_t)TS + kPage - 1) / kPage * kPage;
-    return (int64_t)B * Hq * (tsw * 4 + mass_runs(B, Hq, Hkv, reach_of(has_lens != 0 ? TS : T, window)) * 8);
+    const int64_t most = has_lens != 0 ? TS : T;
+    return (int64_t)B * Hq * (score_row(most) * 4 + mass_runs(B, Hq, Hkv, reach_of(most, window)) * 8);
 }
 
 extern "C" int exkv_attention_mass(const void* q, const void* sm, const void* code, const void* base, const int32_t* rowmask,
