@@ -339,7 +339,7 @@ __device__ inline void take(const SampleArgs& a, int b, const Row& row, uint64_t
     // log w - log S, w from its place and not as it is added up: of an unlikely token's few multiples of 2^-43 a logarithm
     // would be off by up to 0.1
     if (a.logprob != nullptr)
-        a.logprob[b] = (float)(-0.6931471805599453 / kPerOctave * (row.any_place(logit_of(token)) - kBase) - log((double)S / kOne));
+        a.logprob[b] = (float)(0.6931471805599453 / kPerOctave * (kBase - row.any_place(logit_of(token))) - log((double)S / kOne));
 }
 
 // x of lane ^ D.

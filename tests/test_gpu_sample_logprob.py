@@ -66,3 +66,12 @@ def test_weights_at_the_end_of_their_range():
     for u in (0.3, 0.9, 1 - 2.0 ** -10, 1 - 2.0 ** -24):
         drawn += int((_check(x, torch.full((43,), u, device=DEV)) < -0.7).sum())
     assert drawn > 30
+
+
+@pytest.mark.parametrize("V", [3, 9000])
+def test_a_certain_token(V):
+    """Its log-probability is 0, with 0's own sign."""
+    x = torch.full((2, V), -math.inf, device=DEV)
+    x[:, V - 1] = 3.0
+    token, lp = exactkv.sample(x, torch.tensor([0.0, 0.9], device=DEV), logprob=True)
+    assert token.tolist() == [V - 1] * 2 and lp.tolist() == [0.0, 0.0] and not torch.signbit(lp).any()
