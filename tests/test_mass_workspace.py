@@ -28,7 +28,9 @@ def test_a_short_call_takes_little(T):
     torch.cuda.reset_peak_memory_stats()
     before = torch.cuda.memory_allocated()
     exactkv.attention_mass(q, k, T, out=out)
-    assert torch.cuda.max_memory_allocated() - before <= B * Hq * (4 * (T + 15) + 8 * 256) + 512
+    # (torch's allocator rounds up to 512 bytes, and hands out a block of its large pool whole where 2^20 bytes or less would remain of it;
+    # the cache's capacity would be 2^24)
+    assert torch.cuda.max_memory_allocated() - before <= B * Hq * (4 * (T + 15) + 8 * 256) + 512 + 2 ** 20
     assert torch.equal(out[..., :T], exactkv.attention_mass(q, k[:, :T].contiguous(), T)) and (out[..., T:] == 0).all()
     short = exactkv.attention_mass(q, k, lens=torch.tensor([T], dtype=torch.int32, device="cuda"))
     assert torch.allclose(short[..., :T], out[..., :T], rtol=1e-4, atol=1e-9)
