@@ -9,7 +9,8 @@
 // 4 bytes a query head and key, of which the keys' own bytes are 1.5 D a KV head (4 heads of 128: 16 to 192).
 //
 // Bound by the keys' bytes where there are many (8 sequences of 8,192 compressed tokens, 8 KV heads: 105 MB of keys in
-// 24 us, 4.4 TB/s, and 5.5 us for the join; 61 of up to 4,339 in pages, 4 KV heads: 144 MB in 34 us, 4.2 TB/s, and 8.6), by the host's 12 us a call where there are few (one of 997 tokens: 4.2 and 4.2 us).
+// 24 us, 4.4 TB/s, and 5.4 us for the join; 61 of up to 4,339 in pages, 4 KV heads: 144 MB in 34 us, 4.2 TB/s, and 8.5), by the
+// host's 12 us a call where there are few (one of 997 tokens: 4.0 and 4.2 us).
 #include "errors.hpp"
 #include "tile.hpp"
 #include "../../include/exactkv.h"

@@ -17,9 +17,10 @@
 // Both are cut into parts where there are few tiles; parts are joined in order, so a call's bits do not change.
 //
 // Bound by the exponentials, two for each visible pair: one of 8,192 tokens, 32 query and 8 KV heads of 128, needs
-// 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); rows take 247 us,
-// columns 285 us. Prompts of few rows are bound by the latency of their few stages: 64 queries of 32 heads over 16,385 keys
-// 19 + 5 + 27 us (four stages in LDS instead of two do not shorten them: 19.6, and 8,192 tokens' rows take 267).
+// 2 x 1.07e9 of them and twice 275 GFLOP of products (460 us at the rate of a large library product); the call takes 521 to
+// 547 us, by the card, of which under a kernel trace rows 253 and columns 291. Prompts of few rows are bound by the latency of
+// their few stages: 64 queries of 32 heads over 16,385 keys 18 + 4 + 24 us (four stages in LDS instead of two do not shorten
+// the rows: 19.6 us for then 19, and 8,192 tokens' 267 for 253).
 #include "errors.hpp"
 #include "prompt_stage.hpp"
 #include "../../include/exactkv.h"

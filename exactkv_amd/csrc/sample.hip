@@ -20,9 +20,14 @@
 // running sum than that. The log-probability that is returned takes the token's own y, which is not rounded so.
 //
 // Rows of up to 8,192 logits take one launch, a workgroup each; longer ones four, cut into pieces: largest, bins, collected,
-// taken. 256 rows of 152,064 bf16 logits (78 MB): 19, 33, 25 and 9.5 us, the second bound by its fp64 operations, the first and the
-// third by memory (3.1 to 4.1 TB/s); 61 of 50,257 fp32 (12 MB): 4.9, 8.1, 12 and 8.7; one of 128,256: 3.7, 4.7, 6.1
-// and 6.6, each a chain of launches, loads and barriers.
+// taken. 256 rows of 152,064 bf16 logits (78 MB): 19, 33, 25 and 9.4 us, the second bound by its fp64 operations, the first and the
+// third by memory (3.1 to 4.1 TB/s); 61 of 50,257 fp32 (12 MB): 4.9, 8.4, 12 and 8.4; one of 128,256: 4.0, 4.9, 6.6
+// and 6.4, each a chain of launches, loads and barriers.
+//
+// A row of which more than kList tokens lie in the bins in question, or more than kLocal of them in one piece, is walked again
+// by one workgroup in the last launch: flat rows, and with 1,024 rows or more (a piece each) a top_k of 1,025 to 2,048.
+// 64 rows of 128,256: 55 us, at a temperature of 50 (nearly all tokens in a few bins) 314, with top_p 0.9 as well 545; 1,024 of
+// 50,257 with top_k 1,500 298 us, 2,049 (by sums) 131.
 #include "errors.hpp"
 #include "common.hpp"
 #include "../../include/exactkv.h"
@@ -1055,9 +1060,9 @@ struct SamplePlan {
 static SamplePlan plan_sample(int64_t B, int64_t V) {
     SamplePlan p{};
     if (V <= kShort || B == 0) return p;
-    // pieces of whole 2,048 logits, about 1,024 workgroups in all (256 x 152064, 512 / 1,024 / 2,048: 112 / 99 / 102 us; 128
-    // mixed rows 68 / 59 / 62), of 4,096 logits at least (61 x 50257, 2,048 / 4,096: 44.8 / 43.2 us), but not so few that CUs
-    // stay idle (1 x 128256: 24.7 / 27.9)
+    // pieces of whole 2,048 logits, about 1,024 workgroups in all (256 x 152064, 512 / 1,024 / 2,048: 89.3 / 83.0 / 90.2 us; 128
+    // mixed rows, by their inputs, 50 to 60 each), of 4,096 logits at least (61 x 50257, 2,048 / 4,096: 37.4 / 36.0 us), but not
+    // so few that CUs stay idle (1 x 128256: 21.4 / 22.2)
     const int64_t least = B * (V / 4096) < 256 ? 2048 : 4096;
     int64_t pieces = (1024 + B - 1) / B;
     if (pieces > V / least) pieces = V / least;
