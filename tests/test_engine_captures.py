@@ -60,20 +60,30 @@ def test_an_engine_goes_with_its_last_name(paged):
 @pytest.mark.gpu
 @pytest.mark.parametrize("paged", [False, True])
 def test_engines_that_went_while_another_captures(paged):
-    """Engines with captured steps in cycles, nobody's any more, and a collector that runs at every allocation."""
+    """Engines with captured steps in cycles, nobody's any more, and so many objects made during a capture that the collector,
+    did it not rest, would run there and find them."""
     from tests.test_gpu_engine_layers import _ids, _model
     m = _model("llama")
     ids = _ids(2, 30)
+    gone = []
 
-    def run():
+    def run(made):
         if paged:
             eng = exactkv.PagedEngine(m, 2, 64, layer_kernels=True)
             eng.add_many(list(ids[:, :20]))
         else:
             eng = exactkv.Engine(m, 2, 64, layer_kernels=True)
             eng.prefill(ids[:, :20])
+        forward, seen = eng._forward, []
+
+        def with_objects(*args, **kw):
+            seen.append(torch.cuda.is_current_stream_capturing())
+            held = [[i] for i in range(made if seen[-1] else 0)]
+            assert not held or all(r() is not None for r in gone)
+            return forward(*args, **kw)
+        eng._forward = with_objects                    # (and a cycle: only the collector finds this engine)
         out = torch.stack([eng.step(ids[:, t]) for t in range(20, 30)])
-        assert eng.captures == 1
+        assert eng.captures == 1 and seen == [False, True]
         return eng, out
     was = gc.get_threshold()
     gc.collect()
@@ -81,14 +91,17 @@ def test_engines_that_went_while_another_captures(paged):
         gc.disable()
         want = None
         for _ in range(3):
-            eng, out = run()
-            eng.itself = eng                           # a cycle: only the collector finds it
+            eng, out = run(0)
+            gone.append(weakref.ref(eng))
             del eng
             assert want is None or same_bits(out, want)
             want = out
-        gc.set_threshold(1)
+        assert all(r() is not None for r in gone)
+        gc.set_threshold(100000)
         gc.enable()
-        assert same_bits(run()[1], want)
+        assert same_bits(run(200000)[1], want)
+        gc.collect()
+        assert all(r() is None for r in gone)
     finally:
         gc.set_threshold(*was)
         gc.enable()
