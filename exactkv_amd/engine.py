@@ -600,10 +600,11 @@ class PagedEngine:
     def step(self, tok, slots=None):
         """tok: [n] the current token of each slot in `slots` (default: every live slot, in
         order). Returns logits [n, vocab] for their next tokens."""
+        slots = self.table.live_slots() if slots is None else [int(s) for s in slots]
         if self.table._cut:
-            for s in self.table.live_slots() if slots is None else slots:
-                if self.table.dropped(int(s)):
-                    raise RuntimeError(f"slot {int(s)} was cut (evict): its positions are not its places, at which a paged engine's "
+            for s in slots:
+                if self.table.dropped(s):
+                    raise RuntimeError(f"slot {s} was cut (evict): its positions are not its places, at which a paged engine's "
                                        "steps stand")
         slots = self.table.begin_step(slots)
         n = len(slots)

@@ -51,6 +51,19 @@ def test_a_paged_engine_does_not_go_on():
     assert eng.add(torch.arange(30))[0] == slots[1]
 
 
+def test_slots_are_read_once():
+    """A step's slots may be any iterable, beside slots that were cut too."""
+    eng = exactkv.PagedEngine(_tiny("llama").bfloat16(), 3, 64, backend="bf16", graph=False)
+    slots = [eng.add(torch.arange(n))[0] for n in (20, 30)]
+    eng.table.cut(slots[1], 10)
+    seen = []
+    eng.table.begin_step = lambda which: seen.append(list(which)) or [][0]     # (the step's kernels need a GPU: it ends here)
+    for which in (iter(slots[:1]), slots[:1], (s for s in slots[:1])):
+        with pytest.raises(IndexError):
+            eng.step(torch.zeros(1, dtype=torch.long), which)
+    assert seen == [[0]] * 3
+
+
 def test_one_table_of_angles_is_one_distance():
     """rope_append over pages has one table for all rows of a step: slots that were cut by different numbers of tokens are refused."""
     t = exactkv.PageTable(20, 3, 10, device="cpu")
