@@ -548,8 +548,8 @@ int exkv_add_norm(const void* x, int64_t sx, const void* r, int64_t sr, const vo
  * passes u[b] S, and logprob[b] (may be NULL) log(w / S). temperature not above 0: the largest logit, the first of equal
  * ones. u: [0, 1) (clamped). temperature, top_k, top_p, min_p: [B], or NULL for the value of the same name with 0 for every
  * row. NaN and -infinity are never drawn; a row of nothing else gives token 0, log-probability -infinity, and is reported
- * (EXKV_ERR_LOGITS). Weights are fp64, rounded to multiples of 2^-43. ws (16-byte aligned) is the call's own while it
- * runs. One launch up to 8,192 logits a row, four beyond.
+ * (EXKV_ERR_LOGITS). Weights are made in fp64 and added up rounded to multiples of 2^-43, which log(w / S) takes for S alone. ws
+ * (16-byte aligned) is the call's own while it runs. One launch up to 8,192 logits a row, four beyond.
  * No counterpart in the reference, which decodes greedily (engine.py:93-95). */
 int exkv_sample(const void* logits, int64_t stride, int32_t type, int32_t B, int32_t V, const float* u, const float* temperature,
                 const int32_t* top_k, const float* top_p, const float* min_p, float temperature0, int32_t top_k0, float top_p0,
@@ -558,7 +558,7 @@ int exkv_sample(const void* logits, int64_t stride, int32_t type, int32_t B, int
 /* Bytes of that workspace (0: none). */
 int64_t exkv_sample_workspace(int32_t B, int32_t V);
 
-/* Bytes of the workspace that exkv_attention_mass needs (has_lens: lens is given). */
+/* Bytes of the workspace that exkv_attention_mass needs: scores of T tokens a sequence, of TS where lens is given (has_lens). */
 int64_t exkv_mass_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t TS, int32_t has_lens, int32_t window);
 
 /* The attention that cached tokens receive from one query token of each sequence: q [B, Hq, D] over the keys of a
